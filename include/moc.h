@@ -749,6 +749,39 @@ typedef struct {
 int moc_decode_step_group(const moc_decode_layer* layers, int n, int64_t B, int64_t d, int H, int HK, int T, int NS,
                           float scale, int64_t N, size_t workspace_bytes, hipStream_t stream);
 
+/* ------------------------------------------------- end of a sublayer, next norm */
+
+/* u = norm(x) w1 + b1 (post; u = x without), h = alpha residual + gate u, n = norm(h) w2 + b2 (pre), on rows of d
+ * elements (d <= 16,384), f32 in between.  x, n and a full gate of x_dtype, residual and h of r_dtype; weights and
+ * biases f32 [d] or NULL (1 and 0); a channel gate f32 [d].  The no-copy counterpart of the residual add of
+ * MemoryTransformerBlock (memory_block.py:549-558) with a norm behind the block, a gate and a residual scale. */
+#define MOC_GATE_NONE 0
+#define MOC_GATE_SCALAR 1  /* one value */
+#define MOC_GATE_CHANNEL 2 /* f32 [d] */
+#define MOC_GATE_TOKEN 3   /* [rows] */
+#define MOC_GATE_FULL 4    /* [rows][d] of x_dtype */
+typedef struct {
+  const void *x, *residual, *gate;
+  const float *w1, *b1, *w2, *b2;
+  void *h, *n;
+  float* stats; /* f32 [4][rows]: mean and 1 / deviation of x, then of h (NULL: not wanted; the backward's input) */
+  int64_t rows, d;
+  int x_dtype, r_dtype, gate_mode, gate_dtype, norm, post, pre;
+  float alpha, eps;
+} moc_gated_norm;
+int moc_gated_norm_fwd(const moc_gated_norm* a, hipStream_t stream);
+/* Gradients: dh (r_dtype) and dn (x_dtype) arrive (either may be NULL: zero); dx, dres and dgate (token, full) are
+ * written where not NULL; dparams f32 [5 d + 1] = dw1, db1, dw2, db2, the channel gate's gradient (zeros without
+ * one), and the scalar gate's.  a: as the forward's, with its stats. */
+typedef struct {
+  const void *dh, *dn;
+  void *dx, *dres, *dgate;
+  float* dparams;
+} moc_gated_norm_grads;
+size_t moc_gated_norm_bwd_workspace(int64_t rows, int64_t d);
+int moc_gated_norm_bwd(const moc_gated_norm* a, const moc_gated_norm_grads* g, void* workspace, size_t workspace_bytes,
+                       hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,7 @@ a tensor is not on the GPU.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import re
@@ -157,6 +158,9 @@ _SIGS = {
     "moc_bank_touched": (_I, [_P, _I64, _I, _P, _P, _P]),
     "moc_bank_sqnorm_workspace": (_SZ, [_I64, _I64]),
     "moc_bank_sqnorm": (_I, [_P, _P, _P, _I64, _I64, _P, _SZ, _P, _P]),
+    "moc_gated_norm_fwd": (_I, [_P, _P]),
+    "moc_gated_norm_bwd_workspace": (_SZ, [_I64, _I64]),
+    "moc_gated_norm_bwd": (_I, [_P, _P, _P, _SZ, _P]),
 }
 
 _lib = None
@@ -307,3 +311,20 @@ def require_gpu(*tensors: torch.Tensor) -> None:
             raise RuntimeError(
                 "memory_amd runs only on ROCm devices (HIP kernels of libmoc.so); got a tensor on "
                 f"{t.device}. There is no CPU fallback.")
+
+
+def require_one_device(*tensors: torch.Tensor) -> None:
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"expected tensors on one device, got {sorted(map(str, devices))}")
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which `device` is the current one (a launch goes to the current device; nothing to do, and
+    nothing allocated, where it is already)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _here
+    return torch.cuda.device(device)

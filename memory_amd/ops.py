@@ -7,12 +7,14 @@ allocator), the current stream and autograd bookkeeping only.
 
 from __future__ import annotations
 
+import ctypes
 import functools
 from dataclasses import dataclass
 from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from ._lib import call, ptr, stream_ptr
@@ -545,6 +547,150 @@ def row_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]
     if od not in (torch.float32, torch.bfloat16):
         raise ValueError(f"row_norm outputs float32 or bfloat16, got {od}")
     return _RowNorm.apply(x, weight, bias, code, float(eps), od)
+
+
+class _GatedNormArgs(ctypes.Structure):
+    """moc_gated_norm."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "residual", "gate", "w1", "b1", "w2", "b2", "h", "n", "stats")]
+                + [("rows", ctypes.c_int64), ("d", ctypes.c_int64)]
+                + [(n, ctypes.c_int) for n in ("x_dtype", "r_dtype", "gate_mode", "gate_dtype", "norm", "post", "pre")]
+                + [("alpha", ctypes.c_float), ("eps", ctypes.c_float)])
+
+
+class _GatedNormGrads(ctypes.Structure):
+    """moc_gated_norm_grads."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dh", "dn", "dx", "dres", "dgate", "dparams")]
+
+
+_GATE_NONE, _GATE_SCALAR, _GATE_CHANNEL, _GATE_TOKEN, _GATE_FULL = range(5)
+
+
+def _gate_mode(gate: Optional[torch.Tensor], x: torch.Tensor) -> int:
+    if gate is None:
+        return _GATE_NONE
+    d = x.shape[-1]
+    if gate.numel() == 1:
+        return _GATE_SCALAR
+    if gate.shape == (d,):
+        return _GATE_CHANNEL
+    if gate.shape == x.shape[:-1] + (1,):
+        return _GATE_TOKEN
+    if gate.shape == x.shape:
+        return _GATE_FULL
+    raise ValueError(f"gate of shape {tuple(gate.shape)}: expected one value, ({d},), {tuple(x.shape[:-1] + (1,))} or "
+                     f"{tuple(x.shape)}")
+
+
+class _GatedResidualNorm(torch.autograd.Function):
+    """gated_residual_norm on 2-D rows (moc_gated_norm_fwd / _bwd).  The backward reads x and the residual again and
+    forms h from them in float32, so nothing of the forward but the rows' statistics is kept."""
+
+    @staticmethod
+    def forward(ctx, x, r, gate, w1, b1, w2, b2, mode, norm, alpha, eps, trains):
+        R, d = x.shape
+        dev = x.device
+        h = torch.empty_like(r)
+        n = torch.empty_like(x) if w2 is not None else None
+        stats = torch.empty(4, R, device=dev, dtype=torch.float32) if trains else None
+        args = _GatedResidualNorm.args(x, r, gate, w1, b1, w2, b2, mode, norm, alpha, eps, h, n, stats)
+        with L.on_device(dev):
+            call("moc_gated_norm_fwd", ctypes.addressof(args), stream_ptr(dev))
+        if trains:
+            ctx.save_for_backward(x, r, gate, w1, b1, w2, b2, stats)
+            ctx.cfg = (mode, norm, alpha, eps)
+        ctx.set_materialize_grads(False)
+        return (h, n) if n is not None else h
+
+    @staticmethod
+    def args(x, r, gate, w1, b1, w2, b2, mode, norm, alpha, eps, h, n, stats):
+        return _GatedNormArgs(ptr(x), ptr(r), ptr(gate), ptr(w1), ptr(b1), ptr(w2), ptr(b2), ptr(h), ptr(n), ptr(stats),
+                              x.shape[0], x.shape[1], L.dtype_code(x.dtype), L.dtype_code(r.dtype), mode,
+                              0 if gate is None else L.dtype_code(gate.dtype), norm, w1 is not None, w2 is not None, alpha,
+                              eps)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, dn=None):
+        x, r, gate, w1, b1, w2, b2, stats = ctx.saved_tensors
+        mode, norm, alpha, eps = ctx.cfg
+        need = ctx.needs_input_grad
+        if dh is None and dn is None:
+            return (None,) * 12
+        R, d = x.shape
+        dev = x.device
+        dh = None if dh is None else dh.contiguous()
+        dn = None if dn is None else dn.contiguous()
+        dx = torch.empty_like(x) if need[0] else None
+        dr = torch.empty_like(r) if need[1] else None
+        dg = torch.empty_like(gate) if need[2] and mode in (_GATE_TOKEN, _GATE_FULL) else None
+        dp = torch.empty(5 * d + 1, device=dev, dtype=torch.float32)
+        ws_bytes = L.query("moc_gated_norm_bwd_workspace", R, d)
+        ws = torch.empty(ws_bytes // 4, device=dev, dtype=torch.float32)
+        args = _GatedResidualNorm.args(x, r, gate, w1, b1, w2, b2, mode, norm, alpha, eps, None, None, stats)
+        out = _GatedNormGrads(ptr(dh), ptr(dn), ptr(dx), ptr(dr), ptr(dg), ptr(dp))
+        with L.on_device(dev):
+            call("moc_gated_norm_bwd", ctypes.addressof(args), ctypes.addressof(out), ptr(ws), ws_bytes, stream_ptr(dev))
+        if need[2] and mode == _GATE_SCALAR:
+            dg = dp[5 * d:].to(gate.dtype).view(gate.shape)
+        elif need[2] and mode == _GATE_CHANNEL:
+            dg = dp[4 * d:5 * d]
+        col = [dp[i * d:(i + 1) * d] if t is not None and need[3 + i] and (i < 2 or dn is not None) else None
+               for i, t in enumerate((w1, b1, w2, b2))]
+        return (dx, dr, dg, *col, None, None, None, None, None)
+
+
+def gated_residual_norm(x: torch.Tensor, residual: torch.Tensor, *, post_weight: Optional[torch.Tensor] = None,
+                        post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                        residual_scale: float = 1.0, pre_weight: Optional[torch.Tensor] = None,
+                        pre_bias: Optional[torch.Tensor] = None, eps: float = 1e-6, norm: str = "rms",
+                        out_dtype: Optional[torch.dtype] = None):
+    """The end of a sublayer and the next one's norm in one pass over the rows:
+
+        u = norm(x) * post_weight + post_bias        (without a post_weight: u = x)
+        h = residual_scale * residual + gate * u     (residual's dtype)
+        n = norm(h) * pre_weight + pre_bias          (``out_dtype``, default x's; without a pre_weight: None)
+
+    Returns (h, n).  ``norm`` is "rms" or "layer" (biases only there) over the last dim (up to 16,384).  ``gate``: one
+    value, one per channel (d,), one per row (..., 1), or x's shape.  x and residual are float32 or bfloat16 (float16
+    runs as float32) of one shape; everything in between is float32, h and n are rounded once each and n is the norm
+    of the unrounded h.  Differentiable once in every tensor."""
+    if norm not in ("rms", "layer"):
+        raise ValueError(f"norm must be 'rms' or 'layer', got {norm!r}")
+    if x.shape != residual.shape or x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"x {tuple(x.shape)} and residual {tuple(residual.shape)} must be rows of one shape")
+    d = x.shape[-1]
+    if post_weight is None and post_bias is not None or pre_weight is None and pre_bias is not None:
+        raise ValueError("a bias needs the weight of its norm")
+    if norm == "rms" and (post_bias is not None or pre_bias is not None):
+        raise ValueError("RMSNorm has no bias")
+    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight),
+                    ("pre_bias", pre_bias)):
+        if t is not None and t.shape != (d,):
+            raise ValueError(f"{name} of shape {tuple(t.shape)}, expected {(d,)}")
+    mode = _gate_mode(gate, x)
+    od = x.dtype if out_dtype is None else out_dtype
+    if any(not t.is_floating_point() for t in (x, residual)) or not od.is_floating_point:
+        raise ValueError(f"gated_residual_norm takes floating-point rows, got {x.dtype}, {residual.dtype}, {od}")
+    L.require_gpu(x, residual, gate, post_weight, post_bias, pre_weight, pre_bias)
+    L.require_one_device(x, residual, gate, post_weight, post_bias, pre_weight, pre_bias)
+    rd = residual.dtype
+    kt = torch.bfloat16 if x.dtype == torch.bfloat16 and (od == torch.bfloat16 or pre_weight is None) else torch.float32
+    x2 = x.reshape(-1, d).to(kt).contiguous()
+    r2 = residual.reshape(-1, d).to(rd if rd in (torch.float32, torch.bfloat16) else torch.float32).contiguous()
+    if gate is not None:
+        if mode == _GATE_FULL:
+            gate = gate.reshape(-1, d).to(kt)
+        elif mode == _GATE_CHANNEL or gate.dtype not in (torch.float32, torch.bfloat16):
+            gate = gate.float()
+        gate = gate.reshape(-1) if mode == _GATE_TOKEN else gate
+        gate = gate.contiguous()
+    w = [None if t is None else t.float().contiguous() for t in (post_weight, post_bias, pre_weight, pre_bias)]
+    trains = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, r2, gate, *w))
+    out = _GatedResidualNorm.apply(x2, r2, gate, *w, mode, L.MOC_NORM_RMS if norm == "rms" else L.MOC_NORM_LAYERNORM,
+                                   float(residual_scale), float(eps), trains)
+    h, n = out if isinstance(out, tuple) else (out, None)
+    h = h.view(x.shape).to(rd)
+    return h, None if n is None else n.view(x.shape).to(od)
 
 
 class _NormLinear(torch.autograd.Function):
