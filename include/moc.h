@@ -99,6 +99,29 @@ int moc_router_seq_bwd(const float* logits, const int32_t* idx, const float* w, 
                        int64_t R, int64_t C, int S, int k, float scale, const float* dz_in, float* dlogits,
                        hipStream_t stream);
 
+/* The chapter selection as a mixture of experts routes (no reference counterpart; stands beside moc_router_topk):
+ * s = softmax over the chapters c >= S, or sigmoid; key = s + bias (bias f32 [C] or NULL; it steers the selection
+ * only), -inf for a masked logit (-inf); the C - S chapters lie in `groups` runs of equal length, a group scores the
+ * sum of its group_best (1 or 2) largest keys and the top_groups best stay (ties: lower group); the k largest keys
+ * of those, keys descending (compared in f64), equal keys by ascending chapter.  w = scale s / max(sum s, 1e-12)
+ * (renormalize) or scale s.  logits f32 [R] rows of stride ldz; idx i32 [R, k] (global ids); w f32 [R, k];
+ * s_sel f32 [R, k] (the selected s) and row_stats f32 [R, 2] (softmax: maximum and sum of exp) are the backward's
+ * inputs, NULL to skip.  C <= 16,384, k <= 1,024, groups <= 1,024. */
+#define MOC_SCORE_SOFTMAX 0
+#define MOC_SCORE_SIGMOID 1
+int moc_router_select(const float* logits, int64_t ldz, int64_t R, int64_t C, int S, int k, int score, const float* bias,
+                      int groups, int top_groups, int group_best, int renormalize, float scale, int32_t* idx, float* w,
+                      float* s_sel, float* row_stats, hipStream_t stream);
+/* Gradient of w with respect to the logits: every element of dlogits f32 [R, C] is written (idx must hold k
+ * different chapters of [S, C) per row, as moc_router_select writes them). */
+int moc_router_select_bwd(const float* logits, int64_t ldz, const int32_t* idx, const float* s_sel, const float* row_stats,
+                          const float* dw, int64_t R, int64_t C, int S, int k, int score, int renormalize, float scale,
+                          float* dlogits, hipStream_t stream);
+/* Balance step of the bias: counts i32 [C] = how often idx i32 [n] names each chapter (ids outside [0, C) are
+ * skipped), then bias[c] += rate * sign(mean of counts[S..] - counts[c]) for c >= S. */
+int moc_router_balance(const int32_t* idx, int64_t n, int64_t C, int S, float rate, int32_t* counts, float* bias,
+                       hipStream_t stream);
+
 /* Replaces the pooling of ChapterRouter.forward (router.py:96-107 mean; :158-195 rolling
  * mean given as per-position coefficients coef f32 [L], NULL = mean).
  * h [B, L, d] of dtype; pooled f32 [B, d]; workspace from moc_router_pool_workspace. */

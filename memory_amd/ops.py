@@ -159,6 +159,112 @@ def router_topk(logits: torch.Tensor, k: int, exclude_prefix_chapters: int = 0):
     return _RouterTopK.apply(logits, int(k), int(exclude_prefix_chapters))
 
 
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+class _RouterSelect(torch.autograd.Function):
+    """router_select on (R, C) float32 rows (moc_router_select / _bwd)."""
+
+    @staticmethod
+    def forward(ctx, z, bias, k, S, score, groups, top_groups, best, renorm, scale):
+        R, C = z.shape
+        dev = z.device
+        idx = torch.empty(R, k, device=dev, dtype=torch.int32)
+        w = torch.empty(R, k, device=dev, dtype=torch.float32)
+        s_sel = row_stats = None
+        if ctx.needs_input_grad[0]:
+            s_sel = torch.empty(R, k, device=dev, dtype=torch.float32)
+            if score == 0:
+                row_stats = torch.empty(R, 2, device=dev, dtype=torch.float32)
+        with L.on_device(dev):
+            call("moc_router_select", ptr(z), z.stride(0), R, C, S, k, score, ptr(bias), groups, top_groups, best, renorm,
+                 scale, ptr(idx), ptr(w), ptr(s_sel), ptr(row_stats), stream_ptr(dev))
+        ctx.save_for_backward(z, idx, s_sel, row_stats)
+        ctx.cfg = (k, S, score, renorm, scale)
+        ctx.mark_non_differentiable(idx)
+        ctx.set_materialize_grads(False)
+        return idx, w
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _didx, dw):
+        if dw is None:
+            return (None,) * 10
+        z, idx, s_sel, row_stats = ctx.saved_tensors
+        k, S, score, renorm, scale = ctx.cfg
+        R, C = z.shape
+        dev = z.device
+        dw = dw.float().contiguous()
+        dz = torch.empty(R, C, device=dev, dtype=torch.float32)
+        with L.on_device(dev):
+            call("moc_router_select_bwd", ptr(z), z.stride(0), ptr(idx), ptr(s_sel), ptr(row_stats), ptr(dw), R, C, S, k,
+                 score, renorm, scale, ptr(dz), stream_ptr(dev))
+        return (dz,) + (None,) * 9
+
+
+def router_select(logits: torch.Tensor, k: int, exclude_prefix_chapters: int = 0, *, score: str = "softmax",
+                  bias: Optional[torch.Tensor] = None, num_groups: int = 1, top_groups: Optional[int] = None,
+                  group_best: int = 2, renormalize: bool = True, scale: float = 1.0):
+    """Top-k chapters as a mixture of experts routes: (idx int32 (R, k), weights float32 (R, k)) of logits (R, C).
+
+    s is the softmax over the chapters past the excluded prefix, or the sigmoid of each logit; key = s + ``bias``
+    (a (C,) tensor without a gradient that steers the selection and nothing else).  The chapters past the prefix lie
+    in ``num_groups`` runs of equal length; a group scores the sum of its ``group_best`` (1 or 2) largest keys, and
+    only the ``top_groups`` best groups (default: all) are selected from.  Order: key descending (compared in
+    float64), equal keys by ascending chapter.  Weights are ``scale`` times s, divided by the selected scores' sum with
+    ``renormalize``; the gradient (once differentiable) flows to the logits.
+
+    A logit of -inf masks its chapter: it comes after every other, with weight 0 (rows with fewer than k others
+    still name k chapters; a softmax row without any other has NaN weights).  NaN sorts first, as in torch.topk.
+    Up to 16,384 chapters, k up to 1,024."""
+    if score not in _SCORES:
+        raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be 2D (rows, chapters), got shape {tuple(logits.shape)}")
+    R, C = logits.shape
+    S, k, G = int(exclude_prefix_chapters), int(k), int(num_groups)
+    g = G if top_groups is None else int(top_groups)
+    n = C - S
+    if S < 0 or n <= 0:
+        raise ValueError(f"exclude_prefix_chapters must be in [0, {C}), got {S}")
+    if G < 1 or n % G != 0 or not 1 <= g <= G:
+        raise ValueError(f"{n} chapters in num_groups={G}, top_groups={g}: groups of equal length, at least one kept")
+    best = int(group_best)
+    if best not in (1, 2):
+        raise ValueError(f"group_best must be 1 or 2, got {group_best}")
+    best = min(best, n // G)
+    if not 1 <= k <= g * (n // G):
+        raise ValueError(f"k={k} of {g * (n // G)} selectable chapters")
+    if bias is not None and bias.shape != (C,):
+        raise ValueError(f"bias of shape {tuple(bias.shape)}, expected {(C,)}")
+    L.require_gpu(logits, bias)
+    L.require_one_device(logits, bias)
+    z = logits.float()
+    if z.stride(1) != 1 or z.stride(0) < C:
+        z = z.contiguous()
+    if bias is not None:
+        bias = bias.detach().float().contiguous()
+    return _RouterSelect.apply(z, bias, k, S, _SCORES[score], G, g, best, bool(renormalize), float(scale))
+
+
+def router_balance_(bias: torch.Tensor, idx: torch.Tensor, rate: float, exclude_prefix_chapters: int = 0) -> torch.Tensor:
+    """Move the balance bias (C,) float32 in place towards equal use: + rate for chapters past the excluded prefix that
+    ``idx`` (chapter ids of any shape) names less often than their mean, - rate for more often.  Returns how
+    often each chapter is named (C,) int32."""
+    if bias.dim() != 1 or bias.dtype != torch.float32 or not bias.is_contiguous():
+        raise ValueError("the balance bias is a contiguous float32 vector")
+    C, S = bias.shape[0], int(exclude_prefix_chapters)
+    if not 0 <= S < C:
+        raise ValueError(f"exclude_prefix_chapters must be in [0, {C}), got {S}")
+    L.require_gpu(bias, idx)
+    L.require_one_device(bias, idx)
+    ids = idx.reshape(-1).to(torch.int32).contiguous()
+    counts = torch.empty(C, device=bias.device, dtype=torch.int32)
+    with L.on_device(bias.device):
+        call("moc_router_balance", ptr(ids), ids.numel(), C, S, float(rate), ptr(counts), ptr(bias), stream_ptr(bias.device))
+    return counts
+
+
 class _PrependShared(torch.autograd.Function):
     """MemoryTransformer._prepend_shared_chapters (memory_transformer/model.py:356-391)."""
 

@@ -1,0 +1,316 @@
+"""ops.router_select (scores, balance bias, groups, top-k, renormalised weights) against the same selection in
+float64: ids equal, weights and gradients within float32 roundings.
+
+Tolerances, derived: a weight is formed from scores with relative errors of at most 2^-21 (the row's maximum
+subtracted, one exponential, one reciprocal; a softmax sum over C terms adds C 2^-24 in the worst order, 2^-18 for
+64 lanes' sums of 65) and a sum and a quotient of such scores; a gradient from two products and one difference of such
+terms: 2^-16 of the largest term of its row bounds both."""
+
+import pytest
+import torch
+
+from helpers import gen
+
+TOL = 2.0 ** -16
+
+
+# A group's score is a sum of two scores in float64: exp (1 ulp), 1 + e, the quotient, the bias and the sum round
+# it by at most 8 2^-53 of magnitudes below 2.  Two groups whose scores differ by less than this bound are not told
+# apart by float64, and either may stay.  (Sums of scores around one logit come this close: with z = z0 + m 2^-25 two
+# pairs with equal m + m' differ by their second derivative times 2^-50.)
+GROUP_TIE = 2.0 ** -49
+
+
+def reference(z, k, S=0, score="softmax", bias=None, G=1, g=None, best=2, renorm=True, scale=1.0, dw=None, got=None):
+    """(idx, w, dz or None) on the CPU in float64; masked logits (-inf) come after every other.  ``got``: the
+    kernel's ids, which say which of two groups stays where float64 does not tell them apart."""
+    z = z.detach().cpu().double().requires_grad_(dw is not None)
+    R, C = z.shape
+    n, g = C - S, G if g is None else g
+    best = min(best, n // G)
+    body = z[:, S:]
+    s = torch.softmax(body, 1) if score == "softmax" else torch.sigmoid(body)
+    key = s.detach().clone() if bias is not None or (G > g and best == 2) else body.detach().clone()
+    if bias is not None:
+        key = key + bias.cpu().double()[S:]
+    key = torch.where(body.detach() == -torch.inf, -torch.inf, key)
+    key = torch.where(key.isnan(), torch.inf, key)
+    if g < G:
+        top = key.view(R, G, -1).topk(best, dim=2).values
+        if best == 2:
+            top = torch.where(top[:, :, 1:] == -torch.inf, torch.cat([top[:, :, :1], torch.zeros_like(top[:, :, 1:])], 2), top)
+        total = top.sum(2)
+        order = torch.sort(total, dim=1, descending=True, stable=True).indices
+        if got is not None:
+            edge = total.gather(1, order)[:, g - 1:g]
+            near = (total - edge).abs() <= GROUP_TIE
+            used = torch.zeros(R, G, dtype=torch.bool).scatter_(1, (got.cpu().long() - S) // (n // G), True)
+            # certain groups first, then the undecided ones that the kernel kept, then the other undecided ones
+            rank = torch.where(near, torch.where(used, 1.0, 2.0), torch.where(total > edge, 0.0, 3.0))
+            # (groups with the same two keys as the last one kept are truly equal: the lower one stays)
+            same = (top == top.gather(1, order[:, g - 1:g, None].expand(R, 1, best))).all(2)
+            split = (near & ~same).any(1)
+            again = torch.sort(rank, dim=1, stable=True).indices
+            order = torch.where(split[:, None], again, order)
+        live = torch.zeros(R, G, dtype=torch.bool).scatter_(1, order[:, :g], True).repeat_interleave(n // G, 1)
+    else:
+        live = torch.ones(R, n, dtype=torch.bool)
+    # live chapters first, by key descending, ties by position
+    pos = torch.sort(key, dim=1, descending=True, stable=True).indices
+    pos = torch.take_along_dim(pos, torch.sort((~live.gather(1, pos)).int(), dim=1, stable=True).indices, 1)[:, :k]
+    sel = s.gather(1, pos)
+    w = scale * (sel / sel.sum(1, keepdim=True).clamp_min(1e-12) if renorm else sel)
+    dz = torch.autograd.grad(w, z, dw.cpu().double())[0] if dw is not None else None
+    return (pos + S).int(), w.detach(), dz
+
+
+def run(z, k, S, dev, dw=None, bias=None, **kw):
+    from memory_amd import ops
+    zd = z.to(dev).requires_grad_(dw is not None)
+    idx, w = ops.router_select(zd, k, S, bias=None if bias is None else bias.to(dev), **kw)
+    dz = torch.autograd.grad(w, zd, dw.to(dev))[0] if dw is not None else None
+    return idx, w.detach(), dz
+
+
+def compare(z, k, S, dev, seed=0, bias=None, score="softmax", G=1, g=None, best=2, renorm=True, scale=1.0):
+    dw = torch.randn(z.shape[0], k, generator=gen(seed + 77))
+    idx, w, dz = run(z, k, S, dev, dw, bias, score=score, num_groups=G, top_groups=g, group_best=best, renormalize=renorm,
+                     scale=scale)
+    ridx, rw, rdz = reference(z, k, S, score, bias, G, g, best, renorm, scale, dw, idx)
+    assert idx.dtype == torch.int32 and torch.equal(idx.cpu(), ridx)
+    err = ((w.cpu().double() - rw).abs() / rw.abs().amax(1, keepdim=True).clamp_min(1e-30)).max().item()
+    big = rdz.abs().amax(1, keepdim=True) + (rw * dw).abs().amax(1, keepdim=True)
+    gerr = ((dz.cpu().double() - rdz).abs() / big.clamp_min(1e-30)).max().item()
+    print(f"R={z.shape[0]} C={z.shape[1]} k={k} {score} G={G}/{g} weights {err:.2e} gradient {gerr:.2e}", flush=True)
+    assert err <= TOL and gerr <= TOL
+    assert not dz[:, :S].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("G,g,best", [(1, None, 1), (8, 4, 2), (8, 3, 1), (3, 2, 2), (16, 16, 2)])
+def test_forms(gpu_device, score, with_bias, renorm, G, g, best):
+    S, C = 1, 1 + 48 * 7
+    g0 = gen(3)
+    z = torch.randn(70, C, generator=g0)
+    bias = torch.randn(C, generator=g0) * 0.05 if with_bias else None
+    compare(z, 6, S, gpu_device, 1, bias, score, G, g, best, renorm, 2.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,C,S,k,G,g", [(1, 1, 0, 1, 1, 1), (1, 4097, 1, 64, 8, 4), (3, 4097, 1, 64, 1, 1), (65, 4097, 1, 16, 16, 4),
+                                         (200, 4097, 1, 64, 4, 2), (33, 257, 1, 8, 1, 1), (130, 65, 0, 65, 1, 1), (9, 16384, 0, 100, 32, 5),
+                                         (2, 16384, 4, 1024, 1, 1), (70, 129, 1, 1, 128, 1), (66, 4609, 1, 64, 64, 20),
+                                         (67, 5000, 8, 33, 3, 2), (500, 33, 1, 4, 1, 1), (80, 1025, 1, 300, 2, 1), (77, 64, 2, 20, 31, 10),
+                                         (1030, 100, 1, 3, 9, 2), (64, 2049, 1, 128, 1024, 700), (90, 3, 1, 2, 1, 1)])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_sizes(gpu_device, R, C, S, k, G, g, score):
+    g0 = gen(R + C + k)
+    z = torch.randn(R, C, generator=g0) * 0.55
+    bias = torch.randn(C, generator=g0) * 0.02
+    compare(z, k, S, gpu_device, 2, bias, score, G, g, 2, True, 1.0)
+    compare(z, k, S, gpu_device, 3, None, score, G, g, 1, score == "sigmoid", 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [5, 300])
+@pytest.mark.parametrize("score,bias_on", [("sigmoid", True), ("softmax", True), ("sigmoid", False), ("softmax", False)])
+@pytest.mark.parametrize("G,g", [(1, 1), (8, 4)])
+def test_ties_and_near_ties(gpu_device, R, score, bias_on, G, g):
+    """Equal logits go to the lower chapter, also where whole groups are equal; keys one float32 step apart, and keys
+    that float32 cannot tell apart, are ordered as float64 orders them."""
+    C, S, k = 1025, 1, 24
+    g0 = gen(9)
+    bias = torch.randn(C, generator=g0).mul_(0.01) if bias_on else None
+    coarse = (torch.randn(R, C, generator=g0) * 2).round() / 2            # a dozen values
+    if bias_on:
+        bias = (bias * 100).round() / 100
+    compare(coarse, k, S, gpu_device, 1, bias, score, G, g)
+    compare(torch.zeros(R, C), k, S, gpu_device, 1, None if bias is None else bias * 0, score, G, g)
+    close = 0.25 + torch.randint(-40, 40, (R, C), generator=g0) * 2.0 ** -25     # a few float32 steps
+    compare(close, k, S, gpu_device, 1, bias, score, G, g)
+    if bias_on:   # scores + bias that agree to 2^-26 .. 2^-40
+        b = 0.5 - (torch.sigmoid(close[0].double()) if score == "sigmoid" else torch.softmax(close[0, S:].double(), 0).mean())
+        b = b.float().expand(C).contiguous() if b.dim() == 0 else b.float()
+        compare(close, k, S, gpu_device, 1, b, score, G, g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [7, 200])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_masked_logits(gpu_device, R, score):
+    """-inf masks a chapter: rows with fewer live chapters than k, whole groups masked, the lowest finite value."""
+    C, S, k = 513, 1, 16
+    g0 = gen(4)
+    z = torch.randn(R, C, generator=g0)
+    z[torch.rand(R, C, generator=g0) < 0.7] = -torch.inf
+    z[1, 10:] = -torch.inf                       # nine live chapters
+    z[2, S:] = torch.where(torch.arange(C - S) < 256, -torch.inf, z[2, S:])
+    z[3, S:] = torch.randn(C - S, generator=g0)
+    z[3, 200:] = torch.finfo(torch.float32).min
+    z[4, 50:60] = torch.finfo(torch.float32).min
+    bias = torch.randn(C, generator=g0) * 0.3
+    for b in (None, bias):
+        for G, g in ((1, 1), (4, 2)):
+            idx, w, dz = run(z, k, S, gpu_device, torch.ones(R, k), b, score=score, num_groups=G, top_groups=g)
+            ridx, rw, rdz = reference(z, k, S, score, b, G, g, dw=torch.ones(R, k))
+            assert torch.equal(idx.cpu(), ridx)
+            assert (w.cpu().double() - rw).abs().max() <= TOL
+            assert (dz.cpu().double() - rdz).abs().max() <= TOL
+
+
+@pytest.mark.gpu
+def test_nothing_left_and_not_a_number(gpu_device):
+    """A row with every chapter masked names the first k: weight 0 (sigmoid) or NaN (softmax); NaN sorts first; both
+    leave the other rows as they are."""
+    from memory_amd import ops
+    for R in (6, 100):
+        z = torch.randn(R, 300, generator=gen(1)).to(gpu_device)
+        for score in ("sigmoid", "softmax"):
+            i0, w0 = ops.router_select(z, 5, 1, score=score)
+            z1 = z.clone()
+            z1[2] = -torch.inf
+            z1[4, 77] = torch.nan
+            i1, w1 = ops.router_select(z1, 5, 1, score=score)
+            rest = [r for r in range(R) if r not in (2, 4)]
+            assert torch.equal(i0[rest], i1[rest]) and torch.equal(w0[rest], w1[rest])
+            assert i1[2].tolist() == [1, 2, 3, 4, 5]
+            assert not w1[2].any() if score == "sigmoid" else w1[2].isnan().all()
+            assert i1[4, 0] == 77 and w1[4].isnan().all()
+            assert i1[4, 1:].tolist() == [c for c in i0[4].tolist() if c != 77][:4]
+
+
+@pytest.mark.gpu
+def test_layouts_types_and_saturated_scores(gpu_device):
+    from memory_amd import ops
+    z = torch.randn(90, 512, generator=gen(2))
+    wide = z.to(gpu_device)
+    i0, w0 = ops.router_select(wide[:, :257].contiguous(), 8, 1, score="sigmoid")
+    i1, w1 = ops.router_select(wide[:, :257], 8, 1, score="sigmoid")          # rows of a wider matrix
+    assert torch.equal(i0, i1) and torch.equal(w0, w1)
+    i1, w1 = ops.router_select(wide[:, :257].t().contiguous().t(), 8, 1, score="sigmoid")
+    assert torch.equal(i0, i1) and torch.equal(w0, w1)
+    off = torch.empty(90 * 257 + 1, device=gpu_device)[1:].view(90, 257).copy_(wide[:, :257])
+    i1, w1 = ops.router_select(off, 8, 1, score="sigmoid")
+    assert torch.equal(i0, i1) and torch.equal(w0, w1)
+    zb = z[:, :257].bfloat16()
+    compare(zb.float(), 8, 1, gpu_device, bias=torch.randn(257, generator=gen(5)) * 0.1, score="sigmoid")
+    zg = zb.to(gpu_device).requires_grad_(True)
+    idx, w = ops.router_select(zg, 8, 1, score="sigmoid")
+    (dz,) = torch.autograd.grad(w.sum() + (w * w).sum(), zg)
+    assert dz.dtype == torch.bfloat16 and torch.equal(idx.cpu(), reference(zb.float(), 8, 1, "sigmoid")[0])
+    # scores at both ends: 1 - e^-30 and e^-30
+    far = torch.cat([z[:, :128] * 4 + 20, z[:, 128:] * 4 - 20], 1)
+    compare(far, 8, 0, gpu_device, bias=torch.randn(512, generator=gen(6)) * 1e-3, score="sigmoid")
+    compare(far, 8, 0, gpu_device, score="sigmoid", renorm=False)
+    compare(far - 20, 8, 0, gpu_device, score="sigmoid", renorm=True)
+    compare(far, 8, 0, gpu_device, bias=torch.randn(512, generator=gen(6)), score="softmax", renorm=True)
+
+
+@pytest.mark.gpu
+def test_empty_rows_and_repeats(gpu_device):
+    from memory_amd import ops
+    z = torch.zeros(0, 33, device=gpu_device, requires_grad=True)
+    idx, w = ops.router_select(z, 4, 1)
+    assert idx.shape == w.shape == (0, 4)
+    assert torch.autograd.grad(w.sum(), z)[0].shape == (0, 33)
+    z = torch.randn(3000, 513, generator=gen(8))
+    a = run(z, 16, 1, gpu_device, torch.ones(3000, 16), torch.zeros(513), score="sigmoid", num_groups=8, top_groups=3)
+    b = run(z, 16, 1, gpu_device, torch.ones(3000, 16), torch.zeros(513), score="sigmoid", num_groups=8, top_groups=3)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score,R", [("sigmoid", 16), ("softmax", 300)])
+def test_graph_replays(gpu_device, score, R):
+    from memory_amd import ops
+    C = 1025
+    z = torch.randn(R, C, generator=gen(1)).to(gpu_device).requires_grad_(True)
+    bias = torch.randn(C, generator=gen(2)).mul_(0.02).to(gpu_device)
+    dw = torch.randn(R, 16, generator=gen(3)).to(gpu_device)
+
+    def step():
+        idx, w = ops.router_select(z, 16, 1, score=score, bias=bias, num_groups=8, top_groups=4, renormalize=False)
+        return idx, w.detach(), torch.autograd.grad(w, z, dw)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for rep in range(3):
+        with torch.no_grad():
+            z.copy_(torch.randn(R, C, generator=gen(10 + rep)))
+        graph.replay()
+        got = [o.clone() for o in out]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step())), f"replay {rep}"
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences(gpu_device):
+    """Central differences of the weights along random directions that leave the selection as it is."""
+    from memory_amd import ops
+    for score, renorm in (("sigmoid", True), ("sigmoid", False), ("softmax", True), ("softmax", False)):
+        z = torch.randn(4, 65, generator=gen(7))
+        dw = torch.randn(4, 5, generator=gen(8))
+        idx, w, dz = run(z, 5, 1, gpu_device, dw, score=score, renormalize=renorm)
+        v = torch.randn(4, 65, generator=gen(9)) * 2.0 ** -9
+        outs = [reference(z.double() + sgn * v.double(), 5, 1, score, renorm=renorm) for sgn in (1, -1)]
+        assert all(torch.equal(o[0], idx.cpu()) for o in outs)
+        diff = ((outs[0][1] - outs[1][1]) * dw.double()).sum() / 2
+        got = (dz.cpu().double() * v.double()).sum()
+        # third-order term of the difference: |v|^3 times third derivatives below 1, summed over 4 x 65
+        assert abs(diff - got) <= 260 * (8 * 2.0 ** -9) ** 3 + TOL * (dz.cpu().double() * v.double()).abs().sum(), (score, renorm)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,C,S", [(0, 33, 1), (5000, 33, 1), (131072, 4097, 1), (70, 16384, 0)])
+def test_balance(gpu_device, n, C, S):
+    from memory_amd import ops
+    idx = torch.randint(S, C, (n,), generator=gen(n + C)).to(torch.int32)
+    idx[::5] = S
+    bias = torch.randn(C, generator=gen(1))
+    want = torch.bincount(idx.long(), minlength=C)
+    mean = want[S:].double().mean()
+    step = torch.sign(mean - want.double()) * 0.001
+    step[:S] = 0
+    b = bias.to(gpu_device)
+    counts = ops.router_balance_(b, idx.to(gpu_device).view(-1, 1), 0.001, S)
+    assert torch.equal(counts.cpu().long(), want)
+    assert torch.equal(b.cpu(), bias + step.float())
+    stray = torch.tensor([-1, C, S, S], dtype=torch.int32)
+    assert ops.router_balance_(b, stray.to(gpu_device), 0.0, S).sum() == 2
+
+
+def test_refusals():
+    from memory_amd import _lib as L
+    from memory_amd import ops
+    z = torch.zeros(3, 17)
+    for bad in (dict(score="relu"), dict(num_groups=3), dict(num_groups=0), dict(num_groups=4, top_groups=5),
+                dict(num_groups=4, top_groups=0), dict(group_best=3), dict(bias=torch.zeros(16))):
+        with pytest.raises(ValueError):
+            ops.router_select(z, 4, 1, **bad)
+    for k, S in ((0, 1), (17, 1), (4, 17), (4, -1)):
+        with pytest.raises(ValueError):
+            ops.router_select(z, k, S)
+    with pytest.raises(ValueError):
+        ops.router_select(z, 9, 1, num_groups=4, top_groups=2)      # 8 selectable
+    with pytest.raises(ValueError):
+        ops.router_select(z[0], 4, 1)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.router_select(z, 4, 1)
+    with pytest.raises(ValueError, match="float32 vector"):
+        ops.router_balance_(torch.zeros(4, dtype=torch.bfloat16), torch.zeros(2), 0.1)
+    args = lambda **kw: [{**dict(z=16, ld=17, R=3, C=17, S=1, k=4, score=0, b=None, G=1, g=1, best=1, rn=1, sc=1.0, i=16, w=16,
+                                 s=None, st=None, q=None), **kw}[n] for n in ("z", "ld", "R", "C", "S", "k", "score", "b", "G", "g", "best",
+                                                                               "rn", "sc", "i", "w", "s", "st", "q")]
+    for bad in (dict(C=20000, ld=20000), dict(S=17), dict(score=2), dict(G=5), dict(g=2), dict(best=0), dict(k=1025), dict(ld=16),
+                dict(z=None), dict(R=-1)):
+        with pytest.raises(ValueError):
+            L.call("moc_router_select", *args(**bad))
