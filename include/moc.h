@@ -772,6 +772,31 @@ typedef struct {
 int moc_decode_step_group(const moc_decode_layer* layers, int n, int64_t B, int64_t d, int H, int HK, int T, int NS,
                           float scale, int64_t N, size_t workspace_bytes, hipStream_t stream);
 
+/* ------------------------------------------------- decode cache in 8 bits */
+
+/* K / V chapter-head tiles of f32 or bf16 ([tile][64 keys][64 dims], as kv_project's "k" / "v") to e4m3 with one
+ * power-of-two scale per tile: k_tiles [tile][key][dim]; v_tiles [tile][dim][pos], position 16 g + 4 kb + x of a dim
+ * holding key 16 kb + 4 g + x (g, kb, x < 4); k_scale, v_scale f32 [tile].  Values are scale times the e4m3 ones;
+ * infinities become the largest of them, NaN stays. */
+int moc_cache8_pack(int dtype, const void* k, const void* v, int64_t tiles, void* k_tiles, void* v_tiles, float* k_scale,
+                    float* v_scale, hipStream_t stream);
+/* moc_decode_partial and its combine over such tiles (any finite scales >= 0), for L >= 1 query tokens per sequence:
+ * q, out bf16 [B][L][H][64]; k_tiles, v_tiles of C chapters x HK heads; idx i32, omega f32 (>= 0) [B][NS] (ids outside
+ * [0, C): skipped slot) and the chapter plan of idx with its row table (moc_decode_row_table), max_u >= the plan's
+ * n_uniq[0].  A row without slots is 0.  workspace: moc_cache8_attend_workspace bytes, 16-byte aligned.
+ * B NS L H < 2^31. */
+typedef struct {
+  const void *q, *k_tiles, *v_tiles;
+  const float *k_scale, *v_scale, *omega;
+  const int32_t *idx, *uniq, *n_uniq, *csr_off, *csr_edge, *edge_u, *row_tab;
+  void* out;
+  int64_t max_u, B, L, C;
+  int H, HK, NS;
+  float scale;
+} moc_cache8_args;
+size_t moc_cache8_attend_workspace(int64_t B, int64_t L, int H, int HK, int NS);
+int moc_cache8_attend(const moc_cache8_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* ------------------------------------------------- end of a sublayer, next norm */
 
 /* u = norm(x) w1 + b1 (post; u = x without), h = alpha residual + gate u, n = norm(h) w2 + b2 (pre), on rows of d
@@ -789,8 +814,8 @@ typedef struct {
   void *h, *n;
   float* stats; /* f32 [4][rows]: mean and 1 / deviation of x, then of h (NULL: not wanted; the backward's input) */
   int64_t rows, d;
-  int x_dtype, r_dtype, gate_mode, gate_dtype, norm, post, pre;
-  float alpha, eps;
+  int x_dtype, r_dtype, gate_mode, gate_dtype, norm, norm2, post, pre;
+  float alpha, eps, eps2; /* norm, eps of the first norm, norm2, eps2 of the second */
 } moc_gated_norm;
 int moc_gated_norm_fwd(const moc_gated_norm* a, hipStream_t stream);
 /* Gradients: dh (r_dtype) and dn (x_dtype) arrive (either may be NULL: zero); dx, dres and dgate (token, full) are

@@ -158,6 +158,9 @@ _SIGS = {
     "moc_bank_touched": (_I, [_P, _I64, _I, _P, _P, _P]),
     "moc_bank_sqnorm_workspace": (_SZ, [_I64, _I64]),
     "moc_bank_sqnorm": (_I, [_P, _P, _P, _I64, _I64, _P, _SZ, _P, _P]),
+    "moc_cache8_pack": (_I, [_I, _P, _P, _I64, _P, _P, _P, _P, _P]),
+    "moc_cache8_attend_workspace": (_SZ, [_I64, _I64, _I, _I, _I]),
+    "moc_cache8_attend": (_I, [_P, _P, _SZ, _P]),
     "moc_router_select": (_I, [_P, _I64, _I64, _I64, _I, _I, _I, _P, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P]),
     "moc_router_select_bwd": (_I, [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I, _I, _I, _I, _F, _P, _P]),
     "moc_router_balance": (_I, [_P, _I64, _I64, _I, _F, _P, _P, _P]),

@@ -164,8 +164,10 @@ class MemoryStack(nn.Module):
         self.memory_banks = nn.ModuleDict({str(b): _ChapteredBank(self.num_memory_tokens, self.memory_dim,
                                                                   self.num_chapters, init_std)
                                            for b in range(nbanks)})
+        # "router_options" (no reference counterpart): ChapterRouter's selection, of every router
+        options = dict(_cfg(memory, "router_options") or {})
         self.routers = nn.ModuleDict({str(i): ChapterRouter(hidden_dim, self.num_chapters, self.top_k,
-                                                            self.strategy)
+                                                            self.strategy, **options)
                                       for i in self.layer_indices})
         wo0 = bool(_cfg(memory, "wo_init_zero", True))
         self.layers = nn.ModuleDict({str(i): MemorySublayer(hidden_dim, heads, kv_heads, use_rms_norm=use_rms_norm,
@@ -220,7 +222,8 @@ class MemoryStack(nn.Module):
                     unknown.append(k)
             else:
                 unused.append(k)
-        missing = [k for k in own if k not in mem]
+        # (a balance bias starts at 0 where the checkpoint has none)
+        missing = [k for k in own if k not in mem and not k.endswith(".balance_bias")]
         if strict and (missing or unknown):
             raise KeyError(f"reference state dict does not match the memory stack: missing {missing[:8]}, "
                            f"unexpected {unknown[:8]}")

@@ -1,0 +1,522 @@
+// Attention over a decode cache held in 8 bits: K / V tiles of every chapter in e4m3 (OCP), one f32 scale per
+// (chapter, kv head) for K and one for V.
+//
+// For sequence b with slots (chapter c, weight omega) and a query row q of kv head hk:
+//   s_j = omega * ks[c, hk] * scale * (q . k8_j),  o = sum_j softmax_j(s) * omega * vs[c, hk] * v8_j
+// i.e. the decode attention of decode.hip over K = ks k8, V = vs v8; the scales are one factor per 64-key tile and
+// fold into the logit factor and the probabilities, so the products run on the 8-bit values, widened to bf16 (exact).
+//
+// Layout: k_tiles[c][hk][key][dim] and v_tiles[c][hk][dim][pos], position 16 g + 4 kb + x of a dim holding key
+// 16 kb + 4 g + x.  That is the key order of the probabilities in the matrix accumulator (lane group g, values x of
+// key block kb), so that a lane's keys of one dim are 16 consecutive bytes: every operand of both products is one
+// 16-byte load per lane straight into registers, and V needs no transpose.
+#include <algorithm>
+
+#include "moc_common.h"
+
+namespace moc {
+namespace {
+
+constexpr int kC8Dh = 64;
+constexpr int kC8Tile = 64 * 64;   // elements (= bytes) of a tile
+constexpr float kC8Max = 448.f;    // largest e4m3 value
+
+__device__ __forceinline__ float c8_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// eight e4m3 values (two words) as bf16, exact
+__device__ __forceinline__ bf16x8 c8_widen(uint32_t a, uint32_t b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false),
+                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true),
+                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false),
+                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true)};
+  return __builtin_bit_cast(bf16x8, v);
+}
+
+// ------------------------------------------------------------------ quantising
+// One workgroup per tile (blockIdx.y: K or V).  scale = 2^ceil(log2(amax / 448)) of the largest finite magnitude (1
+// for a tile of zeros): x / scale is then exact and every element is rounded once, to nearest even.  Infinities
+// become +-448 scale, NaN stays NaN.
+template <typename T>
+__global__ __launch_bounds__(256) void cache8_pack_kernel(const T* __restrict__ k, const T* __restrict__ v,
+                                                          uint8_t* __restrict__ k8, uint8_t* __restrict__ v8,
+                                                          float* __restrict__ k_scale, float* __restrict__ v_scale) {
+  __shared__ float red[4];
+  __shared__ uint8_t tile[64 * 68];
+  const int64_t t = blockIdx.x;
+  const bool is_v = blockIdx.y == 1;
+  const T* src = (is_v ? v : k) + t * kC8Tile + 16 * threadIdx.x;   // row threadIdx / 4, elements 16 (threadIdx % 4) ..
+  float x[16];
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    x[i] = to_f(src[i]);
+    const float m = fabsf(x[i]);
+    amax = m < INFINITY && m > amax ? m : amax;
+  }
+  amax = wave_max(amax);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = amax;
+  __syncthreads();
+  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  // the exponent e with 448 2^(e-1) < amax <= 448 2^e, within what 2^e and 2^-e can hold
+  int e = 0;
+  if (amax > 0.f) {
+    e = ilogbf(amax) - 8;                       // 2^8 <= 448 < 2^9
+    if (ldexpf(amax, -e) > kC8Max) ++e;
+    e = max(-120, min(120, e));
+  }
+  const float inv = ldexpf(1.f, -e);
+  if (threadIdx.x == 0) (is_v ? v_scale : k_scale)[t] = ldexpf(1.f, e);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      y[j] = x[4 * i + j] * inv;
+      y[j] = y[j] > kC8Max ? kC8Max : y[j] < -kC8Max ? -kC8Max : y[j];   // (NaN passes)
+    }
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], p, true);
+  }
+  if (!is_v) {
+    V16 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.w[i] = w[i];
+    st16(k8 + t * kC8Tile + 16 * threadIdx.x, o);
+    return;
+  }
+  const int key = threadIdx.x >> 2, pos = 16 * ((key >> 2) & 3) + 4 * (key >> 4) + (key & 3);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) tile[(16 * (threadIdx.x & 3) + 4 * i + j) * 68 + pos] = (uint8_t)(w[i] >> (8 * j));
+  __syncthreads();
+  V16 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    o.w[i] = *reinterpret_cast<const uint32_t*>(tile + (threadIdx.x >> 2) * 68 + 16 * (threadIdx.x & 3) + 4 * i);
+  st16(v8 + t * kC8Tile + 16 * threadIdx.x, o);
+}
+
+// ------------------------------------------------------------------ few queries: one wave per (chapter, kv head)
+// Each selected tile is read once however many sequences chose it (the chapter plan over the (sequence, slot) edges),
+// as decode.hip does.  Rows of a unit: edge, query token, head of the kv group; 16 at a time.
+//   S^T = K Q^T (lane = query row), softmax over the 64 keys, O^T = V^T P^T, normalised rows and their log-sum-exp
+// to part rows [edge][token][head][64]; moc_sparse_combine merges the slots.
+// Bound: HBM, or latency where the units are few.  Eight loads of 16 bytes per lane hold the whole tile pair.
+constexpr int kC8Waves = 4;
+
+struct C8Unit {
+  const bf16* q;
+  const uint8_t *k8, *v8;
+  const float *ks, *vs, *omega;
+  const int32_t *uniq, *n_uniq, *csr_off, *csr_edge, *row_tab;
+  bf16* o_part;
+  float* lse_part;
+  int64_t max_u;
+  int L, H, HK, NS;
+  float scale_log2;
+};
+
+__global__ __launch_bounds__(64 * kC8Waves) void cache8_unit_kernel(C8Unit a) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t unit = (int64_t)blockIdx.x * kC8Waves + wave;
+  const int64_t u = unit / a.HK;
+  const int hk = (int)(unit % a.HK);
+  if (u >= a.max_u) return;
+  const int G = a.H / a.HK, GL = G * a.L;
+  // the first 16 rows' edges come with the plan entries, not after them
+  int eid = a.row_tab[u * 16 + min(c16 / GL, 15)];
+  const int nu = a.n_uniq[0];
+  const int64_t c = a.uniq[u];
+  const int p0 = a.csr_off[u], cnt = a.csr_off[u + 1] - p0;
+  if (u >= nu) return;
+  const int nrows = cnt * GL;
+  const int64_t tile = c * a.HK + hk;
+  V16 kw[4], vw[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) kw[i] = ld16(a.k8 + tile * kC8Tile + 64 * (16 * i + c16) + 16 * g);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) vw[i] = ld16(a.v8 + tile * kC8Tile + 64 * (16 * i + c16) + 16 * g);
+  const float ks = a.ks[tile] * a.scale_log2, vs = a.vs[tile];
+  for (int r0 = 0; r0 < nrows; r0 += 16) {
+    const int r = r0 + c16;
+    if (r0 > 0) eid = r < nrows ? a.csr_edge[p0 + r / GL] : -1;
+    else if (r >= nrows) eid = -1;
+    bf16x8 qf[2] = {zero_frag<bf16>(), zero_frag<bf16>()};
+    int64_t row = -1;
+    float w = 1.f;
+    if (eid >= 0) {
+      const int rem = r % GL, l = rem / G, hq = hk * G + rem % G;
+      row = ((int64_t)eid * a.L + l) * a.H + hq;
+      w = a.omega[eid];
+      const bf16* qp = a.q + (((int64_t)(eid / a.NS) * a.L + l) * a.H + hq) * kC8Dh + 16 * g;
+      qf[0] = Load8<bf16, bf16>::run(qp);
+      qf[1] = Load8<bf16, bf16>::run(qp + 8);
+    }
+    // S^T: lane = query row r0 + c16, keys 16 kb + 4 g + x; dims 16 g + 8 ks of both operands
+    f32x4 st[4];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      st[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      mma(st[kb], c8_widen(kw[kb].w[0], kw[kb].w[1]), qf[0]);
+      mma(st[kb], c8_widen(kw[kb].w[2], kw[kb].w[3]), qf[1]);
+    }
+    float mx = st[0][0];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) mx = fmax_fast(mx, st[kb][x]);
+    const float cf = w * ks;
+    const float m = quad_max(mx) * cf;
+    float ps = 0.f;
+    bf16x8 pf[2];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float p = exp2f(st[kb][x] * cf - m);
+        ps += p;
+        pf[kb >> 1][4 * (kb & 1) + x] = (bf16)p;
+      }
+    const float l = quad_sum(ps);
+    // O^T: lane = query row, dims 16 db + 4 g + x
+    f32x4 o[4];
+#pragma unroll
+    for (int db = 0; db < 4; ++db) {
+      o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+      mma(o[db], c8_widen(vw[db].w[0], vw[db].w[1]), pf[0]);
+      mma(o[db], c8_widen(vw[db].w[2], vw[db].w[3]), pf[1]);
+    }
+    if (row >= 0) {
+      const float f = w * vs / l;
+      bf16* op = a.o_part + row * kC8Dh;
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        bf16x4 v;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = (bf16)(o[db][x] * f);
+        *reinterpret_cast<bf16x4*>(op + 16 * db + 4 * g) = v;
+      }
+      if (g == 0) a.lse_part[row] = m + log2f(l);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ many queries: running softmax over the slots
+// One workgroup = 128 query rows (token, head of the kv group) of one (sequence, kv head), 4 waves x 32 rows; the
+// heads of a group share every tile.  A tile pair is 8 KB of e4m3: each thread loads 16 bytes of K and of V one slot
+// ahead, widens them once and puts them into LDS as bf16, double-buffered, for all four waves.  Running maximum
+// (raised lazily) and sum as in the sequence attention (xattn_fwd.hip).
+constexpr int kC8Threads = 256;
+constexpr float kC8Slack = 8.f;
+
+struct C8Prompt {
+  const bf16* q;
+  const uint8_t *k8, *v8;
+  const float *ks, *vs, *omega;
+  const int32_t* idx;
+  bf16* out;
+  float *part, *lse;
+  int64_t C;
+  int B, L, H, HK, NS, nsplit;
+  float scale_log2;
+};
+
+__global__ __launch_bounds__(kC8Threads) void cache8_prompt_kernel(C8Prompt a) {
+  using Tile = SwzTile<bf16, 64>;
+  __shared__ __attribute__((aligned(16))) char sK[2][8192];
+  __shared__ __attribute__((aligned(16))) char sV[2][8192];
+  const int G = a.H / a.HK;
+  const int64_t rows = (int64_t)a.L * G;
+  const int64_t nqb = (rows + 127) / 128;
+  const int64_t t = xcd_tile((int64_t)a.B * a.HK * a.nsplit * nqb);
+  if (t < 0) return;
+  const int64_t bh = t / (a.nsplit * nqb);
+  const int b = (int)(bh / a.HK), hk = (int)(bh % a.HK), sp = (int)((t / nqb) % a.nsplit);
+  const int s_begin = (int)((int64_t)a.NS * sp / a.nsplit), s_end = (int)((int64_t)a.NS * (sp + 1) / a.nsplit);
+  const int64_t q0 = (t % nqb) * 128;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c16 = lane & 15;
+
+  // query rows (token * H + head; -1 past the end) and their fragments
+  int64_t qrow[2];
+  bf16x8 qf[2][2];
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    const int64_t r = q0 + 32 * wave + 16 * qb + c16;
+    qrow[qb] = r < rows ? ((int64_t)b * a.L + r / G) * a.H + hk * G + r % G : -1;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+      qf[qb][ks] = qrow[qb] >= 0 ? Load8<bf16, bf16>::run(a.q + qrow[qb] * kC8Dh + 32 * ks + 8 * g) : zero_frag<bf16>();
+  }
+  float m[2] = {-INFINITY, -INFINITY}, lsum[2] = {0.f, 0.f};
+  bf16x8 ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones[j] = (bf16)1.f;
+  f32x4 o[4][2];
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) o[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int32_t* ids = a.idx + (int64_t)b * a.NS;
+  const float* om = a.omega + (int64_t)b * a.NS;
+  auto slot_tile = [&](int s) -> int64_t {
+    const int64_t c = ids[s];
+    return c >= 0 && c < a.C ? c * a.HK + hk : -1;
+  };
+  V16 kr, vr;
+  auto fetch = [&](int64_t tile) {
+    kr = ld16(a.k8 + tile * kC8Tile + 16 * tid);
+    vr = ld16(a.v8 + tile * kC8Tile + 16 * tid);
+  };
+  auto stage = [&](int buf) {
+    const int row = tid >> 2, col = 16 * (tid & 3);
+    *reinterpret_cast<bf16x8*>(sK[buf] + Tile::off(row, col)) = c8_widen(kr.w[0], kr.w[1]);
+    *reinterpret_cast<bf16x8*>(sK[buf] + Tile::off(row, col + 8)) = c8_widen(kr.w[2], kr.w[3]);
+    *reinterpret_cast<bf16x8*>(sV[buf] + Tile::off(row, col)) = c8_widen(vr.w[0], vr.w[1]);
+    *reinterpret_cast<bf16x8*>(sV[buf] + Tile::off(row, col + 8)) = c8_widen(vr.w[2], vr.w[3]);
+  };
+  int64_t cur = slot_tile(s_begin);
+  if (cur >= 0) {
+    fetch(cur);
+    stage(0);
+  }
+  __syncthreads();
+  for (int s = s_begin; s < s_end; ++s) {
+    const int buf = (s - s_begin) & 1;
+    const int64_t next = s + 1 < s_end ? slot_tile(s + 1) : -1;
+    if (next >= 0) fetch(next);
+    if (cur >= 0) {
+      const float c = om[s] * a.ks[cur] * a.scale_log2, f = om[s] * a.vs[cur];
+      f32x4 st[4][2];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) st[kb][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+          const bf16x8 ka = Tile::frag(sK[buf], 16 * kb + c16, 32 * ks + 8 * g);
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb) mma(st[kb][qb], ka, qf[qb][ks]);
+        }
+      float cm[2];
+      bool grow = false;
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        float mx = st[0][qb][0];
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) mx = fmax_fast(mx, st[kb][qb][x]);
+        cm[qb] = quad_max_pl(mx) * c;   // (c >= 0)
+        grow |= cm[qb] > m[qb] + kC8Slack;
+      }
+      if (__any(grow)) {
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+          const float mn = cm[qb] > m[qb] + kC8Slack ? cm[qb] : m[qb];
+          const float alpha = c8_exp2(m[qb] - mn);
+          m[qb] = mn;
+          lsum[qb] *= alpha;
+#pragma unroll
+          for (int db = 0; db < 4; ++db) o[db][qb] *= alpha;
+        }
+      }
+      bf16x8 pf[2][2];
+      // the value factor f = omega vs goes into the exponent where its logarithm and reciprocal are ordinary
+      // numbers; elsewhere (f = 0, or scales past 2^+-90) it multiplies the probabilities
+      const bool fold = f > 0x1p-90f && f < 0x1p90f;
+      const float lf = fold ? __builtin_amdgcn_logf(f) : 0.f, rf = fold ? __builtin_amdgcn_rcpf(f) : 1.f;
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        const float off = m[qb] - lf;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            pf[qb][h][x] = (bf16)c8_exp2(st[2 * h][qb][x] * c - off);
+            pf[qb][h][4 + x] = (bf16)c8_exp2(st[2 * h + 1][qb][x] * c - off);
+          }
+        // row sums of the rounded probabilities, in units of f
+        f32x4 ls = f32x4{0.f, 0.f, 0.f, 0.f};
+        mma(ls, ones, pf[qb][0]);
+        mma(ls, ones, pf[qb][1]);
+        lsum[qb] += ls[0] * rf;
+        if (!fold) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < 8; ++x) pf[qb][h][x] = (bf16)((float)pf[qb][h][x] * f);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int db = 0; db < 4; ++db) {
+          const bf16x8 va = Tile::frag(sV[buf], 16 * db + c16, 16 * g + 8 * h);
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb) mma(o[db][qb], va, pf[qb][h]);
+        }
+    }
+    if (next >= 0) stage(buf ^ 1);
+    cur = next;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    if (qrow[qb] < 0) continue;
+    const float inv = lsum[qb] > 0.f ? 1.f / lsum[qb] : lsum[qb];   // (no slot: 0; NaN passes)
+    if (a.nsplit > 1) {
+      const int64_t at = (int64_t)sp * a.B * a.L * a.H + qrow[qb];
+#pragma unroll
+      for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(a.part + at * kC8Dh + 16 * db + 4 * g) = o[db][qb] * inv;
+      if (g == 0) a.lse[at] = lsum[qb] > 0.f ? m[qb] + log2f(lsum[qb]) : lsum[qb] == 0.f ? -INFINITY : lsum[qb];
+    } else {
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        bf16x4 v;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = (bf16)(o[db][qb][x] * inv);
+        *reinterpret_cast<bf16x4*>(a.out + qrow[qb] * kC8Dh + 16 * db + 4 * g) = v;
+      }
+    }
+  }
+}
+
+// out = sum_i 2^(lse_i - M) o_i / sum_i 2^(lse_i - M) over the splits of a row: 16 lanes of 4 dims per row.
+__global__ __launch_bounds__(256) void cache8_merge_kernel(const float* __restrict__ part, const float* __restrict__ lse,
+                                                           int nsplit, int64_t rows, bf16* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i >> 4;
+  if (row >= rows) return;
+  const int ch = (int)(i & 15);
+  float M = -INFINITY;
+  for (int s = 0; s < nsplit; ++s) M = fmax_fast(M, lse[s * rows + row]);
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  float den = 0.f;
+  if (!(M == -INFINITY)) {
+    for (int s = 0; s < nsplit; ++s) {
+      const float w = c8_exp2(lse[s * rows + row] - M);
+      den += w;
+      acc += w * *reinterpret_cast<const f32x4*>(part + (s * rows + row) * kC8Dh + 4 * ch);
+    }
+    acc *= 1.f / den;
+  }
+  bf16x4 v;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) v[x] = (bf16)acc[x];
+  *reinterpret_cast<bf16x4*>(out + row * kC8Dh + 4 * ch) = v;
+}
+
+// One plan unit per tile against one pass over a row block's slots: rows of one slot's tile up to which the unit
+// form is taken.
+constexpr int kC8UnitRows = 16;
+bool c8_units(int L, int H, int HK) { return L == 1 || (int64_t)L * (H / HK) <= kC8UnitRows; }
+
+// slots of a row block split over workgroups until about two workgroups per CU are busy
+int c8_splits(int64_t B, int64_t L, int H, int HK, int NS) {
+  const int64_t tiles = B * HK * ((L * (H / HK) + 127) / 128);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(NS, 512 / std::max<int64_t>(tiles, 1)));
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+struct C8Ws {
+  size_t o_part = 0, lse_part, lse, bytes;
+  C8Ws(int64_t B, int64_t L, int H, int HK, int NS) {
+    const size_t rows = (size_t)B * L * H;
+    if (c8_units((int)L, H, HK)) {
+      lse_part = up256(rows * NS * kC8Dh * 2);
+      lse = lse_part + up256(rows * NS * 4);
+      bytes = lse + up256(rows * 4);
+    } else {
+      const int ns = c8_splits(B, L, H, HK, NS);
+      lse_part = lse = ns > 1 ? up256(rows * ns * kC8Dh * 4) : 0;
+      bytes = ns > 1 ? lse_part + up256(rows * ns * 4) : 0;
+    }
+  }
+};
+
+bool c8_shape_ok(int64_t B, int64_t L, int H, int HK, int NS) {
+  return B >= 0 && L > 0 && L < (1 << 24) && H > 0 && HK > 0 && H % HK == 0 && NS > 0 &&
+         (B == 0 || (L * H < ((int64_t)1 << 31) / 64 && B * NS * L * H < ((int64_t)1 << 31)));
+}
+
+}  // namespace
+}  // namespace moc
+
+using namespace moc;
+
+extern "C" {
+
+int moc_cache8_pack(int dtype, const void* k, const void* v, int64_t tiles, void* k_tiles, void* v_tiles, float* k_scale,
+                    float* v_scale, hipStream_t stream) {
+  MOC_REQUIRE(tiles >= 0 && tiles < ((int64_t)1 << 31), MOC_ERR_ARG, "moc_cache8_pack: %lld tiles", (long long)tiles);
+  if (tiles == 0) return MOC_OK;
+  MOC_REQUIRE(k && v && k_tiles && v_tiles && k_scale && v_scale, MOC_ERR_ARG, "moc_cache8_pack: null pointer");
+  MOC_REQUIRE((((uintptr_t)k_tiles | (uintptr_t)v_tiles) & 15) == 0, MOC_ERR_ARG, "moc_cache8_pack: unaligned tiles");
+  const dim3 grid((unsigned)tiles, 2);
+  if (dtype == MOC_BF16)
+    hipLaunchKernelGGL(cache8_pack_kernel<bf16>, grid, dim3(256), 0, stream, (const bf16*)k, (const bf16*)v, (uint8_t*)k_tiles,
+                       (uint8_t*)v_tiles, k_scale, v_scale);
+  else if (dtype == MOC_F32)
+    hipLaunchKernelGGL(cache8_pack_kernel<float>, grid, dim3(256), 0, stream, (const float*)k, (const float*)v,
+                       (uint8_t*)k_tiles, (uint8_t*)v_tiles, k_scale, v_scale);
+  else
+    return set_error(MOC_ERR_UNSUPPORTED, "moc_cache8_pack: dtype %d", dtype);
+  return check_launch("cache8_pack_kernel");
+}
+
+size_t moc_cache8_attend_workspace(int64_t B, int64_t L, int H, int HK, int NS) {
+  return c8_shape_ok(B, L, H, HK, NS) && B > 0 ? C8Ws(B, L, H, HK, NS).bytes : 0;
+}
+
+int moc_cache8_attend(const moc_cache8_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  MOC_REQUIRE(a, MOC_ERR_ARG, "moc_cache8_attend: null pointer");
+  MOC_REQUIRE(c8_shape_ok(a->B, a->L, a->H, a->HK, a->NS) && a->C > 0 && a->max_u >= 0 &&
+                  a->max_u * a->HK < ((int64_t)1 << 32),
+              MOC_ERR_ARG, "moc_cache8_attend: B=%lld L=%lld H=%d HK=%d NS=%d C=%lld", (long long)a->B, (long long)a->L, a->H,
+              a->HK, a->NS, (long long)a->C);
+  if (a->B == 0) return MOC_OK;
+  MOC_REQUIRE(a->q && a->k_tiles && a->v_tiles && a->k_scale && a->v_scale && a->idx && a->omega && a->uniq && a->n_uniq &&
+                  a->csr_off && a->csr_edge && a->edge_u && a->row_tab && a->out,
+              MOC_ERR_ARG, "moc_cache8_attend: null pointer");
+  MOC_REQUIRE((((uintptr_t)a->q | (uintptr_t)a->k_tiles | (uintptr_t)a->v_tiles | (uintptr_t)a->out) & 15) == 0, MOC_ERR_ARG,
+              "moc_cache8_attend: 16-byte aligned q / tiles / out");
+  const C8Ws y(a->B, a->L, a->H, a->HK, a->NS);
+  MOC_REQUIRE(y.bytes == 0 || (workspace && workspace_bytes >= y.bytes && ((uintptr_t)workspace & 15) == 0), MOC_ERR_ARG,
+              "moc_cache8_attend: workspace %zu < %zu bytes, or unaligned", workspace_bytes, y.bytes);
+  char* ws = (char*)workspace;
+  const float sl2 = a->scale * 1.4426950408889634f;
+  if (c8_units((int)a->L, a->H, a->HK)) {
+    const int64_t units = a->max_u * a->HK;
+    if (units > 0) {
+      C8Unit k{(const bf16*)a->q, (const uint8_t*)a->k_tiles, (const uint8_t*)a->v_tiles, a->k_scale, a->v_scale, a->omega,
+               a->uniq, a->n_uniq, a->csr_off, a->csr_edge, a->row_tab, (bf16*)(ws + y.o_part), (float*)(ws + y.lse_part),
+               a->max_u, (int)a->L, a->H, a->HK, a->NS, sl2};
+      hipLaunchKernelGGL(cache8_unit_kernel, dim3((unsigned)((units + kC8Waves - 1) / kC8Waves)), dim3(64 * kC8Waves), 0,
+                         stream, k);
+      if (int rc = check_launch("cache8_unit_kernel")) return rc;
+    }
+    const int rpe = (int)(a->L * a->H);
+    return moc_sparse_combine(MOC_BF16, ws + y.o_part, (const float*)(ws + y.lse_part), a->edge_u, nullptr, 1, a->NS, rpe, a->B,
+                              rpe, 0, a->out, (float*)(ws + y.lse), stream);
+  }
+  const int nsplit = c8_splits(a->B, a->L, a->H, a->HK, a->NS);
+  const int64_t nqb = (a->L * (a->H / a->HK) + 127) / 128, tiles = a->B * a->HK * nsplit * nqb;
+  C8Prompt p{(const bf16*)a->q, (const uint8_t*)a->k_tiles, (const uint8_t*)a->v_tiles, a->k_scale, a->v_scale, a->omega, a->idx,
+             (bf16*)a->out, (float*)ws, (float*)(ws + y.lse_part), a->C, (int)a->B, (int)a->L, a->H, a->HK, a->NS, nsplit, sl2};
+  hipLaunchKernelGGL(cache8_prompt_kernel, dim3(xcd_grid(tiles)), dim3(kC8Threads), 0, stream, p);
+  if (int rc = check_launch("cache8_prompt_kernel")) return rc;
+  if (nsplit == 1) return MOC_OK;
+  const int64_t rows = a->B * a->L * a->H;
+  hipLaunchKernelGGL(cache8_merge_kernel, dim3((unsigned)((rows * 16 + 255) / 256)), dim3(256), 0, stream, (const float*)p.part,
+                     (const float*)p.lse, nsplit, rows, (bf16*)a->out);
+  return check_launch("cache8_merge_kernel");
+}
+
+}  // extern "C"

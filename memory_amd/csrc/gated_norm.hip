@@ -98,16 +98,15 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_fwd_kernel(m
     }
   }
   const float inv_d = 1.f / (float)d;
-  const bool layer = a.norm == MOC_NORM_LAYERNORM;
   float h[KCH][VEC];
 #pragma unroll
   for (int i = 0; i < KCH; ++i)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) h[i][e] = t + 64 * W * i < nch ? gn_get<TX, VEC>(xv[i], e) : 0.f;
   float mu = 0.f, rs = 1.f;
-  auto stats = [&]() {
+  auto stats = [&](int norm, float eps) {
     mu = 0.f;
-    if (layer) {
+    if (norm == MOC_NORM_LAYERNORM) {
       float s[1] = {0.f};
 #pragma unroll
       for (int i = 0; i < KCH; ++i)
@@ -127,10 +126,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_fwd_kernel(m
         }
       }
     gn_row_sum<W, 1>(q, red, wave, lane);
-    rs = 1.f / sqrtf(q[0] * inv_d + a.eps);
+    rs = 1.f / sqrtf(q[0] * inv_d + eps);
   };
   if (a.post) {
-    stats();
+    stats(a.norm, a.eps);
     if (a.stats && t == 0) {
       a.stats[r] = mu;
       a.stats[a.rows + r] = rs;
@@ -159,7 +158,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_fwd_kernel(m
     gn_store<TR, VEC>((TR*)a.h + r * d + VEC * c, o);
   }
   if (!a.pre) return;
-  stats();
+  stats(a.norm2, a.eps2);
   if (a.stats && t == 0) {
     a.stats[2 * a.rows + r] = mu;
     a.stats[3 * a.rows + r] = rs;
@@ -194,7 +193,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(m
   const int t = W == 1 ? lane : (int)threadIdx.x;
   const int d = (int)a.d, nch = d / VEC;
   const float inv_d = 1.f / (float)d;
-  const bool layer = a.norm == MOC_NORM_LAYERNORM;
+  const bool layer = a.norm == MOC_NORM_LAYERNORM, layer2 = a.norm2 == MOC_NORM_LAYERNORM;
   float acc[kQ][KCH][VEC];
 #pragma unroll
   for (int q = 0; q < kQ; ++q)
@@ -257,7 +256,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(m
       }
     }
     if (o.dn) gn_row_sum<W, 3>(s, red, wave, lane);
-    const float c0 = layer ? s[0] * inv_d : 0.f, c1 = s[1] * inv_d;
+    const float c0 = layer2 ? s[0] * inv_d : 0.f, c1 = s[1] * inv_d;
     float p[3] = {0.f, 0.f, 0.f};
     // g2 becomes dH, hh becomes g1 = du w1
 #pragma unroll
@@ -388,7 +387,9 @@ int gn_check(const char* who, const moc_gated_norm* a) {
   MOC_REQUIRE(a->rows >= 0 && a->d > 0 && a->d <= kGnMaxD, MOC_ERR_UNSUPPORTED, "%s: rows=%lld d=%lld (d up to %d)", who,
               (long long)a->rows, (long long)a->d, kGnMaxD);
   MOC_REQUIRE(a->rows < ((int64_t)1 << 31), MOC_ERR_UNSUPPORTED, "%s: rows=%lld", who, (long long)a->rows);
-  MOC_REQUIRE(a->norm == MOC_NORM_RMS || a->norm == MOC_NORM_LAYERNORM, MOC_ERR_ARG, "%s: norm %d", who, a->norm);
+  MOC_REQUIRE((a->norm == MOC_NORM_RMS || a->norm == MOC_NORM_LAYERNORM) &&
+                  (a->norm2 == MOC_NORM_RMS || a->norm2 == MOC_NORM_LAYERNORM),
+              MOC_ERR_ARG, "%s: norm %d, %d", who, a->norm, a->norm2);
   MOC_REQUIRE(dtype_size(a->x_dtype) && dtype_size(a->r_dtype), MOC_ERR_UNSUPPORTED, "%s: dtypes x %d residual %d", who,
               a->x_dtype, a->r_dtype);
   MOC_REQUIRE(a->gate_mode >= MOC_GATE_NONE && a->gate_mode <= MOC_GATE_FULL && (a->gate_mode == MOC_GATE_NONE || a->gate || a->rows == 0),
@@ -396,7 +397,7 @@ int gn_check(const char* who, const moc_gated_norm* a) {
   MOC_REQUIRE(a->gate_mode == MOC_GATE_NONE || (a->gate_mode == MOC_GATE_CHANNEL ? a->gate_dtype == MOC_F32
               : a->gate_mode == MOC_GATE_FULL ? a->gate_dtype == a->x_dtype : dtype_size(a->gate_dtype) != 0),
               MOC_ERR_UNSUPPORTED, "%s: gate dtype %d of gate mode %d", who, a->gate_dtype, a->gate_mode);
-  MOC_REQUIRE(a->eps >= 0.f, MOC_ERR_ARG, "%s: eps < 0", who);
+  MOC_REQUIRE(a->eps >= 0.f && a->eps2 >= 0.f, MOC_ERR_ARG, "%s: eps < 0", who);
   return MOC_OK;
 }
 

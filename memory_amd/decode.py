@@ -22,8 +22,33 @@ from . import ops
 from ._lib import call, ptr, stream_ptr
 
 
+FP8 = torch.float8_e4m3fn
+# position -> key of a V tile's dim in 8 bits (its own inverse): the key order of the attention's probabilities
+_V8_KEYS = [16 * kb + 4 * g + x for g in range(4) for kb in range(4) for x in range(4)]
+
+
+def _v8_permuted(v: torch.Tensor) -> torch.Tensor:
+    """[..., keys, dims] -> [..., dims, positions], or back."""
+    keys = torch.tensor(_V8_KEYS, device=v.device)
+    return v.view(torch.uint8).transpose(-1, -2)[..., keys].contiguous().view(FP8)
+
+
+def _v8_natural(v: torch.Tensor) -> torch.Tensor:
+    keys = torch.tensor(_V8_KEYS, device=v.device)
+    return v.view(torch.uint8)[..., keys].transpose(-1, -2).contiguous().view(FP8)
+
+
 class MemoryDecodeCache:
-    """Per-layer K and V tiles [C][HK][64 keys][64 dims] of the whole bank (optionally row-normalised)."""
+    """Per-layer K and V tiles [C][HK][64 keys][64 dims] of the whole bank (optionally row-normalised).
+
+    ``dtype=torch.float8_e4m3fn`` (or ``quantized()`` of a float32 / bfloat16 cache) holds them in 8 bits: half the
+    memory and half the bytes of a step.  Each (chapter, kv head) has a float32 scale for K and one for V
+    (``k_scale``, ``v_scale`` [C][HK], powers of two), a value is scale times its e4m3 value, and ``v_tiles`` is then
+    held as [C][HK][64 dims][64 positions] in the order the kernels read (``dequantized()`` gives both back as
+    [keys][dims])."""
+
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
 
     def __init__(self, bank: torch.Tensor, wk: torch.Tensor, wv: torch.Tensor, *, num_chapters: int,
                  tokens_per_chapter: int, num_kv_heads: int, norm_type: Optional[str] = None, eps: float = 1e-6,
@@ -31,6 +56,11 @@ class MemoryDecodeCache:
         L.require_gpu(bank, wk, wv)
         C, T = int(num_chapters), int(tokens_per_chapter)
         self.num_chapters, self.T, self.HK, self.dtype = C, T, int(num_kv_heads), dtype
+        if dtype == FP8:
+            full = MemoryDecodeCache(bank, wk, wv, num_chapters=C, tokens_per_chapter=T, num_kv_heads=num_kv_heads,
+                                     norm_type=norm_type, eps=eps)
+            self._pack(full)
+            return
         with torch.no_grad():
             plan = ops.identity_plan(C, bank.device)
             code = ops.norm_code(norm_type)
@@ -41,52 +71,116 @@ class MemoryDecodeCache:
             self.k_tiles, self.v_tiles = ops.kv_project(bank.contiguous(), plan, T, wkv, self.HK, 64, mean, rstd,
                                                         dtype, ("k", "v"))
 
+    def _pack(self, full: "MemoryDecodeCache") -> None:
+        if full.T != 64:
+            raise ValueError(f"an 8-bit decode cache needs 64 tokens per chapter, got {full.T}")
+        shape, dev = full.k_tiles.shape, full.k_tiles.device
+        self.k_tiles = torch.empty(shape, device=dev, dtype=FP8)
+        self.v_tiles = torch.empty(shape, device=dev, dtype=FP8)
+        self.k_scale = torch.empty(shape[:2], device=dev, dtype=torch.float32)
+        self.v_scale = torch.empty(shape[:2], device=dev, dtype=torch.float32)
+        with L.on_device(dev):
+            call("moc_cache8_pack", L.dtype_code(full.dtype), ptr(full.k_tiles), ptr(full.v_tiles), shape[0] * shape[1],
+                 ptr(self.k_tiles), ptr(self.v_tiles), ptr(self.k_scale), ptr(self.v_scale), stream_ptr(dev))
+
+    def quantized(self) -> "MemoryDecodeCache":
+        """This cache in 8 bits: per (chapter, kv head) the scale is the smallest power of two that brings the tile's
+        largest finite magnitude to 448 or below; infinities become +-448 times it."""
+        if self.dtype == FP8:
+            return self
+        out = MemoryDecodeCache.__new__(MemoryDecodeCache)
+        out.num_chapters, out.T, out.HK, out.dtype = self.num_chapters, self.T, self.HK, FP8
+        out._pack(self)
+        return out
+
+    def dequantized(self):
+        """(K, V) float32 [C][HK][64 keys][64 dims] that the cache stands for."""
+        if self.dtype != FP8:
+            return self.k_tiles.float(), self.v_tiles.float()
+        return (self.k_tiles.float() * self.k_scale[:, :, None, None],
+                _v8_natural(self.v_tiles).float() * self.v_scale[:, :, None, None])
+
     @property
     def nbytes(self) -> int:
-        return self.k_tiles.numel() * self.k_tiles.element_size() * 2
+        scales = 0 if self.k_scale is None else 8 * self.k_scale.numel()
+        return self.k_tiles.numel() * self.k_tiles.element_size() * 2 + scales
 
     # File format of a saved cache (safetensors): tensors ``k_tiles`` and ``v_tiles``, each
     # [num_chapters][num_kv_heads][tokens_per_chapter keys][64 dims] in the cache dtype (the
     # projected, optionally row-normalised bank, K = norm(M) Wk^T and V = norm(M) Wv^T per
     # chapter), and string metadata: format, num_chapters, tokens_per_chapter, num_kv_heads,
-    # dtype.  The K/V of one memory layer; omega is applied at attention time.
+    # dtype.  The K/V of one memory layer; omega is applied at attention time.  An 8-bit cache is
+    # written under a format of its own, with its scales ``k_scale`` and ``v_scale`` [num_chapters][num_kv_heads]
+    # (float32) and both tiles as [keys][dims].
     FORMAT = "moc-decode-kv/1"
+    FORMAT_8BIT = "moc-decode-kv-e4m3/1"
 
     def save(self, path: str) -> None:
         from safetensors.torch import save_file
-        meta = {"format": self.FORMAT, "num_chapters": str(self.num_chapters), "tokens_per_chapter": str(self.T),
+        eight = self.dtype == FP8
+        meta = {"format": self.FORMAT_8BIT if eight else self.FORMAT, "num_chapters": str(self.num_chapters), "tokens_per_chapter": str(self.T),
                 "num_kv_heads": str(self.HK), "dtype": str(self.dtype).replace("torch.", "")}
-        save_file({"k_tiles": self.k_tiles.contiguous().cpu(), "v_tiles": self.v_tiles.contiguous().cpu()}, path,
-                  metadata=meta)
+        tensors = {"k_tiles": self.k_tiles.contiguous().cpu(),
+                   "v_tiles": (_v8_natural(self.v_tiles) if eight else self.v_tiles.contiguous()).cpu()}
+        if eight:
+            tensors.update(k_scale=self.k_scale.cpu(), v_scale=self.v_scale.cpu())
+        save_file(tensors, path, metadata=meta)
 
     @classmethod
     def load(cls, path: str, device: torch.device) -> "MemoryDecodeCache":
         from safetensors import safe_open
         with safe_open(path, framework="pt", device="cpu") as f:
             meta = f.metadata() or {}
-            if meta.get("format") != cls.FORMAT:
-                raise ValueError(f"{path}: not a {cls.FORMAT} decode cache (format {meta.get('format')!r})")
+            if meta.get("format") not in (cls.FORMAT, cls.FORMAT_8BIT):
+                raise ValueError(f"{path}: not a {cls.FORMAT} or {cls.FORMAT_8BIT} decode cache (format "
+                                 f"{meta.get('format')!r})")
             k, v = f.get_tensor("k_tiles"), f.get_tensor("v_tiles")
+            scales = {}
+            if meta["format"] == cls.FORMAT_8BIT:
+                scales = {n: f.get_tensor(n).to(device) for n in ("k_scale", "v_scale")}
         C, T, HK = int(meta["num_chapters"]), int(meta["tokens_per_chapter"]), int(meta["num_kv_heads"])
         if tuple(k.shape) != (C, HK, T, 64) or k.shape != v.shape:
             raise ValueError(f"{path}: tile shape {tuple(k.shape)} does not match the metadata")
-        return cls.from_tiles(k.to(device), v.to(device), num_chapters=C, tokens_per_chapter=T, num_kv_heads=HK)
+        return cls.from_tiles(k.to(device), v.to(device), num_chapters=C, tokens_per_chapter=T, num_kv_heads=HK, **scales)
 
     @classmethod
     def from_tiles(cls, k_tiles: torch.Tensor, v_tiles: torch.Tensor, *, num_chapters: int, tokens_per_chapter: int,
-                   num_kv_heads: int) -> "MemoryDecodeCache":
-        """A cache over already projected tiles [num_chapters][num_kv_heads][T][64]."""
-        L.require_gpu(k_tiles, v_tiles)
-        if k_tiles.dtype not in (torch.float32, torch.bfloat16) or v_tiles.dtype != k_tiles.dtype:
-            raise ValueError("decode cache tiles must be float32 or bfloat16, both of one dtype")
+                   num_kv_heads: int, k_scale: Optional[torch.Tensor] = None,
+                   v_scale: Optional[torch.Tensor] = None) -> "MemoryDecodeCache":
+        """A cache over already projected tiles [num_chapters][num_kv_heads][T][64] (keys, dims).  Tiles in
+        float8_e4m3fn come with their scales [num_chapters][num_kv_heads], finite and not negative (checked here, which
+        waits for the stream)."""
+        L.require_gpu(k_tiles, v_tiles, k_scale, v_scale)
+        L.require_one_device(k_tiles, v_tiles, k_scale, v_scale)
+        eight = k_tiles.dtype == FP8
+        if k_tiles.dtype not in (torch.float32, torch.bfloat16, FP8) or v_tiles.dtype != k_tiles.dtype:
+            raise ValueError("decode cache tiles must be float32, bfloat16 or float8_e4m3fn, both of one dtype")
+        if eight != (k_scale is not None) or eight != (v_scale is not None):
+            raise ValueError("float8_e4m3fn tiles need k_scale and v_scale, others take none")
         if k_tiles.shape != (num_chapters, num_kv_heads, tokens_per_chapter, 64) or v_tiles.shape != k_tiles.shape:
             raise ValueError(f"tiles of shape {tuple(k_tiles.shape)}, expected "
                              f"{(num_chapters, num_kv_heads, tokens_per_chapter, 64)}")
         self = cls.__new__(cls)
         self.num_chapters, self.T, self.HK, self.dtype = int(num_chapters), int(tokens_per_chapter), \
             int(num_kv_heads), k_tiles.dtype
-        self.k_tiles, self.v_tiles = k_tiles.contiguous(), v_tiles.contiguous()
+        if not eight:
+            self.k_tiles, self.v_tiles = k_tiles.contiguous(), v_tiles.contiguous()
+            return self
+        if self.T != 64:
+            raise ValueError(f"an 8-bit decode cache needs 64 tokens per chapter, got {self.T}")
+        self.k_tiles, self.v_tiles = _aligned(k_tiles), _v8_permuted(v_tiles)
+        for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+            s = s.float().contiguous()
+            if s.shape != (self.num_chapters, self.HK) or not bool((s.isfinite() & (s >= 0)).all()):
+                raise ValueError(f"{name}: finite scales >= 0 of shape {(self.num_chapters, self.HK)}, got "
+                                 f"{tuple(s.shape)}")
+            setattr(self, name, s)
         return self
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 class DecodeRouting:
@@ -217,7 +311,8 @@ class DecodeRouter:
         r = self.router.router
         C, S = self.num_chapters, self.num_shared
         k = min(int(self.router.top_k), C - S)
-        if (S > 0 and k > 0 and pooled.shape[0] > 0 and pooled.dtype == torch.float32 and pooled.is_contiguous()
+        plain = getattr(self.router, "plain_selection", True)
+        if (plain and S > 0 and k > 0 and pooled.shape[0] > 0 and pooled.dtype == torch.float32 and pooled.is_contiguous()
                 and r.weight.dtype in (torch.float32, torch.bfloat16) and r.weight.shape == (C, pooled.shape[1])
                 and r.weight.is_cuda and (r.bias is None or r.bias.is_cuda) and L.KERNEL_EVENTS is None):
             routing, self.last_logits = DecodeRouting._decided(pooled, r, C, S, k, self.routed_scale)
@@ -225,7 +320,7 @@ class DecodeRouter:
         logits = ops.router_linear(pooled, r.weight, r.bias)
         self.last_logits = logits
         if k > 0:
-            idx, w = ops.router_topk(logits, k, S)
+            idx, w = ops.router_topk(logits, k, S) if plain else self.router.select(logits, k, S)
         else:
             idx = torch.empty((pooled.shape[0], 0), dtype=torch.int32, device=pooled.device)
             w = torch.empty((pooled.shape[0], 0), dtype=torch.float32, device=pooled.device)
@@ -285,9 +380,64 @@ class DecodeRouter:
         return self._decide(self._own_states(hidden_states))
 
 
+class _Cache8Args(ctypes.Structure):
+    """moc_cache8_args."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k_tiles", "v_tiles", "k_scale", "v_scale", "omega", "idx", "uniq",
+                                                "n_uniq", "csr_off", "csr_edge", "edge_u", "row_tab", "out")]
+                + [(n, ctypes.c_int64) for n in ("max_u", "B", "L", "C")]
+                + [(n, ctypes.c_int) for n in ("H", "HK", "NS")] + [("scale", ctypes.c_float)])
+
+
+def _attend8(q: torch.Tensor, B: int, Lq: int, H: int, cache: MemoryDecodeCache, routing: DecodeRouting) -> torch.Tensor:
+    """q (B, [L,] H, 64) over an 8-bit cache (moc_cache8_attend)."""
+    q = _aligned(q.to(torch.bfloat16))
+    pl, dev = routing.plan, q.device
+    out = torch.empty_like(q)
+    nbytes = L.query("moc_cache8_attend_workspace", B, Lq, H, cache.HK, routing.NS)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    args = _Cache8Args(ptr(q), ptr(cache.k_tiles), ptr(cache.v_tiles), ptr(cache.k_scale), ptr(cache.v_scale),
+                       ptr(routing.omega), ptr(routing.idx), ptr(pl.uniq), ptr(pl.n_uniq), ptr(pl.csr_off),
+                       ptr(pl.csr_edge), ptr(pl.edge_u), ptr(routing.row_tab), ptr(out), routing.max_units, B, Lq,
+                       pl.num_chapters, H, cache.HK, routing.NS, 0.125)
+    with L.on_device(dev):
+        call("moc_cache8_attend", ctypes.addressof(args), ptr(ws), nbytes, stream_ptr(dev))
+    return out
+
+
+def _attend_tokens(q: torch.Tensor, cache: MemoryDecodeCache, routing: DecodeRouting) -> torch.Tensor:
+    """q (B, L, H, 64) over a float32 or bfloat16 cache: the sequence attention on the cache's tiles."""
+    B, Lq, H, D = q.shape
+    if cache.T != 64:
+        raise ValueError(f"the decode cache's attention needs 64 tokens per chapter, got {cache.T}")
+    q = _aligned(q.to(cache.dtype))
+    dev, HK = q.device, cache.HK
+    idx = torch.where(routing.idx < routing.plan.num_chapters, routing.idx, -1)
+    lse = torch.empty(B, H, (Lq + 127) // 128 * 128, device=dev, dtype=torch.float32)
+    out = torch.empty_like(q)
+    call("moc_xattn_fwd", L.dtype_code(cache.dtype), ptr(q), ptr(cache.k_tiles), ptr(cache.v_tiles), cache.k_tiles.numel(),
+         HK * 4096, 4096, 64, ptr(idx), ptr(routing.omega), B, Lq, H, HK, D, 64, routing.NS, 0.125, ptr(out), ptr(lse),
+         stream_ptr(dev))
+    return out
+
+
 def decode_attention(q: torch.Tensor, cache: MemoryDecodeCache, routing: DecodeRouting) -> torch.Tensor:
-    """q (B, H, 64) -> attention output (B, H, 64) over the routed chapters (joint softmax, omega-weighted)."""
+    """q (B, H, 64) -> attention output (B, H, 64) over the routed chapters (joint softmax, omega-weighted), or for
+    several query tokens of each sequence (B, L, H, 64) -> (B, L, H, 64).  The result has the cache's type, bfloat16
+    over an 8-bit cache."""
     L.require_gpu(q)
+    if q.dim() not in (3, 4) or q.shape[-1] != 64 or q.shape[0] != routing.B or q.shape[-2] % cache.HK != 0:
+        raise ValueError(f"queries of shape {tuple(q.shape)}: expected ({routing.B}, [tokens,] heads, 64) with heads a "
+                         f"multiple of {cache.HK}")
+    L.require_one_device(q, cache.k_tiles, routing.idx)
+    if routing.plan.num_chapters > cache.num_chapters:
+        raise ValueError(f"routing over {routing.plan.num_chapters} chapters, cache of {cache.num_chapters}")
+    Lq = q.shape[1] if q.dim() == 4 else 1
+    if q.numel() == 0 or routing.NS == 0:
+        return torch.zeros(q.shape, device=q.device, dtype=torch.bfloat16 if cache.dtype == FP8 else cache.dtype)
+    if cache.dtype == FP8:
+        return _attend8(q, q.shape[0], Lq, q.shape[-2], cache, routing)
+    if q.dim() == 4:
+        return _attend_tokens(q, cache, routing)
     B, H, D = q.shape
     if q.dtype != cache.dtype:
         q = q.to(cache.dtype)
@@ -322,11 +472,16 @@ def _step_native(x, wq, wo, H: int, cache: MemoryDecodeCache, routing: DecodeRou
 
 def memory_decode_step(memory_attn, hidden: torch.Tensor, cache: MemoryDecodeCache,
                        routing: DecodeRouting) -> torch.Tensor:
-    """One decode step of a memory sublayer: hidden (B, 1, d) -> (B, 1, d) (before the residual)."""
+    """One decode step of a memory sublayer: hidden (B, 1, d) -> (B, 1, d) (before the residual); or L tokens
+    of each sequence, (B, L, d) -> (B, L, d), over one routing (a prompt served from the cache)."""
     B = hidden.shape[0]
     H = memory_attn.num_heads
     with torch.no_grad():
         wq, wo = memory_attn.q_proj.weight, memory_attn.o_proj.weight
+        if hidden.dim() == 3 and hidden.shape[1] != 1:
+            q = ops.linear(hidden.to(wq.dtype), wq).view(B, hidden.shape[1], H, memory_attn.head_dim)
+            a = decode_attention(q, cache, routing)
+            return ops.linear(a.reshape(B, hidden.shape[1], -1).to(wo.dtype), wo)
         x = hidden.reshape(B, -1).to(wq.dtype)
         if _step_native(x, wq, wo, H, cache, routing):
             x, wq, wo = x.contiguous(), wq.contiguous(), wo.contiguous()

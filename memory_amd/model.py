@@ -160,7 +160,7 @@ class RoutedMemoryLayer(nn.Module):
                  normalize_shared_routed_before_mixing: bool = False, shared_routed_norm_type: str = "rms",
                  shared_routed_norm_eps: float = 1e-6, routing_strategy: str = "sequence",
                  routing_window_size: Optional[int] = None, wo_init_zero: bool = True,
-                 gradient_checkpointing: bool = False):
+                 gradient_checkpointing: bool = False, router_options: Optional[Dict] = None):
         super().__init__()
         self.num_chapters = int(num_chapters)
         self.tokens_per_chapter = int(tokens_per_chapter)
@@ -170,7 +170,8 @@ class RoutedMemoryLayer(nn.Module):
         self.norm_type = shared_routed_norm_type
         self.norm_eps = float(shared_routed_norm_eps)
         self.routing_window_size = routing_window_size
-        self.router = ChapterRouter(hidden_dim, num_chapters, top_k, routing_strategy)
+        # router_options: ChapterRouter's selection (score, num_groups, top_groups, balance_bias, ...)
+        self.router = ChapterRouter(hidden_dim, num_chapters, top_k, routing_strategy, **(router_options or {}))
         self.memory_attn = MemoryCrossAttention(hidden_dim, num_heads, num_kv_heads, wo_init_zero=wo_init_zero,
                                                 gradient_checkpointing=gradient_checkpointing)
         # run the whole layer as one autograd function (memory_amd.seq_layer) where it applies;
@@ -192,7 +193,7 @@ class RoutedMemoryLayer(nn.Module):
 
     def _fused(self, hidden_states: torch.Tensor, bank: torch.Tensor):
         """The whole layer as one autograd function (memory_amd.seq_layer) when it applies."""
-        if not self.fused:
+        if not self.fused or not getattr(self.router, "plain_selection", True):
             return None
         attn = self.memory_attn
         strategy = self.router.routing_strategy
@@ -258,7 +259,7 @@ class TokenRoutedMemoryLayer(nn.Module):
                  num_shared_chapters: int = 1, routed_scaling_factor: float = 2.5, num_kv_heads: Optional[int] = None,
                  normalize_shared_routed_before_mixing: bool = False, shared_routed_norm_type: str = "rms",
                  shared_routed_norm_eps: float = 1e-6, weighted: bool = True, kernel_version: str = "v4",
-                 wo_init_zero: bool = True):
+                 wo_init_zero: bool = True, router_options: Optional[Dict] = None):
         super().__init__()
         self.num_chapters = int(num_chapters)
         self.tokens_per_chapter = int(tokens_per_chapter)
@@ -269,7 +270,7 @@ class TokenRoutedMemoryLayer(nn.Module):
         self.norm_eps = float(shared_routed_norm_eps)
         self.weighted = bool(weighted)
         self.kernel_version = kernel_version
-        self.router = ChapterRouter(hidden_dim, num_chapters, top_k, "token")
+        self.router = ChapterRouter(hidden_dim, num_chapters, top_k, "token", **(router_options or {}))
         self.memory_attn = MemoryCrossAttention(hidden_dim, num_heads, num_kv_heads, wo_init_zero=wo_init_zero)
 
     @float16_via_float32

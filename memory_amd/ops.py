@@ -659,8 +659,8 @@ class _GatedNormArgs(ctypes.Structure):
     """moc_gated_norm."""
     _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "residual", "gate", "w1", "b1", "w2", "b2", "h", "n", "stats")]
                 + [("rows", ctypes.c_int64), ("d", ctypes.c_int64)]
-                + [(n, ctypes.c_int) for n in ("x_dtype", "r_dtype", "gate_mode", "gate_dtype", "norm", "post", "pre")]
-                + [("alpha", ctypes.c_float), ("eps", ctypes.c_float)])
+                + [(n, ctypes.c_int) for n in ("x_dtype", "r_dtype", "gate_mode", "gate_dtype", "norm", "norm2", "post", "pre")]
+                + [(n, ctypes.c_float) for n in ("alpha", "eps", "eps2")])
 
 
 class _GatedNormGrads(ctypes.Structure):
@@ -692,33 +692,33 @@ class _GatedResidualNorm(torch.autograd.Function):
     forms h from them in float32, so nothing of the forward but the rows' statistics is kept."""
 
     @staticmethod
-    def forward(ctx, x, r, gate, w1, b1, w2, b2, mode, norm, alpha, eps, trains):
+    def forward(ctx, x, r, gate, w1, b1, w2, b2, mode, norms, alpha, eps, trains):
         R, d = x.shape
         dev = x.device
         h = torch.empty_like(r)
         n = torch.empty_like(x) if w2 is not None else None
         stats = torch.empty(4, R, device=dev, dtype=torch.float32) if trains else None
-        args = _GatedResidualNorm.args(x, r, gate, w1, b1, w2, b2, mode, norm, alpha, eps, h, n, stats)
+        args = _GatedResidualNorm.args(x, r, gate, w1, b1, w2, b2, mode, norms, alpha, eps, h, n, stats)
         with L.on_device(dev):
             call("moc_gated_norm_fwd", ctypes.addressof(args), stream_ptr(dev))
         if trains:
             ctx.save_for_backward(x, r, gate, w1, b1, w2, b2, stats)
-            ctx.cfg = (mode, norm, alpha, eps)
+            ctx.cfg = (mode, norms, alpha, eps)
         ctx.set_materialize_grads(False)
         return (h, n) if n is not None else h
 
     @staticmethod
-    def args(x, r, gate, w1, b1, w2, b2, mode, norm, alpha, eps, h, n, stats):
+    def args(x, r, gate, w1, b1, w2, b2, mode, norms, alpha, eps, h, n, stats):
         return _GatedNormArgs(ptr(x), ptr(r), ptr(gate), ptr(w1), ptr(b1), ptr(w2), ptr(b2), ptr(h), ptr(n), ptr(stats),
                               x.shape[0], x.shape[1], L.dtype_code(x.dtype), L.dtype_code(r.dtype), mode,
-                              0 if gate is None else L.dtype_code(gate.dtype), norm, w1 is not None, w2 is not None, alpha,
-                              eps)
+                              0 if gate is None else L.dtype_code(gate.dtype), *norms, w1 is not None, w2 is not None,
+                              alpha, *eps)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, dn=None):
         x, r, gate, w1, b1, w2, b2, stats = ctx.saved_tensors
-        mode, norm, alpha, eps = ctx.cfg
+        mode, norms, alpha, eps = ctx.cfg
         need = ctx.needs_input_grad
         if dh is None and dn is None:
             return (None,) * 12
@@ -732,7 +732,7 @@ class _GatedResidualNorm(torch.autograd.Function):
         dp = torch.empty(5 * d + 1, device=dev, dtype=torch.float32)
         ws_bytes = L.query("moc_gated_norm_bwd_workspace", R, d)
         ws = torch.empty(ws_bytes // 4, device=dev, dtype=torch.float32)
-        args = _GatedResidualNorm.args(x, r, gate, w1, b1, w2, b2, mode, norm, alpha, eps, None, None, stats)
+        args = _GatedResidualNorm.args(x, r, gate, w1, b1, w2, b2, mode, norms, alpha, eps, None, None, stats)
         out = _GatedNormGrads(ptr(dh), ptr(dn), ptr(dx), ptr(dr), ptr(dg), ptr(dp))
         with L.on_device(dev):
             call("moc_gated_norm_bwd", ctypes.addressof(args), ctypes.addressof(out), ptr(ws), ws_bytes, stream_ptr(dev))
@@ -749,6 +749,7 @@ def gated_residual_norm(x: torch.Tensor, residual: torch.Tensor, *, post_weight:
                         post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
                         residual_scale: float = 1.0, pre_weight: Optional[torch.Tensor] = None,
                         pre_bias: Optional[torch.Tensor] = None, eps: float = 1e-6, norm: str = "rms",
+                        pre_eps: Optional[float] = None, pre_norm: Optional[str] = None,
                         out_dtype: Optional[torch.dtype] = None):
     """The end of a sublayer and the next one's norm in one pass over the rows:
 
@@ -756,18 +757,22 @@ def gated_residual_norm(x: torch.Tensor, residual: torch.Tensor, *, post_weight:
         h = residual_scale * residual + gate * u     (residual's dtype)
         n = norm(h) * pre_weight + pre_bias          (``out_dtype``, default x's; without a pre_weight: None)
 
-    Returns (h, n).  ``norm`` is "rms" or "layer" (biases only there) over the last dim (up to 16,384).  ``gate``: one
+    Returns (h, n).  ``norm`` is "rms" or "layer" (biases only there) over the last dim (up to 16,384), ``pre_norm`` and
+    ``pre_eps`` are those of the second norm where it differs from the first.  ``gate``: one
     value, one per channel (d,), one per row (..., 1), or x's shape.  x and residual are float32 or bfloat16 (float16
     runs as float32) of one shape; everything in between is float32, h and n are rounded once each and n is the norm
     of the unrounded h.  Differentiable once in every tensor."""
-    if norm not in ("rms", "layer"):
-        raise ValueError(f"norm must be 'rms' or 'layer', got {norm!r}")
+    pre_norm = norm if pre_norm is None else pre_norm
+    pre_eps = eps if pre_eps is None else pre_eps
+    codes = {"rms": L.MOC_NORM_RMS, "layer": L.MOC_NORM_LAYERNORM}
+    if norm not in codes or pre_norm not in codes:
+        raise ValueError(f"norm must be 'rms' or 'layer', got {norm!r}, {pre_norm!r}")
     if x.shape != residual.shape or x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"x {tuple(x.shape)} and residual {tuple(residual.shape)} must be rows of one shape")
     d = x.shape[-1]
     if post_weight is None and post_bias is not None or pre_weight is None and pre_bias is not None:
         raise ValueError("a bias needs the weight of its norm")
-    if norm == "rms" and (post_bias is not None or pre_bias is not None):
+    if norm == "rms" and post_bias is not None or pre_norm == "rms" and pre_bias is not None:
         raise ValueError("RMSNorm has no bias")
     for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight),
                     ("pre_bias", pre_bias)):
@@ -792,8 +797,8 @@ def gated_residual_norm(x: torch.Tensor, residual: torch.Tensor, *, post_weight:
         gate = gate.contiguous()
     w = [None if t is None else t.float().contiguous() for t in (post_weight, post_bias, pre_weight, pre_bias)]
     trains = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, r2, gate, *w))
-    out = _GatedResidualNorm.apply(x2, r2, gate, *w, mode, L.MOC_NORM_RMS if norm == "rms" else L.MOC_NORM_LAYERNORM,
-                                   float(residual_scale), float(eps), trains)
+    out = _GatedResidualNorm.apply(x2, r2, gate, *w, mode, (codes[norm], codes[pre_norm]), float(residual_scale),
+                                   (float(eps), float(pre_eps)), trains)
     h, n = out if isinstance(out, tuple) else (out, None)
     h = h.view(x.shape).to(rd)
     return h, None if n is None else n.view(x.shape).to(od)

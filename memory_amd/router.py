@@ -49,9 +49,17 @@ def compute_router_losses(logits: torch.Tensor, probs: Optional[torch.Tensor], i
 
 
 class ChapterRouter(nn.Module):
-    """Top-k chapter router (memory_transformer/router.py:15-340)."""
+    """Top-k chapter router (memory_transformer/router.py:15-340).
 
-    def __init__(self, hidden_dim: int, num_chapters: int, top_k: int = 1, routing_strategy: str = "sequence"):
+    Beside the reference's softmax top-k it selects as a mixture of experts does (``ops.router_select``): ``score``
+    "softmax" or "sigmoid", ``num_groups`` groups of the routed chapters of which ``top_groups`` stay (scored by their
+    ``group_best`` largest keys), weights renormalised or not, and with ``balance_bias`` a float32 buffer of that name
+    that is added to the scores for the selection only and moved by ``update_balance``.  Groups divide the chapters
+    past the excluded (shared) prefix."""
+
+    def __init__(self, hidden_dim: int, num_chapters: int, top_k: int = 1, routing_strategy: str = "sequence", *,
+                 score: str = "softmax", num_groups: int = 1, top_groups: Optional[int] = None, group_best: int = 2,
+                 renormalize: bool = True, balance_bias: bool = False):
         super().__init__()
         if num_chapters <= 0:
             raise ValueError(f"num_chapters must be > 0, got {num_chapters}")
@@ -63,9 +71,49 @@ class ChapterRouter(nn.Module):
         self.num_chapters = num_chapters
         self.top_k = top_k
         self.routing_strategy = routing_strategy
+        if score not in ("softmax", "sigmoid"):
+            raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+        if num_groups < 1 or (top_groups is not None and not 1 <= top_groups <= num_groups):
+            raise ValueError(f"num_groups={num_groups}, top_groups={top_groups}")
+        if group_best not in (1, 2):
+            raise ValueError(f"group_best must be 1 or 2, got {group_best}")
+        self.score = score
+        self.num_groups = int(num_groups)
+        self.top_groups = self.num_groups if top_groups is None else int(top_groups)
+        self.group_best = int(group_best)
+        self.renormalize = bool(renormalize)
+        if balance_bias:
+            self.register_buffer("balance_bias", torch.zeros(num_chapters))
+        else:
+            self.balance_bias = None
         self.router = nn.Linear(hidden_dim, num_chapters, bias=True)
         nn.init.normal_(self.router.weight, mean=0.0, std=0.02)
         nn.init.zeros_(self.router.bias)
+
+    # -- selection ------------------------------------------------------------
+    @property
+    def plain_selection(self) -> bool:
+        """Whether the selection is the reference's softmax top-k (which the fused layers run)."""
+        return (self.score == "softmax" and self.top_groups == self.num_groups and self.renormalize
+                and self.balance_bias is None)
+
+    def select(self, logits: torch.Tensor, k: int, exclude_prefix_chapters: int = 0):
+        """(idx int32 (R, k), weights float32 (R, k)) of logits (R, C)."""
+        if self.plain_selection:
+            return ops.router_topk(logits, k, exclude_prefix_chapters)
+        grouped = self.top_groups < self.num_groups
+        return ops.router_select(logits, k, exclude_prefix_chapters, score=self.score, bias=self.balance_bias,
+                                 num_groups=self.num_groups if grouped else 1,
+                                 top_groups=self.top_groups if grouped else 1, group_best=self.group_best,
+                                 renormalize=self.renormalize)
+
+    @torch.no_grad()
+    def update_balance(self, indices: torch.Tensor, rate: float = 1e-3, exclude_prefix_chapters: int = 0) -> torch.Tensor:
+        """After a step: moves the balance bias by ``rate`` towards equal use of the chapters past the excluded prefix,
+        given the step's selections (chapter ids of any shape).  Returns how often each chapter was selected."""
+        if self.balance_bias is None:
+            raise ValueError("this router has no balance bias (balance_bias=True)")
+        return ops.router_balance_(self.balance_bias, indices, rate, exclude_prefix_chapters)
 
     # -- logits ---------------------------------------------------------------
     def sequence_logits(self, hidden_states: torch.Tensor, rolling_window_size: Optional[int] = None) -> torch.Tensor:
@@ -105,7 +153,7 @@ class ChapterRouter(nn.Module):
             idx = torch.empty((B, 0), dtype=torch.int32, device=hidden_states.device)
             w = torch.empty((B, 0), dtype=torch.float32, device=hidden_states.device)
         else:
-            idx, w = ops.router_topk(logits, k, S)
+            idx, w = self.select(logits, k, S)
         losses = {}
         if return_losses:
             losses = compute_router_losses(logits, None, idx, self.num_chapters)
@@ -131,7 +179,11 @@ class ChapterRouter(nn.Module):
             if return_losses:
                 losses = compute_router_losses(logits, None, idx.reshape(B * T, 0), C)
             return idx, w, losses
-        logits, idx32, w = ops.token_router(hidden_states, self.router.weight, self.router.bias, k, S)
+        if self.plain_selection:
+            logits, idx32, w = ops.token_router(hidden_states, self.router.weight, self.router.bias, k, S)
+        else:
+            logits = ops.router_token_logits(hidden_states, self.router.weight, self.router.bias)
+            idx32, w = self.select(logits, k, S)
         idx = (idx32 if ids32 else idx32.long()).view(B, T, k)
         losses = {}
         if return_losses:

@@ -1,0 +1,352 @@
+"""The decode cache in 8 bits (e4m3 tiles with one scale per chapter and kv head): its quantisation bit by bit, and
+the attention over it against float64.
+
+Tolerances, derived: the products run on exact operands (bfloat16 queries, e4m3 values widened exactly) with float32
+sums; probabilities are rounded to bfloat16 (2^-8 each), part rows of a chapter once more, the result once, and row
+sums may carry the probabilities' rounding: 2^-8 |o| + 3 2^-8 sum_j p_j |v_j|.  A logit's float32 sum of 64 products is off
+by at most 64 2^-24 sum |q k|, which moves a probability by as much: 2^-17 times the largest logit's terms."""
+
+import pytest
+import torch
+
+from helpers import gen
+
+BF, F32, FP8 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
+H8 = 2.0 ** -8
+
+
+def make_tiles(C, HK, seed, spread=0.5):
+    g0 = gen(seed)
+    x = torch.randn(C, HK, 64, 64, generator=g0) * torch.exp(spread * torch.randn(C, HK, 1, 1, generator=g0))
+    s = torch.exp2(torch.ceil(torch.log2(x.abs().amax((2, 3)).double() / 448))).float()
+    return (x / s[:, :, None, None]).to(FP8), s
+
+
+def reference(q, k8, ks, v8, vs, idx, omega):
+    """(o, bound) float64 of q (B, L, H, 64); slots whose id is out of range are left out."""
+    B, Lq, H, D = q.shape
+    C, HK = ks.shape
+    out, bound = torch.zeros(B, Lq, H, D, dtype=torch.float64), torch.zeros(B, Lq, H, D, dtype=torch.float64)
+    for b in range(B):
+        sl = [s for s in range(idx.shape[1]) if 0 <= int(idx[b, s]) < C]
+        if not sl:
+            continue
+        ids = idx[b, sl].long()
+        om = omega[b, sl].double()
+        k = k8[ids].to(F32).double() * ks[ids].double()[:, :, None, None] * om[:, None, None, None]
+        v = v8[ids].to(F32).double() * vs[ids].double()[:, :, None, None] * om[:, None, None, None]
+        for h in range(H):
+            kk, vv = k[:, h // (H // HK)].reshape(-1, D), v[:, h // (H // HK)].reshape(-1, D)
+            qd = q[b, :, h].double()
+            p = torch.softmax(qd @ kk.t() / 8, dim=1)
+            out[b, :, h] = p @ vv
+            mag = p @ vv.abs()
+            logit = (qd.abs() @ kk.abs().t() / 8).amax(1, keepdim=True)
+            bound[b, :, h] = H8 * out[b, :, h].abs() + (3 * H8 + 2.0 ** -16 * logit) * mag
+    return out, bound
+
+
+def make(B, L, H, HK, C, NS, seed, distinct=True):
+    g0 = gen(seed)
+    k8, ks = make_tiles(C, HK, seed + 1)
+    v8, vs = make_tiles(C, HK, seed + 2)
+    q = torch.randn(B, L, H, 64, generator=g0).to(BF)
+    if distinct and NS <= C:
+        idx = torch.stack([torch.randperm(C, generator=g0)[:NS] for _ in range(B)]).int()
+    else:
+        idx = torch.randint(0, C, (B, NS), generator=g0).int()
+    omega = torch.rand(B, NS, generator=g0) * 1.5
+    return q, k8, ks, v8, vs, idx, omega
+
+
+def attend(dev, q, k8, ks, v8, vs, idx, omega, sync=True):
+    from memory_amd.decode import DecodeRouting, MemoryDecodeCache, decode_attention
+    C, HK = ks.shape
+    cache = MemoryDecodeCache.from_tiles(k8.to(dev), v8.to(dev), num_chapters=C, tokens_per_chapter=64, num_kv_heads=HK,
+                                         k_scale=ks.to(dev), v_scale=vs.to(dev))
+    routing = DecodeRouting(idx.to(dev), omega.to(dev), C, sync=sync)
+    qd = q.to(dev)
+    out = decode_attention(qd[:, 0] if q.shape[1] == 1 else qd, cache, routing)
+    assert out.dtype == BF
+    return out.view(q.shape)
+
+
+def check(got, q, k8, ks, v8, vs, idx, omega):
+    want, bound = reference(q, k8, ks, v8, vs, idx, omega)
+    err = (got.cpu().double() - want).abs()
+    worst = (err / (bound + 1e-30)).max().item() if err.numel() else 0
+    print(f"q {tuple(q.shape)} C={ks.shape[0]} HK={ks.shape[1]} NS={idx.shape[1]}: worst {worst:.3f} of the bound", flush=True)
+    assert (err <= bound + 1e-30).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_pack(gpu_device, dtype):
+    """Scales and bytes equal the definition's, on ordinary tiles and on zeros, infinities, NaN, magnitudes at a
+    scale's edge, subnormal and huge ones."""
+    from memory_amd.decode import MemoryDecodeCache, _v8_natural
+    g0 = gen(1)
+    C, HK = 12, 3
+    k = torch.randn(C, HK, 64, 64, generator=g0) * torch.exp(3 * torch.randn(C, HK, 1, 1, generator=g0))
+    v = torch.randn(C, HK, 64, 64, generator=g0)
+    k[0, 0] = 0
+    k[0, 1].clamp_(-1, 1)[3, 4] = 448.0
+    k[0, 2].clamp_(-1, 1)[3, 4] = -450.0
+    k[1, 0].clamp_(-1, 1)[63, 63] = 256.0
+    k[1, 1, 5, 6] = float("inf")
+    k[1, 1, 7, 8] = float("-inf")
+    k[1, 2, 0, 0] = float("nan")
+    k[2, 0] = float("nan")
+    k[2, 1] *= 1e-30
+    k[2, 2] = k[2, 2].clamp(-3, 3) * 1e37
+    k[3, 0] = torch.randn(64, 64, generator=g0) * 1e-39 if dtype == F32 else 0
+    k[3, 1] = float("inf")
+    k, v = k.to(dtype), v.to(dtype)
+    cache = MemoryDecodeCache.from_tiles(k.to(gpu_device), v.to(gpu_device), num_chapters=C, tokens_per_chapter=64,
+                                         num_kv_heads=HK).quantized()
+    for x, tiles, scale in ((k, cache.k_tiles, cache.k_scale), (v, _v8_natural(cache.v_tiles), cache.v_scale)):
+        x = x.double()
+        fin = torch.where(x.isfinite(), x.abs(), 0.0).amax((2, 3))
+        e = torch.where(fin > 0, torch.ceil(torch.log2(fin / 448)), 0.0)
+        # log2 of 448 2^e itself may round either way: decide by the definition
+        e = torch.where((fin > 0) & (fin > 448 * torch.exp2(e)), e + 1, e)
+        e = torch.where((fin > 0) & (fin <= 448 * torch.exp2(e - 1)), e - 1, e).clamp(-120, 120)
+        assert torch.equal(scale.cpu().double(), torch.exp2(e))
+        y = (x / torch.exp2(e)[:, :, None, None]).clamp(-448, 448).float().to(FP8)
+        got = tiles.cpu()
+        nan = x.isnan()
+        assert got.float()[nan].isnan().all()
+        assert torch.equal(got.float()[~nan], y.float()[~nan])
+    kd, vd = cache.dequantized()
+    assert kd.shape == (C, HK, 64, 64) and torch.equal(vd.cpu(), (y.float() * scale.cpu()[:, :, None, None]))
+    assert cache.nbytes == 2 * C * HK * 4096 + 8 * C * HK and cache.quantized() is cache
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,L,H,HK,C,NS", [(1, 1, 1, 1, 1, 1), (1, 1, 12, 12, 65, 65), (3, 1, 8, 1, 20, 5), (5, 1, 16, 4, 40, 33),
+                                           (64, 1, 4, 2, 33, 9), (2, 1, 32, 2, 10, 70), (40, 1, 12, 4, 8, 5), (300, 1, 2, 1, 9, 3),
+                                           (2, 2, 4, 4, 20, 7), (3, 3, 8, 2, 20, 65), (2, 16, 2, 2, 9, 4), (1, 17, 2, 2, 9, 4),
+                                           (2, 5, 16, 4, 30, 12), (1, 33, 16, 1, 30, 65), (2, 129, 4, 2, 12, 9), (1, 509, 4, 4, 70, 65),
+                                           (3, 300, 8, 8, 9, 1), (1, 2, 64, 1, 5, 3), (1, 1000, 3, 3, 7, 2)])
+def test_attention(gpu_device, B, L, H, HK, C, NS):
+    case = make(B, L, H, HK, C, NS, B + L + H + C)
+    check(attend(gpu_device, *case), *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L", [1, 4, 40])
+def test_slots_weights_and_scales(gpu_device, L):
+    """Skipped slots (ids out of range), rows without any slot, a chapter chosen twice, weights of 0, scales that are
+    no powers of two, 0, or far from 1."""
+    q, k8, ks, v8, vs, idx, omega = make(6, L, 4, 2, 12, 8, 5, distinct=False)
+    idx[0, 2], idx[0, 5], idx[1, 0] = -1, 12, 2 ** 31 - 1
+    idx[2] = -7
+    idx[3] = 4
+    omega[4, :3] = 0
+    omega[5] = 0
+    ks = ks * (0.5 + torch.rand(12, 2, generator=gen(3)))
+    vs = vs * (0.5 + torch.rand(12, 2, generator=gen(4)))
+    ks[3], vs[5], ks[7], vs[7] = 0.0, 0.0, 1e-30, 1e-30
+    vs[8], vs[9] = 1e30, 1e-35
+    case = (q, k8, ks, v8, vs, idx, omega)
+    for sync in (True, False):
+        got = attend(gpu_device, *case, sync=sync)
+        check(got, *case)
+        assert not got[2].any() and not got[5].any()
+    none = (q, k8, ks, v8, vs, torch.full_like(idx, -1), omega)
+    assert not attend(gpu_device, *none).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L", [1, 24])
+def test_large_logits_and_nan(gpu_device, L):
+    """Logits of several hundred (one key takes all), and a NaN that stays in the sequences and heads that read it."""
+    case = list(make(3, L, 4, 2, 10, 4, 8))
+    case[2] = case[2] * 60
+    check(attend(gpu_device, *case), *case)
+    clean = attend(gpu_device, *case)
+    k8 = case[1].view(torch.uint8).clone()
+    hit = int(case[5][1, 2])
+    k8[hit, 1, 3, 3] = 0x7f
+    case[1] = k8.view(FP8)
+    got = attend(gpu_device, *case)
+    for b in range(3):
+        reads = hit in case[5][b].tolist()
+        assert torch.equal(got[b, :, :2], clean[b, :, :2])
+        assert got[b, :, 2:].isnan().all() if reads else torch.equal(got[b], clean[b])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L", [1, 6, 70])
+def test_query_layouts_and_types(gpu_device, L):
+    from memory_amd.decode import DecodeRouting, MemoryDecodeCache, decode_attention
+    q, k8, ks, v8, vs, idx, omega = make(2, L, 4, 2, 9, 5, 3)
+    want = attend(gpu_device, q, k8, ks, v8, vs, idx, omega)
+    cache = MemoryDecodeCache.from_tiles(k8.to(gpu_device), v8.to(gpu_device), num_chapters=9, tokens_per_chapter=64,
+                                         num_kv_heads=2, k_scale=ks.to(gpu_device), v_scale=vs.to(gpu_device))
+    routing = DecodeRouting(idx.to(gpu_device), omega.to(gpu_device), 9)
+    qd = q.to(gpu_device)
+    views = [qd.float(), qd.transpose(1, 2).contiguous().transpose(1, 2), qd.half().float().half()]
+    off = torch.zeros(qd.numel() + 3, device=gpu_device, dtype=BF)[3:].view(q.shape).copy_(qd)
+    for v in views[:2] + [off]:
+        got = decode_attention(v[:, 0] if L == 1 else v, cache, routing).view(q.shape)
+        assert torch.equal(got, want)
+    assert decode_attention(qd[:, :0], cache, routing).shape == (2, 0, 4, 64)
+
+
+@pytest.mark.gpu
+def test_tiles_past_four_gib(gpu_device):
+    """A cache whose last tiles lie past 2^32 bytes."""
+    from memory_amd.decode import DecodeRouting, MemoryDecodeCache, decode_attention
+    C, HK = 16384, 66
+    q, k8, ks, v8, vs, idx, omega = make(2, 1, HK, HK, 4, 4, 9)
+    tiles = torch.zeros(C, HK, 64, 64, device=gpu_device, dtype=torch.uint8)
+    scale = torch.ones(C, HK, device=gpu_device)
+    for L in (1, 20):
+        caches = []
+        for t8, s in ((k8, ks), (v8, vs)):
+            t, sc = tiles.clone(), scale.clone()
+            t[-4:] = t8.view(torch.uint8).to(gpu_device)
+            sc[-4:] = s.to(gpu_device)
+            caches.append((t, sc))
+        cache = MemoryDecodeCache.__new__(MemoryDecodeCache)
+        cache.num_chapters, cache.T, cache.HK, cache.dtype = C, 64, HK, FP8
+        cache.k_tiles, cache.k_scale = caches[0][0].view(FP8), caches[0][1]
+        from memory_amd.decode import _v8_permuted
+        caches[1][0][-4:] = _v8_permuted(v8.to(gpu_device)).view(torch.uint8)
+        cache.v_tiles, cache.v_scale = caches[1][0].view(FP8), caches[1][1]
+        qq = q.expand(2, L, HK, 64).contiguous()
+        routing = DecodeRouting((idx + C - 4).to(gpu_device), omega.to(gpu_device), C)
+        qd = qq.to(gpu_device)
+        got = decode_attention(qd[:, 0] if L == 1 else qd, cache, routing).view(qq.shape)
+        check(got, qq, k8, ks, v8, vs, idx, omega)
+        del cache, caches
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L", [1, 5, 40])
+def test_graph_replays(gpu_device, L):
+    from memory_amd.decode import DecodeRouting, MemoryDecodeCache, decode_attention
+    q, k8, ks, v8, vs, idx, omega = make(7, L, 8, 4, 30, 9, 2)
+    cache = MemoryDecodeCache.from_tiles(k8.to(gpu_device), v8.to(gpu_device), num_chapters=30, tokens_per_chapter=64,
+                                         num_kv_heads=4, k_scale=ks.to(gpu_device), v_scale=vs.to(gpu_device))
+    routing = DecodeRouting(idx.to(gpu_device), omega.to(gpu_device), 30)
+    qd = (q[:, 0] if L == 1 else q).to(gpu_device)
+    decode_attention(qd, cache, routing)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = decode_attention(qd, cache, routing)
+    for rep in range(3):
+        qd.copy_(torch.randn(qd.shape, generator=gen(rep)).to(BF))
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, decode_attention(qd, cache, routing)), f"replay {rep}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,tol", [(BF, 2e-2), (F32, 1e-4)])
+def test_tokens_over_a_full_cache(gpu_device, dtype, tol):
+    """Several query tokens over a bfloat16 or float32 cache (the sequence attention on its tiles)."""
+    from memory_amd.decode import DecodeRouting, MemoryDecodeCache, decode_attention
+    q, k8, ks, v8, vs, idx, omega = make(3, 37, 8, 2, 12, 6, 4)
+    idx[1, 2], idx[2, 0] = -1, 12
+    k, v = (t.float() * s[:, :, None, None] for t, s in ((k8, ks), (v8, vs)))
+    cache = MemoryDecodeCache.from_tiles(k.to(gpu_device, dtype), v.to(gpu_device, dtype), num_chapters=12, tokens_per_chapter=64,
+                                         num_kv_heads=2)
+    out = decode_attention(q.to(gpu_device), cache, DecodeRouting(idx.to(gpu_device), omega.to(gpu_device), 12))
+    want, _ = reference(q, k8, ks, v8, vs, idx, omega)
+    assert out.dtype == dtype and (out.cpu().double() - want).abs().max() <= tol * want.abs().max()
+
+
+@pytest.mark.gpu
+def test_cache_from_a_bank_saved_and_loaded(gpu_device, tmp_path):
+    """The 8-bit cache of a bank is the quantised bfloat16 one; a file gives back the same bytes; a decode step and a
+    prompt through it, eager and as a DecodeStepGraph."""
+    from memory_amd.decode import DecodeRouting, DecodeStepGraph, MemoryDecodeCache, memory_decode_step
+    from memory_amd.memory_attention import MemoryCrossAttention
+    g0 = gen(3)
+    C, d, H, HK, B = 9, 256, 4, 2, 5
+    bank = (torch.randn(C * 64, d, generator=g0) * 0.5).to(gpu_device)
+    attn = MemoryCrossAttention(d, H, HK, wo_init_zero=False).to(gpu_device, BF)
+    kw = dict(num_chapters=C, tokens_per_chapter=64, num_kv_heads=HK, norm_type="rms")
+    full = MemoryDecodeCache(bank, attn.k_proj.weight, attn.v_proj.weight, **kw)
+    eight = MemoryDecodeCache(bank, attn.k_proj.weight, attn.v_proj.weight, dtype=FP8, **kw)
+    again = full.quantized()
+    same = lambda a, b: all(torch.equal(getattr(a, n).view(torch.uint8), getattr(b, n).view(torch.uint8))
+                            for n in ("k_tiles", "v_tiles", "k_scale", "v_scale"))
+    assert same(eight, again) and eight.nbytes < 0.51 * full.nbytes
+    path = str(tmp_path / "cache.safetensors")
+    eight.save(path)
+    assert same(MemoryDecodeCache.load(path, gpu_device), eight)
+    idx = torch.stack([torch.randperm(C, generator=g0)[:5] for _ in range(B)]).int().to(gpu_device)
+    routing = DecodeRouting(idx, torch.rand(B, 5, generator=g0).to(gpu_device), C)
+    k, v = eight.dequantized()
+    exact = MemoryDecodeCache.from_tiles(k, v, num_chapters=C, tokens_per_chapter=64, num_kv_heads=HK)
+    attn32 = MemoryCrossAttention(d, H, HK, wo_init_zero=False).to(gpu_device)
+    attn32.load_state_dict({n: p.float() for n, p in attn.state_dict().items()})
+    for L in (1, 12):
+        h = torch.randn(B, L, d, generator=g0).to(gpu_device, BF)
+        got = memory_decode_step(attn, h, eight, routing)
+        want = memory_decode_step(attn32, h.float(), exact, routing)
+        # bfloat16 queries, attention and result: each 2^-8 of magnitudes that the projections mix
+        assert got.shape == h.shape and (got.float() - want).abs().max() <= 2e-2 * want.abs().max()
+        graph = DecodeStepGraph([(attn, eight, routing)], [h])
+        for rep in range(3):
+            x = torch.randn(B, L, d, generator=gen(rep)).to(gpu_device, BF)
+            out = graph.run([x])[0].clone()
+            torch.cuda.synchronize()
+            assert torch.equal(out, memory_decode_step(attn, x, eight, routing))
+
+
+@pytest.mark.gpu
+def test_refusals(gpu_device):
+    from memory_amd.decode import DecodeRouting, MemoryDecodeCache, decode_attention
+    k8, s = make_tiles(4, 2, 1)
+    k8, s = k8.to(gpu_device), s.to(gpu_device)
+    kw = dict(num_chapters=4, tokens_per_chapter=64, num_kv_heads=2)
+    for bad in (dict(), dict(k_scale=s), dict(k_scale=s, v_scale=-s), dict(k_scale=s * float("inf"), v_scale=s),
+                dict(k_scale=s[:, :1], v_scale=s)):
+        with pytest.raises(ValueError):
+            MemoryDecodeCache.from_tiles(k8, k8, **kw, **bad)
+    with pytest.raises(ValueError):
+        MemoryDecodeCache.from_tiles(k8.float(), k8.float(), **kw, k_scale=s, v_scale=s)
+    cache = MemoryDecodeCache.from_tiles(k8, k8, **kw, k_scale=s, v_scale=s)
+    idx = torch.zeros(3, 2, device=gpu_device, dtype=torch.int32)
+    routing = DecodeRouting(idx, torch.ones(3, 2, device=gpu_device), 4)
+    for shape in ((2, 4, 64), (3, 3, 64), (3, 4, 32), (3, 64), (3, 1, 1, 4, 64)):
+        with pytest.raises(ValueError):
+            decode_attention(torch.zeros(shape, device=gpu_device, dtype=BF), cache, routing)
+    wide = DecodeRouting(idx, torch.ones(3, 2, device=gpu_device), 5)
+    with pytest.raises(ValueError, match="cache of 4"):
+        decode_attention(torch.zeros(3, 4, 64, device=gpu_device, dtype=BF), cache, wide)
+
+
+def test_refusals_of_the_entry_points():
+    import ctypes
+    from memory_amd import _lib as L
+    from memory_amd.decode import _Cache8Args, _v8_natural, _v8_permuted
+    v = torch.randint(0, 255, (3, 2, 64, 64), dtype=torch.uint8, generator=gen(1)).view(FP8)
+    p = _v8_permuted(v).view(torch.uint8)
+    for g in range(4):
+        for kb in range(4):
+            for x in range(4):
+                assert torch.equal(p[..., 16 * g + 4 * kb + x], v.view(torch.uint8)[..., 16 * kb + 4 * g + x, :])
+    assert torch.equal(_v8_natural(_v8_permuted(v)).view(torch.uint8), v.view(torch.uint8))
+    with pytest.raises(ValueError, match="null"):
+        L.call("moc_cache8_pack", L.MOC_BF16, None, None, 3, None, None, None, None, None)
+    with pytest.raises(ValueError, match="dtype"):
+        L.call("moc_cache8_pack", 7, 16, 16, 3, 16, 16, 16, 16, None)
+    ok = dict(B=1, L=1, H=2, HK=1, NS=3, C=4, max_u=3)
+    for bad in (dict(), dict(H=3, HK=2), dict(NS=0), dict(L=0), dict(C=0), dict(max_u=-1), dict(B=1 << 20, L=1 << 11)):
+        a = _Cache8Args(**{**ok, **bad})
+        with pytest.raises(ValueError):
+            L.call("moc_cache8_attend", ctypes.addressof(a), None, 0, None)
+    ptrs = {n: 256 for n, t in _Cache8Args._fields_ if t is ctypes.c_void_p}
+    a = _Cache8Args(**ok, **ptrs)
+    with pytest.raises(ValueError, match="workspace"):
+        L.call("moc_cache8_attend", ctypes.addressof(a), 256, 16, None)
+    a.q = 8
+    with pytest.raises(ValueError, match="aligned"):
+        L.call("moc_cache8_attend", ctypes.addressof(a), 256, 1 << 20, None)

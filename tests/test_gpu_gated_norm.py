@@ -4,7 +4,7 @@ formulas in float64.
 Tolerances, derived: between loads and stores every value is float32, with at most 256 roundings of 2^-24 on the
 way of any element of a row (sums over a row are formed from lane sums of at most 32 terms, six cross-lane
 additions and at most 16 waves; a gradient passes four such sums), each relative to the largest term of its row; the
-store rounds by half a step (2^-9 relative to the value for bfloat16).  Column sums over R rows add at most
+store rounds by half a step (2^-8 relative to the value for bfloat16).  Column sums over R rows add at most
 R + 64 roundings relative to the sum of the terms' magnitudes."""
 
 import pytest
@@ -268,6 +268,6 @@ def test_refusals():
     a.d = 16385
     with pytest.raises(ValueError, match="16384"):
         L.call("moc_gated_norm_fwd", ctypes.addressof(a), None)
-    a.d, a.norm, a.gate_mode = 8, 1, 9
+    a.d, a.norm, a.norm2, a.gate_mode = 8, 1, 1, 9
     with pytest.raises(ValueError, match="gate mode"):
         L.call("moc_gated_norm_fwd", ctypes.addressof(a), None)
