@@ -819,8 +819,9 @@ typedef struct {
 } moc_gated_norm;
 int moc_gated_norm_fwd(const moc_gated_norm* a, hipStream_t stream);
 /* Gradients: dh (r_dtype) and dn (x_dtype) arrive (either may be NULL: zero); dx, dres and dgate (token, full) are
- * written where not NULL; dparams f32 [5 d + 1] = dw1, db1, dw2, db2, the channel gate's gradient (zeros without
- * one), and the scalar gate's.  a: as the forward's, with its stats. */
+ * written where not NULL; dparams f32 [5 d + 1] = dw1, db1, dw2, db2, the channel gate's gradient and the scalar
+ * gate's, each written where its parameter is there (w2's and b2's: where dn is).  a: as the forward's, with its
+ * stats; dx, dres and dgate may not overlap the inputs. */
 typedef struct {
   const void *dh, *dn;
   void *dx, *dres, *dgate;

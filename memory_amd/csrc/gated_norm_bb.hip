@@ -1,0 +1,7 @@
+// gated_norm.h for x of bf16 and a residual of bf16.
+#include "gated_norm.h"
+
+int moc::gn_fwd_bb(const moc_gated_norm& a, bool vec, hipStream_t stream) { return gn::fwd_types<bf16, bf16>(a, vec, stream); }
+int moc::gn_bwd_bb(const moc_gated_norm& a, const moc_gated_norm_grads& g, bool vec, const GnStrips& s, hipStream_t stream) {
+  return gn::bwd_types<bf16, bf16>(a, g, vec, s, stream);
+}

@@ -729,7 +729,7 @@ class _GatedResidualNorm(torch.autograd.Function):
         dx = torch.empty_like(x) if need[0] else None
         dr = torch.empty_like(r) if need[1] else None
         dg = torch.empty_like(gate) if need[2] and mode in (_GATE_TOKEN, _GATE_FULL) else None
-        dp = torch.empty(5 * d + 1, device=dev, dtype=torch.float32)
+        dp = (torch.empty if R else torch.zeros)(5 * d + 1, device=dev, dtype=torch.float32)
         ws_bytes = L.query("moc_gated_norm_bwd_workspace", R, d)
         ws = torch.empty(ws_bytes // 4, device=dev, dtype=torch.float32)
         args = _GatedResidualNorm.args(x, r, gate, w1, b1, w2, b2, mode, norms, alpha, eps, None, None, stats)
