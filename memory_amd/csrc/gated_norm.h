@@ -22,13 +22,14 @@ int gn_bwd_bb(const moc_gated_norm& a, const moc_gated_norm_grads& g, bool vec, 
 // column sums kept by a strip, in the order of moc_gated_norm_grads::dparams
 enum { kGnDw1, kGnDb1, kGnDw2, kGnDb2, kGnDg, kGnSums };
 
+constexpr int kGnWaves = 4;   // of a workgroup with several rows
 // waves of a row and rows in parallel of the backward's workgroups: one load of eight (or four scalar ones) per lane
 // and operand up to 8,192 (4,096) elements
 inline int gn_bwd_waves(int64_t d, bool vec) {
   const int64_t per = vec ? 512 : 256;
   return d <= per ? 1 : d <= 2 * per ? 2 : d <= 4 * per ? 4 : d <= 8 * per ? 8 : 16;
 }
-inline int gn_bwd_rows(int waves) { return waves <= 2 ? 8 / waves : 1; }
+inline int gn_bwd_rows(int waves) { return waves < kGnWaves ? kGnWaves / waves : 1; }
 
 namespace gn {
 
@@ -75,11 +76,24 @@ template <int VEC> __device__ __forceinline__ void load_w(const float* p, int j,
   }
 }
 
+// Sum over the wave, the same bits in every lane: neighbours, pairs, quads and halves of a 16-lane row by DPP, then
+// the rows by permutes; no LDS (against six rounds of ds_bpermute).
+template <int kCtrl> __device__ __forceinline__ float dpp_add(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), kCtrl, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lanes_sum(float v) {
+  v = dpp_add<0xB1>(v);    // quad_perm [1, 0, 3, 2]
+  v = dpp_add<0x4E>(v);    // quad_perm [2, 3, 0, 1]
+  v = dpp_add<0x141>(v);   // row_half_mirror
+  v = dpp_add<0x140>(v);   // row_mirror
+  return quad_sum_pl(v);
+}
+
 // sums of N values over the W waves of a row (waves w0 .. w0 + W - 1 of the workgroup), the same bits in every
 // lane.  W > 1: every wave of the workgroup calls it.
 template <int W, int N> __device__ __forceinline__ void row_sum(float (&v)[N], float* red, int wave) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  for (int i = 0; i < N; ++i) v[i] = lanes_sum(v[i]);
   if constexpr (W > 1) {
     __syncthreads();   // the previous sums have been read
     if ((threadIdx.x & 63) == 0) {
@@ -237,40 +251,55 @@ __global__ __launch_bounds__(64 * W * RPB) void gated_norm_bwd_kernel(moc_gated_
     for (int e = 0; e < VEC; ++e) dw1[i][e] = db1[i][e] = dw2[i][e] = db2[i][e] = dgc[i][e] = 0.f;
   }
   float dscal = 0.f;
-  // (every wave takes part in every round: the sums of a row over its waves synchronise the workgroup)
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
-    const int64_t r = r0 + grp;
-    const bool live = r < a.rows;
+  // a row's operands, loaded one round ahead (raw: nothing here waits for a load)
+  struct Row {
     typename Vec<TX, VEC>::type xv[KCH], gv[KCH], nv[KCH];
     typename Vec<TR, VEC>::type rv[KCH], hv[KCH];
+    float mu1, rs1, mu2, rs2;
+    uint32_t gate;
+  };
+  auto fetch = [&](Row& n, int64_t r) {
+    n.mu1 = n.mu2 = n.rs2 = 0.f;
+    n.rs1 = 1.f;
+    n.gate = 0;
+    if (r >= a.rows) return;
 #pragma unroll
     for (int i = 0; i < KCH; ++i) {
       const int c = t + 64 * W * i;
-      if (c < nch && live) {
+      if (c < nch) {
         const int64_t at = r * d + VEC * c;
-        xv[i] = load<TX, VEC>(a.x, at);
+        n.xv[i] = load<TX, VEC>(a.x, at);
         if (has_dn) {
-          rv[i] = load<TR, VEC>(a.residual, at);
-          nv[i] = load<TX, VEC>(o.dn, at);
+          n.rv[i] = load<TR, VEC>(a.residual, at);
+          n.nv[i] = load<TX, VEC>(o.dn, at);
         }
-        if (o.dh) hv[i] = load<TR, VEC>(o.dh, at);
-        if constexpr (FULL) gv[i] = load<TX, VEC>(a.gate, at);
+        if (o.dh) n.hv[i] = load<TR, VEC>(o.dh, at);
+        if constexpr (FULL) n.gv[i] = load<TX, VEC>(a.gate, at);
       }
     }
-    float mu1 = 0.f, rs1 = 1.f, mu2 = 0.f, rs2 = 0.f, grow = 1.f;
-    if (live) {
-      if (a.post) {
-        mu1 = a.stats[r];
-        rs1 = a.stats[a.rows + r];
-      }
-      if (has_dn) {
-        mu2 = a.stats[2 * a.rows + r];
-        rs2 = a.stats[3 * a.rows + r];
-      }
-      grow = gate_row(a, r);
+    if (a.post) {
+      n.mu1 = a.stats[r];
+      n.rs1 = a.stats[a.rows + r];
     }
+    if (has_dn) {
+      n.mu2 = a.stats[2 * a.rows + r];
+      n.rs2 = a.stats[3 * a.rows + r];
+    }
+    if (!FULL && (a.gate_mode == MOC_GATE_SCALAR || a.gate_mode == MOC_GATE_TOKEN)) {
+      const int64_t at = a.gate_mode == MOC_GATE_TOKEN ? r : 0;
+      if (a.gate_dtype == MOC_F32) n.gate = ((const uint32_t*)a.gate)[at];
+      else n.gate = ((const uint16_t*)a.gate)[at];
+    }
+  };
+  // (every wave takes part in every round: the sums of a row over its waves synchronise the workgroup)
+  auto process = [&](const Row& cur, int64_t r) {
+    const bool live = r < a.rows;
+    const float mu1 = cur.mu1, rs1 = cur.rs1, mu2 = cur.mu2, rs2 = cur.rs2;
+    float grow = 1.f;   // (a bf16's bits are the upper half of the float's)
+    if (!FULL && (a.gate_mode == MOC_GATE_SCALAR || a.gate_mode == MOC_GATE_TOKEN))
+      grow = __uint_as_float(a.gate_dtype == MOC_F32 ? cur.gate : cur.gate << 16);
     auto gate_of = [&](int i, int e) {
-      if constexpr (FULL) return get<TX, VEC>(gv[i], e);
+      if constexpr (FULL) return get<TX, VEC>(cur.gv[i], e);
       else if constexpr (CHAN) return gc[i][e] * grow;   // (one of the two is 1)
       else return grow;
     };
@@ -278,17 +307,18 @@ __global__ __launch_bounds__(64 * W * RPB) void gated_norm_bwd_kernel(moc_gated_
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < KCH; ++i) {
-      const bool in = t + 64 * W * i < nch && live;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        xh[i][e] = hh[i][e] = g2[i][e] = 0.f;
-        if (in) {
-          xh[i][e] = (get<TX, VEC>(xv[i], e) - mu1) * rs1;
-          if (has_dn) {
+      for (int e = 0; e < VEC; ++e) xh[i][e] = hh[i][e] = g2[i][e] = 0.f;
+      if (t + 64 * W * i < nch && live) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) xh[i][e] = (get<TX, VEC>(cur.xv[i], e) - mu1) * rs1;
+        if (has_dn) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
             const float u = xh[i][e] * w1[i][e] + b1[i][e];
-            const float h = a.alpha * get<TR, VEC>(rv[i], e) + gate_of(i, e) * u;
+            const float h = a.alpha * get<TR, VEC>(cur.rv[i], e) + gate_of(i, e) * u;
             hh[i][e] = (h - mu2) * rs2;
-            const float dn = get<TX, VEC>(nv[i], e);
+            const float dn = get<TX, VEC>(cur.nv[i], e);
             dw2[i][e] += dn * hh[i][e];
             if constexpr (BIAS) db2[i][e] += dn;
             g2[i][e] = dn * w2[i][e];
@@ -301,20 +331,29 @@ __global__ __launch_bounds__(64 * W * RPB) void gated_norm_bwd_kernel(moc_gated_
     if (has_dn) row_sum<W, 2>(s, red, wave);
     const float c0 = layer2 ? s[0] * inv_d : 0.f, c1 = s[1] * inv_d;
     float p[3] = {0.f, 0.f, 0.f};
-    // hh becomes g1 = du w1
+    // g2 becomes dH, hh becomes g1 = du w1
 #pragma unroll
     for (int i = 0; i < KCH; ++i) {
       const int c = t + 64 * W * i;
       if (c >= nch || !live) continue;
-      float dr[VEC], dg[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) g2[i][e] = rs2 * (g2[i][e] - c0 - hh[i][e] * c1);
+      if (o.dh) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) g2[i][e] += get<TR, VEC>(cur.hv[i], e);
+      }
+      if (o.dres) {
+        float dr[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) dr[e] = a.alpha * g2[i][e];
+        store<TR, VEC>(o.dres, r * d + VEC * c, dr);
+      }
+      float dg[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        float dH = rs2 * (g2[i][e] - c0 - hh[i][e] * c1);
-        if (o.dh) dH += get<TR, VEC>(hv[i], e);
-        dr[e] = a.alpha * dH;
-        dg[e] = dH * (xh[i][e] * w1[i][e] + b1[i][e]);
+        dg[e] = g2[i][e] * (xh[i][e] * w1[i][e] + b1[i][e]);
         p[2] += dg[e];
-        const float du = gate_of(i, e) * dH;
+        const float du = gate_of(i, e) * g2[i][e];
         if constexpr (CHAN) dgc[i][e] += dg[e];
         dw1[i][e] += du * xh[i][e];
         if constexpr (BIAS) db1[i][e] += du;
@@ -322,7 +361,6 @@ __global__ __launch_bounds__(64 * W * RPB) void gated_norm_bwd_kernel(moc_gated_
         p[0] += hh[i][e];
         p[1] += hh[i][e] * xh[i][e];
       }
-      if (o.dres) store<TR, VEC>(o.dres, r * d + VEC * c, dr);
       if constexpr (FULL) {
         if (o.dgate) store<TX, VEC>(o.dgate, r * d + VEC * c, dg);
       }
@@ -345,6 +383,20 @@ __global__ __launch_bounds__(64 * W * RPB) void gated_norm_bwd_kernel(moc_gated_
         store<TX, VEC>(o.dx, r * d + VEC * c, dx);
       }
     }
+  };
+  // two rows' operands in turn: a copy from one to the other would wait for the loads
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t r0 = (int64_t)blockIdx.x * RPB;
+  Row even, odd;
+  fetch(even, r0 + grp);
+  while (r0 < a.rows) {
+    fetch(odd, r0 + step + grp);
+    process(even, r0 + grp);
+    r0 += step;
+    if (r0 >= a.rows) break;
+    fetch(even, r0 + step + grp);
+    process(odd, r0 + grp);
+    r0 += step;
   }
   // the strip's column sums; several row groups add theirs through LDS, in order
   const int64_t strip = blockIdx.x;
@@ -393,7 +445,8 @@ __global__ __launch_bounds__(64 * W * RPB) void gated_norm_bwd_kernel(moc_gated_
   }
 }
 
-// Shapes.  Forward, eight per load: one wave up to 1,024 elements, four up to 8,192, sixteen up to 16,384.
+// Shapes.  Forward, eight per load: one wave up to 512 elements, two up to 1,024 (8,192 x 768: 15.8 us, one wave with two
+// loads per lane 18.3), four up to 4,096 (6,123 x 4,096 with two loads per lane: 38.5 us, eight waves 41.9).
 template <typename TX, typename TR, int VEC, int W, int KCH> int fwd_shape(const moc_gated_norm& a, hipStream_t stream) {
   const dim3 grid((unsigned)(W == 1 ? (a.rows + 3) / 4 : a.rows)), block(W == 1 ? 256 : 64 * W);
   if (a.gate_mode == MOC_GATE_FULL)
@@ -406,7 +459,7 @@ template <typename TX, typename TR> int fwd_types(const moc_gated_norm& a, bool 
   const int64_t d = a.d;
   if (vec) {
     if (d <= 512) return fwd_shape<TX, TR, 8, 1, 1>(a, s);
-    if (d <= 1024) return fwd_shape<TX, TR, 8, 1, 2>(a, s);
+    if (d <= 1024) return fwd_shape<TX, TR, 8, 2, 1>(a, s);
     if (d <= 2048) return fwd_shape<TX, TR, 8, 4, 1>(a, s);
     if (d <= 4096) return fwd_shape<TX, TR, 8, 4, 2>(a, s);
     if (d <= 8192) return fwd_shape<TX, TR, 8, 16, 1>(a, s);
@@ -442,16 +495,16 @@ template <typename TX, typename TR>
 int bwd_types(const moc_gated_norm& a, const moc_gated_norm_grads& g, bool vec, const GnStrips& s, hipStream_t st) {
   const int w = gn_bwd_waves(a.d, vec);
   if (vec) {
-    if (w == 1) return bwd_shape<TX, TR, 8, 1, 8, 1>(a, g, s, st);
-    if (w == 2) return bwd_shape<TX, TR, 8, 2, 4, 1>(a, g, s, st);
-    if (w == 4) return bwd_shape<TX, TR, 8, 4, 1, 1>(a, g, s, st);
+    if (w == 1) return bwd_shape<TX, TR, 8, 1, kGnWaves, 1>(a, g, s, st);
+    if (w == 2) return bwd_shape<TX, TR, 8, 2, kGnWaves / 2, 1>(a, g, s, st);
+    if (w == 4) return bwd_shape<TX, TR, 8, 4, kGnWaves / 4, 1>(a, g, s, st);
     if (w == 8) return bwd_shape<TX, TR, 8, 8, 1, 1>(a, g, s, st);
     if (a.d <= 8192) return bwd_shape<TX, TR, 8, 16, 1, 1>(a, g, s, st);
     return bwd_shape<TX, TR, 8, 16, 1, 2>(a, g, s, st);
   }
-  if (w == 1) return bwd_shape<TX, TR, 1, 1, 8, 4>(a, g, s, st);
-  if (w == 2) return bwd_shape<TX, TR, 1, 2, 4, 4>(a, g, s, st);
-  if (w == 4) return bwd_shape<TX, TR, 1, 4, 1, 4>(a, g, s, st);
+  if (w == 1) return bwd_shape<TX, TR, 1, 1, kGnWaves, 4>(a, g, s, st);
+  if (w == 2) return bwd_shape<TX, TR, 1, 2, kGnWaves / 2, 4>(a, g, s, st);
+  if (w == 4) return bwd_shape<TX, TR, 1, 4, kGnWaves / 4, 4>(a, g, s, st);
   if (w == 8) return bwd_shape<TX, TR, 1, 8, 1, 4>(a, g, s, st);
   if (a.d <= 4096) return bwd_shape<TX, TR, 1, 16, 1, 4>(a, g, s, st);
   return bwd_shape<TX, TR, 1, 16, 1, 16>(a, g, s, st);

@@ -23,7 +23,6 @@ namespace moc {
 namespace {
 
 constexpr int kGnMaxD = 16384;
-constexpr int kGnMaxStrips = 512;   // two workgroups on every CU
 
 // grads[q][j] = sum over the strips: eight lanes of four columns each, 128 groups of strips, added in a fixed order.
 __global__ __launch_bounds__(1024) void gated_norm_cols_kernel(const float* __restrict__ part, int strips, int d, unsigned live,
@@ -59,9 +58,10 @@ __global__ __launch_bounds__(1024) void gated_norm_cols_kernel(const float* __re
   if (threadIdx.x < 32 && c < d) out[(int64_t)q * d + c] = buf[0][threadIdx.x];
 }
 
+// Strips (workgroups) of the backward: two waves on every SIMD, which is what its registers allow.
 int64_t gn_strips(int64_t rows, int64_t d, bool vec) {
-  const int rpb = gn_bwd_rows(gn_bwd_waves(d, vec));
-  return std::max<int64_t>(1, std::min<int64_t>((rows + rpb - 1) / rpb, kGnMaxStrips));
+  const int waves = gn_bwd_waves(d, vec), rpb = gn_bwd_rows(waves);
+  return std::max<int64_t>(1, std::min<int64_t>((rows + rpb - 1) / rpb, 2048 / (waves * rpb)));
 }
 
 int gn_check(const char* who, const moc_gated_norm* a) {
