@@ -14,8 +14,10 @@
 //   sigmoid: dz_j = ds_j s_j (1 - s_j) on the selected, 0 elsewhere
 //   softmax: dz_c = s_c (ds_c [selected] - sum_j ds_j s_j); the sum is 0 for renormalised weights.
 //
-// One workgroup per row, every key of the row in LDS as an ordered 64-bit integer: the k-th largest by eight
-// passes over bytes, then the selected in order.
+// Rows are held in registers by one wave, or by four where there are few; what does not fit them, or cannot be decided
+// from f32 keys with a few exact ones, goes to a workgroup with every exact key in LDS.
+#include <cfloat>
+
 #include <algorithm>
 
 #include "moc_common.h"
@@ -27,6 +29,7 @@ constexpr int kSelThreads = 256;
 constexpr int kSelMaxK = 1024;
 constexpr int kSelMaxG = 1024;
 constexpr int kSelMaxC = 16384;
+constexpr int64_t kSelFewRows = 1024;   // up to which four waves take a row
 
 // doubles (and NaN) to integers of the same order; 0 stays free for "not selectable"
 __device__ __forceinline__ uint64_t key64(double v) {
@@ -60,9 +63,10 @@ template <int NT> __device__ __forceinline__ double blk_sum(double v, double* re
   return s;
 }
 
-__global__ __launch_bounds__(kSelThreads) void router_select_kernel(SelArgs a) {
+// One row on a workgroup, any shape: every key of the row in LDS as an ordered 64-bit integer, the k-th largest by
+// eight passes over bytes, then the selected in order.  Every thread calls it.
+__device__ __forceinline__ void select_row(const SelArgs& a, int64_t r, char* lds) {
   constexpr int NT = kSelThreads;
-  extern __shared__ char lds[];
   uint64_t* keys = (uint64_t*)lds;                       // [n]
   uint64_t* gkey = keys + a.n;                           // [G]
   uint64_t* sel_key = gkey + a.G;                        // [k]
@@ -72,7 +76,6 @@ __global__ __launch_bounds__(kSelThreads) void router_select_kernel(SelArgs a) {
   __shared__ double red[NT / 64];
   __shared__ int hist[256];
   __shared__ int pick[4];
-  const int64_t r = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* z = a.z + r * a.ldz + a.S;
   const float* b = a.bias ? a.bias + a.S : nullptr;
@@ -82,11 +85,7 @@ __global__ __launch_bounds__(kSelThreads) void router_select_kernel(SelArgs a) {
   double m = 0.0, Z = 1.0;
   float mf = -INFINITY;
   if (!a.sigmoid) {
-    bool nan = false;
-    for (int c = tid; c < n; c += NT) {
-      nan |= z[c] != z[c];
-      mf = fmaxf(mf, z[c]);
-    }
+    for (int c = tid; c < n; c += NT) mf = fmaxf(mf, z[c]);
     mf = wave_max(mf);
     __syncthreads();
     if (lane == 0) red[wave] = mf;
@@ -230,6 +229,463 @@ __global__ __launch_bounds__(kSelThreads) void router_select_kernel(SelArgs a) {
   }
 }
 
+__global__ __launch_bounds__(kSelThreads) void router_select_kernel(SelArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  select_row(a, blockIdx.x, lds);
+}
+
+inline size_t select_row_lds(int n, int G, int k) { return (size_t)n * 8 + (size_t)G * 9 + (size_t)k * 16; }
+
+// --------------------------------------------------------- rows in registers
+// Rows of up to 64 * 72 (NW = 1) logits with k <= 64, and up to 64 groups: a team of NW waves holds the row's keys in
+// registers as f32, E per lane, a group's chapters on lanes of its own (four consecutive ones per load).
+//   1. keys in f32, within eps = kSelEps + 2^-24 |key| of the exact ones (the bound below); per lane the two largest, and four
+//      maxima (NW = 1; one for NW = 4): 256 per row.
+//   2. the groups' scores from the lanes' pairs; groups too close to the cut for these keys are scored again from
+//      exact keys of their few largest.
+//   3. t = a lower bound of the k-th largest of the 256 maxima: k keys are >= t.  With fewer live maxima than k, t by
+//      bisection over the keys themselves.
+//   4. every key >= t - 2 eps is a candidate (a few dozen; more than 256: select_row).  Only these are evaluated in
+//      f64 and ranked exactly.
+// Why no selected chapter is missed: k keys are >= t in f32, so the exact k-th largest is >= t - eps, and a chapter at
+// or above that has an f32 key >= t - 2 eps.
+// Error of the keys, with v_exp_f32 and v_rcp_f32 good to 1 ulp (2^-23).  Sigmoid: the argument z log2(e) is off by
+// 1.5 |z| 2^-24 (its rounding and the constant's), which moves s by |z| s (1 - s) 1.5 2^-24 < 0.34 2^-24; the exponential moves
+// it by s (1 - s) 2^-23 <= 0.5 2^-24; 1 + e and the reciprocal by 3 2^-24 s: below 4 2^-24 = 2^-22.  Softmax: the
+// argument is off by 3 2^-24 |z - m| (difference, product, constant), which moves p by |z - m| p 3 2^-24 <= 1.2 2^-24 with
+// p <= 1 (x e^-x <= 0.37), the exponential and 1 / Z by 2 2^-24 p each...: together below 2^-21.  The bias' addition
+// rounds by 2^-24 |key|.
+constexpr float kSelEps = 0x1p-21f;
+constexpr int kSelMaxima = 256;
+constexpr int kSelCand = 256;
+constexpr int kSelTeamK = 64;
+
+enum { kKeyLogit, kKeySigmoid, kKeySoftmax };
+
+template <int NW> struct SelTeam {
+  uint64_t key[kSelCand];
+  int32_t id[kSelCand];
+  uint32_t maxima[kSelMaxima];
+  float top[64 * NW][2];
+  double part[NW];
+  int count[NW];
+};
+
+__device__ __forceinline__ uint32_t key32(float v) {
+  const uint32_t u = __float_as_uint(v + 0.f);
+  return (u >> 31) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float key32_inv(uint32_t k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
+
+template <int NW> __device__ __forceinline__ void team_sync() {
+  if constexpr (NW == 1) wave_lds_sync();
+  else __syncthreads();
+}
+template <int NW> __device__ __forceinline__ double team_sum(double v, SelTeam<NW>& sm, int wave) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  if constexpr (NW > 1) {
+    team_sync<NW>();
+    if ((threadIdx.x & 63) == 0) sm.part[wave] = v;
+    team_sync<NW>();
+    v = 0.0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) v += sm.part[i];
+  }
+  return v;
+}
+template <int NW> __device__ __forceinline__ float team_max(float v, SelTeam<NW>& sm, int wave) {
+  v = wave_max(v);
+  if constexpr (NW > 1) {
+    team_sync<NW>();
+    if ((threadIdx.x & 63) == 0) sm.part[wave] = (double)v;
+    team_sync<NW>();
+#pragma unroll
+    for (int i = 0; i < NW; ++i) v = fmaxf(v, (float)sm.part[i]);
+  }
+  return v;
+}
+template <int NW> __device__ __forceinline__ int team_add(int v, SelTeam<NW>& sm, int wave) {
+  if constexpr (NW > 1) {
+    team_sync<NW>();
+    if ((threadIdx.x & 63) == 0) sm.count[wave] = v;
+    team_sync<NW>();
+    v = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) v += sm.count[i];
+  }
+  return v;
+}
+
+// bit 4 j + e: v[j][e] >= cut
+template <int E> __device__ __forceinline__ void lane_bits(const float (&v)[E / 4][4], float cut, uint32_t (&bits)[(E + 31) / 32]) {
+#pragma unroll
+  for (int i = 0; i < (E + 31) / 32; ++i) bits[i] = 0;
+#pragma unroll
+  for (int j = 0; j < E / 4; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bits[(4 * j + e) >> 5] |= (v[j][e] >= cut ? 1u : 0u) << ((4 * j + e) & 31);
+}
+
+// True where the row is done, false where select_row has to take it (the same in every lane of the team).
+template <int NW, int E, int MODE>
+__device__ __forceinline__ bool select_team(const SelArgs& a, int64_t r, SelTeam<NW>& sm, int tl) {
+  constexpr int TL = 64 * NW, E4 = E / 4, Q = 4 / NW;
+  const int lane = tl & 63, wave = tl >> 6;
+  const bool grouped = a.top < a.G;
+  const int Ge = grouped ? a.G : 1, per = a.n / Ge, lpg = TL / Ge;
+  const int grp = tl / lpg, pos = tl - grp * lpg;
+  const bool active = grp < Ge;
+  const int mine = active ? per : 0;   // chapters of the lane's group
+  const int c0 = grp * per;
+  const float* z = a.z + r * a.ldz + a.S;
+  const float* b = a.bias ? a.bias + a.S : nullptr;
+  typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+  float v[E4][4];
+#pragma unroll
+  for (int j = 0; j < E4; ++j) {
+    const int i = 4 * (pos + lpg * j);
+    if (i + 4 <= mine) {
+      const f32x4u t = __builtin_nontemporal_load(reinterpret_cast<const f32x4u*>(z + c0 + i));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j][e] = t[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j][e] = i + e < mine ? z[c0 + i + e] : -INFINITY;
+    }
+  }
+  // softmax statistics
+  float m = -INFINITY;
+  double Z = 1.0;
+  if (!a.sigmoid) {
+#pragma unroll
+    for (int j = 0; j < E4; ++j) m = fmaxf(m, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
+    m = team_max<NW>(m, sm, wave);
+    if (!(m > -INFINITY && m < INFINITY)) return false;
+    double s = 0.0;
+#pragma unroll
+    for (int j = 0; j < E4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = __builtin_amdgcn_exp2f((v[j][e] - m) * 1.4426950408889634f);
+        s += (double)p;
+        if constexpr (MODE == kKeySoftmax) v[j][e] = v[j][e] == -INFINITY ? -INFINITY : p;
+      }
+    Z = team_sum<NW>(s, sm, wave);
+    if (a.row_stats && tl == 0) {
+      a.row_stats[2 * r] = m;
+      a.row_stats[2 * r + 1] = (float)Z;
+    }
+  }
+  // keys
+  if constexpr (MODE != kKeyLogit) {
+    const float rz = MODE == kKeySoftmax ? (float)(1.0 / Z) : 1.f;
+#pragma unroll
+    for (int j = 0; j < E4; ++j) {
+      float w[4] = {0.f, 0.f, 0.f, 0.f};
+      const int i = 4 * (pos + lpg * j);
+      if (b) {
+        if (i + 4 <= mine) {
+          const f32x4u t = *reinterpret_cast<const f32x4u*>(b + c0 + i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = t[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = i + e < mine ? b[c0 + i + e] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = v[j][e];
+        float s;
+        if constexpr (MODE == kKeySigmoid) s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
+        else s = x * rz;
+        v[j][e] = x == -INFINITY ? -INFINITY : s + w[e];
+      }
+    }
+  }
+  // the lane's maxima (NaN stays in them) and its two largest keys
+  float mx[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    mx[e] = v[0][e];
+#pragma unroll
+    for (int j = 1; j < E4; ++j) mx[e] = fmax_fast(mx[e], v[j][e]);
+  }
+  float k1 = fmax_fast(fmax_fast(mx[0], mx[1]), fmax_fast(mx[2], mx[3]));
+  const bool odd = !(k1 < INFINITY);   // NaN or infinity
+  if (team_add<NW>(__popcll(__ballot(odd)), sm, wave) != 0) return false;
+  uint64_t keep = ~0ull;
+  if (grouped) {
+    float k2 = -INFINITY;
+    if (a.best == 2) {
+      k1 = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < E4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          k2 = __builtin_amdgcn_fmed3f(k1, k2, v[j][e]);
+          k1 = fmaxf(k1, v[j][e]);
+        }
+    }
+    sm.top[tl][0] = k1;
+    sm.top[tl][1] = k2;
+    team_sync<NW>();
+    // (every wave for itself) lane g: group g's score, its rank, and how clear the cut is
+    float g1 = -INFINITY, g2 = -INFINITY;
+    if (lane < Ge) {
+      for (int i = 0; i < lpg; ++i) {
+        const float t1 = sm.top[lane * lpg + i][0], t2 = sm.top[lane * lpg + i][1];
+        g2 = fmaxf(__builtin_amdgcn_fmed3f(g1, g2, t1), t2);
+        g1 = fmaxf(g1, t1);
+      }
+    }
+    const float sc = a.best == 2 && g2 > -INFINITY ? g1 + g2 : g1;
+    int rank = 0;
+    for (int i = 0; i < Ge; ++i) {
+      const float o = __shfl(sc, i, 64);
+      rank += o > sc || (o == sc && i < lane);
+    }
+    const bool in = lane < Ge;
+    keep = __ballot(in && rank < a.top);
+    if constexpr (MODE != kKeyLogit) {
+      // groups whose score is within the errors of the last one kept and the first one dropped are scored again
+      // from exact keys: of those, the best by (score, lower group) stay
+      const float last = __shfl(sc, __builtin_ctzll(__ballot(in && rank == a.top - 1)), 64);
+      const float first = __shfl(sc, __builtin_ctzll(__ballot(in && rank == a.top)), 64);
+      // (the error of a score: two keys and their sum)
+      float err = in && sc > -INFINITY ? 0x1p-24f * (fabsf(g1) + (g2 > -INFINITY ? fabsf(g2) : 0.f) + fabsf(sc)) : 0.f;
+      err = 2.f * kSelEps + wave_max(err);
+      if (!(last - first > 2.f * err)) {
+        if (!(first > -INFINITY)) return false;
+        const uint64_t near = __ballot(in && sc >= first - 2.f * err && sc <= last + 2.f * err);
+        const uint64_t sure = __ballot(in && sc > last + 2.f * err);
+        uint64_t score = 0;   // lane g: group g's exact score, ordered
+        for (uint64_t todo = near; todo; todo &= todo - 1) {
+          const int g = __builtin_ctzll(todo);
+          const float lo = __shfl(a.best == 2 ? g2 : g1, g, 64);
+          const float cut = lo - 2.f * (kSelEps + 0x1p-24f * fabsf(lo));
+          uint64_t e1 = 0, e2 = 0;   // the lane's two largest exact keys of the group
+          if (active && grp == g) {
+            uint32_t bits[(E + 31) / 32];
+            lane_bits<E>(v, fmaxf(cut, -FLT_MAX), bits);
+#pragma unroll
+            for (int i = 0; i < (E + 31) / 32; ++i)
+              for (uint32_t w = bits[i]; w; w &= w - 1) {
+                const int q = 32 * i + __builtin_ctz(w), c = c0 + 4 * (pos + lpg * (q >> 2)) + (q & 3);
+                const double x = (double)z[c];
+                const double s = a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - (double)m) / Z;
+                const uint64_t k = key64(s + (b ? (double)b[c] : 0.0));
+                e2 = k > e1 ? e1 : k > e2 ? k : e2;
+                e1 = k > e1 ? k : e1;
+              }
+          }
+#pragma unroll
+          for (int o = 32; o >= 1; o >>= 1) {
+            const uint64_t p1 = __shfl_xor((unsigned long long)e1, o, 64), p2 = __shfl_xor((unsigned long long)e2, o, 64);
+            const uint64_t low = min(e1, p1);
+            e1 = max(e1, p1);
+            e2 = max(low, max(e2, p2));
+          }
+          if constexpr (NW > 1) {
+            team_sync<NW>();
+            if (lane == 0) {
+              sm.key[2 * wave] = e1;
+              sm.key[2 * wave + 1] = e2;
+            }
+            team_sync<NW>();
+            e1 = e2 = 0;
+            for (int i = 0; i < 2 * NW; ++i) {
+              const uint64_t k = sm.key[i];
+              e2 = k > e1 ? e1 : k > e2 ? k : e2;
+              e1 = k > e1 ? k : e1;
+            }
+          }
+          const double s1 = key64_inv(e1);
+          if (lane == g) score = a.best == 1 || e2 == 0 ? e1 : key64(s1 + key64_inv(e2));
+        }
+        const int room = a.top - __popcll(sure);
+        int place = 0;
+        for (uint64_t todo = near; todo; todo &= todo - 1) {
+          const int g = __builtin_ctzll(todo);
+          const uint64_t o = __shfl((unsigned long long)score, g, 64);
+          place += o > score || (o == score && g < lane);
+        }
+        keep = sure | __ballot((near >> lane & 1) && place < room);
+      }
+    }
+  }
+  const bool live = active && (keep >> (grp & 63) & 1) != 0;
+  // (maxima of live lanes that hold chapters)
+  const int maxima = (grouped ? a.top : 1) * (Q == 4 ? min(4 * lpg, per) : min(lpg, (per + 3) / 4));
+  uint32_t T = 0;
+  if (maxima >= a.k) {
+    if constexpr (Q == 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e] = live ? __uint_as_float(key32(mx[e])) : 0.f;
+    } else {
+      sm.maxima[tl] = live ? key32(fmax_fast(fmax_fast(mx[0], mx[1]), fmax_fast(mx[2], mx[3]))) : 0u;
+      team_sync<NW>();
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sm.maxima[lane + 64 * e]);
+    }
+    // (the low byte is left out: t may lie a little below the k-th maximum)
+    for (int bit = 31; bit >= 8; --bit) {
+      const uint32_t t = T | 1u << bit;
+      int cnt = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) cnt += __popcll(__ballot(__float_as_uint(mx[e]) >= t));
+      if (cnt >= a.k) {
+        T = t;
+        if (cnt == a.k) break;
+      }
+    }
+  } else {
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t t = T | 1u << bit;
+      const float tf = key32_inv(t);
+      int cnt = 0;
+      if (live && t > 0x007fffffu) {
+#pragma unroll
+        for (int j = 0; j < E4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) cnt += v[j][e] >= tf;
+      }
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) cnt += __shfl_xor(cnt, o, 64);
+      cnt = team_add<NW>(cnt, sm, wave);
+      if (cnt >= a.k) {
+        T = t;
+        if (cnt <= 2 * a.k + 32) break;
+      }
+    }
+  }
+  if (T <= 0x007fffffu) return false;   // fewer than k keys above -inf
+  const float t0 = key32_inv(T), thr = MODE == kKeyLogit ? t0 : t0 - 2.f * (kSelEps + 0x1p-24f * fabsf(t0));
+  // candidates: the lane's as bits, then a list in lane order
+  uint32_t bits[(E + 31) / 32];
+  lane_bits<E>(v, thr, bits);
+  int cnt = 0;
+#pragma unroll
+  for (int i = 0; i < (E + 31) / 32; ++i) {
+    bits[i] = live ? bits[i] : 0u;
+    cnt += __popc(bits[i]);
+  }
+  int at = cnt;   // inclusive sum over the lanes
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int t = __shfl_up(at, o, 64);
+    if (lane >= o) at += t;
+  }
+  int ncand = __shfl(at, 63, 64);
+  at -= cnt;
+  if constexpr (NW > 1) {
+    team_sync<NW>();
+    if (lane == 0) sm.count[wave] = ncand;
+    team_sync<NW>();
+    ncand = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      at += i < wave ? sm.count[i] : 0;
+      ncand += sm.count[i];
+    }
+  }
+  if (ncand > kSelCand) return false;
+#pragma unroll
+  for (int i = 0; i < (E + 31) / 32; ++i) {
+    uint32_t w = bits[i];
+    while (w) {
+      const int q = 32 * i + __builtin_ctz(w);
+      w &= w - 1;
+      sm.id[at++] = c0 + 4 * (pos + lpg * (q >> 2)) + (q & 3);
+    }
+  }
+  team_sync<NW>();
+  // exact keys of the candidates
+  constexpr int NC = kSelCand / TL;
+  uint64_t key[NC];
+  double sc[NC];
+  int32_t id[NC];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    key[i] = 0;
+    sc[i] = 0.0;
+    id[i] = 0;
+    const int p = tl + TL * i;
+    if (p < ncand) {
+      id[i] = sm.id[p];
+      const float x = z[id[i]];
+      if (MODE != kKeyLogit || NC == 1) sc[i] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x)) : exp((double)x - (double)m) / Z;
+      key[i] = key64(MODE == kKeyLogit ? (double)x : sc[i] + (b ? (double)b[id[i]] : 0.0));
+      sm.key[p] = key[i];
+    }
+  }
+  team_sync<NW>();
+  int rank[NC];
+  bool unclear = false;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    rank[i] = kSelCand;
+    if (TL * i < ncand) {   // (the same in every lane)
+      int rk = 0;
+      for (int j = 0; j < ncand; ++j) {
+        const uint64_t kj = sm.key[j];
+        const int32_t ij = sm.id[j];
+        rk += kj > key[i] || (kj == key[i] && ij < id[i]);
+        if constexpr (MODE == kKeySoftmax) {
+          // Z is off by up to 2^-21, which moves a pair of keys by as much of their scores' difference
+          const double gap = fabs(key64_inv(kj) - key64_inv(key[i]));
+          unclear |= tl + TL * i < ncand && ij != id[i] && gap <= 0x1p-20 * sc[i] && z[ij] != z[id[i]];
+        }
+      }
+      if (tl + TL * i < ncand) rank[i] = rk;
+    }
+  }
+  if constexpr (MODE == kKeySoftmax) {
+    if (team_add<NW>(__popcll(__ballot(unclear)), sm, wave) != 0) return false;
+  }
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    if (MODE == kKeyLogit && NC > 1 && rank[i] < a.k) {
+      const float x = z[id[i]];
+      sc[i] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x)) : exp((double)x - (double)m) / Z;
+    }
+    sum += rank[i] < a.k ? sc[i] : 0.0;
+  }
+  sum = team_sum<NW>(sum, sm, wave);
+  const double f = (double)a.scale / (a.renorm ? fmax(sum, 1e-12) : 1.0);
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+    if (rank[i] < a.k) {
+      const int64_t o = r * a.k + rank[i];
+      a.idx[o] = id[i] + a.S;
+      a.w[o] = (float)(sc[i] * f);
+      if (a.s_sel) a.s_sel[o] = (float)sc[i];
+    }
+  return true;
+}
+
+// Four waves: four rows (NW = 1) or one (NW = 4); rows that select_team leaves are then taken by the whole workgroup.
+template <int NW, int E, int MODE>
+__global__ __launch_bounds__(kSelThreads) void router_select_team_kernel(SelArgs a) {
+  constexpr int kTeams = 4 / NW;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ int left[kTeams];
+  SelTeam<NW>* teams = (SelTeam<NW>*)lds;
+  const int team = NW == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const int tl = NW == 1 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
+  const int64_t r0 = (int64_t)blockIdx.x * kTeams, r = r0 + team;
+  const bool done = r >= a.R || select_team<NW, E, MODE>(a, r, teams[team], tl);
+  if (tl == 0) left[team] = !done;
+  __syncthreads();
+  for (int t = 0; t < kTeams; ++t)
+    if (left[t]) {
+      select_row(a, r0 + t, lds);
+      __syncthreads();
+    }
+}
+
 struct SelBwdArgs {
   const float *z, *dw, *s_sel, *row_stats;
   const int32_t* idx;
@@ -307,6 +763,46 @@ __global__ __launch_bounds__(1024) void balance_update_kernel(const int32_t* __r
   }
 }
 
+template <int NW, int E> int select_team_launch(const SelArgs& a, int mode, hipStream_t stream) {
+  const size_t lds = std::max(sizeof(SelTeam<NW>) * (4 / NW), select_row_lds(a.n, a.G, a.k));
+  const dim3 grid((unsigned)((a.R + 4 / NW - 1) / (4 / NW)));
+  if (mode == kKeyLogit)
+    hipLaunchKernelGGL((router_select_team_kernel<NW, E, kKeyLogit>), grid, dim3(kSelThreads), lds, stream, a);
+  else if (mode == kKeySigmoid)
+    hipLaunchKernelGGL((router_select_team_kernel<NW, E, kKeySigmoid>), grid, dim3(kSelThreads), lds, stream, a);
+  else
+    hipLaunchKernelGGL((router_select_team_kernel<NW, E, kKeySoftmax>), grid, dim3(kSelThreads), lds, stream, a);
+  return check_launch("router_select_team_kernel");
+}
+
+int select_launch(const SelArgs& a, hipStream_t stream) {
+  const bool grouped = a.top < a.G;
+  const int Ge = grouped ? a.G : 1;
+  // a group's score adds two keys: scores are needed then, or where a bias is added to them
+  const int mode = !a.bias && (!grouped || a.best == 1) ? kKeyLogit : a.sigmoid ? kKeySigmoid : kKeySoftmax;
+  const int NW = a.R <= kSelFewRows ? 4 : 1;
+  // elements per lane: four consecutive chapters of the lane's group per load
+  const int lanes = 64 * NW / std::max(Ge, 1);
+  const int e = lanes > 0 ? 4 * ((a.n / Ge + 4 * lanes - 1) / (4 * lanes)) : 1 << 30;
+  if (a.k <= kSelTeamK && Ge <= 64 && e <= (NW == 1 ? 72 : 24)) {
+    if (NW == 4) {
+      if (e <= 4) return select_team_launch<4, 4>(a, mode, stream);
+      if (e <= 16) return select_team_launch<4, 16>(a, mode, stream);
+      return select_team_launch<4, 24>(a, mode, stream);
+    }
+    if (e <= 4) return select_team_launch<1, 4>(a, mode, stream);
+    if (e <= 16) return select_team_launch<1, 16>(a, mode, stream);
+    if (e <= 32) return select_team_launch<1, 32>(a, mode, stream);
+    if (e <= 64) return select_team_launch<1, 64>(a, mode, stream);
+    return select_team_launch<1, 72>(a, mode, stream);
+  }
+  const size_t lds = select_row_lds(a.n, a.G, a.k);
+  if (lds > 65536)
+    MOC_HIP(hipFuncSetAttribute((const void*)router_select_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  hipLaunchKernelGGL(router_select_kernel, dim3((unsigned)a.R), dim3(kSelThreads), lds, stream, a);
+  return check_launch("router_select_kernel");
+}
+
 }  // namespace
 }  // namespace moc
 
@@ -334,10 +830,7 @@ int moc_router_select(const float* logits, int64_t ldz, int64_t R, int64_t C, in
   MOC_REQUIRE(logits && idx && w, MOC_ERR_ARG, "moc_router_select: null pointer");
   SelArgs a{logits, bias, R, ldz, (int)n, S, k, score == MOC_SCORE_SIGMOID, groups, top_groups, group_best,
             renormalize != 0, scale, idx, w, s_sel, row_stats};
-  const size_t lds = (size_t)n * 8 + (size_t)groups * 9 + (size_t)k * 16;
-  MOC_HIP(hipFuncSetAttribute((const void*)router_select_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  hipLaunchKernelGGL(router_select_kernel, dim3((unsigned)R), dim3(kSelThreads), lds, stream, a);
-  return check_launch("router_select_kernel");
+  return select_launch(a, stream);
 }
 
 int moc_router_select_bwd(const float* logits, int64_t ldz, const int32_t* idx, const float* s_sel, const float* row_stats,

@@ -115,7 +115,23 @@ def test_sizes(gpu_device, R, C, S, k, G, g, score):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("R", [5, 300])
+@pytest.mark.parametrize("C,S,k,G,g", [(4097, 1, 16, 8, 4), (4097, 1, 64, 1, 1), (4097, 1, 64, 16, 1), (4609, 1, 33, 64, 20),
+                                       (257, 1, 8, 1, 1), (65, 1, 64, 1, 1), (301, 1, 20, 3, 1), (4096, 0, 5, 2, 1),
+                                       (1366 * 3 + 1, 1, 40, 3, 2), (130, 2, 64, 32, 16), (2049, 1, 64, 4, 1), (17, 1, 16, 1, 1)])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_many_rows(gpu_device, C, S, k, G, g, score):
+    """More rows than four waves each are taken for: one wave per row, in registers."""
+    R = 1030
+    g0 = gen(C + k)
+    z = torch.randn(R, C, generator=g0) * 0.55
+    bias = torch.randn(C, generator=g0) * 0.02
+    compare(z, k, S, gpu_device, 2, bias, score, G, g, 2, True, 1.0)
+    compare(z, k, S, gpu_device, 3, None, score, G, g, 1, False, 1.0)
+    compare(z, k, S, gpu_device, 4, None, score, G, g, 2, True, 2.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [5, 300, 1100])
 @pytest.mark.parametrize("score,bias_on", [("sigmoid", True), ("softmax", True), ("sigmoid", False), ("softmax", False)])
 @pytest.mark.parametrize("G,g", [(1, 1), (8, 4)])
 def test_ties_and_near_ties(gpu_device, R, score, bias_on, G, g):
@@ -138,7 +154,7 @@ def test_ties_and_near_ties(gpu_device, R, score, bias_on, G, g):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("R", [7, 200])
+@pytest.mark.parametrize("R", [7, 200, 1100])
 @pytest.mark.parametrize("score", ["sigmoid", "softmax"])
 def test_masked_logits(gpu_device, R, score):
     """-inf masks a chapter: rows with fewer live chapters than k, whole groups masked, the lowest finite value."""
@@ -166,7 +182,7 @@ def test_nothing_left_and_not_a_number(gpu_device):
     """A row with every chapter masked names the first k: weight 0 (sigmoid) or NaN (softmax); NaN sorts first; both
     leave the other rows as they are."""
     from memory_amd import ops
-    for R in (6, 100):
+    for R in (6, 100, 1100):
         z = torch.randn(R, 300, generator=gen(1)).to(gpu_device)
         for score in ("sigmoid", "softmax"):
             i0, w0 = ops.router_select(z, 5, 1, score=score)
