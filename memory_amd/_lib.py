@@ -319,10 +319,13 @@ def require_gpu(*tensors: torch.Tensor) -> None:
                 f"{t.device}. There is no CPU fallback.")
 
 
-def require_one_device(*tensors: torch.Tensor) -> None:
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"expected tensors on one device, got {sorted(map(str, devices))}")
+def require_same_gpu(first: torch.Tensor, *tensors: torch.Tensor) -> None:
+    """require_gpu, and all on the first one's device."""
+    require_gpu(first, *tensors)
+    dev = first.device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"expected tensors on one device, got {dev} and {t.device}")
 
 
 _here = contextlib.nullcontext()

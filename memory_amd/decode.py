@@ -150,8 +150,7 @@ class MemoryDecodeCache:
         """A cache over already projected tiles [num_chapters][num_kv_heads][T][64] (keys, dims).  Tiles in
         float8_e4m3fn come with their scales [num_chapters][num_kv_heads], finite and not negative (checked here, which
         waits for the stream)."""
-        L.require_gpu(k_tiles, v_tiles, k_scale, v_scale)
-        L.require_one_device(k_tiles, v_tiles, k_scale, v_scale)
+        L.require_same_gpu(k_tiles, v_tiles, k_scale, v_scale)
         eight = k_tiles.dtype == FP8
         if k_tiles.dtype not in (torch.float32, torch.bfloat16, FP8) or v_tiles.dtype != k_tiles.dtype:
             raise ValueError("decode cache tiles must be float32, bfloat16 or float8_e4m3fn, both of one dtype")
@@ -424,11 +423,10 @@ def decode_attention(q: torch.Tensor, cache: MemoryDecodeCache, routing: DecodeR
     """q (B, H, 64) -> attention output (B, H, 64) over the routed chapters (joint softmax, omega-weighted), or for
     several query tokens of each sequence (B, L, H, 64) -> (B, L, H, 64).  The result has the cache's type, bfloat16
     over an 8-bit cache."""
-    L.require_gpu(q)
+    L.require_same_gpu(q, cache.k_tiles, routing.idx)
     if q.dim() not in (3, 4) or q.shape[-1] != 64 or q.shape[0] != routing.B or q.shape[-2] % cache.HK != 0:
         raise ValueError(f"queries of shape {tuple(q.shape)}: expected ({routing.B}, [tokens,] heads, 64) with heads a "
                          f"multiple of {cache.HK}")
-    L.require_one_device(q, cache.k_tiles, routing.idx)
     if routing.plan.num_chapters > cache.num_chapters:
         raise ValueError(f"routing over {routing.plan.num_chapters} chapters, cache of {cache.num_chapters}")
     Lq = q.shape[1] if q.dim() == 4 else 1

@@ -162,25 +162,29 @@ def router_topk(logits: torch.Tensor, k: int, exclude_prefix_chapters: int = 0):
 _SCORES = {"softmax": 0, "sigmoid": 1}
 
 
+def _router_select_forward(z, bias, cfg, trains):
+    k, S, score, groups, top_groups, best, renorm, scale = cfg
+    R, C = z.shape
+    dev = z.device
+    idx = torch.empty((R, k), device=dev, dtype=torch.int32)
+    w = torch.empty((R, k), device=dev, dtype=torch.float32)
+    # what a backward reads: the selected scores, and softmax's row statistics
+    kept = torch.empty(R * (k + (2 if score == 0 else 0)), device=dev, dtype=torch.float32) if trains else None
+    at = None if kept is None else kept.data_ptr()
+    with L.on_device(dev):
+        call("moc_router_select", z.data_ptr(), z.stride(0), R, C, S, k, score, ptr(bias), groups, top_groups, best, renorm,
+             scale, idx.data_ptr(), w.data_ptr(), at, at + 4 * R * k if trains and score == 0 else None, stream_ptr(dev))
+    return idx, w, kept
+
+
 class _RouterSelect(torch.autograd.Function):
     """router_select on (R, C) float32 rows (moc_router_select / _bwd)."""
 
     @staticmethod
-    def forward(ctx, z, bias, k, S, score, groups, top_groups, best, renorm, scale):
-        R, C = z.shape
-        dev = z.device
-        idx = torch.empty(R, k, device=dev, dtype=torch.int32)
-        w = torch.empty(R, k, device=dev, dtype=torch.float32)
-        s_sel = row_stats = None
-        if ctx.needs_input_grad[0]:
-            s_sel = torch.empty(R, k, device=dev, dtype=torch.float32)
-            if score == 0:
-                row_stats = torch.empty(R, 2, device=dev, dtype=torch.float32)
-        with L.on_device(dev):
-            call("moc_router_select", ptr(z), z.stride(0), R, C, S, k, score, ptr(bias), groups, top_groups, best, renorm,
-                 scale, ptr(idx), ptr(w), ptr(s_sel), ptr(row_stats), stream_ptr(dev))
-        ctx.save_for_backward(z, idx, s_sel, row_stats)
-        ctx.cfg = (k, S, score, renorm, scale)
+    def forward(ctx, z, bias, cfg):
+        idx, w, kept = _router_select_forward(z, bias, cfg, True)
+        ctx.save_for_backward(z, idx, kept)
+        ctx.cfg = cfg
         ctx.mark_non_differentiable(idx)
         ctx.set_materialize_grads(False)
         return idx, w
@@ -189,17 +193,19 @@ class _RouterSelect(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, _didx, dw):
         if dw is None:
-            return (None,) * 10
-        z, idx, s_sel, row_stats = ctx.saved_tensors
-        k, S, score, renorm, scale = ctx.cfg
+            return None, None, None
+        z, idx, kept = ctx.saved_tensors
+        k, S, score, _, _, _, renorm, scale = ctx.cfg
         R, C = z.shape
         dev = z.device
-        dw = dw.float().contiguous()
-        dz = torch.empty(R, C, device=dev, dtype=torch.float32)
+        if dw.dtype != torch.float32 or not dw.is_contiguous():
+            dw = dw.float().contiguous()
+        dz = torch.empty((R, C), device=dev, dtype=torch.float32)
+        at = kept.data_ptr()
         with L.on_device(dev):
-            call("moc_router_select_bwd", ptr(z), z.stride(0), ptr(idx), ptr(s_sel), ptr(row_stats), ptr(dw), R, C, S, k,
-                 score, renorm, scale, ptr(dz), stream_ptr(dev))
-        return (dz,) + (None,) * 9
+            call("moc_router_select_bwd", z.data_ptr(), z.stride(0), idx.data_ptr(), at, at + 4 * R * k if score == 0 else None,
+                 dw.data_ptr(), R, C, S, k, score, renorm, scale, dz.data_ptr(), stream_ptr(dev))
+        return dz, None, None
 
 
 def router_select(logits: torch.Tensor, k: int, exclude_prefix_chapters: int = 0, *, score: str = "softmax",
@@ -237,14 +243,16 @@ def router_select(logits: torch.Tensor, k: int, exclude_prefix_chapters: int = 0
         raise ValueError(f"k={k} of {g * (n // G)} selectable chapters")
     if bias is not None and bias.shape != (C,):
         raise ValueError(f"bias of shape {tuple(bias.shape)}, expected {(C,)}")
-    L.require_gpu(logits, bias)
-    L.require_one_device(logits, bias)
-    z = logits.float()
+    L.require_same_gpu(logits, bias)
+    z = logits if logits.dtype == torch.float32 else logits.float()
     if z.stride(1) != 1 or z.stride(0) < C:
         z = z.contiguous()
-    if bias is not None:
+    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
         bias = bias.detach().float().contiguous()
-    return _RouterSelect.apply(z, bias, k, S, _SCORES[score], G, g, best, bool(renormalize), float(scale))
+    cfg = (k, S, _SCORES[score], G, g, best, bool(renormalize), float(scale))
+    if z.requires_grad and torch.is_grad_enabled():
+        return _RouterSelect.apply(z, None if bias is None else bias.detach(), cfg)
+    return _router_select_forward(z, bias, cfg, False)[:2]
 
 
 def router_balance_(bias: torch.Tensor, idx: torch.Tensor, rate: float, exclude_prefix_chapters: int = 0) -> torch.Tensor:
@@ -256,8 +264,7 @@ def router_balance_(bias: torch.Tensor, idx: torch.Tensor, rate: float, exclude_
     C, S = bias.shape[0], int(exclude_prefix_chapters)
     if not 0 <= S < C:
         raise ValueError(f"exclude_prefix_chapters must be in [0, {C}), got {S}")
-    L.require_gpu(bias, idx)
-    L.require_one_device(bias, idx)
+    L.require_same_gpu(bias, idx)
     ids = idx.reshape(-1).to(torch.int32).contiguous()
     counts = torch.empty(C, device=bias.device, dtype=torch.int32)
     with L.on_device(bias.device):
@@ -687,62 +694,102 @@ def _gate_mode(gate: Optional[torch.Tensor], x: torch.Tensor) -> int:
                      f"{tuple(x.shape)}")
 
 
+def _gated_norm_args(x, r, gate, w1, b1, w2, b2, cfg, h, n, stats):
+    mode, norms, alpha, eps = cfg
+    d = x.shape[-1]
+    return _GatedNormArgs(x.data_ptr(), r.data_ptr(), ptr(gate), ptr(w1), ptr(b1), ptr(w2), ptr(b2), ptr(h), ptr(n),
+                          ptr(stats), x.numel() // d, d, L.dtype_code(x.dtype), L.dtype_code(r.dtype), mode,
+                          0 if gate is None else L.dtype_code(gate.dtype), *norms, w1 is not None, w2 is not None, alpha,
+                          *eps)
+
+
+def _gated_norm_forward(x, r, gate, w1, b1, w2, b2, cfg, trains):
+    h = torch.empty_like(r)
+    n = torch.empty_like(x) if w2 is not None else None
+    stats = torch.empty(4 * (x.numel() // x.shape[-1]), device=x.device, dtype=torch.float32) if trains else None
+    args = _gated_norm_args(x, r, gate, w1, b1, w2, b2, cfg, h, n, stats)
+    with L.on_device(x.device):
+        call("moc_gated_norm_fwd", ctypes.addressof(args), stream_ptr(x.device))
+    return h, n, stats
+
+
+@functools.lru_cache(maxsize=1024)
+def _gated_norm_workspace(rows: int, d: int) -> int:
+    """float32 elements of the backward's workspace."""
+    return L.query("moc_gated_norm_bwd_workspace", rows, d) // 4
+
+
 class _GatedResidualNorm(torch.autograd.Function):
-    """gated_residual_norm on 2-D rows (moc_gated_norm_fwd / _bwd).  The backward reads x and the residual again and
-    forms h from them in float32, so nothing of the forward but the rows' statistics is kept."""
+    """gated_residual_norm on contiguous rows (moc_gated_norm_fwd / _bwd).  The backward reads x and the residual again
+    and forms h from them in float32, so nothing of the forward but the rows' statistics is kept."""
 
     @staticmethod
-    def forward(ctx, x, r, gate, w1, b1, w2, b2, mode, norms, alpha, eps, trains):
-        R, d = x.shape
-        dev = x.device
-        h = torch.empty_like(r)
-        n = torch.empty_like(x) if w2 is not None else None
-        stats = torch.empty(4, R, device=dev, dtype=torch.float32) if trains else None
-        args = _GatedResidualNorm.args(x, r, gate, w1, b1, w2, b2, mode, norms, alpha, eps, h, n, stats)
-        with L.on_device(dev):
-            call("moc_gated_norm_fwd", ctypes.addressof(args), stream_ptr(dev))
-        if trains:
-            ctx.save_for_backward(x, r, gate, w1, b1, w2, b2, stats)
-            ctx.cfg = (mode, norms, alpha, eps)
+    def forward(ctx, x, r, gate, w1, b1, w2, b2, cfg):
+        h, n, stats = _gated_norm_forward(x, r, gate, w1, b1, w2, b2, cfg, True)
+        ctx.save_for_backward(x, r, gate, w1, b1, w2, b2, stats)
+        ctx.cfg = cfg
         ctx.set_materialize_grads(False)
         return (h, n) if n is not None else h
-
-    @staticmethod
-    def args(x, r, gate, w1, b1, w2, b2, mode, norms, alpha, eps, h, n, stats):
-        return _GatedNormArgs(ptr(x), ptr(r), ptr(gate), ptr(w1), ptr(b1), ptr(w2), ptr(b2), ptr(h), ptr(n), ptr(stats),
-                              x.shape[0], x.shape[1], L.dtype_code(x.dtype), L.dtype_code(r.dtype), mode,
-                              0 if gate is None else L.dtype_code(gate.dtype), *norms, w1 is not None, w2 is not None,
-                              alpha, *eps)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, dn=None):
         x, r, gate, w1, b1, w2, b2, stats = ctx.saved_tensors
-        mode, norms, alpha, eps = ctx.cfg
+        cfg = ctx.cfg
+        mode = cfg[0]
         need = ctx.needs_input_grad
         if dh is None and dn is None:
-            return (None,) * 12
-        R, d = x.shape
+            return (None,) * 8
+        d = x.shape[-1]
+        R = x.numel() // d
         dev = x.device
-        dh = None if dh is None else dh.contiguous()
-        dn = None if dn is None else dn.contiguous()
+        if dh is not None and not dh.is_contiguous():
+            dh = dh.contiguous()
+        if dn is not None and not dn.is_contiguous():
+            dn = dn.contiguous()
         dx = torch.empty_like(x) if need[0] else None
         dr = torch.empty_like(r) if need[1] else None
         dg = torch.empty_like(gate) if need[2] and mode in (_GATE_TOKEN, _GATE_FULL) else None
-        dp = (torch.empty if R else torch.zeros)(5 * d + 1, device=dev, dtype=torch.float32)
-        ws_bytes = L.query("moc_gated_norm_bwd_workspace", R, d)
-        ws = torch.empty(ws_bytes // 4, device=dev, dtype=torch.float32)
-        args = _GatedResidualNorm.args(x, r, gate, w1, b1, w2, b2, mode, norms, alpha, eps, None, None, stats)
-        out = _GatedNormGrads(ptr(dh), ptr(dn), ptr(dx), ptr(dr), ptr(dg), ptr(dp))
+        # the parameters' gradients and the workspace in one allocation (16-byte aligned parts)
+        n_par = (5 * d + 4) // 4 * 4
+        buf = torch.empty(n_par + _gated_norm_workspace(R, d), device=dev, dtype=torch.float32)
+        if R == 0:
+            buf.zero_()
+        args = _gated_norm_args(x, r, gate, w1, b1, w2, b2, cfg, None, None, stats)
+        at = buf.data_ptr()
+        out = _GatedNormGrads(ptr(dh), ptr(dn), ptr(dx), ptr(dr), ptr(dg), at)
         with L.on_device(dev):
-            call("moc_gated_norm_bwd", ctypes.addressof(args), ctypes.addressof(out), ptr(ws), ws_bytes, stream_ptr(dev))
+            call("moc_gated_norm_bwd", ctypes.addressof(args), ctypes.addressof(out), at + 4 * n_par, 4 * (buf.numel() - n_par),
+                 stream_ptr(dev))
+        dw1 = db1 = dw2 = db2 = None
+        if w1 is not None and need[3]:
+            dw1 = buf[:d]
+        if b1 is not None and need[4]:
+            db1 = buf[d:2 * d]
+        if dn is not None:
+            if w2 is not None and need[5]:
+                dw2 = buf[2 * d:3 * d]
+            if b2 is not None and need[6]:
+                db2 = buf[3 * d:4 * d]
         if need[2] and mode == _GATE_SCALAR:
-            dg = dp[5 * d:].to(gate.dtype).view(gate.shape)
+            dg = buf[5 * d:5 * d + 1].to(gate.dtype).view(gate.shape)
         elif need[2] and mode == _GATE_CHANNEL:
-            dg = dp[4 * d:5 * d]
-        col = [dp[i * d:(i + 1) * d] if t is not None and need[3 + i] and (i < 2 or dn is not None) else None
-               for i, t in enumerate((w1, b1, w2, b2))]
-        return (dx, dr, dg, *col, None, None, None, None, None)
+            dg = buf[4 * d:5 * d]
+        return dx, dr, dg, dw1, db1, dw2, db2, None
+
+
+def _f32_vector(t: Optional[torch.Tensor], d: int, name: str) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.dim() != 1 or t.shape[0] != d:
+        raise ValueError(f"{name} of shape {tuple(t.shape)}, expected {(d,)}")
+    if t.dtype != torch.float32:
+        t = t.float()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+_NORM_KINDS = {"rms": L.MOC_NORM_RMS, "layer": L.MOC_NORM_LAYERNORM}
+_ROWS = (torch.float32, torch.bfloat16)
 
 
 def gated_residual_norm(x: torch.Tensor, residual: torch.Tensor, *, post_weight: Optional[torch.Tensor] = None,
@@ -762,46 +809,45 @@ def gated_residual_norm(x: torch.Tensor, residual: torch.Tensor, *, post_weight:
     value, one per channel (d,), one per row (..., 1), or x's shape.  x and residual are float32 or bfloat16 (float16
     runs as float32) of one shape; everything in between is float32, h and n are rounded once each and n is the norm
     of the unrounded h.  Differentiable once in every tensor."""
-    pre_norm = norm if pre_norm is None else pre_norm
-    pre_eps = eps if pre_eps is None else pre_eps
-    codes = {"rms": L.MOC_NORM_RMS, "layer": L.MOC_NORM_LAYERNORM}
-    if norm not in codes or pre_norm not in codes:
+    kind, kind2 = _NORM_KINDS.get(norm), _NORM_KINDS.get(norm if pre_norm is None else pre_norm)
+    if kind is None or kind2 is None:
         raise ValueError(f"norm must be 'rms' or 'layer', got {norm!r}, {pre_norm!r}")
-    if x.shape != residual.shape or x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"x {tuple(x.shape)} and residual {tuple(residual.shape)} must be rows of one shape")
-    d = x.shape[-1]
+    shape, d = x.shape, x.shape[-1] if x.dim() else 0
+    if shape != residual.shape or d == 0:
+        raise ValueError(f"x {tuple(shape)} and residual {tuple(residual.shape)} must be rows of one shape")
     if post_weight is None and post_bias is not None or pre_weight is None and pre_bias is not None:
         raise ValueError("a bias needs the weight of its norm")
-    if norm == "rms" and post_bias is not None or pre_norm == "rms" and pre_bias is not None:
+    if kind == L.MOC_NORM_RMS and post_bias is not None or kind2 == L.MOC_NORM_RMS and pre_bias is not None:
         raise ValueError("RMSNorm has no bias")
-    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight),
-                    ("pre_bias", pre_bias)):
-        if t is not None and t.shape != (d,):
-            raise ValueError(f"{name} of shape {tuple(t.shape)}, expected {(d,)}")
+    w1, b1 = _f32_vector(post_weight, d, "post_weight"), _f32_vector(post_bias, d, "post_bias")
+    w2, b2 = _f32_vector(pre_weight, d, "pre_weight"), _f32_vector(pre_bias, d, "pre_bias")
     mode = _gate_mode(gate, x)
-    od = x.dtype if out_dtype is None else out_dtype
-    if any(not t.is_floating_point() for t in (x, residual)) or not od.is_floating_point:
-        raise ValueError(f"gated_residual_norm takes floating-point rows, got {x.dtype}, {residual.dtype}, {od}")
-    L.require_gpu(x, residual, gate, post_weight, post_bias, pre_weight, pre_bias)
-    L.require_one_device(x, residual, gate, post_weight, post_bias, pre_weight, pre_bias)
-    rd = residual.dtype
-    kt = torch.bfloat16 if x.dtype == torch.bfloat16 and (od == torch.bfloat16 or pre_weight is None) else torch.float32
-    x2 = x.reshape(-1, d).to(kt).contiguous()
-    r2 = residual.reshape(-1, d).to(rd if rd in (torch.float32, torch.bfloat16) else torch.float32).contiguous()
+    od, rd = x.dtype if out_dtype is None else out_dtype, residual.dtype
+    if not (x.is_floating_point() and residual.is_floating_point() and od.is_floating_point):
+        raise ValueError(f"gated_residual_norm takes floating-point rows, got {x.dtype}, {rd}, {od}")
+    L.require_same_gpu(x, residual, gate, w1, b1, w2, b2)
+    # the kernels' row types: bfloat16 only where x and n both have it
+    kt = torch.bfloat16 if x.dtype == torch.bfloat16 and (od == torch.bfloat16 or w2 is None) else torch.float32
+    x2 = x if x.dtype == kt else x.to(kt)
+    x2 = x2 if x2.is_contiguous() else x2.contiguous()
+    r2 = residual if rd in _ROWS else residual.float()
+    r2 = r2 if r2.is_contiguous() else r2.contiguous()
     if gate is not None:
         if mode == _GATE_FULL:
-            gate = gate.reshape(-1, d).to(kt)
-        elif mode == _GATE_CHANNEL or gate.dtype not in (torch.float32, torch.bfloat16):
+            gate = gate.to(kt)
+        elif mode == _GATE_CHANNEL or gate.dtype not in _ROWS:
             gate = gate.float()
-        gate = gate.reshape(-1) if mode == _GATE_TOKEN else gate
         gate = gate.contiguous()
-    w = [None if t is None else t.float().contiguous() for t in (post_weight, post_bias, pre_weight, pre_bias)]
-    trains = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, r2, gate, *w))
-    out = _GatedResidualNorm.apply(x2, r2, gate, *w, mode, (codes[norm], codes[pre_norm]), float(residual_scale),
-                                   (float(eps), float(pre_eps)), trains)
-    h, n = out if isinstance(out, tuple) else (out, None)
-    h = h.view(x.shape).to(rd)
-    return h, None if n is None else n.view(x.shape).to(od)
+    cfg = (mode, (kind, kind2), float(residual_scale), (float(eps), float(eps if pre_eps is None else pre_eps)))
+    if torch.is_grad_enabled() and (x2.requires_grad or r2.requires_grad or any(
+            t is not None and t.requires_grad for t in (gate, w1, b1, w2, b2))):
+        out = _GatedResidualNorm.apply(x2, r2, gate, w1, b1, w2, b2, cfg)
+        h, n = out if w2 is not None else (out, None)
+    else:
+        h, n, _ = _gated_norm_forward(x2, r2, gate, w1, b1, w2, b2, cfg, False)
+    if h.dtype != rd:
+        h = h.to(rd)
+    return h, n if n is None or n.dtype == od else n.to(od)
 
 
 class _NormLinear(torch.autograd.Function):
