@@ -21,6 +21,12 @@ constexpr int kC8Dh = 64;
 constexpr int kC8Tile = 64 * 64;   // elements (= bytes) of a tile
 constexpr float kC8Max = 448.f;    // largest e4m3 value
 
+// the maximum over the wave (NaN stays)
+__device__ __forceinline__ float wave_max_nan(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = fmax_fast(v, __shfl_xor(v, o, 64));
+  return v;
+}
 __device__ __forceinline__ float c8_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // eight e4m3 values (two words) as bf16, exact
@@ -31,6 +37,22 @@ __device__ __forceinline__ bf16x8 c8_widen(uint32_t a, uint32_t b) {
                        __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false),
                        __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true)};
   return __builtin_bit_cast(bf16x8, v);
+}
+
+typedef _Float16 f16;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+// the same as f16 (exact as well: e4m3 spans 2^-9 .. 448)
+__device__ __forceinline__ f16x8 c8_widen_f16(uint32_t a, uint32_t b) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  const f16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false),
+                      __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true),
+                      __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false),
+                      __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true)};
+  return __builtin_bit_cast(f16x8, v);
+}
+__device__ __forceinline__ void mma16(f32x4& c, const f16x8& a, const f16x8& b) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 // ------------------------------------------------------------------ quantising
@@ -102,8 +124,11 @@ __global__ __launch_bounds__(256) void cache8_pack_kernel(const T* __restrict__ 
 // ------------------------------------------------------------------ few queries: one wave per (chapter, kv head)
 // Each selected tile is read once however many sequences chose it (the chapter plan over the (sequence, slot) edges),
 // as decode.hip does.  Rows of a unit: edge, query token, head of the kv group; 16 at a time.
-//   S^T = K Q^T (lane = query row), softmax over the 64 keys, O^T = V^T P^T, normalised rows and their log-sum-exp
-// to part rows [edge][token][head][64]; moc_sparse_combine merges the slots.
+//   S^T = K Q^T (lane = query row), softmax over the 64 keys, O^T = V^T P^T, normalised rows to part rows
+// [edge][token][head][64] with their log-sum-exp and value factor omega vs; cache8_combine_kernel merges the slots.
+// Probabilities (at most 1) and part rows (averages of e4m3 values, at most 448) are rounded to f16, 2^-11 where bf16
+// would round by 2^-8 at the same bytes: with bf16 the result was 1.7 times as far from the exact one as its own
+// rounding.
 // Bound: HBM, or latency where the units are few.  Eight loads of 16 bytes per lane hold the whole tile pair.
 constexpr int kC8Waves = 4;
 
@@ -112,8 +137,8 @@ struct C8Unit {
   const uint8_t *k8, *v8;
   const float *ks, *vs, *omega;
   const int32_t *uniq, *n_uniq, *csr_off, *csr_edge, *row_tab;
-  bf16* o_part;
-  float* lse_part;
+  f16* o_part;
+  float2* lse_part;
   int64_t max_u;
   int L, H, HK, NS;
   float scale_log2;
@@ -128,7 +153,7 @@ __global__ __launch_bounds__(64 * kC8Waves) void cache8_unit_kernel(C8Unit a) {
   if (u >= a.max_u) return;
   const int G = a.H / a.HK, GL = G * a.L;
   // the first 16 rows' edges come with the plan entries, not after them
-  int eid = a.row_tab[u * 16 + min(c16 / GL, 15)];
+  const int eid = a.row_tab[u * 16 + c16 / GL];
   const int nu = a.n_uniq[0];
   const int64_t c = a.uniq[u];
   const int p0 = a.csr_off[u], cnt = a.csr_off[u + 1] - p0;
@@ -141,21 +166,39 @@ __global__ __launch_bounds__(64 * kC8Waves) void cache8_unit_kernel(C8Unit a) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) vw[i] = ld16(a.v8 + tile * kC8Tile + 64 * (16 * i + c16) + 16 * g);
   const float ks = a.ks[tile] * a.scale_log2, vs = a.vs[tile];
-  for (int r0 = 0; r0 < nrows; r0 += 16) {
-    const int r = r0 + c16;
-    if (r0 > 0) eid = r < nrows ? a.csr_edge[p0 + r / GL] : -1;
-    else if (r >= nrows) eid = -1;
-    bf16x8 qf[2] = {zero_frag<bf16>(), zero_frag<bf16>()};
-    int64_t row = -1;
-    float w = 1.f;
-    if (eid >= 0) {
-      const int rem = r % GL, l = rem / G, hq = hk * G + rem % G;
-      row = ((int64_t)eid * a.L + l) * a.H + hq;
-      w = a.omega[eid];
-      const bf16* qp = a.q + (((int64_t)(eid / a.NS) * a.L + l) * a.H + hq) * kC8Dh + 16 * g;
-      qf[0] = Load8<bf16, bf16>::run(qp);
-      qf[1] = Load8<bf16, bf16>::run(qp + 8);
+  // a row block's operands: its edges two blocks ahead, its queries one (a chapter that every sequence selects has many)
+  struct Rows {
+    bf16x8 qf[2];
+    int64_t row;
+    float w;
+  };
+  auto edge_of = [&](int r0) { return r0 + c16 < nrows ? a.csr_edge[p0 + (r0 + c16) / GL] : -1; };
+  auto fetch = [&](int r0, int e) {
+    Rows x;
+    x.qf[0] = x.qf[1] = zero_frag<bf16>();
+    x.row = -1;
+    x.w = 1.f;
+    if (e >= 0) {
+      const int rem = (r0 + c16) % GL, l = rem / G, hq = hk * G + rem % G;
+      x.row = ((int64_t)e * a.L + l) * a.H + hq;
+      x.w = a.omega[e];
+      const bf16* qp = a.q + (((int64_t)(e / a.NS) * a.L + l) * a.H + hq) * kC8Dh + 16 * g;
+      x.qf[0] = Load8<bf16, bf16>::run(qp);
+      x.qf[1] = Load8<bf16, bf16>::run(qp + 8);
     }
+    return x;
+  };
+  Rows cur = fetch(0, c16 < nrows ? eid : -1);
+  int ahead = nrows > 16 ? edge_of(16) : -1;
+  for (int r0 = 0; r0 < nrows; r0 += 16) {
+    Rows next = cur;
+    if (r0 + 16 < nrows) {   // (the same in every lane)
+      next = fetch(r0 + 16, ahead);
+      ahead = edge_of(r0 + 32);
+    }
+    const bf16x8 (&qf)[2] = cur.qf;
+    const int64_t row = cur.row;
+    const float w = cur.w;
     // S^T: lane = query row r0 + c16, keys 16 kb + 4 g + x; dims 16 g + 8 ks of both operands
     f32x4 st[4];
 #pragma unroll
@@ -172,14 +215,14 @@ __global__ __launch_bounds__(64 * kC8Waves) void cache8_unit_kernel(C8Unit a) {
     const float cf = w * ks;
     const float m = quad_max(mx) * cf;
     float ps = 0.f;
-    bf16x8 pf[2];
+    f16x8 pf[2];
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const float p = exp2f(st[kb][x] * cf - m);
+        const float p = c8_exp2(st[kb][x] * cf - m);
         ps += p;
-        pf[kb >> 1][4 * (kb & 1) + x] = (bf16)p;
+        pf[kb >> 1][4 * (kb & 1) + x] = (f16)p;
       }
     const float l = quad_sum(ps);
     // O^T: lane = query row, dims 16 db + 4 g + x
@@ -187,21 +230,86 @@ __global__ __launch_bounds__(64 * kC8Waves) void cache8_unit_kernel(C8Unit a) {
 #pragma unroll
     for (int db = 0; db < 4; ++db) {
       o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
-      mma(o[db], c8_widen(vw[db].w[0], vw[db].w[1]), pf[0]);
-      mma(o[db], c8_widen(vw[db].w[2], vw[db].w[3]), pf[1]);
+      mma16(o[db], c8_widen_f16(vw[db].w[0], vw[db].w[1]), pf[0]);
+      mma16(o[db], c8_widen_f16(vw[db].w[2], vw[db].w[3]), pf[1]);
     }
     if (row >= 0) {
-      const float f = w * vs / l;
-      bf16* op = a.o_part + row * kC8Dh;
+      const float inv = 1.f / l;
+      f16* op = a.o_part + row * kC8Dh;
 #pragma unroll
       for (int db = 0; db < 4; ++db) {
-        bf16x4 v;
+        f16x4 v;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) v[x] = (bf16)(o[db][x] * f);
-        *reinterpret_cast<bf16x4*>(op + 16 * db + 4 * g) = v;
+        for (int x = 0; x < 4; ++x) v[x] = (f16)(o[db][x] * inv);
+        *reinterpret_cast<f16x4*>(op + 16 * db + 4 * g) = v;
       }
-      if (g == 0) a.lse_part[row] = m + log2f(l);
+      if (g == 0) a.lse_part[row] = make_float2(m + __builtin_amdgcn_logf(l), w * vs);
     }
+    cur = next;
+  }
+}
+
+// out = sum_s 2^(lse_s - M) f_s o_s / sum_s 2^(lse_s - M) over a row's slots: one wave per row, lane s holding slot s's
+// statistics, eight lanes of 16 bytes per part row.  A skipped slot's entries were never written: its factor is 0 and what
+// was read of its row is dropped by a select.
+__global__ __launch_bounds__(256) void cache8_combine_kernel(const f16* __restrict__ o_part, const float2* __restrict__ lse_part,
+                                                             const int32_t* __restrict__ edge_u, int NS, int rpe, int64_t rows,
+                                                             bf16* __restrict__ out) {
+  const int lane = threadIdx.x & 63, sg = lane >> 3, ch = lane & 7;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int64_t e0 = row / rpe * NS;
+  const int r = (int)(row % rpe);
+  constexpr int kSlots = 72;   // of a round: nine loads per lane, all in flight before the statistics are used
+  float M = -INFINITY, den = 0.f;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < NS; s0 += kSlots) {
+    const int n = min(kSlots, NS - s0);
+    f16x8 v[kSlots / 8];
+#pragma unroll
+    for (int i = 0; i < kSlots / 8; ++i)
+      v[i] = 8 * i + sg < n ? *reinterpret_cast<const f16x8*>(o_part + ((e0 + s0 + 8 * i + sg) * rpe + r) * kC8Dh + 8 * ch) : f16x8{};
+    float2 st[2];   // slots lane and 64 + lane of the round
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int64_t e = e0 + s0 + lane + 64 * q;
+      st[q] = make_float2(-INFINITY, 0.f);
+      if (lane + 64 * q < n) {
+        const int u = edge_u[e];
+        const float2 t = lse_part[e * rpe + r];
+        if (u >= 0) st[q] = t;
+      }
+    }
+    const float Mn = fmax_fast(M, wave_max_nan(fmax_fast(st[0].x, st[1].x)));
+    const float scale = M == Mn ? 1.f : c8_exp2(M - Mn);   // (NaN passes)
+    float a[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float p = st[q].x == -INFINITY ? 0.f : c8_exp2(st[q].x - Mn);
+      den = (q == 0 ? den * scale : den) + p;
+      a[q] = st[q].x == -INFINITY ? 0.f : p * st[q].y;
+    }
+    M = Mn;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) acc[x] *= scale;
+#pragma unroll
+    for (int i = 0; i < kSlots / 8; ++i) {
+      const float aj = __shfl(8 * i < 64 ? a[0] : a[1], (8 * i + sg) & 63, 64);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) acc[x] += aj != 0.f ? aj * (float)v[i][x] : 0.f;
+    }
+  }
+  den = wave_sum(den);
+#pragma unroll
+  for (int o = 8; o < 64; o <<= 1)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) acc[x] += __shfl_xor(acc[x], o, 64);
+  if (lane < 8) {
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    bf16x8 v;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] = (bf16)(acc[x] * inv);
+    *reinterpret_cast<bf16x8*>(out + row * kC8Dh + 8 * lane) = v;
   }
 }
 
@@ -225,7 +333,7 @@ struct C8Prompt {
   float scale_log2;
 };
 
-__global__ __launch_bounds__(kC8Threads) void cache8_prompt_kernel(C8Prompt a) {
+__global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a) {
   using Tile = SwzTile<bf16, 64>;
   __shared__ __attribute__((aligned(16))) char sK[2][8192];
   __shared__ __attribute__((aligned(16))) char sV[2][8192];
@@ -426,16 +534,15 @@ int c8_splits(int64_t B, int64_t L, int H, int HK, int NS) {
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 struct C8Ws {
-  size_t o_part = 0, lse_part, lse, bytes;
+  size_t o_part = 0, lse_part, bytes;
   C8Ws(int64_t B, int64_t L, int H, int HK, int NS) {
     const size_t rows = (size_t)B * L * H;
     if (c8_units((int)L, H, HK)) {
       lse_part = up256(rows * NS * kC8Dh * 2);
-      lse = lse_part + up256(rows * NS * 4);
-      bytes = lse + up256(rows * 4);
+      bytes = lse_part + up256(rows * NS * 8);
     } else {
       const int ns = c8_splits(B, L, H, HK, NS);
-      lse_part = lse = ns > 1 ? up256(rows * ns * kC8Dh * 4) : 0;
+      lse_part = ns > 1 ? up256(rows * ns * kC8Dh * 4) : 0;
       bytes = ns > 1 ? lse_part + up256(rows * ns * 4) : 0;
     }
   }
@@ -496,15 +603,16 @@ int moc_cache8_attend(const moc_cache8_args* a, void* workspace, size_t workspac
     const int64_t units = a->max_u * a->HK;
     if (units > 0) {
       C8Unit k{(const bf16*)a->q, (const uint8_t*)a->k_tiles, (const uint8_t*)a->v_tiles, a->k_scale, a->v_scale, a->omega,
-               a->uniq, a->n_uniq, a->csr_off, a->csr_edge, a->row_tab, (bf16*)(ws + y.o_part), (float*)(ws + y.lse_part),
+               a->uniq, a->n_uniq, a->csr_off, a->csr_edge, a->row_tab, (f16*)(ws + y.o_part), (float2*)(ws + y.lse_part),
                a->max_u, (int)a->L, a->H, a->HK, a->NS, sl2};
       hipLaunchKernelGGL(cache8_unit_kernel, dim3((unsigned)((units + kC8Waves - 1) / kC8Waves)), dim3(64 * kC8Waves), 0,
                          stream, k);
       if (int rc = check_launch("cache8_unit_kernel")) return rc;
     }
-    const int rpe = (int)(a->L * a->H);
-    return moc_sparse_combine(MOC_BF16, ws + y.o_part, (const float*)(ws + y.lse_part), a->edge_u, nullptr, 1, a->NS, rpe, a->B,
-                              rpe, 0, a->out, (float*)(ws + y.lse), stream);
+    const int64_t rows = a->B * a->L * a->H;
+    hipLaunchKernelGGL(cache8_combine_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, (const f16*)(ws + y.o_part),
+                       (const float2*)(ws + y.lse_part), a->edge_u, a->NS, (int)(a->L * a->H), rows, (bf16*)a->out);
+    return check_launch("cache8_combine_kernel");
   }
   const int nsplit = c8_splits(a->B, a->L, a->H, a->HK, a->NS);
   const int64_t nqb = (a->L * (a->H / a->HK) + 127) / 128, tiles = a->B * a->HK * nsplit * nqb;

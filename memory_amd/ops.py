@@ -14,10 +14,20 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
+from torch.autograd import function as autograd_function
 
 from . import _lib as L
 from ._lib import call, ptr, stream_ptr
+
+
+def once_differentiable(backward):
+    """torch's once_differentiable, which a backward that is not itself recorded does not go through (3 us)."""
+    recorded = autograd_function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def recorded_backward(fn, inputs, needs, grad_outputs):

@@ -246,6 +246,24 @@ def test_graph_replays_forward_and_backward(gpu_device):
         assert all(torch.equal(a, b) for a, b in zip(got, step())), f"replay {rep}"
 
 
+@pytest.mark.gpu
+def test_second_derivatives_are_refused(gpu_device):
+    """A recorded backward gives first derivatives and refuses to be differentiated itself."""
+    from memory_amd import ops
+    x = torch.randn(5, 64, device=gpu_device, requires_grad=True)
+    w = torch.ones(64, device=gpu_device)
+    h, n = ops.gated_residual_norm(x, x.detach() * 2, post_weight=w, pre_weight=w)
+    (g,) = torch.autograd.grad(n.square().sum(), x, create_graph=True)
+    h2, n2 = ops.gated_residual_norm(x, x.detach() * 2, post_weight=w, pre_weight=w)
+    assert torch.equal(g, torch.autograd.grad(n2.square().sum(), x)[0])
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    z = torch.randn(5, 33, device=gpu_device, requires_grad=True)
+    (g,) = torch.autograd.grad(ops.router_select(z, 4, 1)[1].square().sum(), z, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_refusals():
     from memory_amd import ops
     x, w = torch.zeros(3, 8), torch.ones(8)
