@@ -11,6 +11,8 @@
 // key block kb), so that a lane's keys of one dim are 16 consecutive bytes: every operand of both products is one
 // 16-byte load per lane straight into registers, and V needs no transpose.
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "moc_common.h"
 
@@ -141,6 +143,7 @@ struct C8Unit {
   float2* lse_part;
   int64_t max_u;
   int L, H, HK, NS;
+  uint32_t ns_mul, ns_shift;   // e / NS = e ns_mul >> ns_shift for e < 2^31
   float scale_log2;
 };
 
@@ -172,29 +175,44 @@ __global__ __launch_bounds__(64 * kC8Waves) void cache8_unit_kernel(C8Unit a) {
     int64_t row;
     float w;
   };
-  auto edge_of = [&](int r0) { return r0 + c16 < nrows ? a.csr_edge[p0 + (r0 + c16) / GL] : -1; };
-  auto fetch = [&](int r0, int e) {
+  // row r0 + c16 is row `rem` of edge number j of the chapter; both move on by 16 rows without a division
+  const int step_j = 16 / GL, step_rem = 16 % GL;
+  int j = c16 / GL, rem = c16 % GL;
+  auto move_on = [&] {
+    j += step_j;
+    rem += step_rem;
+    if (rem >= GL) {
+      rem -= GL;
+      ++j;
+    }
+  };
+  auto fetch = [&](int e, int rm) {
     Rows x;
     x.qf[0] = x.qf[1] = zero_frag<bf16>();
     x.row = -1;
     x.w = 1.f;
     if (e >= 0) {
-      const int rem = (r0 + c16) % GL, l = rem / G, hq = hk * G + rem % G;
-      x.row = ((int64_t)e * a.L + l) * a.H + hq;
+      const int l = a.L == 1 ? 0 : rm / G, at = l * a.H + hk * G + (a.L == 1 ? rm : rm % G);   // (token, head)
+      const int64_t lh = (int64_t)a.L * a.H;
+      x.row = e * lh + at;
       x.w = a.omega[e];
-      const bf16* qp = a.q + (((int64_t)(e / a.NS) * a.L + l) * a.H + hq) * kC8Dh + 16 * g;
+      const int64_t seq = (int64_t)(((uint64_t)(uint32_t)e * a.ns_mul) >> a.ns_shift);
+      const bf16* qp = a.q + (seq * lh + at) * kC8Dh + 16 * g;
       x.qf[0] = Load8<bf16, bf16>::run(qp);
       x.qf[1] = Load8<bf16, bf16>::run(qp + 8);
     }
     return x;
   };
-  Rows cur = fetch(0, c16 < nrows ? eid : -1);
-  int ahead = nrows > 16 ? edge_of(16) : -1;
+  Rows cur = fetch(c16 < nrows ? eid : -1, rem);
+  move_on();
+  int ahead = 16 + c16 < nrows ? a.csr_edge[p0 + j] : -1, ahead_rem = rem;
   for (int r0 = 0; r0 < nrows; r0 += 16) {
     Rows next = cur;
     if (r0 + 16 < nrows) {   // (the same in every lane)
-      next = fetch(r0 + 16, ahead);
-      ahead = edge_of(r0 + 32);
+      next = fetch(ahead, ahead_rem);
+      move_on();
+      ahead = r0 + 32 + c16 < nrows ? a.csr_edge[p0 + j] : -1;
+      ahead_rem = rem;
     }
     const bf16x8 (&qf)[2] = cur.qf;
     const int64_t row = cur.row;
@@ -213,7 +231,7 @@ __global__ __launch_bounds__(64 * kC8Waves) void cache8_unit_kernel(C8Unit a) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) mx = fmax_fast(mx, st[kb][x]);
     const float cf = w * ks;
-    const float m = quad_max(mx) * cf;
+    const float m = quad_max_pl(mx) * cf;
     float ps = 0.f;
     f16x8 pf[2];
 #pragma unroll
@@ -224,7 +242,7 @@ __global__ __launch_bounds__(64 * kC8Waves) void cache8_unit_kernel(C8Unit a) {
         ps += p;
         pf[kb >> 1][4 * (kb & 1) + x] = (f16)p;
       }
-    const float l = quad_sum(ps);
+    const float l = quad_sum_pl(ps);
     // O^T: lane = query row, dims 16 db + 4 g + x
     f32x4 o[4];
 #pragma unroll
@@ -314,11 +332,14 @@ __global__ __launch_bounds__(256) void cache8_combine_kernel(const f16* __restri
 }
 
 // ------------------------------------------------------------------ many queries: running softmax over the slots
-// One workgroup = 128 query rows (token, head of the kv group) of one (sequence, kv head), 4 waves x 32 rows; the
-// heads of a group share every tile.  A tile pair is 8 KB of e4m3: each thread loads 16 bytes of K and of V one slot
-// ahead, widens them once and puts them into LDS as bf16, double-buffered, for all four waves.  Running maximum
+// One workgroup = 256 query rows (token, head of the kv group) of one (sequence, kv head), 8 waves x 32 rows; the
+// heads of a group share every tile.  A tile pair is 8 KB of e4m3: each thread loads eight bytes of K and of V one slot
+// ahead (two ahead took more registers than there are: 200 us), widens them once and puts them into LDS as bf16,
+// double-buffered, for all waves (four waves of 16 bytes: 191 us against 183 for 4 x 2,048 tokens of 16 heads, 764 TFLOP/s).
+// Bound: the exponentials and the products, which hardly overlap (matrix units busy 0.34, VALU 0.6 of the time).  Running maximum
 // (raised lazily) and sum as in the sequence attention (xattn_fwd.hip).
-constexpr int kC8Threads = 256;
+constexpr int kC8Threads = 512;
+constexpr int kC8Rows = kC8Threads / 2;   // 32 per wave
 constexpr float kC8Slack = 8.f;
 
 struct C8Prompt {
@@ -339,25 +360,28 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
   __shared__ __attribute__((aligned(16))) char sV[2][8192];
   const int G = a.H / a.HK;
   const int64_t rows = (int64_t)a.L * G;
-  const int64_t nqb = (rows + 127) / 128;
+  const int64_t nqb = (rows + kC8Rows - 1) / kC8Rows;
   const int64_t t = xcd_tile((int64_t)a.B * a.HK * a.nsplit * nqb);
   if (t < 0) return;
   const int64_t bh = t / (a.nsplit * nqb);
   const int b = (int)(bh / a.HK), hk = (int)(bh % a.HK), sp = (int)((t / nqb) % a.nsplit);
   const int s_begin = (int)((int64_t)a.NS * sp / a.nsplit), s_end = (int)((int64_t)a.NS * (sp + 1) / a.nsplit);
-  const int64_t q0 = (t % nqb) * 128;
+  const int64_t q0 = (t % nqb) * kC8Rows;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c16 = lane & 15;
 
-  // query rows (token * H + head; -1 past the end) and their fragments
-  int64_t qrow[2];
+  // query rows (of the sequence: token * H + head; -1 past the end) and their fragments
+  const bf16* qb0 = a.q + (int64_t)b * a.L * a.H * kC8Dh;
+  auto query_row = [&](int qb) {
+    const int r = (int)q0 + 32 * wave + 16 * qb + c16;
+    return r < rows ? r / G * a.H + hk * G + r % G : -1;
+  };
   bf16x8 qf[2][2];
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
-    const int64_t r = q0 + 32 * wave + 16 * qb + c16;
-    qrow[qb] = r < rows ? ((int64_t)b * a.L + r / G) * a.H + hk * G + r % G : -1;
+    const int qr = query_row(qb);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
-      qf[qb][ks] = qrow[qb] >= 0 ? Load8<bf16, bf16>::run(a.q + qrow[qb] * kC8Dh + 32 * ks + 8 * g) : zero_frag<bf16>();
+      qf[qb][ks] = qr >= 0 ? Load8<bf16, bf16>::run(qb0 + (int64_t)qr * kC8Dh + 32 * ks + 8 * g) : zero_frag<bf16>();
   }
   float m[2] = {-INFINITY, -INFINITY}, lsum[2] = {0.f, 0.f};
   bf16x8 ones;
@@ -375,30 +399,39 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
     const int64_t c = ids[s];
     return c >= 0 && c < a.C ? c * a.HK + hk : -1;
   };
-  V16 kr, vr;
+  uint2 kr, vr;
   auto fetch = [&](int64_t tile) {
-    kr = ld16(a.k8 + tile * kC8Tile + 16 * tid);
-    vr = ld16(a.v8 + tile * kC8Tile + 16 * tid);
+    kr = *reinterpret_cast<const uint2*>(a.k8 + tile * kC8Tile + 8 * tid);
+    vr = *reinterpret_cast<const uint2*>(a.v8 + tile * kC8Tile + 8 * tid);
   };
+  const int st_off = Tile::off(tid >> 3, 8 * (tid & 7));
   auto stage = [&](int buf) {
-    const int row = tid >> 2, col = 16 * (tid & 3);
-    *reinterpret_cast<bf16x8*>(sK[buf] + Tile::off(row, col)) = c8_widen(kr.w[0], kr.w[1]);
-    *reinterpret_cast<bf16x8*>(sK[buf] + Tile::off(row, col + 8)) = c8_widen(kr.w[2], kr.w[3]);
-    *reinterpret_cast<bf16x8*>(sV[buf] + Tile::off(row, col)) = c8_widen(vr.w[0], vr.w[1]);
-    *reinterpret_cast<bf16x8*>(sV[buf] + Tile::off(row, col + 8)) = c8_widen(vr.w[2], vr.w[3]);
+    *reinterpret_cast<bf16x8*>(sK[buf] + st_off) = c8_widen(kr.x, kr.y);
+    *reinterpret_cast<bf16x8*>(sV[buf] + st_off) = c8_widen(vr.x, vr.y);
   };
+  // a slot's logit and value factors are loaded with its tile, its chapter id one slot before that
   int64_t cur = slot_tile(s_begin);
+  int64_t next = s_begin + 1 < s_end ? slot_tile(s_begin + 1) : -1;
+  float c = 0.f, f = 0.f;
   if (cur >= 0) {
     fetch(cur);
+    c = om[s_begin] * a.ks[cur] * a.scale_log2;
+    f = om[s_begin] * a.vs[cur];
     stage(0);
   }
   __syncthreads();
+  auto slots = [&](auto busy) {
   for (int s = s_begin; s < s_end; ++s) {
     const int buf = (s - s_begin) & 1;
-    const int64_t next = s + 1 < s_end ? slot_tile(s + 1) : -1;
-    if (next >= 0) fetch(next);
-    if (cur >= 0) {
-      const float c = om[s] * a.ks[cur] * a.scale_log2, f = om[s] * a.vs[cur];
+    float w1 = 0.f, ks1 = 0.f, vs1 = 0.f;
+    if (next >= 0) {
+      fetch(next);
+      w1 = om[s + 1];
+      ks1 = a.ks[next];
+      vs1 = a.vs[next];
+    }
+    const int64_t after = s + 2 < s_end ? slot_tile(s + 2) : -1;
+    if constexpr (decltype(busy)::value) if (cur >= 0) {
       f32x4 st[4][2];
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
@@ -412,22 +445,23 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
 #pragma unroll
           for (int qb = 0; qb < 2; ++qb) mma(st[kb][qb], ka, qf[qb][ks]);
         }
-      float cm[2];
+      // a lane's keys tell whether a row's reference has to rise; only then is the row's maximum formed
+      float mx[2];
       bool grow = false;
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
-        float mx = st[0][qb][0];
+        mx[qb] = st[0][qb][0];
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) mx = fmax_fast(mx, st[kb][qb][x]);
-        cm[qb] = quad_max_pl(mx) * c;   // (c >= 0)
-        grow |= cm[qb] > m[qb] + kC8Slack;
+          for (int x = 0; x < 4; ++x) mx[qb] = fmax_fast(mx[qb], st[kb][qb][x]);
+        grow |= mx[qb] * c > m[qb] + kC8Slack;   // (c >= 0)
       }
       if (__any(grow)) {
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
-          const float mn = cm[qb] > m[qb] + kC8Slack ? cm[qb] : m[qb];
+          const float cm = quad_max_pl(mx[qb]) * c;
+          const float mn = cm > m[qb] + kC8Slack ? cm : m[qb];
           const float alpha = c8_exp2(m[qb] - mn);
           m[qb] = mn;
           lsum[qb] *= alpha;
@@ -456,10 +490,12 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
         mma(ls, ones, pf[qb][1]);
         lsum[qb] += ls[0] * rf;
         if (!fold) {
+          float fo = f;   // (kept out of the other path, which the compiler would otherwise convert twice for)
+          asm volatile("" : "+v"(fo));
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int x = 0; x < 8; ++x) pf[qb][h][x] = (bf16)((float)pf[qb][h][x] * f);
+            for (int x = 0; x < 8; ++x) pf[qb][h][x] = (bf16)((float)pf[qb][h][x] * fo);
         }
       }
 #pragma unroll
@@ -473,14 +509,23 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
     }
     if (next >= 0) stage(buf ^ 1);
     cur = next;
+    next = after;
+    c = w1 * ks1 * a.scale_log2;
+    f = w1 * vs1;
     __syncthreads();
   }
+  };
+  // a wave without rows only helps to stage the tiles
+  if (q0 + 32 * wave < rows) slots(std::true_type{});
+  else slots(std::false_type{});
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
-    if (qrow[qb] < 0) continue;
+    const int qr = query_row(qb);
+    if (qr < 0) continue;
+    const int64_t row = (int64_t)b * a.L * a.H + qr;
     const float inv = lsum[qb] > 0.f ? 1.f / lsum[qb] : lsum[qb];   // (no slot: 0; NaN passes)
     if (a.nsplit > 1) {
-      const int64_t at = (int64_t)sp * a.B * a.L * a.H + qrow[qb];
+      const int64_t at = (int64_t)sp * a.B * a.L * a.H + row;
 #pragma unroll
       for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(a.part + at * kC8Dh + 16 * db + 4 * g) = o[db][qb] * inv;
       if (g == 0) a.lse[at] = lsum[qb] > 0.f ? m[qb] + log2f(lsum[qb]) : lsum[qb] == 0.f ? -INFINITY : lsum[qb];
@@ -490,7 +535,7 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
         bf16x4 v;
 #pragma unroll
         for (int x = 0; x < 4; ++x) v[x] = (bf16)(o[db][qb][x] * inv);
-        *reinterpret_cast<bf16x4*>(a.out + qrow[qb] * kC8Dh + 16 * db + 4 * g) = v;
+        *reinterpret_cast<bf16x4*>(a.out + row * kC8Dh + 16 * db + 4 * g) = v;
       }
     }
   }
@@ -504,10 +549,12 @@ __global__ __launch_bounds__(256) void cache8_merge_kernel(const float* __restri
   if (row >= rows) return;
   const int ch = (int)(i & 15);
   float M = -INFINITY;
+#pragma unroll 8
   for (int s = 0; s < nsplit; ++s) M = fmax_fast(M, lse[s * rows + row]);
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
   float den = 0.f;
   if (!(M == -INFINITY)) {
+#pragma unroll 8
     for (int s = 0; s < nsplit; ++s) {
       const float w = c8_exp2(lse[s * rows + row] - M);
       den += w;
@@ -521,15 +568,25 @@ __global__ __launch_bounds__(256) void cache8_merge_kernel(const float* __restri
   *reinterpret_cast<bf16x4*>(out + row * kC8Dh + 4 * ch) = v;
 }
 
-// One plan unit per tile against one pass over a row block's slots: rows of one slot's tile up to which the unit
-// form is taken.
-constexpr int kC8UnitRows = 16;
-bool c8_units(int L, int H, int HK) { return L == 1 || (int64_t)L * (H / HK) <= kC8UnitRows; }
-
-// slots of a row block split over workgroups until about two workgroups per CU are busy
+// Slots of a row block split over workgroups, up to one per CU: a prompt of 509 tokens of 12 heads 24 + 7 us with its
+// merge; two per CU 25 + 13 (the f32 part rows), 144 in all 27 + 5.  Blocks of few rows, whose part rows are small: two.
 int c8_splits(int64_t B, int64_t L, int H, int HK, int NS) {
-  const int64_t tiles = B * HK * ((L * (H / HK) + 127) / 128);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(NS, 512 / std::max<int64_t>(tiles, 1)));
+  const int64_t rows = L * (H / HK), tiles = B * HK * ((rows + kC8Rows - 1) / kC8Rows);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(NS, 32), (rows <= 64 ? 512 : 256) / std::max<int64_t>(tiles, 1)));
+}
+
+// Whether the unit form is taken for several tokens: by estimated times (us).  Unit form: one wave takes the 16-row
+// blocks of a chapter that every sequence selects one after the other, ~1 us each, and part rows are written and
+// read.  Row blocks: ~1.2 us per slot and workgroup of a CU, and the merge.  Measured, unit form / row blocks, at 65 of 4,097
+// chapters: 1 x 64 tokens of 12 heads 17 / 22 us, 4 x 64 35 / 23, 16 x 16 37 / 60, 16 x 64 109 / 60, 64 x 8 80 / 185; 16 heads on
+// 4: 8 x 4 18 / 20, 8 x 16 42 / 20, 37 x 8 88 / 41, 37 x 16 165 / 44.
+bool c8_units(int64_t B, int64_t L, int H, int HK, int NS) {
+  if (L == 1) return true;
+  const double rows = (double)L * (H / HK), tiles = (double)B * HK * std::ceil(rows / kC8Rows);
+  const double units = 9 + B * rows / 16 + (double)B * NS * L * H * 256 / 5e6;
+  const int ns = c8_splits(B, L, H, HK, NS);
+  const double blocks = 10 + 1.2 * NS / ns * std::max(1.0, tiles * ns / 256) + (ns > 1 ? 5 : 0);
+  return units <= blocks;
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -537,7 +594,7 @@ struct C8Ws {
   size_t o_part = 0, lse_part, bytes;
   C8Ws(int64_t B, int64_t L, int H, int HK, int NS) {
     const size_t rows = (size_t)B * L * H;
-    if (c8_units((int)L, H, HK)) {
+    if (c8_units(B, L, H, HK, NS)) {
       lse_part = up256(rows * NS * kC8Dh * 2);
       bytes = lse_part + up256(rows * NS * 8);
     } else {
@@ -599,12 +656,17 @@ int moc_cache8_attend(const moc_cache8_args* a, void* workspace, size_t workspac
               "moc_cache8_attend: workspace %zu < %zu bytes, or unaligned", workspace_bytes, y.bytes);
   char* ws = (char*)workspace;
   const float sl2 = a->scale * 1.4426950408889634f;
-  if (c8_units((int)a->L, a->H, a->HK)) {
+  if (c8_units(a->B, a->L, a->H, a->HK, a->NS)) {
     const int64_t units = a->max_u * a->HK;
     if (units > 0) {
       C8Unit k{(const bf16*)a->q, (const uint8_t*)a->k_tiles, (const uint8_t*)a->v_tiles, a->k_scale, a->v_scale, a->omega,
                a->uniq, a->n_uniq, a->csr_off, a->csr_edge, a->row_tab, (f16*)(ws + y.o_part), (float2*)(ws + y.lse_part),
-               a->max_u, (int)a->L, a->H, a->HK, a->NS, sl2};
+               a->max_u, (int)a->L, a->H, a->HK, a->NS, 0, 0, sl2};
+      // division by NS as a product: with s = ceil(log2 NS), floor(2^(31 + s) / NS) + 1 < 2^32 is exact below 2^31
+      int s = 0;
+      while ((1 << s) < a->NS) ++s;
+      k.ns_shift = 31 + s;
+      k.ns_mul = (uint32_t)(((uint64_t)1 << (31 + s)) / a->NS + 1);
       hipLaunchKernelGGL(cache8_unit_kernel, dim3((unsigned)((units + kC8Waves - 1) / kC8Waves)), dim3(64 * kC8Waves), 0,
                          stream, k);
       if (int rc = check_launch("cache8_unit_kernel")) return rc;
@@ -615,7 +677,7 @@ int moc_cache8_attend(const moc_cache8_args* a, void* workspace, size_t workspac
     return check_launch("cache8_combine_kernel");
   }
   const int nsplit = c8_splits(a->B, a->L, a->H, a->HK, a->NS);
-  const int64_t nqb = (a->L * (a->H / a->HK) + 127) / 128, tiles = a->B * a->HK * nsplit * nqb;
+  const int64_t nqb = (a->L * (a->H / a->HK) + kC8Rows - 1) / kC8Rows, tiles = a->B * a->HK * nsplit * nqb;
   C8Prompt p{(const bf16*)a->q, (const uint8_t*)a->k_tiles, (const uint8_t*)a->v_tiles, a->k_scale, a->v_scale, a->omega, a->idx,
              (bf16*)a->out, (float*)ws, (float*)(ws + y.lse_part), a->C, (int)a->B, (int)a->L, a->H, a->HK, a->NS, nsplit, sl2};
   hipLaunchKernelGGL(cache8_prompt_kernel, dim3(xcd_grid(tiles)), dim3(kC8Threads), 0, stream, p);
