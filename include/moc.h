@@ -784,7 +784,7 @@ int moc_cache8_pack(int dtype, const void* k, const void* v, int64_t tiles, void
  * q, out bf16 [B][L][H][64]; k_tiles, v_tiles of C chapters x HK heads; idx i32, omega f32 (>= 0) [B][NS] (ids outside
  * [0, C): skipped slot) and the chapter plan of idx with its row table (moc_decode_row_table), max_u >= the plan's
  * n_uniq[0].  A row without slots is 0.  workspace: moc_cache8_attend_workspace bytes, 16-byte aligned.
- * B NS L H < 2^31. */
+ * B NS < 2^31, L H < 2^25; one token: B NS H / HK < 2^31. */
 typedef struct {
   const void *q, *k_tiles, *v_tiles;
   const float *k_scale, *v_scale, *omega;

@@ -582,6 +582,7 @@ int c8_splits(int64_t B, int64_t L, int H, int HK, int NS) {
 // 4: 8 x 4 18 / 20, 8 x 16 42 / 20, 37 x 8 88 / 41, 37 x 16 165 / 44.
 bool c8_units(int64_t B, int64_t L, int H, int HK, int NS) {
   if (L == 1) return true;
+  if (B * NS * L >= ((int64_t)1 << 31) / (H / HK)) return false;
   const double rows = (double)L * (H / HK), tiles = (double)B * HK * std::ceil(rows / kC8Rows);
   const double units = 9 + B * rows / 16 + (double)B * NS * L * H * 256 / 5e6;
   const int ns = c8_splits(B, L, H, HK, NS);
@@ -606,8 +607,11 @@ struct C8Ws {
 };
 
 bool c8_shape_ok(int64_t B, int64_t L, int H, int HK, int NS) {
-  return B >= 0 && L > 0 && L < (1 << 24) && H > 0 && HK > 0 && H % HK == 0 && NS > 0 &&
-         (B == 0 || (L * H < ((int64_t)1 << 31) / 64 && B * NS * L * H < ((int64_t)1 << 31)));
+  if (B < 0 || L <= 0 || H <= 0 || HK <= 0 || H % HK != 0 || NS <= 0) return false;
+  const int64_t cap = (int64_t)1 << 31;
+  if (B >= cap / NS || L >= ((int64_t)1 << 25) / H) return false;   // edges, and rows of a sequence
+  if (c8_units(B, L, H, HK, NS)) return B * NS * L < cap / (H / HK) && B * L * H < cap;   // rows of a unit
+  return B * HK * c8_splits(B, L, H, HK, NS) * ((L * (H / HK) + kC8Rows - 1) / kC8Rows) < cap && B * L * H < cap * 8;
 }
 
 }  // namespace

@@ -201,34 +201,26 @@ __device__ __forceinline__ void select_row(const SelArgs& a, int64_t r, char* ld
     }
   }
   __syncthreads();
-  // their order and scores
-  double mine[(kSelMaxK + NT - 1) / NT];
-  int rank[(kSelMaxK + NT - 1) / NT];
-  double sum = 0.0;
-#pragma unroll
-  for (int q = 0; q < (kSelMaxK + NT - 1) / NT; ++q) {
-    const int i = tid + NT * q;
-    if (i < a.k) {
-      const uint64_t ki = sel_key[i];
-      const int32_t ii = sel_id[i];
-      int rk = 0;
-      for (int j = 0; j < a.k; ++j) rk += sel_key[j] > ki || (sel_key[j] == ki && sel_id[j] < ii);
-      rank[q] = rk;
-      mine[q] = score(z[ii]);
-      sum += mine[q];
-    }
+  // their order, and scores and weights in that order (the list's own order is not fixed, a sum over it would not be)
+  int32_t* id_at = (int32_t*)keys;   // (the keys are done)
+  for (int i = tid; i < a.k; i += NT) {
+    const uint64_t ki = sel_key[i];
+    const int32_t ii = sel_id[i];
+    int rk = 0;
+    for (int j = 0; j < a.k; ++j) rk += sel_key[j] > ki || (sel_key[j] == ki && sel_id[j] < ii);
+    sel_s[rk] = (float)score(z[ii]);
+    id_at[rk] = ii;
   }
+  __syncthreads();
+  double sum = 0.0;
+  for (int i = tid; i < a.k; i += NT) sum += (double)sel_s[i];
   sum = blk_sum<NT>(sum, red);
   const double D = a.renorm ? (sum > 1e-12 ? sum : (sum == sum ? 1e-12 : sum)) : 1.0;
-#pragma unroll
-  for (int q = 0; q < (kSelMaxK + NT - 1) / NT; ++q) {
-    const int i = tid + NT * q;
-    if (i < a.k) {
-      const int64_t o = r * a.k + rank[q];
-      a.idx[o] = sel_id[i] + a.S;
-      a.w[o] = (float)((double)a.scale * mine[q] / D);
-      if (a.s_sel) a.s_sel[o] = (float)mine[q];
-    }
+  for (int i = tid; i < a.k; i += NT) {
+    const int64_t o = r * a.k + i;
+    a.idx[o] = id_at[i] + a.S;
+    a.w[o] = (float)((double)a.scale * (double)sel_s[i] / D);
+    if (a.s_sel) a.s_sel[o] = sel_s[i];
   }
 }
 

@@ -13,6 +13,7 @@ sequence's slots -> o_proj.  Inference only (no autograd).
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -178,7 +179,7 @@ class MemoryDecodeCache:
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
+    t = t if t.is_contiguous() else t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -387,19 +388,25 @@ class _Cache8Args(ctypes.Structure):
                 + [(n, ctypes.c_int) for n in ("H", "HK", "NS")] + [("scale", ctypes.c_float)])
 
 
+@functools.lru_cache(maxsize=1024)
+def _attend8_workspace(B: int, Lq: int, H: int, HK: int, NS: int) -> int:
+    return L.query("moc_cache8_attend_workspace", B, Lq, H, HK, NS)
+
+
 def _attend8(q: torch.Tensor, B: int, Lq: int, H: int, cache: MemoryDecodeCache, routing: DecodeRouting) -> torch.Tensor:
     """q (B, [L,] H, 64) over an 8-bit cache (moc_cache8_attend)."""
-    q = _aligned(q.to(torch.bfloat16))
+    q = _aligned(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16))
     pl, dev = routing.plan, q.device
     out = torch.empty_like(q)
-    nbytes = L.query("moc_cache8_attend_workspace", B, Lq, H, cache.HK, routing.NS)
+    nbytes = _attend8_workspace(B, Lq, H, cache.HK, routing.NS)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    args = _Cache8Args(ptr(q), ptr(cache.k_tiles), ptr(cache.v_tiles), ptr(cache.k_scale), ptr(cache.v_scale),
-                       ptr(routing.omega), ptr(routing.idx), ptr(pl.uniq), ptr(pl.n_uniq), ptr(pl.csr_off),
-                       ptr(pl.csr_edge), ptr(pl.edge_u), ptr(routing.row_tab), ptr(out), routing.max_units, B, Lq,
-                       pl.num_chapters, H, cache.HK, routing.NS, 0.125)
+    args = _Cache8Args(q.data_ptr(), cache.k_tiles.data_ptr(), cache.v_tiles.data_ptr(), cache.k_scale.data_ptr(),
+                       cache.v_scale.data_ptr(), routing.omega.data_ptr(), routing.idx.data_ptr(), pl.uniq.data_ptr(),
+                       pl.n_uniq.data_ptr(), pl.csr_off.data_ptr(), pl.csr_edge.data_ptr(), pl.edge_u.data_ptr(),
+                       routing.row_tab.data_ptr(), out.data_ptr(), routing.max_units, B, Lq, pl.num_chapters, H, cache.HK,
+                       routing.NS, 0.125)
     with L.on_device(dev):
-        call("moc_cache8_attend", ctypes.addressof(args), ptr(ws), nbytes, stream_ptr(dev))
+        call("moc_cache8_attend", ctypes.addressof(args), ws.data_ptr(), nbytes, stream_ptr(dev))
     return out
 
 

@@ -236,6 +236,9 @@ def test_empty_rows_and_repeats(gpu_device):
     a = run(z, 16, 1, gpu_device, torch.ones(3000, 16), torch.zeros(513), score="sigmoid", num_groups=8, top_groups=3)
     b = run(z, 16, 1, gpu_device, torch.ones(3000, 16), torch.zeros(513), score="sigmoid", num_groups=8, top_groups=3)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+    z[:, ::2] = 0.5      # crowded with equal keys: every row takes the general path
+    runs = [run(z, 60, 1, gpu_device, torch.ones(3000, 60), torch.zeros(513), score=s) for s in ("softmax", "sigmoid") * 2]
+    assert all(torch.equal(x, y) for i in (0, 1) for x, y in zip(runs[i], runs[i + 2]))
 
 
 @pytest.mark.gpu
