@@ -783,7 +783,8 @@ int moc_cache8_pack(int dtype, const void* k, const void* v, int64_t tiles, void
 /* moc_decode_partial and its combine over such tiles (any finite scales >= 0), for L >= 1 query tokens per sequence:
  * q, out bf16 [B][L][H][64]; k_tiles, v_tiles of C chapters x HK heads; idx i32, omega f32 (>= 0) [B][NS] (ids outside
  * [0, C): skipped slot) and the chapter plan of idx with its row table (moc_decode_row_table), max_u >= the plan's
- * n_uniq[0].  A row without slots is 0.  workspace: moc_cache8_attend_workspace bytes, 16-byte aligned.
+ * n_uniq[0].  A row without slots is 0; of value factors omega v_scale that differ by more than 2^90 within a sequence the
+ * smaller may count as 0.  workspace: moc_cache8_attend_workspace bytes, 16-byte aligned.
  * B NS < 2^31, L H < 2^25; one token: B NS H / HK < 2^31. */
 typedef struct {
   const void *q, *k_tiles, *v_tiles;

@@ -334,10 +334,12 @@ __global__ __launch_bounds__(256) void cache8_combine_kernel(const f16* __restri
 // ------------------------------------------------------------------ many queries: running softmax over the slots
 // One workgroup = 256 query rows (token, head of the kv group) of one (sequence, kv head), 8 waves x 32 rows; the
 // heads of a group share every tile.  A tile pair is 8 KB of e4m3: each thread loads eight bytes of K and of V one slot
-// ahead (two ahead took more registers than there are: 200 us), widens them once and puts them into LDS as bf16,
-// double-buffered, for all waves (four waves of 16 bytes: 191 us against 183 for 4 x 2,048 tokens of 16 heads, 764 TFLOP/s).
-// Bound: the exponentials and the products, which hardly overlap (matrix units busy 0.34, VALU 0.6 of the time).  Running maximum
-// (raised lazily) and sum as in the sequence attention (xattn_fwd.hip).
+// ahead (two ahead took more registers than there are: 200 us), widens them once and puts them into LDS, K as bf16 and V
+// as f16, double-buffered, for all waves (four waves of 16 bytes: 191 us against 183).  Probabilities are f16: with bf16 the
+// kernel took 183 us for 4 x 2,048 tokens of 16 heads in place of 188 to 194, at 1.4 times the error against float64
+// (0.0024; 0.0017 is what rounding the result to bf16 alone gives).  174 us a call in a row of calls: 803 TFLOP/s, 0.66 of a
+// large matrix product's rate.  Bound: the exponentials and the products, which hardly overlap (matrix units busy 0.34,
+// VALU 0.6 of the time).  Running maximum (raised lazily) and sum as in the sequence attention (xattn_fwd.hip).
 constexpr int kC8Threads = 512;
 constexpr int kC8Rows = kC8Threads / 2;   // 32 per wave
 constexpr float kC8Slack = 8.f;
@@ -384,9 +386,10 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
       qf[qb][ks] = qr >= 0 ? Load8<bf16, bf16>::run(qb0 + (int64_t)qr * kC8Dh + 32 * ks + 8 * g) : zero_frag<bf16>();
   }
   float m[2] = {-INFINITY, -INFINITY}, lsum[2] = {0.f, 0.f};
-  bf16x8 ones;
+  float F = 0.f, inv_F = INFINITY;
+  f16x8 ones;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) ones[j] = (bf16)1.f;
+  for (int j = 0; j < 8; ++j) ones[j] = (f16)1.f;
   f32x4 o[4][2];
 #pragma unroll
   for (int db = 0; db < 4; ++db)
@@ -407,7 +410,7 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
   const int st_off = Tile::off(tid >> 3, 8 * (tid & 7));
   auto stage = [&](int buf) {
     *reinterpret_cast<bf16x8*>(sK[buf] + st_off) = c8_widen(kr.x, kr.y);
-    *reinterpret_cast<bf16x8*>(sV[buf] + st_off) = c8_widen(vr.x, vr.y);
+    *reinterpret_cast<f16x8*>(sV[buf] + st_off) = c8_widen_f16(vr.x, vr.y);
   };
   // a slot's logit and value factors are loaded with its tile, its chapter id one slot before that
   int64_t cur = slot_tile(s_begin);
@@ -469,42 +472,49 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
           for (int db = 0; db < 4; ++db) o[db][qb] *= alpha;
         }
       }
-      bf16x8 pf[2][2];
-      // the value factor f = omega vs goes into the exponent where its logarithm and reciprocal are ordinary
-      // numbers; elsewhere (f = 0, or scales past 2^+-90) it multiplies the probabilities
-      const bool fold = f > 0x1p-90f && f < 0x1p90f;
-      const float lf = fold ? __builtin_amdgcn_logf(f) : 0.f, rf = fold ? __builtin_amdgcn_rcpf(f) : 1.f;
+      // O is held in units of F, a value factor omega vs met before; a slot's probabilities carry f / F, in the
+      // exponent.  Within 2^-1 .. 2^6 of F they stay below 2^14, and one that f16's smallest step rounds away is
+      // below 2^-24 of the row's largest; past that F becomes f.  f = 0 leaves O alone and counts in the sum, and so
+      // does an f 2^-90 of F.
+      float r = f * inv_F;
+      const bool none = f == 0.f || r < 0x1p-90f;
+      if (!none && !(r > 0x1p-1f && r < 0x1p6f)) {   // (the first slot; NaN too)
+        const float beta = F / f;
+        F = f;
+        inv_F = 1.f / f;
+        r = 1.f;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb) o[db][qb] *= beta;
+      }
+      r = none ? 1.f : r;
+      const float lr = __builtin_amdgcn_logf(r), rr = __builtin_amdgcn_rcpf(r);
+      f16x8 pf[2][2];
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
-        const float off = m[qb] - lf;
+        const float off = m[qb] - lr;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            pf[qb][h][x] = (bf16)c8_exp2(st[2 * h][qb][x] * c - off);
-            pf[qb][h][4 + x] = (bf16)c8_exp2(st[2 * h + 1][qb][x] * c - off);
+            pf[qb][h][x] = (f16)c8_exp2(st[2 * h][qb][x] * c - off);
+            pf[qb][h][4 + x] = (f16)c8_exp2(st[2 * h + 1][qb][x] * c - off);
           }
-        // row sums of the rounded probabilities, in units of f
+        // row sums of the rounded probabilities, in units of r
         f32x4 ls = f32x4{0.f, 0.f, 0.f, 0.f};
-        mma(ls, ones, pf[qb][0]);
-        mma(ls, ones, pf[qb][1]);
-        lsum[qb] += ls[0] * rf;
-        if (!fold) {
-          float fo = f;   // (kept out of the other path, which the compiler would otherwise convert twice for)
-          asm volatile("" : "+v"(fo));
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int x = 0; x < 8; ++x) pf[qb][h][x] = (bf16)((float)pf[qb][h][x] * fo);
-        }
+        mma16(ls, ones, pf[qb][0]);
+        mma16(ls, ones, pf[qb][1]);
+        lsum[qb] += ls[0] * rr;
       }
+      if (!none)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int db = 0; db < 4; ++db) {
-          const bf16x8 va = Tile::frag(sV[buf], 16 * db + c16, 16 * g + 8 * h);
+          const f16x8 va = __builtin_bit_cast(f16x8, Tile::frag(sV[buf], 16 * db + c16, 16 * g + 8 * h));
 #pragma unroll
-          for (int qb = 0; qb < 2; ++qb) mma(o[db][qb], va, pf[qb][h]);
+          for (int qb = 0; qb < 2; ++qb) mma16(o[db][qb], va, pf[qb][h]);
         }
     }
     if (next >= 0) stage(buf ^ 1);
@@ -523,7 +533,7 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
     const int qr = query_row(qb);
     if (qr < 0) continue;
     const int64_t row = (int64_t)b * a.L * a.H + qr;
-    const float inv = lsum[qb] > 0.f ? 1.f / lsum[qb] : lsum[qb];   // (no slot: 0; NaN passes)
+    const float inv = lsum[qb] > 0.f ? F / lsum[qb] : lsum[qb];   // (no slot: 0; NaN passes)
     if (a.nsplit > 1) {
       const int64_t at = (int64_t)sp * a.B * a.L * a.H + row;
 #pragma unroll

@@ -484,9 +484,12 @@ def memory_decode_step(memory_attn, hidden: torch.Tensor, cache: MemoryDecodeCac
     with torch.no_grad():
         wq, wo = memory_attn.q_proj.weight, memory_attn.o_proj.weight
         if hidden.dim() == 3 and hidden.shape[1] != 1:
-            q = ops.linear(hidden.to(wq.dtype), wq).view(B, hidden.shape[1], H, memory_attn.head_dim)
+            Lx = hidden.shape[1]
+            if hidden.numel() == 0:
+                return torch.zeros(B, Lx, wo.shape[0], device=hidden.device, dtype=wo.dtype)
+            q = ops.linear(hidden.to(wq.dtype), wq).view(B, Lx, H, memory_attn.head_dim)
             a = decode_attention(q, cache, routing)
-            return ops.linear(a.reshape(B, hidden.shape[1], -1).to(wo.dtype), wo)
+            return ops.linear(a.reshape(B, Lx, H * memory_attn.head_dim).to(wo.dtype), wo)
         x = hidden.reshape(B, -1).to(wq.dtype)
         if _step_native(x, wq, wo, H, cache, routing):
             x, wq, wo = x.contiguous(), wq.contiguous(), wo.contiguous()

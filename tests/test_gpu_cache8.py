@@ -159,6 +159,30 @@ def test_slots_weights_and_scales(gpu_device, L):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("L", [1, 24])
+def test_value_factors_far_apart_and_long_tails(gpu_device, L):
+    """Value factors over twenty powers of two in one sequence, the largest on a chapter that hardly counts, and
+    probabilities of 2^-13 of the largest whose sum is an eighth of it: none may be rounded away."""
+    C = 24
+    q, k8, ks, v8, vs, idx, omega = make(3, L, 4, 2, C, C, 12)
+    k, q = torch.zeros(C, 2, 64, 64), q.abs().clamp(0.5, 1)
+    q[..., 0] = 8
+    k[:, :, 1:, 0] = -9.0            # logit -9 beside one key's 0 in chapter 5: e^-9 = 2^-13
+    k[:, :, 0, 0] = -9.0
+    k[5, :, 7, 0] = 0.0
+    k[0] = 0
+    k[0, :, :, 0] = -30.0
+    omega = torch.ones_like(omega)
+    vs = torch.full((C, 2), 2.0 ** -11)
+    vs[0], vs[11], vs[17] = 1.0, 2.0 ** -5, 2.0 ** -20
+    case = (q, k.to(FP8), torch.ones(C, 2), v8.float().abs().to(FP8), vs, idx, omega)
+    check(attend(gpu_device, *case), *case)
+    for order in (idx.sort(1).values, idx.sort(1, descending=True).values):
+        case = (*case[:5], order, omega)
+        check(attend(gpu_device, *case), *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L", [1, 24])
 def test_large_logits_and_nan(gpu_device, L):
     """Logits of several hundred (one key takes all), and a NaN that stays in the sequences and heads that read it."""
     case = list(make(3, L, 4, 2, 10, 4, 8))
@@ -286,6 +310,7 @@ def test_cache_from_a_bank_saved_and_loaded(gpu_device, tmp_path):
     exact = MemoryDecodeCache.from_tiles(k, v, num_chapters=C, tokens_per_chapter=64, num_kv_heads=HK)
     attn32 = MemoryCrossAttention(d, H, HK, wo_init_zero=False).to(gpu_device)
     attn32.load_state_dict({n: p.float() for n, p in attn.state_dict().items()})
+    assert memory_decode_step(attn, torch.zeros(B, 0, d, device=gpu_device, dtype=BF), eight, routing).shape == (B, 0, d)
     for L in (1, 12):
         h = torch.randn(B, L, d, generator=g0).to(gpu_device, BF)
         got = memory_decode_step(attn, h, eight, routing)
