@@ -420,9 +420,10 @@ def _attend_tokens(q: torch.Tensor, cache: MemoryDecodeCache, routing: DecodeRou
     idx = torch.where(routing.idx < routing.plan.num_chapters, routing.idx, -1)
     lse = torch.empty(B, H, (Lq + 127) // 128 * 128, device=dev, dtype=torch.float32)
     out = torch.empty_like(q)
-    call("moc_xattn_fwd", L.dtype_code(cache.dtype), ptr(q), ptr(cache.k_tiles), ptr(cache.v_tiles), cache.k_tiles.numel(),
-         HK * 4096, 4096, 64, ptr(idx), ptr(routing.omega), B, Lq, H, HK, D, 64, routing.NS, 0.125, ptr(out), ptr(lse),
-         stream_ptr(dev))
+    with L.on_device(dev):
+        call("moc_xattn_fwd", L.dtype_code(cache.dtype), ptr(q), ptr(cache.k_tiles), ptr(cache.v_tiles), cache.k_tiles.numel(),
+             HK * 4096, 4096, 64, ptr(idx), ptr(routing.omega), B, Lq, H, HK, D, 64, routing.NS, 0.125, ptr(out), ptr(lse),
+             stream_ptr(dev))
     return out
 
 

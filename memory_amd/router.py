@@ -107,10 +107,19 @@ class ChapterRouter(nn.Module):
                                  top_groups=self.top_groups if grouped else 1, group_best=self.group_best,
                                  renormalize=self.renormalize)
 
+    def _apply(self, fn, recurse=True):
+        # a conversion of the module to 16 bits leaves the balance bias in float32: steps of 1e-3 would be lost in it
+        kept = self.balance_bias
+        super()._apply(fn, recurse)
+        if kept is not None and self.balance_bias.dtype != torch.float32:
+            self.balance_bias = kept.to(self.balance_bias.device)
+        return self
+
     @torch.no_grad()
     def update_balance(self, indices: torch.Tensor, rate: float = 1e-3, exclude_prefix_chapters: int = 0) -> torch.Tensor:
         """After a step: moves the balance bias by ``rate`` towards equal use of the chapters past the excluded prefix,
-        given the step's selections (chapter ids of any shape).  Returns how often each chapter was selected."""
+        given the step's selections (chapter ids of any shape; where several ranks train one model, those of all of them, gathered,
+        so that their biases stay alike).  Returns how often each chapter was selected."""
         if self.balance_bias is None:
             raise ValueError("this router has no balance bias (balance_bias=True)")
         return ops.router_balance_(self.balance_bias, indices, rate, exclude_prefix_chapters)

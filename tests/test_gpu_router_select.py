@@ -333,3 +333,15 @@ def test_refusals():
                 dict(z=None), dict(R=-1)):
         with pytest.raises(ValueError):
             L.call("moc_router_select", *args(**bad))
+
+
+def test_balance_bias_stays_in_float32():
+    from memory_amd.router import ChapterRouter
+    r = ChapterRouter(32, 9, 2, balance_bias=True)
+    r.balance_bias.copy_(torch.linspace(-0.01, 0.01, 9))
+    want = r.balance_bias.clone()
+    r = r.to(torch.bfloat16)
+    assert r.router.weight.dtype == torch.bfloat16 and r.balance_bias.dtype == torch.float32
+    assert torch.equal(r.balance_bias, want) and "balance_bias" in r.state_dict()
+    assert torch.equal(r.half().float().balance_bias, want) and r.balance_bias is dict(r.named_buffers())["balance_bias"]
+    assert ChapterRouter(32, 9, 2).to(torch.bfloat16).balance_bias is None
