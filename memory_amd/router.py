@@ -86,6 +86,8 @@ class ChapterRouter(nn.Module):
             self.register_buffer("balance_bias", torch.zeros(num_chapters))
         else:
             self.balance_bias = None
+        # ids (R, k) of the last selection in training mode, for update_balance (with a balance bias only)
+        self.selected: Optional[torch.Tensor] = None
         self.router = nn.Linear(hidden_dim, num_chapters, bias=True)
         nn.init.normal_(self.router.weight, mean=0.0, std=0.02)
         nn.init.zeros_(self.router.bias)
@@ -102,10 +104,13 @@ class ChapterRouter(nn.Module):
         if self.plain_selection:
             return ops.router_topk(logits, k, exclude_prefix_chapters)
         grouped = self.top_groups < self.num_groups
-        return ops.router_select(logits, k, exclude_prefix_chapters, score=self.score, bias=self.balance_bias,
-                                 num_groups=self.num_groups if grouped else 1,
-                                 top_groups=self.top_groups if grouped else 1, group_best=self.group_best,
-                                 renormalize=self.renormalize)
+        idx, w = ops.router_select(logits, k, exclude_prefix_chapters, score=self.score, bias=self.balance_bias,
+                                   num_groups=self.num_groups if grouped else 1,
+                                   top_groups=self.top_groups if grouped else 1, group_best=self.group_best,
+                                   renormalize=self.renormalize)
+        if self.balance_bias is not None and self.training:
+            self.selected = idx
+        return idx, w
 
     def _apply(self, fn, recurse=True):
         # a conversion of the module to 16 bits leaves the balance bias in float32: steps of 1e-3 would be lost in it
@@ -116,12 +121,18 @@ class ChapterRouter(nn.Module):
         return self
 
     @torch.no_grad()
-    def update_balance(self, indices: torch.Tensor, rate: float = 1e-3, exclude_prefix_chapters: int = 0) -> torch.Tensor:
+    def update_balance(self, indices: Optional[torch.Tensor] = None, rate: float = 1e-3,
+                       exclude_prefix_chapters: int = 0) -> torch.Tensor:
         """After a step: moves the balance bias by ``rate`` towards equal use of the chapters past the excluded prefix,
-        given the step's selections (chapter ids of any shape; where several ranks train one model, those of all of them, gathered,
-        so that their biases stay alike).  Returns how often each chapter was selected."""
+        given the step's selections: chapter ids of any shape, by default ``selected``, the last ones of training mode.
+        Where several ranks train one model, pass those of all of them, gathered, so that their biases stay alike.
+        Returns how often each chapter was selected."""
         if self.balance_bias is None:
             raise ValueError("this router has no balance bias (balance_bias=True)")
+        if indices is None:
+            indices = self.selected
+            if indices is None:
+                raise ValueError("no selection in training mode yet: pass the step's chapter ids")
         return ops.router_balance_(self.balance_bias, indices, rate, exclude_prefix_chapters)
 
     # -- logits ---------------------------------------------------------------

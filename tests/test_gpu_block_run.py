@@ -254,3 +254,31 @@ def test_sublayer_forms(gpu_device):
     half = MemorySublayer(d, H, wo_init_zero=False, post_norm=True, gate="scalar").to(dev).half()
     o16, n16 = half(h.half(), mem.half(), next_norm=nxt)
     assert o16.dtype == n16.dtype == torch.float16
+
+
+def test_balance_from_the_last_training_step(gpu_device):
+    """update_balance without ids counts the last selection made in training mode, and no other."""
+    from memory_amd.model import RoutedMemoryLayer, TokenRoutedMemoryLayer
+    dev, d, H, C, k = gpu_device, 128, 2, 17, 4
+    bank = (torch.randn(C * 64, d, generator=gen(2)) * 0.5).to(dev)
+    for cls, rows in ((RoutedMemoryLayer, 3), (TokenRoutedMemoryLayer, 3 * 20)):
+        lay = cls(d, H, C, 64, k, router_options=dict(score="sigmoid", balance_bias=True)).to(dev)
+        router = lay.router
+        with pytest.raises(ValueError):
+            router.update_balance()
+        h = torch.randn(3, 20, d, generator=gen(4)).to(dev)
+        out, _ = lay(h, bank)
+        out.sum().backward()
+        seen = router.selected.clone()
+        assert seen.shape == (rows, k)
+        lay.eval()
+        lay(torch.randn(5, 20, d, generator=gen(5)).to(dev), bank)
+        assert torch.equal(router.selected, seen)
+        counts = router.update_balance(rate=0.5, exclude_prefix_chapters=1)
+        want = torch.bincount(seen.reshape(-1).cpu().long(), minlength=C)
+        assert torch.equal(counts.cpu().long(), want)
+        moved = 0.5 * torch.sign(want[1:].double().mean() - want[1:].double())
+        assert torch.equal(router.balance_bias[1:].cpu().double(), moved) and router.balance_bias[0] == 0
+        plain = cls(d, H, C, 64, k).to(dev)
+        plain(h, bank)
+        assert plain.router.selected is None
