@@ -388,6 +388,9 @@ class _Cache8Args(ctypes.Structure):
                 + [(n, ctypes.c_int) for n in ("H", "HK", "NS")] + [("scale", ctypes.c_float)])
 
 
+_pack_cache8 = L.packer(_Cache8Args)
+
+
 @functools.lru_cache(maxsize=1024)
 def _attend8_workspace(B: int, Lq: int, H: int, HK: int, NS: int) -> int:
     return L.query("moc_cache8_attend_workspace", B, Lq, H, HK, NS)
@@ -400,13 +403,13 @@ def _attend8(q: torch.Tensor, B: int, Lq: int, H: int, cache: MemoryDecodeCache,
     out = torch.empty_like(q)
     nbytes = _attend8_workspace(B, Lq, H, cache.HK, routing.NS)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    args = _Cache8Args(q.data_ptr(), cache.k_tiles.data_ptr(), cache.v_tiles.data_ptr(), cache.k_scale.data_ptr(),
-                       cache.v_scale.data_ptr(), routing.omega.data_ptr(), routing.idx.data_ptr(), pl.uniq.data_ptr(),
-                       pl.n_uniq.data_ptr(), pl.csr_off.data_ptr(), pl.csr_edge.data_ptr(), pl.edge_u.data_ptr(),
-                       routing.row_tab.data_ptr(), out.data_ptr(), routing.max_units, B, Lq, pl.num_chapters, H, cache.HK,
-                       routing.NS, 0.125)
+    args = _pack_cache8(q.data_ptr(), cache.k_tiles.data_ptr(), cache.v_tiles.data_ptr(), cache.k_scale.data_ptr(),
+                        cache.v_scale.data_ptr(), routing.omega.data_ptr(), routing.idx.data_ptr(), pl.uniq.data_ptr(),
+                        pl.n_uniq.data_ptr(), pl.csr_off.data_ptr(), pl.csr_edge.data_ptr(), pl.edge_u.data_ptr(),
+                        routing.row_tab.data_ptr(), out.data_ptr(), routing.max_units, B, Lq, pl.num_chapters, H, cache.HK,
+                        routing.NS, 0.125)
     with L.on_device(dev):
-        call("moc_cache8_attend", ctypes.addressof(args), ws.data_ptr(), nbytes, stream_ptr(dev))
+        call("moc_cache8_attend", args, ws.data_ptr(), nbytes, stream_ptr(dev))
     return out
 
 

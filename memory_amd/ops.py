@@ -17,7 +17,7 @@ import torch.nn.functional as F
 from torch.autograd import function as autograd_function
 
 from . import _lib as L
-from ._lib import call, ptr, stream_ptr
+from ._lib import call, ptr, ptr0, stream_ptr
 
 
 def once_differentiable(backward):
@@ -685,6 +685,8 @@ class _GatedNormGrads(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("dh", "dn", "dx", "dres", "dgate", "dparams")]
 
 
+_pack_gated_norm, _pack_gated_norm_grads = L.packer(_GatedNormArgs), L.packer(_GatedNormGrads)
+
 _GATE_NONE, _GATE_SCALAR, _GATE_CHANNEL, _GATE_TOKEN, _GATE_FULL = range(5)
 
 
@@ -707,10 +709,10 @@ def _gate_mode(gate: Optional[torch.Tensor], x: torch.Tensor) -> int:
 def _gated_norm_args(x, r, gate, w1, b1, w2, b2, cfg, h, n, stats):
     mode, norms, alpha, eps = cfg
     d = x.shape[-1]
-    return _GatedNormArgs(x.data_ptr(), r.data_ptr(), ptr(gate), ptr(w1), ptr(b1), ptr(w2), ptr(b2), ptr(h), ptr(n),
-                          ptr(stats), x.numel() // d, d, L.dtype_code(x.dtype), L.dtype_code(r.dtype), mode,
-                          0 if gate is None else L.dtype_code(gate.dtype), *norms, w1 is not None, w2 is not None, alpha,
-                          *eps)
+    return _pack_gated_norm(x.data_ptr(), r.data_ptr(), ptr0(gate), ptr0(w1), ptr0(b1), ptr0(w2), ptr0(b2), ptr0(h),
+                            ptr0(n), ptr0(stats), x.numel() // d, d, L.dtype_code(x.dtype), L.dtype_code(r.dtype), mode,
+                            0 if gate is None else L.dtype_code(gate.dtype), *norms, w1 is not None, w2 is not None,
+                            alpha, *eps)
 
 
 def _gated_norm_forward(x, r, gate, w1, b1, w2, b2, cfg, trains):
@@ -719,7 +721,7 @@ def _gated_norm_forward(x, r, gate, w1, b1, w2, b2, cfg, trains):
     stats = torch.empty(4 * (x.numel() // x.shape[-1]), device=x.device, dtype=torch.float32) if trains else None
     args = _gated_norm_args(x, r, gate, w1, b1, w2, b2, cfg, h, n, stats)
     with L.on_device(x.device):
-        call("moc_gated_norm_fwd", ctypes.addressof(args), stream_ptr(x.device))
+        call("moc_gated_norm_fwd", args, stream_ptr(x.device))
     return h, n, stats
 
 
@@ -767,10 +769,9 @@ class _GatedResidualNorm(torch.autograd.Function):
             buf.zero_()
         args = _gated_norm_args(x, r, gate, w1, b1, w2, b2, cfg, None, None, stats)
         at = buf.data_ptr()
-        out = _GatedNormGrads(ptr(dh), ptr(dn), ptr(dx), ptr(dr), ptr(dg), at)
+        out = _pack_gated_norm_grads(ptr0(dh), ptr0(dn), ptr0(dx), ptr0(dr), ptr0(dg), at)
         with L.on_device(dev):
-            call("moc_gated_norm_bwd", ctypes.addressof(args), ctypes.addressof(out), at + 4 * n_par, 4 * (buf.numel() - n_par),
-                 stream_ptr(dev))
+            call("moc_gated_norm_bwd", args, out, at + 4 * n_par, 4 * (buf.numel() - n_par), stream_ptr(dev))
         dw1 = db1 = dw2 = db2 = None
         if w1 is not None and need[3]:
             dw1 = buf[:d]
