@@ -341,7 +341,7 @@ __global__ __launch_bounds__(256) void cache8_combine_kernel(const f16* __restri
 // ahead (two ahead took more registers than there are: 200 us), widens them once and puts them into LDS, K as bf16 and V
 // as f16, double-buffered, for all waves (four waves of 16 bytes: 191 us against 183).  Probabilities are f16: with bf16 the
 // kernel took 183 us for 4 x 2,048 tokens of 16 heads in place of 188 to 194, at 1.4 times the error against float64
-// (0.0024; 0.0017 is what rounding the result to bf16 alone gives).  174 us a call in a row of calls: 803 TFLOP/s, 0.66 of a
+// (0.0024; 0.0017 is what rounding the result to bf16 alone gives).  173 to 177 us a call in a row of calls: 800 TFLOP/s, 0.65 of a
 // large matrix product's rate.  Bound: the exponentials and the products, which hardly overlap (matrix units busy 0.34,
 // VALU 0.6 of the time).  Running maximum (raised lazily) and sum as in the sequence attention (xattn_fwd.hip).
 constexpr int kC8Threads = 512;
