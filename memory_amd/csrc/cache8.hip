@@ -390,7 +390,7 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
       qf[qb][ks] = qr >= 0 ? Load8<bf16, bf16>::run(qb0 + (int64_t)qr * kC8Dh + 32 * ks + 8 * g) : zero_frag<bf16>();
   }
   float m[2] = {-INFINITY, -INFINITY}, lsum[2] = {0.f, 0.f};
-  float F = 0.f, inv_F = INFINITY;
+  float F = 0.f, inv_F = INFINITY, f_min = 0.f;   // (f_min: 2^-90 of the largest factor met)
   f16x8 ones;
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = (f16)1.f;
@@ -479,9 +479,11 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
       // O is held in units of F, a value factor omega vs met before; a slot's probabilities carry f / F, in the
       // exponent.  Within 2^-1 .. 2^6 of F they stay below 2^14, and one that f16's smallest step rounds away is
       // below 2^-24 of the row's largest; past that F becomes f.  f = 0 leaves O alone and counts in the sum, and so
-      // does an f 2^-90 of F.
+      // does an f below 2^-90 of the largest factor met, so that F stays above that and O in f32's range (448 2^90
+      // times the sum of the probabilities), however the factors fall from slot to slot.
       float r = f * inv_F;
-      const bool none = f == 0.f || r < 0x1p-90f;
+      const bool none = f == 0.f || f < f_min;
+      f_min = fmaxf(f_min, f * 0x1p-90f);
       if (!none && !(r > 0x1p-1f && r < 0x1p6f)) {   // (the first slot; NaN too)
         const float beta = F / f;
         F = f;

@@ -375,3 +375,134 @@ def test_refusals_of_the_entry_points():
     a.q = 8
     with pytest.raises(ValueError, match="aligned"):
         L.call("moc_cache8_attend", ctypes.addressof(a), 256, 1 << 20, None)
+
+
+def tight(q, k8, ks, v8, vs, idx, omega):
+    """(o, bound) with the bound of float16 probabilities and part rows: the result's rounding 2^-8 |o|; probabilities, row
+    sums or part rows 2^-11 each and 2^-11 for everything in float32 (sums of up to 2^11 terms of 2^-24, exponentials,
+    quotients) on sum_j p_j |v_j|; the logits' float32 sums, 2^-16 of the largest logit's terms; float16's smallest
+    step, 2^-24 of the row's largest probability per key (in its numerator and, for the row sum, on |o|) and 2^-25 of a
+    value factor for a part row."""
+    B, Lq, H, D = q.shape
+    C, HK = ks.shape
+    out, bound = torch.zeros(B, Lq, H, D, dtype=torch.float64), torch.zeros(B, Lq, H, D, dtype=torch.float64)
+    for b in range(B):
+        sl = [s for s in range(idx.shape[1]) if 0 <= int(idx[b, s]) < C]
+        if not sl:
+            continue
+        ids, om = idx[b, sl].long(), omega[b, sl].double()
+        k = k8[ids].to(F32).double() * ks[ids].double()[:, :, None, None] * om[:, None, None, None]
+        f = vs[ids].double() * om[:, None]                              # value factors [slots][HK]
+        v = v8[ids].to(F32).double() * f[:, :, None, None]
+        qd = q[b].double().transpose(0, 1).view(HK, H // HK, Lq, D)
+        for hk in range(HK):
+            kk, vv = k[:, hk].reshape(-1, D), v[:, hk].reshape(-1, D)
+            x = qd[hk].reshape(-1, D)
+            p = torch.softmax(x @ kk.t() / 8, dim=1)
+            o, mag = p @ vv, p @ vv.abs()
+            logit = (x.abs() @ kk.abs().t() / 8).amax(1, keepdim=True)
+            top = p.amax(1, keepdim=True)
+            part = p.view(p.shape[0], len(sl), 64).sum(2) @ f[:, hk, None].abs()
+            e = (H8 * o.abs() + (3 * 2.0 ** -11 + 2.0 ** -16 * logit) * mag + 2.0 ** -24 * top * vv.abs().sum(0)
+                 + 2.0 ** -24 * 64 * len(sl) * top * o.abs() + 2.0 ** -25 * part)
+            at = slice(hk * (H // HK), (hk + 1) * (H // HK))
+            out[b, :, at] = o.view(H // HK, Lq, D).transpose(0, 1)
+            bound[b, :, at] = e.view(H // HK, Lq, D).transpose(0, 1)
+    return out, bound
+
+
+def check_tight(got, *case):
+    want, bound = tight(*case)
+    err = (got.cpu().double() - want).abs()
+    print(f"q {tuple(case[0].shape)}: worst {(err / (bound + 1e-30)).max().item():.3f} of the bound", flush=True)
+    assert (err <= bound + 1e-30).all()      # (NaN and infinity fail too)
+
+
+def prompts(B, Lq, H, HK, C, NS, seed):
+    """make() of a shape whose row blocks each take all slots in one workgroup (no part rows, so no workspace)."""
+    from memory_amd.decode import _attend8_workspace
+    assert _attend8_workspace(B, Lq, H, HK, NS) == 0
+    return make(B, Lq, H, HK, C, NS, seed)
+
+
+MANY = [(160, 65, 1, 1, 30, 24), (33, 130, 4, 2, 40, 17), (3, 400, 32, 8, 40, 33)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", MANY)
+def test_prompts_of_many_slots_per_workgroup(gpu_device, shape):
+    """Many slots one after the other in one workgroup: ordinary ones, skipped ids between live ones (the first and the
+    last among them), zero factors in the middle, whole sequences without a slot."""
+    case = list(prompts(*shape, seed=41))
+    check_tight(attend(gpu_device, *case), *case)
+    idx, omega, vs = case[5].clone(), case[6].clone(), case[4].clone()
+    B, NS = idx.shape
+    idx[torch.rand(B, NS, generator=gen(5)) < 0.3] = -1
+    idx[0, 0], idx[0, -1], idx[1, 3:6] = -1, 99, -5
+    idx[2] = -1
+    omega[torch.rand(B, NS, generator=gen(6)) < 0.2] = 0
+    vs[::5] = 0
+    case[4], case[5], case[6] = vs, idx, omega
+    got = attend(gpu_device, *case)
+    check_tight(got, *case)
+    assert not got[2].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", MANY[:2])
+def test_prompts_whose_logits_rise(gpu_device, shape):
+    """Logits of several hundred that rise, fall or mix from slot to slot: the running maximum is raised at most slots;
+    and a tile of NaN in the middle stays in the rows that read it."""
+    case = list(prompts(*shape, seed=43))
+    C, (B, NS) = shape[4], case[5].shape
+    for order in ("rise", "fall", "mix"):
+        size = {"rise": torch.linspace(0.2, 40, C), "fall": torch.linspace(40, 0.2, C), "mix": torch.rand(C, generator=gen(2)) * 40}[order]
+        c = [*case]
+        c[2] = case[2] * 0.3 * size[:, None]
+        c[5] = case[5].sort(1).values
+        check_tight(attend(gpu_device, *c), *c)
+    clean = attend(gpu_device, *c)
+    k8 = c[1].view(torch.uint8).clone()
+    hit = int(c[5][1, NS // 2])
+    k8[hit, -1, 3, 3] = 0x7f
+    c[1] = k8.view(FP8)
+    got = attend(gpu_device, *c)
+    HK, G = shape[3], shape[2] // shape[3]
+    for b in range(B):
+        own = slice((HK - 1) * G, HK * G)
+        assert torch.equal(got[b, :, :(HK - 1) * G], clean[b, :, :(HK - 1) * G])
+        assert got[b, :, own].isnan().all() if (c[5][b] == hit).any() else torch.equal(got[b, :, own], clean[b, :, own])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", MANY[:2])
+@pytest.mark.parametrize("chain", [(60, -20, -80), (60, 0, -29, -60, -90, -100), (-120, -60, 0, 60, 100), (110, 30, 25, -50, -120),
+                                   (-100, 60, -20, -80, 60, -29, -110), (0, -80, -125)])
+@pytest.mark.parametrize("by", ["scale"])
+def test_chains_of_value_factors(gpu_device, shape, chain, by):
+    """Value factors that fall, rise or alternate by up to 2^80 a slot and 2^230 in all, from the scales or (to 2^-125)
+    from the routing weights, in slot order: finite, and right within the factors that may count as nothing (below
+    2^-90 of the largest, which are far below the bound where the probabilities are alike)."""
+    if by == "weight" and max(chain) > 60:
+        chain = tuple(e - max(chain) for e in chain)
+    case = list(prompts(*shape, seed=47))
+    q, k8, ks, v8, vs, idx, omega = case
+    B, NS = idx.shape
+    C = ks.shape[0]
+    f = torch.exp2(torch.tensor(chain, dtype=F32).clamp(min=-125))
+    per = -(-NS // len(chain))
+    order = torch.arange(NS) // per
+    idx = torch.stack([torch.randperm(C, generator=gen(b))[:NS] for b in range(B)]).sort(1).values.int()
+    idx[:] = idx[0]                      # slots of all sequences alike, so that a chapter's scale is its slot's
+    q = (q.float() * 0.1).to(BF)
+    if by == "scale":
+        vs = torch.ones_like(vs)
+        vs[idx[0].long()] = f[order][:, None]
+        omega = torch.ones_like(omega)
+    else:
+        vs, omega = torch.ones_like(vs), f[order].expand(B, NS).contiguous()
+        omega = omega * torch.where(omega == omega.max(), 0.3, 1.0)
+    case = (q, k8, ks, v8, vs, idx, omega)
+    got = attend(gpu_device, *case)
+    assert got.isfinite().all()
+    check_tight(got, *case)
