@@ -234,14 +234,15 @@ __global__ __launch_bounds__(64 * kC8Waves) void cache8_unit_kernel(C8Unit a) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) mx = fmax_fast(mx, st[kb][x]);
     const float cf = w * ks;
-    const float m = quad_max_pl(mx) * cf;
+    mx = quad_max_pl(mx);
+    const float m = mx * cf;
     float ps = 0.f;
     f16x8 pf[2];
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const float p = c8_exp2(st[kb][x] * cf - m);
+        const float p = c8_exp2((st[kb][x] - mx) * cf);   // (at most 1, however large the logits)
         ps += p;
         pf[kb >> 1][4 * (kb & 1) + x] = (f16)p;
       }
@@ -496,16 +497,31 @@ __global__ __launch_bounds__(kC8Threads, 4) void cache8_prompt_kernel(C8Prompt a
       }
       r = none ? 1.f : r;
       const float lr = __builtin_amdgcn_logf(r), rr = __builtin_amdgcn_rcpf(r);
+      // Past 2^22 the product's rounding in m shows in the exponent (the difference below is fused): there the logits are
+      // rounded alike and subtracted first, and are at most kC8Slack.
+      float cc = c;
+      float off[2] = {m[0] - lr, m[1] - lr};
+      if (__any(fmax_fast(fabsf(m[0]), fabsf(m[1])) > 0x1p22f)) {
+#pragma clang fp contract(off)
+        cc = 1.f;
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+          off[qb] = -lr;
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) st[kb][qb][x] = st[kb][qb][x] * c - m[qb];
+        }
+      }
       f16x8 pf[2][2];
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
-        const float off = m[qb] - lr;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            pf[qb][h][x] = (f16)c8_exp2(st[2 * h][qb][x] * c - off);
-            pf[qb][h][4 + x] = (f16)c8_exp2(st[2 * h + 1][qb][x] * c - off);
+            pf[qb][h][x] = (f16)c8_exp2(st[2 * h][qb][x] * cc - off[qb]);
+            pf[qb][h][4 + x] = (f16)c8_exp2(st[2 * h + 1][qb][x] * cc - off[qb]);
           }
         // row sums of the rounded probabilities, in units of r
         f32x4 ls = f32x4{0.f, 0.f, 0.f, 0.f};

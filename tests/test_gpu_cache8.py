@@ -478,7 +478,7 @@ def test_prompts_whose_logits_rise(gpu_device, shape):
 @pytest.mark.parametrize("shape", MANY[:2])
 @pytest.mark.parametrize("chain", [(60, -20, -80), (60, 0, -29, -60, -90, -100), (-120, -60, 0, 60, 100), (110, 30, 25, -50, -120),
                                    (-100, 60, -20, -80, 60, -29, -110), (0, -80, -125)])
-@pytest.mark.parametrize("by", ["scale"])
+@pytest.mark.parametrize("by", ["scale", "weight"])
 def test_chains_of_value_factors(gpu_device, shape, chain, by):
     """Value factors that fall, rise or alternate by up to 2^80 a slot and 2^230 in all, from the scales or (to 2^-125)
     from the routing weights, in slot order: finite, and right within the factors that may count as nothing (below
@@ -506,3 +506,34 @@ def test_chains_of_value_factors(gpu_device, shape, chain, by):
     got = attend(gpu_device, *case)
     assert got.isfinite().all()
     check_tight(got, *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L", [1, 4, 65])
+@pytest.mark.parametrize("size", [2.0 ** 14, 2.0 ** 24, 2.0 ** 40, 2.0 ** 60])
+def test_logits_without_a_fraction(gpu_device, L, size):
+    """Logits so large that float32 holds no fraction of them: every row is finite, and where the largest leads by more
+    than their rounding (2^-16 of the largest logit's terms, and 30 for the others' probabilities) it takes all."""
+    case = prompts(160, 65, 1, 1, 30, 24, 59) if L == 65 else make(16, L, 4, 2, 12, 5, 59)
+    q, k8, ks, v8, vs, idx, omega = case
+    omega = 0.5 + omega / 2
+    ks = ks * size
+    case = (q, k8, ks, v8, vs, idx, omega)
+    got = attend(gpu_device, *case)
+    assert got.isfinite().all()
+    want, _ = reference(*case)
+    B, Lq, H, _ = q.shape
+    HK, rows, clear = ks.shape[1], 0, 0
+    for b in range(B):
+        ids, om = idx[b].long(), omega[b].double()
+        for h in range(H):
+            k = (k8[ids].to(F32).double() * ks[ids].double()[:, :, None, None] * om[:, None, None, None])[:, h // (H // HK)].reshape(-1, 64)
+            s, terms = q[b, :, h].double() @ k.t() / 8, (q[b, :, h].double().abs() @ k.abs().t() / 8).amax(1)
+            two = s.topk(2, dim=1).values
+            lead = two[:, 0] - two[:, 1] > 2.0 ** -16 * terms + 30
+            err = (got[b, :, h].cpu().double() - want[b, :, h]).abs()[lead]
+            # half a step of the result, and of the values' float32 factors
+            assert (err <= (H8 + 2.0 ** -20) * want[b, :, h].abs()[lead] + 2.0 ** -30).all()
+            rows, clear = rows + Lq, clear + int(lead.sum())
+    print(f"{clear} of {rows} rows are clear", flush=True)
+    assert clear > rows // 2
