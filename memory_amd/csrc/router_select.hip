@@ -250,7 +250,12 @@ inline size_t select_row_lds(int n, int G, int k) { return (size_t)n * 8 + (size
 // argument is off by 3 2^-24 |z - m| (difference, product, constant), which moves p by |z - m| p 3 2^-24 <= 1.2 2^-24 with
 // p <= 1 (x e^-x <= 0.37), the exponential and 1 / Z by 2 2^-24 p each...: together below 2^-21.  The bias' addition
 // rounds by 2^-24 |key|.
+// The softmax's sum Z itself is off by (3 sum p |z - m| + 2) 2^-24 of it, below 20 2^-24 for up to 6,144 chapters (sum
+// p |z - m| = y log(n / y) / (1 + y) <= 5.9, n chapters of one logit that together weigh y times the largest).  It moves all keys
+// of a row to the same side, by p times it, below 9 2^-24; a difference of two keys, whose own errors are below 1 and
+// 4 2^-24 where p is that large, stays within twice the bound above.
 constexpr float kSelEps = 0x1p-21f;
+constexpr double kSelSumErr = 0x1p-19;
 constexpr int kSelMaxima = 256;
 constexpr int kSelCand = 256;
 constexpr int kSelTeamK = 64;
@@ -509,11 +514,13 @@ __device__ __forceinline__ bool select_team(const SelArgs& a, int64_t r, SelTeam
         const uint64_t near = __ballot(in && sc >= first - 2.f * err && sc <= last + 2.f * err);
         const uint64_t sure = __ballot(in && sc > last + 2.f * err);
         uint64_t score = 0;   // lane g: group g's exact score, ordered
+        float most = 0.f;     // and the largest of its chapters' scores in it
         for (uint64_t todo = near; todo; todo &= todo - 1) {
           const int g = __builtin_ctzll(todo);
           const float lo = __shfl(a.best == 2 ? g2 : g1, g, 64);
           const float cut = lo - 2.f * (kSelEps + 0x1p-24f * fabsf(lo));
           uint64_t e1 = 0, e2 = 0;   // the lane's two largest exact keys of the group
+          float sg = 0.f;            // the largest score among the group's keys in question
           if (active && grp == g) {
             uint32_t bits[(E + 31) / 32];
             lane_bits<E>(v, fmaxf(cut, -FLT_MAX), bits);
@@ -521,9 +528,11 @@ __device__ __forceinline__ bool select_team(const SelArgs& a, int64_t r, SelTeam
             for (int i = 0; i < (E + 31) / 32; ++i)
               for (uint32_t w = bits[i]; w; w &= w - 1) {
                 const int c = c0 + chapter(32 * i + __builtin_ctz(w));
-                const uint64_t k = key64(score64(z[c], a.sigmoid, m, Z) + (b ? (double)b[c] : 0.0));
+                const double sc64 = score64(z[c], a.sigmoid, m, Z);
+                const uint64_t k = key64(sc64 + (b ? (double)b[c] : 0.0));
                 e2 = k > e1 ? e1 : k > e2 ? k : e2;
                 e1 = k > e1 ? k : e1;
+                if constexpr (MODE == kKeySoftmax) sg = fmaxf(sg, (float)sc64);
               }
           }
 #pragma unroll
@@ -549,6 +558,10 @@ __device__ __forceinline__ bool select_team(const SelArgs& a, int64_t r, SelTeam
           }
           const double s1 = key64_inv(e1);
           if (lane == g) score = a.best == 1 || e2 == 0 ? e1 : key64(s1 + key64_inv(e2));
+          if constexpr (MODE == kKeySoftmax) {
+            sg = team_max<NW>(sg, sm, wave);
+            if (lane == g) most = sg;
+          }
         }
         const int room = a.top - __popcll(sure);
         int place = 0;
@@ -557,7 +570,22 @@ __device__ __forceinline__ bool select_team(const SelArgs& a, int64_t r, SelTeam
           const uint64_t o = __shfl((unsigned long long)score, g, 64);
           place += o > score || (o == score && g < lane);
         }
-        keep = sure | __ballot((near >> lane & 1) && place < room);
+        const uint64_t chosen = __ballot((near >> lane & 1) && place < room);
+        keep = sure | chosen;
+        if constexpr (MODE == kKeySoftmax) {
+          // Z's error moves two groups' totals by as much of the difference of their scores, which biases may hide: it is
+          // below twice the larger score.  A pair across the cut that is no further apart goes to exact sums.
+          if (b) {
+            bool unclear = false;
+            for (uint64_t todo = near & ~chosen; todo; todo &= todo - 1) {
+              const int g = __builtin_ctzll(todo);
+              const double o = key64_inv(__shfl((unsigned long long)score, g, 64));
+              const float om = __shfl(most, g, 64);
+              unclear |= (chosen >> lane & 1) && key64_inv(score) - o <= 2.0 * kSelSumErr * (double)fmaxf(most, om);
+            }
+            if (__any(unclear)) return false;   // (the same in every wave)
+          }
+        }
       }
     }
   }
@@ -689,9 +717,9 @@ __device__ __forceinline__ bool select_team(const SelArgs& a, int64_t r, SelTeam
       if (TL * i < ncand) {   // (the same in every lane)
         rank[i] += kj > key[i] || (kj == key[i] && ij < id[i]);
         if constexpr (MODE == kKeySoftmax) {
-          // Z is off by up to 2^-21, which moves a pair of keys by as much of their scores' difference
+          // Z's error moves a pair of keys by as much of their scores' difference
           const double gap = fabs(key64_inv(kj) - key64_inv(key[i]));
-          unclear |= tl + TL * i < ncand && ij != id[i] && gap <= 0x1p-20 * (double)sc[i] && z[ij] != z[id[i]];
+          unclear |= tl + TL * i < ncand && ij != id[i] && gap <= kSelSumErr * (double)sc[i] && z[ij] != z[id[i]];
         }
       }
     }

@@ -345,3 +345,53 @@ def test_balance_bias_stays_in_float32():
     assert torch.equal(r.balance_bias, want) and "balance_bias" in r.state_dict()
     assert torch.equal(r.half().float().balance_bias, want) and r.balance_bias is dict(r.named_buffers())["balance_bias"]
     assert ChapterRouter(32, 9, 2).to(torch.bfloat16).balance_bias is None
+
+
+def near_cut(R, C, S, best, seed):
+    """Peaked softmax rows of two groups, and a bias on the best chapter of the second one: the groups' totals differ
+    by 2^-27 .. 2^-40 either way, their scores' sums by about a half.  Two chapters outside either group's best give
+    the sum of exponentials its value."""
+    g0 = gen(seed)
+    n, per = C - S, (C - S) // 2
+    z = torch.randn(R, n, generator=g0) - 1
+    z[:, per - 2:per] = -20.0                        # the two chapters that set the sum
+    z[:, [3, 5]] = 8 + 0.02 * torch.rand(R, 2, generator=g0)
+    z[:, [per + 2, per + 7]] = 6.5 + 0.02 * torch.rand(R, 2, generator=g0)
+    bias = torch.zeros(C)
+    e = z.double().exp()
+    pairs = lambda x: x.topk(best, dim=1).values.sum(1)
+    # the best of group two with the bias on its chapter: that chapter (and the larger other one)
+    two = e[:, per + 2] + (e[:, per + 7] if best == 2 else 0)
+    gap = torch.exp2(-27 - 13 * torch.rand(R, generator=g0, dtype=torch.float64)) * torch.where(torch.rand(R, generator=g0) < 0.5, 1.0, -1.0)
+    rest = e[:, :per - 2].sum(1) + e[:, per:].sum(1)
+    apart = pairs(e[:, :per]) - two
+    bias[S + per + 2] = (apart / (rest + 700)).median().float()
+    total = apart / (bias[S + per + 2].double() + gap)        # sum of exponentials for which the totals differ by gap
+    assert (total - rest > 1).all() and (total - rest < 1500).all()
+    z[:, per - 2] = torch.log(total - rest - 2.0 ** -7).float()
+    z[:, per - 1] = torch.log(total - rest - z[:, per - 2].double().exp()).float()
+    s = torch.softmax(z.double(), 1)
+    have = pairs(s[:, :per]) - s[:, per + 2] - (s[:, per + 7] if best == 2 else 0) - bias[S + per + 2].double()
+    assert (have.sign() == gap.sign()).all() and (have.abs() > 2.0 ** -42).all() and (have.abs() < 2.0 ** -26).all()
+    return torch.cat([torch.zeros(R, S), z], 1), bias
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [5, 1100])
+@pytest.mark.parametrize("C,k", [(1025, 16), (257, 8), (4097, 64), (1025, 70)])
+@pytest.mark.parametrize("best", [1, 2])
+def test_softmax_groups_near_the_cut_with_unequal_biases(gpu_device, R, C, k, best):
+    """Groups whose totals (scores and biases) differ by less than a float32 sum of exponentials tells apart."""
+    z, bias = near_cut(R, C, 1, best, R + C + best)
+    compare(z, k, 1, gpu_device, 1, bias, "softmax", 2, 1, best)
+
+
+def test_near_cut_tells_a_float32_sum_from_an_exact_one():
+    """Rows of near_cut change sides where the sum of exponentials is 2^-23 off."""
+    z, bias = near_cut(400, 1025, 1, 2, 3)
+    zd = z[:, 1:].double()
+    sides = []
+    for off in (0.0, 2.0 ** -23):
+        s = zd.exp() / (zd.exp().sum(1, keepdim=True) * (1 + off)) + bias[1:].double()
+        sides.append(s[:, :512].topk(2).values.sum(1) > s[:, 512:].topk(2).values.sum(1))
+    assert (sides[0] != sides[1]).float().mean() > 0.2
