@@ -824,7 +824,14 @@ __global__ __launch_bounds__(kSelThreads) void router_select_bwd_kernel(SelBwdAr
   __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
   for (int j = tid; j < a.k; j += NT) {
     const double s = a.s_sel[r * a.k + j], ds = f * ((double)a.dw[r * a.k + j] - shift);
-    row[a.idx[r * a.k + j]] = (float)(a.sigmoid ? ds * s * (1.0 - s) : s * (ds - t));
+    const int32_t c = a.idx[r * a.k + j];
+    if (a.sigmoid) {
+      // s (1 - s) from the logit, e^-|z| / (1 + e^-|z|)^2: a score near 1 that was rounded to f32 has lost 1 - s
+      const double e = exp(-fabs((double)a.z[r * a.ldz + c])), q = 1.0 + e;
+      row[c] = (float)(ds * (e / (q * q)));
+    } else {
+      row[c] = (float)(s * (ds - t));
+    }
   }
 }
 

@@ -395,3 +395,34 @@ def test_near_cut_tells_a_float32_sum_from_an_exact_one():
         s = zd.exp() / (zd.exp().sum(1, keepdim=True) * (1 + off)) + bias[1:].double()
         sides.append(s[:, :512].topk(2).values.sum(1) > s[:, 512:].topk(2).values.sum(1))
     assert (sides[0] != sides[1]).float().mean() > 0.2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [9, 1100])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_sigmoid_gradient_of_saturated_scores(gpu_device, R, renorm):
+    """Every element's gradient ds s (1 - s) on its own scale, also where the score rounds to 1 in float32.  The kernel
+    forms s (1 - s) from the logit and ds from scores rounded to float32 (2^-24 each), in float64, and rounds the
+    result (2^-24): 2^-21 of the terms of ds times s (1 - s), and half a subnormal step."""
+    C, S, k = 301, 1, 12
+    g0 = gen(31)
+    z = torch.randn(R, C, generator=g0)
+    at = torch.randperm(C - S, generator=g0)[:k] + S
+    z[:, at] = 8 + 50 * torch.rand(R, k, generator=g0)             # s to 1 - e^-58
+    z[1] = -60 - 25 * torch.rand(C, generator=g0)                  # and down to e^-85
+    dw = torch.randn(R, k, generator=g0)
+    idx, w, dz = run(z, k, S, gpu_device, dw, score="sigmoid", renormalize=renorm, scale=1.5)
+    ridx, rw, _ = reference(z, k, S, "sigmoid", renorm=renorm, scale=1.5)
+    assert torch.equal(idx.cpu(), ridx)
+    zs, d = z.double().gather(1, ridx.long()), dw.double()
+    s, slope = torch.sigmoid(zs), torch.sigmoid(zs) * torch.sigmoid(-zs)
+    if renorm:
+        D = s.sum(1, keepdim=True).clamp_min(1e-12)
+        shift = torch.where(s.sum(1, keepdim=True) > 1e-12, (d * s).sum(1, keepdim=True) / D, 0.0)
+        ds, terms = 1.5 * (d - shift) / D, 1.5 * (d.abs() + (d * s).abs().sum(1, keepdim=True) / D) / D
+    else:
+        ds, terms = 1.5 * d, 1.5 * d.abs()
+    err = (dz.cpu().double().gather(1, ridx.long()) - ds * slope).abs()
+    bound = 2.0 ** -21 * terms * slope + 2.0 ** -150
+    print(f"worst {(err / bound).max().item():.3f} of the bound", flush=True)
+    assert (err <= bound).all()
