@@ -105,8 +105,8 @@ int moc_router_seq_bwd(const float* logits, const int32_t* idx, const float* w, 
  * sum of its group_best (1 or 2) largest keys and the top_groups best stay (ties: lower group); the k largest keys
  * of those, keys descending (compared in f64), equal keys by ascending chapter.  w = scale s / max(sum s, 1e-12)
  * (renormalize) or scale s.  logits f32 [R] rows of stride ldz; idx i32 [R, k] (global ids); w f32 [R, k];
- * s_sel f32 [R, k] (the selected s) and row_stats f32 [R, 2] (softmax: maximum and sum of exp) are the backward's
- * inputs, NULL to skip.  C <= 16,384, k <= 1,024, groups <= 1,024. */
+ * s_sel f32 [R, k] (the selected s) and row_stats f32 [R, 3] (softmax: maximum, sum of exp, and the share of the
+ * chapters that are not selected) are the backward's inputs, NULL to skip.  C <= 16,384, k <= 1,024, groups <= 1,024. */
 #define MOC_SCORE_SOFTMAX 0
 #define MOC_SCORE_SIGMOID 1
 int moc_router_select(const float* logits, int64_t ldz, int64_t R, int64_t C, int S, int k, int score, const float* bias,

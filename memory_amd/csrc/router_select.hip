@@ -12,7 +12,8 @@
 //
 // Backward, ds_j = scale (dw_j - [sum > 1e-12] (sum_i dw_i s_i) / D) / D with D = max(sum, 1e-12), or scale dw_j:
 //   sigmoid: dz_j = ds_j s_j (1 - s_j) on the selected, 0 elsewhere
-//   softmax: dz_c = s_c (ds_c [selected] - sum_j ds_j s_j); the sum is 0 for renormalised weights.
+//   softmax: dz_c = s_c (ds_c [selected] - sum_j ds_j s_j); the sum is 0 for renormalised weights.  ds_c - sum_j ds_j s_j is
+//   formed as ds_c (1 - sum_j s_j) + sum_j (ds_c - ds_j) s_j with the mass that is not selected from the forward.
 //
 // Rows are held in registers by one wave, or by four where there are few; what does not fit them, or cannot be decided
 // from f32 keys with a few exact ones, goes to a workgroup with every exact key in LDS.
@@ -50,6 +51,13 @@ struct SelArgs {
   int32_t* idx;
   float *w, *s_sel, *row_stats;
 };
+
+// the softmax's maximum, sum, and the part of its mass that is not selected (sel: the selected's part of the sum)
+__device__ __forceinline__ void put_row_stats(const SelArgs& a, int64_t r, float m, double Z, double sel) {
+  a.row_stats[3 * r] = m;
+  a.row_stats[3 * r + 1] = (float)Z;
+  a.row_stats[3 * r + 2] = (float)((Z > sel ? Z - sel : 0.0) / Z);
+}
 
 // a chapter's exact score (m, Z: the row's maximum and sum for softmax); one exponential and one quotient in the code
 __device__ __forceinline__ double score64(float x, int sigmoid, float m, double Z) {
@@ -100,10 +108,6 @@ __device__ __forceinline__ void select_row(const SelArgs& a, int64_t r, char* ld
     double s = 0.0;
     for (int c = tid; c < n; c += NT) s += exp((double)z[c] - (double)mf);   // (every logit -inf: NaN, as the formula)
     Z = blk_sum<NT>(s, red);
-    if (a.row_stats && tid == 0) {
-      a.row_stats[2 * r] = mf;
-      a.row_stats[2 * r + 1] = (float)Z;
-    }
   }
   auto score = [&](float v) { return score64(v, a.sigmoid, mf, Z); };
   for (int c = tid; c < n; c += NT) {
@@ -215,6 +219,12 @@ __device__ __forceinline__ void select_row(const SelArgs& a, int64_t r, char* ld
   double sum = 0.0;
   for (int i = tid; i < a.k; i += NT) sum += (double)sel_s[i];
   sum = blk_sum<NT>(sum, red);
+  if (a.row_stats) {
+    double e = 0.0;
+    for (int i = tid; i < a.k; i += NT) e += exp((double)z[id_at[i]] - (double)mf);
+    e = blk_sum<NT>(e, red);
+    if (tid == 0) put_row_stats(a, r, mf, Z, e);
+  }
   const double D = a.renorm ? (sum > 1e-12 ? sum : (sum == sum ? 1e-12 : sum)) : 1.0;
   for (int i = tid; i < a.k; i += NT) {
     const int64_t o = r * a.k + i;
@@ -431,10 +441,6 @@ __device__ __forceinline__ bool select_team(const SelArgs& a, int64_t r, SelTeam
         if constexpr (MODE == kKeySoftmax) v[j][e] = v[j][e] == -INFINITY ? -INFINITY : p;
       }
     Z = team_sum<NW>(s, sm, wave);
-    if (a.row_stats && tl == 0) {
-      a.row_stats[2 * r] = m;
-      a.row_stats[2 * r + 1] = (float)Z;
-    }
   }
   // keys
   if constexpr (MODE != kKeyLogit) {
@@ -739,6 +745,17 @@ __device__ __forceinline__ bool select_team(const SelArgs& a, int64_t r, SelTeam
 #pragma unroll
   for (int i = 0; i < NC; ++i) sum += rank[i] < a.k ? (double)sc[i] : 0.0;
   sum = team_sum<NW>(sum, sm, wave);
+  if constexpr (MODE != kKeySigmoid) {
+    if (a.row_stats) {
+      // (the same bits that the selected have in Z)
+      double e = 0.0;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        e += rank[i] < a.k ? (double)__builtin_amdgcn_exp2f((z[id[i]] - m) * 1.4426950408889634f) : 0.0;
+      e = team_sum<NW>(e, sm, wave);
+      if (tl == 0) put_row_stats(a, r, m, Z, e);
+    }
+  }
   const double f = (double)a.scale / (a.renorm ? fmax(sum, 1e-12) : 1.0);
 #pragma unroll
   for (int i = 0; i < NC; ++i)
@@ -811,11 +828,13 @@ __global__ __launch_bounds__(kSelThreads) void router_select_bwd_kernel(SelBwdAr
   const double t = a.sigmoid || (a.renorm && !clamped) ? 0.0 : (double)a.scale * dot / D;
   const double f = (double)a.scale / D, shift = a.renorm && !clamped ? dot / D : 0.0;   // ds_j = f (dw_j - shift)
   float* row = a.dz + r * a.C;
+  double rest = 0.0;   // of the softmax's mass: what is not selected
   if (t == 0.0) {
     for (int64_t c = tid; c < a.C; c += NT) row[c] = 0.f;
   } else {
-    const float m = a.row_stats[2 * r];
-    const float ft = (float)(-t / (double)a.row_stats[2 * r + 1]);
+    const float m = a.row_stats[3 * r];
+    const float ft = (float)(-t / (double)a.row_stats[3 * r + 1]);
+    rest = (double)a.row_stats[3 * r + 2];
     for (int64_t c = tid; c < a.C; c += NT) row[c] = c < a.S ? 0.f : expf(a.z[r * a.ldz + c] - m) * ft;
   }
   // (the row's stores are done before the entries')
@@ -830,7 +849,8 @@ __global__ __launch_bounds__(kSelThreads) void router_select_bwd_kernel(SelBwdAr
       const double e = exp(-fabs((double)a.z[r * a.ldz + c])), q = 1.0 + e;
       row[c] = (float)(ds * (e / (q * q)));
     } else {
-      row[c] = (float)(s * (ds - t));
+      // (1 - sum s from the rest of the row: a score near 1 that was rounded to f32 has lost it)
+      row[c] = (float)(s * (t == 0.0 ? ds : ds * rest + (ds * sum - t)));
     }
   }
 }

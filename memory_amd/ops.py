@@ -179,7 +179,7 @@ def _router_select_forward(z, bias, cfg, trains):
     idx = torch.empty((R, k), device=dev, dtype=torch.int32)
     w = torch.empty((R, k), device=dev, dtype=torch.float32)
     # what a backward reads: the selected scores, and softmax's row statistics
-    kept = torch.empty(R * (k + (2 if score == 0 else 0)), device=dev, dtype=torch.float32) if trains else None
+    kept = torch.empty(R * (k + (3 if score == 0 else 0)), device=dev, dtype=torch.float32) if trains else None
     at = None if kept is None else kept.data_ptr()
     with L.on_device(dev):
         call("moc_router_select", z.data_ptr(), z.stride(0), R, C, S, k, score, ptr(bias), groups, top_groups, best, renorm,

@@ -426,3 +426,31 @@ def test_sigmoid_gradient_of_saturated_scores(gpu_device, R, renorm):
     bound = 2.0 ** -21 * terms * slope + 2.0 ** -150
     print(f"worst {(err / bound).max().item():.3f} of the bound", flush=True)
     assert (err <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [9, 1100])
+@pytest.mark.parametrize("C,k", [(301, 12), (301, 1), (301, 70), (70, 69)])
+def test_softmax_gradient_of_saturated_scores(gpu_device, R, C, k):
+    """Scores that are not renormalised, one of them near 1: dz_j = s_j (ds_j (1 - sum of the selected s) + sum_i (ds_j
+    - ds_i) s_i), each element on the scale of these terms (TOL, as everywhere in this file)."""
+    S = 1
+    g0 = gen(33)
+    z = torch.randn(R, C, generator=g0)
+    z[:, 7] = 2 + 35 * torch.rand(R, generator=g0)
+    dw = torch.randn(R, k, generator=g0)
+    idx, w, dz = run(z, k, S, gpu_device, dw, score="softmax", renormalize=False, scale=1.5)
+    ridx, rw, _ = reference(z, k, S, "softmax", renorm=False, scale=1.5)
+    assert torch.equal(idx.cpu(), ridx)
+    p = z[:, S:].double()
+    p = (p - torch.logsumexp(p, 1, keepdim=True)).exp()
+    s, ds = p.gather(1, ridx.long() - S), 1.5 * dw.double()
+    left = p.scatter(1, ridx.long() - S, 0.0).sum(1, keepdim=True)
+    pairs = ds[:, :, None] - ds[:, None, :]
+    want = s * (ds * left + (pairs * s[:, None, :]).sum(2))
+    scale = s * (ds.abs() * left + (pairs.abs() * s[:, None, :]).sum(2))
+    err = (dz.cpu().double().gather(1, ridx.long()) - want).abs()
+    # (float64's own sums of the row leave 2^-48; float32's smallest step)
+    bound = TOL * scale + 2.0 ** -48 * s * ds.abs().amax(1, keepdim=True) + 2.0 ** -149
+    print(f"worst {(err / bound).max().item():.3f} of the bound", flush=True)
+    assert (err <= bound).all()
