@@ -172,6 +172,11 @@ def router_topk(logits: torch.Tensor, k: int, exclude_prefix_chapters: int = 0):
 _SCORES = {"softmax": 0, "sigmoid": 1}
 
 
+def _row_stride(z: torch.Tensor) -> int:
+    """Elements from row to row; of a single row, whose stride may be anything, its length."""
+    return z.stride(0) if z.shape[0] > 1 else z.shape[1]
+
+
 def _router_select_forward(z, bias, cfg, trains):
     k, S, score, groups, top_groups, best, renorm, scale = cfg
     R, C = z.shape
@@ -182,7 +187,7 @@ def _router_select_forward(z, bias, cfg, trains):
     kept = torch.empty(R * (k + (3 if score == 0 else 0)), device=dev, dtype=torch.float32) if trains else None
     at = None if kept is None else kept.data_ptr()
     with L.on_device(dev):
-        call("moc_router_select", z.data_ptr(), z.stride(0), R, C, S, k, score, ptr(bias), groups, top_groups, best, renorm,
+        call("moc_router_select", z.data_ptr(), _row_stride(z), R, C, S, k, score, ptr(bias), groups, top_groups, best, renorm,
              scale, idx.data_ptr(), w.data_ptr(), at, at + 4 * R * k if trains and score == 0 else None, stream_ptr(dev))
     return idx, w, kept
 
@@ -213,7 +218,7 @@ class _RouterSelect(torch.autograd.Function):
         dz = torch.empty((R, C), device=dev, dtype=torch.float32)
         at = kept.data_ptr()
         with L.on_device(dev):
-            call("moc_router_select_bwd", z.data_ptr(), z.stride(0), idx.data_ptr(), at, at + 4 * R * k if score == 0 else None,
+            call("moc_router_select_bwd", z.data_ptr(), _row_stride(z), idx.data_ptr(), at, at + 4 * R * k if score == 0 else None,
                  dw.data_ptr(), R, C, S, k, score, renorm, scale, dz.data_ptr(), stream_ptr(dev))
         return dz, None, None
 
@@ -255,7 +260,7 @@ def router_select(logits: torch.Tensor, k: int, exclude_prefix_chapters: int = 0
         raise ValueError(f"bias of shape {tuple(bias.shape)}, expected {(C,)}")
     L.require_same_gpu(logits, bias)
     z = logits if logits.dtype == torch.float32 else logits.float()
-    if z.stride(1) != 1 or z.stride(0) < C:
+    if z.stride(1) != 1 or (R > 1 and z.stride(0) < C):
         z = z.contiguous()
     if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
         bias = bias.detach().float().contiguous()

@@ -454,3 +454,23 @@ def test_softmax_gradient_of_saturated_scores(gpu_device, R, C, k):
     bound = TOL * scale + 2.0 ** -48 * s * ds.abs().amax(1, keepdim=True) + 2.0 ** -149
     print(f"worst {(err / bound).max().item():.3f} of the bound", flush=True)
     assert (err <= bound).all()
+
+
+@pytest.mark.gpu
+def test_one_row_of_any_strides(gpu_device):
+    """A single row whose row stride says nothing (a transposed column), forward and backward."""
+    from memory_amd import ops
+    z = torch.randn(1, 257, generator=gen(12)).to(gpu_device)
+    dw = torch.randn(1, 8, generator=gen(13)).to(gpu_device)
+    column = z.reshape(257, 1).t()
+    assert column.stride() == (1, 1)
+    for score in ("sigmoid", "softmax"):
+        outs = []
+        for view in (z, column, z.expand(3, 257)[1:2], z.as_strided((1, 257), (5, 1))):
+            leaf = view.detach().requires_grad_(True)
+            idx, w = ops.router_select(leaf, 8, 1, score=score, renormalize=False)
+            outs.append((idx, w, torch.autograd.grad(w, leaf, dw)[0]))
+            with torch.no_grad():
+                assert all(torch.equal(a, b) for a, b in zip(outs[0], ops.router_select(view, 8, 1, score=score, renormalize=False)))
+        for o in outs[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(outs[0], o))
