@@ -767,16 +767,16 @@ class _GatedResidualNorm(torch.autograd.Function):
         dx = torch.empty_like(x) if need[0] else None
         dr = torch.empty_like(r) if need[1] else None
         dg = torch.empty_like(gate) if need[2] and mode in (_GATE_TOKEN, _GATE_FULL) else None
-        # the parameters' gradients and the workspace in one allocation (16-byte aligned parts)
-        n_par = (5 * d + 4) // 4 * 4
-        buf = torch.empty(n_par + _gated_norm_workspace(R, d), device=dev, dtype=torch.float32)
+        # (the parameters' gradients outlive the call, as .grad: they share nothing with its workspace)
+        buf = torch.empty(5 * d + 1, device=dev, dtype=torch.float32)
+        n_ws = _gated_norm_workspace(R, d)
+        ws = torch.empty(n_ws, device=dev, dtype=torch.float32)
         if R == 0:
             buf.zero_()
         args = _gated_norm_args(x, r, gate, w1, b1, w2, b2, cfg, None, None, stats)
-        at = buf.data_ptr()
-        out = _pack_gated_norm_grads(ptr0(dh), ptr0(dn), ptr0(dx), ptr0(dr), ptr0(dg), at)
+        out = _pack_gated_norm_grads(ptr0(dh), ptr0(dn), ptr0(dx), ptr0(dr), ptr0(dg), buf.data_ptr())
         with L.on_device(dev):
-            call("moc_gated_norm_bwd", args, out, at + 4 * n_par, 4 * (buf.numel() - n_par), stream_ptr(dev))
+            call("moc_gated_norm_bwd", args, out, ws.data_ptr(), 4 * n_ws, stream_ptr(dev))
         dw1 = db1 = dw2 = db2 = None
         if w1 is not None and need[3]:
             dw1 = buf[:d]

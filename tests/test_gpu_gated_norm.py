@@ -289,3 +289,14 @@ def test_refusals():
     a.d, a.norm, a.norm2, a.gate_mode = 8, 1, 1, 9
     with pytest.raises(ValueError, match="gate mode"):
         L.call("moc_gated_norm_fwd", ctypes.addressof(a), None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["scalar", "channel", "token"])
+def test_parameter_gradients_hold_no_workspace(gpu_device, gate):
+    """What stays allocated behind the parameters' gradients is their own size, not the backward's workspace."""
+    d = 768
+    t, dh, dn = make((2048, d), BF, F32, "layer", gate, 21)
+    _, _, g = run(t, gpu_device, "layer", 1.0, 1e-5, dh, dn)
+    for name in ("w1", "b1", "w2", "b2") + (("gate",) if gate != "token" else ()):
+        assert g[name].untyped_storage().nbytes() <= 4 * (5 * d + 64), name
