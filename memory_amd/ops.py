@@ -14,7 +14,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd import function as autograd_function
+from torch.autograd import forward_ad, function as autograd_function
 
 from . import _lib as L
 from ._lib import call, ptr, ptr0, stream_ptr
@@ -28,6 +28,14 @@ def once_differentiable(backward):
     def run(ctx, *grads):
         return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
+
+
+def _differentiated(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a call on these tensors goes through its autograd function: one of them wants a gradient, or a
+    forward-mode level is open, where the function refuses a tangent that the kernels would drop."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def recorded_backward(fn, inputs, needs, grad_outputs):
@@ -265,7 +273,7 @@ def router_select(logits: torch.Tensor, k: int, exclude_prefix_chapters: int = 0
     if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
         bias = bias.detach().float().contiguous()
     cfg = (k, S, _SCORES[score], G, g, best, bool(renormalize), float(scale))
-    if z.requires_grad and torch.is_grad_enabled():
+    if _differentiated(z):
         return _RouterSelect.apply(z, None if bias is None else bias.detach(), cfg)
     return _router_select_forward(z, bias, cfg, False)[:2]
 
@@ -855,8 +863,7 @@ def gated_residual_norm(x: torch.Tensor, residual: torch.Tensor, *, post_weight:
             gate = gate.float()
         gate = gate.contiguous()
     cfg = (mode, (kind, kind2), float(residual_scale), (float(eps), float(eps if pre_eps is None else pre_eps)))
-    if torch.is_grad_enabled() and (x2.requires_grad or r2.requires_grad or any(
-            t is not None and t.requires_grad for t in (gate, w1, b1, w2, b2))):
+    if _differentiated(x2, r2, gate, w1, b1, w2, b2):
         out = _GatedResidualNorm.apply(x2, r2, gate, w1, b1, w2, b2, cfg)
         h, n = out if w2 is not None else (out, None)
     else:

@@ -300,3 +300,22 @@ def test_parameter_gradients_hold_no_workspace(gpu_device, gate):
     _, _, g = run(t, gpu_device, "layer", 1.0, 1e-5, dh, dn)
     for name in ("w1", "b1", "w2", "b2") + (("gate",) if gate != "token" else ()):
         assert g[name].untyped_storage().nbytes() <= 4 * (5 * d + 64), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["x", "r", "gate", "w1", "w2"])
+def test_forward_mode_is_refused(gpu_device, which):
+    """A tangent raises, as in the single norm: it is never dropped."""
+    import torch.autograd.forward_ad as fwd
+    from memory_amd import ops
+    t, _, _ = make((5, 64), F32, F32, "rms", "channel", 1)
+    t = {k: v.to(gpu_device) for k, v in t.items() if v is not None}
+    go = lambda v: ops.gated_residual_norm(v["x"], v["r"], gate=v["gate"], post_weight=v["w1"], pre_weight=v["w2"])
+    want = go(t)
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError):
+            ops.row_norm(fwd.make_dual(t["x"], torch.ones_like(t["x"])), t["w1"], None, 1e-6, "rms")
+        with pytest.raises(NotImplementedError):
+            go({**t, which: fwd.make_dual(t[which], torch.ones_like(t[which]))})
+        got = go(t)                                  # (no tangent: as outside)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -474,3 +474,20 @@ def test_one_row_of_any_strides(gpu_device):
                 assert all(torch.equal(a, b) for a, b in zip(outs[0], ops.router_select(view, 8, 1, score=score, renormalize=False)))
         for o in outs[1:]:
             assert all(torch.equal(a, b) for a, b in zip(outs[0], o))
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(gpu_device):
+    """A tangent raises, as in the other selection: it is never dropped."""
+    import torch.autograd.forward_ad as fwd
+    from memory_amd import ops
+    z = torch.randn(5, 33, generator=gen(1)).to(gpu_device)
+    with fwd.dual_level():
+        dual = fwd.make_dual(z, torch.ones_like(z))
+        for f in (ops.router_topk, ops.router_select):
+            with pytest.raises(NotImplementedError):
+                f(dual, 4, 1)
+        idx, w = ops.router_select(z, 4, 1)          # (no tangent: as outside)
+    assert all(torch.equal(a, b) for a, b in zip((idx, w), ops.router_select(z, 4, 1)))
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda t: ops.router_select(t, 4, 1)[1], (z,), (torch.ones_like(z),))
