@@ -164,7 +164,8 @@ class MemoryDecodeCache:
         self.num_chapters, self.T, self.HK, self.dtype = int(num_chapters), int(tokens_per_chapter), \
             int(num_kv_heads), k_tiles.dtype
         if not eight:
-            self.k_tiles, self.v_tiles = k_tiles.contiguous(), v_tiles.contiguous()
+            # (the attention over several tokens copies 16-byte pieces of them to LDS)
+            self.k_tiles, self.v_tiles = _aligned(k_tiles), _aligned(v_tiles)
             return self
         if self.T != 64:
             raise ValueError(f"an 8-bit decode cache needs 64 tokens per chapter, got {self.T}")

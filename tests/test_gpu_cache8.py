@@ -537,3 +537,21 @@ def test_logits_without_a_fraction(gpu_device, L, size):
             rows, clear = rows + Lq, clear + int(lead.sum())
     print(f"{clear} of {rows} rows are clear", flush=True)
     assert clear > rows // 2
+
+
+@pytest.mark.gpu
+def test_full_tiles_of_any_address(gpu_device):
+    """bfloat16 and float32 tiles that start off a 16-byte boundary are copied to one when a cache is made of them."""
+    from memory_amd.decode import DecodeRouting, MemoryDecodeCache, decode_attention
+    q, k8, ks, v8, vs, idx, omega = make(3, 37, 4, 2, 12, 6, 4)
+    kw = dict(num_chapters=12, tokens_per_chapter=64, num_kv_heads=2)
+    routing = DecodeRouting(idx.to(gpu_device), omega.to(gpu_device), 12)
+    for dtype in (BF, F32):
+        k, v = ((t.float() * s[:, :, None, None]).to(gpu_device, dtype) for t, s in ((k8, ks), (v8, vs)))
+        off = [torch.empty(t.numel() + 1, device=gpu_device, dtype=dtype)[1:].view(t.shape).copy_(t) for t in (k, v)]
+        caches = [MemoryDecodeCache.from_tiles(*t, **kw) for t in ((k, v), off)]
+        assert caches[0].k_tiles.data_ptr() == k.data_ptr()
+        assert all(t.data_ptr() % 16 == 0 for c in caches for t in (c.k_tiles, c.v_tiles))
+        for x in (q, q[:, 0]):
+            a, b = (decode_attention(x.to(gpu_device), c, routing) for c in caches)
+            assert torch.equal(a, b)
