@@ -233,6 +233,9 @@ class MemoryStack(nn.Module):
         with torch.no_grad():
             for k, v in mem.items():
                 own[k].copy_(v.to(own[k].dtype))
+            for k, v in own.items():
+                if k.endswith(".balance_bias") and k not in mem and k[:-len("balance_bias")] + "router.weight" in mem:
+                    v.zero_()
             # a bank stepped by BankAdamW: its chapters were all brought to the last step before
             # the copy (state_dict above flushes), so the loaded values are current; the bf16
             # mirror the kernels read is refreshed from them

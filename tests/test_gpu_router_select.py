@@ -491,3 +491,23 @@ def test_forward_mode_is_refused(gpu_device):
     assert all(torch.equal(a, b) for a, b in zip((idx, w), ops.router_select(z, 4, 1)))
     with pytest.raises((RuntimeError, NotImplementedError)):
         torch.func.jvp(lambda t: ops.router_select(t, 4, 1)[1], (z,), (torch.ones_like(z),))
+
+
+def test_a_checkpoint_without_a_bias_starts_it_at_zero():
+    """Weights loaded over a router whose bias has moved: the bias of a checkpoint that has one, 0 of one that has
+    none; a state dict without that router leaves it alone."""
+    from memory_amd.checkpoint import MemoryStack
+    mem = dict(use_chapters=True, num_chapters=9, num_memory_tokens=9 * 64, top_k_chapters=2, num_shared_chapters=1,
+               router_options=dict(balance_bias=True))
+    stack = MemoryStack(hidden_dim=64, num_layers=1, num_heads=1, num_kv_heads=None, memory=mem)
+    moved = torch.linspace(-1, 1, 9)
+    router = next(iter(stack.routers.values()))
+    router.balance_bias.copy_(moved)
+    whole = {k: v.clone() for k, v in stack.state_dict().items()}
+    router.balance_bias.zero_()
+    stack.load_reference_state_dict(whole)
+    assert torch.equal(router.balance_bias, moved)
+    stack.load_reference_state_dict({k: v for k, v in whole.items() if not k.startswith("routers")}, strict=False)
+    assert torch.equal(router.balance_bias, moved)
+    stack.load_reference_state_dict({k: v for k, v in whole.items() if not k.endswith("balance_bias")})
+    assert not router.balance_bias.any()
