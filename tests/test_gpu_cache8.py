@@ -6,6 +6,8 @@ sums; probabilities are rounded to bfloat16 (2^-8 each), part rows of a chapter 
 sums may carry the probabilities' rounding: 2^-8 |o| + 3 2^-8 sum_j p_j |v_j|.  A logit's float32 sum of 64 products is off
 by at most 64 2^-24 sum |q k|, which moves a probability by as much: 2^-17 times the largest logit's terms."""
 
+import math
+
 import pytest
 import torch
 
@@ -555,3 +557,43 @@ def test_full_tiles_of_any_address(gpu_device):
         for x in (q, q[:, 0]):
             a, b = (decode_attention(x.to(gpu_device), c, routing) for c in caches)
             assert torch.equal(a, b)
+
+
+def half_way(L, sign):
+    """Half of a chapter's keys with probabilities just below (or above) the middle of two bfloat16 values, the other
+    half with 1/2 of the largest, values that cancel between the halves: roundings to bfloat16 all fall on one side."""
+    case = list(make(16, L, 4, 2, 3, 1, 53))
+    q, k, v = torch.zeros(16, L, 4, 64), torch.zeros(3, 2, 64, 64), torch.ones(3, 2, 64, 64)
+    k[:, :, 1:33, 0:4], k[:, :, 33:, 4:8] = -1.0, -1.0
+    v[:, :, 33:] = -1.0
+    for at, p in ((0, 0.5 + 2.0 ** -9 + sign * 2.0 ** -13), (4, 0.5)):
+        rest = -8 * math.log(p)
+        for i in range(4):
+            q[..., at + i] = float(torch.tensor(rest).to(BF))
+            rest -= float(q[0, 0, 0, at + i])
+    one = torch.ones(3, 2)
+    return q.to(BF), k.to(FP8), one, v.to(FP8), one, case[5], torch.ones_like(case[6])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L", [1, 4, 24])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_roundings_are_float16(gpu_device, L, sign):
+    """Where bfloat16 probabilities would be off by more than the bound."""
+    case = half_way(L, sign)
+    check_tight(attend(gpu_device, *case), *case)
+
+
+def test_bound_tells_bfloat16_probabilities():
+    """The same attention with probabilities rounded to bfloat16 is off by more than the bound, with float16 by less."""
+    for dt, fits in ((BF, False), (torch.float16, True)):
+        for sign in (-1, 1):
+            q, k8, ks, v8, vs, idx, omega = half_way(1, sign)
+            want, bound = tight(q, k8, ks, v8, vs, idx, omega)
+            s = q[0, 0, :1].double() @ k8[int(idx[0, 0]), 0].to(F32).double().t() / 8
+            p = torch.exp(s - s.amax(1, keepdim=True)).to(dt).double()
+            v = v8[int(idx[0, 0]), 0].to(F32).double()
+            for total in (p.sum(1, keepdim=True), torch.exp(s - s.amax(1, keepdim=True)).sum(1, keepdim=True)):
+                worst = (((p @ v / total).to(BF).double() - want[0, 0, :1]).abs() / bound[0, 0, :1]).max().item()
+                print(dt, sign, worst)
+                assert (worst <= 1) == fits
