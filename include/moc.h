@@ -117,7 +117,7 @@ int moc_router_select(const float* logits, int64_t ldz, int64_t R, int64_t C, in
 int moc_router_select_bwd(const float* logits, int64_t ldz, const int32_t* idx, const float* s_sel, const float* row_stats,
                           const float* dw, int64_t R, int64_t C, int S, int k, int score, int renormalize, float scale,
                           float* dlogits, hipStream_t stream);
-/* Balance step of the bias: counts i32 [C] = how often idx i32 [n] names each chapter (ids outside [0, C) are
+/* Balance step of the bias: counts i32 [C] = how often idx i32 [n] (n < 2^31) names each chapter (ids outside [0, C) are
  * skipped), then bias[c] += rate * sign(mean of counts[S..] - counts[c]) for c >= S. */
 int moc_router_balance(const int32_t* idx, int64_t n, int64_t C, int S, float rate, int32_t* counts, float* bias,
                        hipStream_t stream);

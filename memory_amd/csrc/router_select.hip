@@ -976,7 +976,7 @@ int moc_router_select_bwd(const float* logits, int64_t ldz, const int32_t* idx, 
 
 int moc_router_balance(const int32_t* idx, int64_t n, int64_t C, int S, float rate, int32_t* counts, float* bias,
                        hipStream_t stream) {
-  MOC_REQUIRE(n >= 0 && n < ((int64_t)1 << 38) && C > 0 && C <= kSelMaxC && S >= 0 && S < C, MOC_ERR_ARG,
+  MOC_REQUIRE(n >= 0 && n < ((int64_t)1 << 31) && C > 0 && C <= kSelMaxC && S >= 0 && S < C, MOC_ERR_ARG,
               "moc_router_balance: n=%lld C=%lld S=%d", (long long)n, (long long)C, S);
   MOC_REQUIRE(counts && bias && (idx || n == 0), MOC_ERR_ARG, "moc_router_balance: null pointer");
   hipLaunchKernelGGL(select_clear_kernel, dim3((unsigned)((C + 255) / 256)), dim3(256), 0, stream, counts, C);

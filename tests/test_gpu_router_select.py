@@ -511,3 +511,10 @@ def test_a_checkpoint_without_a_bias_starts_it_at_zero():
     assert torch.equal(router.balance_bias, moved)
     stack.load_reference_state_dict({k: v for k, v in whole.items() if not k.endswith("balance_bias")})
     assert not router.balance_bias.any()
+
+
+def test_balance_refuses_more_ids_than_it_counts():
+    from memory_amd import _lib as L
+    for n in (-1, 1 << 31, 1 << 37):      # (the counts have 32 bits)
+        with pytest.raises(ValueError, match="moc_router_balance"):
+            L.call("moc_router_balance", 16, n, 9, 1, 0.1, 16, 16, None)
