@@ -102,8 +102,10 @@ int moc_router_seq_bwd(const float* logits, const int32_t* idx, const float* w, 
 /* The chapter selection as a mixture of experts routes (no reference counterpart; stands beside moc_router_topk):
  * s = softmax over the chapters c >= S, or sigmoid; key = s + bias (bias f32 [C] or NULL; it steers the selection
  * only), -inf for a masked logit (-inf); the C - S chapters lie in `groups` runs of equal length, a group scores the
- * sum of its group_best (1 or 2) largest keys and the top_groups best stay (ties: lower group); the k largest keys
- * of those, keys descending (compared in f64), equal keys by ascending chapter.  w = scale s / max(sum s, 1e-12)
+ * sum of its group_best (1 or 2) largest keys (a masked second one adds nothing: its largest alone) and the top_groups
+ * best stay (ties: lower group); the k largest keys of those, keys descending (compared in f64; without a bias, and
+ * with groups scored by at most one key, as their logits, which also orders scores that f64 rounds alike), equal keys
+ * by ascending chapter.  w = scale s / max(sum s, 1e-12)
  * (renormalize) or scale s.  logits f32 [R] rows of stride ldz; idx i32 [R, k] (global ids); w f32 [R, k];
  * s_sel f32 [R, k] (the selected s) and row_stats f32 [R, 3] (softmax: maximum, sum of exp, and the share of the
  * chapters that are not selected) are the backward's inputs, NULL to skip.  C <= 16,384, k <= 1,024, groups <= 1,024. */
@@ -784,7 +786,8 @@ int moc_cache8_pack(int dtype, const void* k, const void* v, int64_t tiles, void
  * q, out bf16 [B][L][H][64]; k_tiles, v_tiles of C chapters x HK heads; idx i32, omega f32 (>= 0) [B][NS] (ids outside
  * [0, C): skipped slot) and the chapter plan of idx with its row table (moc_decode_row_table), max_u >= the plan's
  * n_uniq[0].  A row without slots is 0; of value factors omega v_scale that differ by more than 2^90 within a sequence the
- * smaller may count as 0.  workspace: moc_cache8_attend_workspace bytes, 16-byte aligned.
+ * smaller may count as 0.  Logits omega k_scale scale q.k are f32: the order of larger ones than 2^24 is that of their
+ * roundings.  workspace: moc_cache8_attend_workspace bytes, 16-byte aligned.
  * B NS < 2^31, L H < 2^25; one token: B NS H / HK < 2^31. */
 typedef struct {
   const void *q, *k_tiles, *v_tiles;

@@ -60,8 +60,8 @@ __device__ __forceinline__ void mma16(f32x4& c, const f16x8& a, const f16x8& b) 
 // ------------------------------------------------------------------ quantising
 // One workgroup per tile (blockIdx.y: K or V).  scale = 2^ceil(log2(amax / 448)) of the largest finite magnitude (1
 // for a tile of zeros): x / scale is then exact and every element is rounded once, to nearest even.  Infinities
-// become +-448 scale, NaN stays NaN.  Bound: HBM (read once into registers, a tile's maximum through LDS); run once per
-// bank update.
+// become +-448 scale, NaN stays NaN.  Bound: HBM (read once into registers, a tile's maximum through LDS): 4,097 chapters of 12
+// heads in bf16 206 us, 5.9 TB/s, in f32 350 us, 5.8 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void cache8_pack_kernel(const T* __restrict__ k, const T* __restrict__ v,
                                                           uint8_t* __restrict__ k8, uint8_t* __restrict__ v8,
@@ -134,7 +134,8 @@ __global__ __launch_bounds__(256) void cache8_pack_kernel(const T* __restrict__ 
 // rounding.
 // Bound: HBM, or latency where the units are few.  Eight loads of 16 bytes per lane hold the whole tile pair.  64 sequences
 // with 65 of 4,097 chapters, 12 heads (256 MB of tiles): 40 us, 6.3 TB/s, where a copy of 1 GiB reaches 5.2 (part of the tiles
-// stays in the last-level cache); 37 sequences of 16 heads on 4: 16 us; one sequence: 4 us.
+// stays in the last-level cache); one sequence: 4 us.  37 sequences of 16 heads on 4: 17 us, most of it the one wave per kv head
+// that takes the shared chapter's 148 rows, ten blocks of about 1 us one after the other.
 constexpr int kC8Waves = 4;
 
 struct C8Unit {
@@ -342,8 +343,8 @@ __global__ __launch_bounds__(256) void cache8_combine_kernel(const f16* __restri
 // ahead (two ahead took more registers than there are: 200 us), widens them once and puts them into LDS, K as bf16 and V
 // as f16, double-buffered, for all waves (four waves of 16 bytes: 191 us against 183).  Probabilities are f16: with bf16 the
 // kernel took 183 us for 4 x 2,048 tokens of 16 heads in place of 188 to 194, at 1.4 times the error against float64
-// (0.0024; 0.0017 is what rounding the result to bf16 alone gives).  173 to 177 us a call in a row of calls: 800 TFLOP/s, 0.65 of a
-// large matrix product's rate.  Bound: the exponentials and the products, which hardly overlap (matrix units busy 0.34,
+// (0.0024; 0.0017 is what rounding the result to bf16 alone gives).  163 to 177 us a call in a row of calls, 178 to 188 alone, by card:
+// 790 to 857 TFLOP/s, 0.65 to 0.70 of a large matrix product's rate.  Bound: the exponentials and the products, which hardly overlap (matrix units busy 0.34,
 // VALU 0.6 of the time).  Running maximum (raised lazily) and sum as in the sequence attention (xattn_fwd.hip).
 constexpr int kC8Threads = 512;
 constexpr int kC8Rows = kC8Threads / 2;   // 32 per wave

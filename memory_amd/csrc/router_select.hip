@@ -30,7 +30,10 @@ constexpr int kSelThreads = 256;
 constexpr int kSelMaxK = 1024;
 constexpr int kSelMaxG = 1024;
 constexpr int kSelMaxC = 16384;
-constexpr int64_t kSelFewRows = 1024;   // up to which four waves take a row
+// Up to which four waves take a row, one behind it.  Sigmoid with a bias, four waves / one, us: 4,097 chapters in 8 groups, 16
+// selected: 7.2 / 10.3 for 64 rows, 10.9 / 11.1 for 1,024, 19.1 / 14.4 for 2,048; 64 selected: 10.5 / 27.6, 16.0 / 28.9,
+// 27.6 / 33.5; 257 chapters, 8 selected: 5.2 / 5.6, 7.3 / 5.8, 11.6 / 6.5.
+constexpr int64_t kSelFewRows = 1024;
 
 // doubles (and NaN) to integers of the same order; 0 stays free for "not selectable"
 __device__ __forceinline__ uint64_t key64(double v) {
@@ -769,9 +772,10 @@ __device__ __forceinline__ bool select_team(const SelArgs& a, int64_t r, SelTeam
 }
 
 // Four waves: four rows (NW = 1) or one (NW = 4); rows that select_team leaves are then taken by the whole workgroup.
-// Bound: the bisection for the k-th key and the ranks of the candidates, dependent steps of one wave; HBM moves 134 MB in
-// 26 us.  Of 4,097 chapters: 16 rows, k = 64, four waves each 10.6 us; 2,039 rows, k = 16 17.6 us; 8,192 rows, k = 16 44 us
-// (3.0 TB/s).  16,001 rows of 257, k = 8, softmax: 29 us, a wave a row whose lanes hold four or five logits.
+// Bound, few rows: dependent steps (the bisection for the k-th key, the ranks of the candidates): 16 rows of 4,097, k = 64, four
+// waves each 10.6 us, the waves waiting for 0.54 of it.  Many rows: the VALU, at work for 0.57 to 0.61 of the time: 8,192 rows of
+// 4,097, k = 16 44 us (3.0 TB/s; HBM moves these 134 MB in 26); 16,001 rows of 257, k = 8, softmax with a backward's statistics
+// 32 us, the same steps of a wave whose lanes hold four or five logits.  2,039 rows of 4,097 17.6 us, two rounds of waves.
 template <int NW, int E, int MODE>
 __global__ __launch_bounds__(kSelThreads, E <= 64 ? 3 : 2) void router_select_team_kernel(SelArgs a) {
   constexpr int kTeams = 4 / NW;
@@ -801,7 +805,8 @@ struct SelBwdArgs {
 };
 
 // A team of NT threads per row (a wave: four rows per workgroup): the row of zeros, or of the softmax's dense part, then
-// the selected entries over it.  Bound by the stores: 8,192 x 4,097 (134 MB) 22 us, a plain fill of as much 18.2.
+// the selected entries over it.  Bound by the stores: 8,192 x 4,097 (134 MB) 22 to 24 us by card, a plain fill of as much
+// 18.2.  With the softmax's dense part (16,001 x 257) 14 us, where reading the logits and writing takes 6.4.
 template <int NT>
 __global__ __launch_bounds__(kSelThreads) void router_select_bwd_kernel(SelBwdArgs a) {
   constexpr int kRows = kSelThreads / NT;
@@ -868,7 +873,8 @@ __global__ __launch_bounds__(256) void select_clear_kernel(int32_t* __restrict__
   if (i < C) counts[i] = 0;
 }
 // bias[c] += rate * sign(mean count - count[c]) for the routed chapters c >= S (mean over them; compared as
-// integers: count * (C - S) against the total).
+// integers: count * (C - S) against the total).  With the clearing and the counting 16 us for 131,072 ids of 4,097 chapters,
+// three launches at their latency, once a training step.
 __global__ __launch_bounds__(1024) void balance_update_kernel(const int32_t* __restrict__ counts, int64_t C, int S, float rate,
                                                               float* __restrict__ bias) {
   __shared__ long long part[16];

@@ -46,7 +46,7 @@ class MemoryDecodeCache:
     memory and half the bytes of a step.  Each (chapter, kv head) has a float32 scale for K and one for V
     (``k_scale``, ``v_scale`` [C][HK], powers of two), a value is scale times its e4m3 value, and ``v_tiles`` is then
     held as [C][HK][64 dims][64 positions] in the order the kernels read (``dequantized()`` gives both back as
-    [keys][dims])."""
+    [keys][dims]).  A bank's 8-bit cache is that of its bfloat16 projection: rounded by 2^-8 there, by 2^-4 here."""
 
     k_scale: Optional[torch.Tensor] = None
     v_scale: Optional[torch.Tensor] = None
@@ -398,7 +398,8 @@ def _attend8_workspace(B: int, Lq: int, H: int, HK: int, NS: int) -> int:
 
 
 def _attend8(q: torch.Tensor, B: int, Lq: int, H: int, cache: MemoryDecodeCache, routing: DecodeRouting) -> torch.Tensor:
-    """q (B, [L,] H, 64) over an 8-bit cache (moc_cache8_attend)."""
+    """q (B, [L,] H, 64) over an 8-bit cache (moc_cache8_attend).  The matrix products take bfloat16 queries: others are
+    rounded to them, 2^-8 of a query, a sixteenth of the cache's own rounding."""
     q = _aligned(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16))
     pl, dev = routing.plan, q.device
     out = torch.empty_like(q)
@@ -433,8 +434,8 @@ def _attend_tokens(q: torch.Tensor, cache: MemoryDecodeCache, routing: DecodeRou
 
 def decode_attention(q: torch.Tensor, cache: MemoryDecodeCache, routing: DecodeRouting) -> torch.Tensor:
     """q (B, H, 64) -> attention output (B, H, 64) over the routed chapters (joint softmax, omega-weighted), or for
-    several query tokens of each sequence (B, L, H, 64) -> (B, L, H, 64).  The result has the cache's type, bfloat16
-    over an 8-bit cache."""
+    several query tokens of each sequence (B, L, H, 64) -> (B, L, H, 64), over a float32 or bfloat16 cache of up to 4 GiB
+    for K.  The result has the cache's type, bfloat16 over an 8-bit cache."""
     L.require_same_gpu(q, cache.k_tiles, routing.idx)
     if q.dim() not in (3, 4) or q.shape[-1] != 64 or q.shape[0] != routing.B or q.shape[-2] % cache.HK != 0:
         raise ValueError(f"queries of shape {tuple(q.shape)}: expected ({routing.B}, [tokens,] heads, 64) with heads a "

@@ -238,9 +238,10 @@ def router_select(logits: torch.Tensor, k: int, exclude_prefix_chapters: int = 0
 
     s is the softmax over the chapters past the excluded prefix, or the sigmoid of each logit; key = s + ``bias``
     (a (C,) tensor without a gradient that steers the selection and nothing else).  The chapters past the prefix lie
-    in ``num_groups`` runs of equal length; a group scores the sum of its ``group_best`` (1 or 2) largest keys, and
-    only the ``top_groups`` best groups (default: all) are selected from.  Order: key descending (compared in
-    float64), equal keys by ascending chapter.  Weights are ``scale`` times s, divided by the selected scores' sum with
+    in ``num_groups`` runs of equal length; a group scores the sum of its ``group_best`` (1 or 2) largest keys (of its
+    largest alone where the second is masked), and only the ``top_groups`` best groups (default: all) are selected from.
+    Order: key descending (compared in float64; without a bias, and with groups scored by at most one key, the logits
+    themselves are, which also orders scores that float64 rounds alike), equal keys by ascending chapter.  Weights are ``scale`` times s, divided by the selected scores' sum with
     ``renormalize``; the gradient (once differentiable) flows to the logits.
 
     A logit of -inf masks its chapter: it comes after every other, with weight 0 (rows with fewer than k others
