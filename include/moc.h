@@ -835,6 +835,86 @@ size_t moc_gated_norm_bwd_workspace(int64_t rows, int64_t d);
 int moc_gated_norm_bwd(const moc_gated_norm* a, const moc_gated_norm_grads* g, void* workspace, size_t workspace_bytes,
                        hipStream_t stream);
 
+/* ---------------------------- attention over keys and values of another length */
+
+/* o_i = sum_j softmax_j(scale q_i . k_j) v_j for L queries of H heads over N keys of HK kv heads (H % HK == 0), the
+ * dense cross-attention of memory_attention.py:402-478 for any N, ragged or masked keys, D 64 or 128.  Element (b, row,
+ * head, i) of a tensor at b * xb + row * xl (xn) + head * xh + i; strides multiples of 16 bytes, tensors 16-byte aligned;
+ * out, dq [B][L][H][D] and dk, dv [B][N][HK][D] contiguous.  lengths i32 [B] or NULL: keys from lengths[b] on do not
+ * count (values are clamped to 0 .. N).  words u64 [B][ceil(N / 64)] or NULL: bit j of word t says whether key 64 t + j
+ * counts (moc_key_words, which takes lengths in).  Keys that do not count may hold anything; rows without keys are 0 and
+ * give no gradient.  lse f32 [B][HK][moc_cross_rows]: log2-domain log-sum-exp for the backward (forward: may be NULL). */
+typedef struct {
+  const void *q, *k, *v, *dout;
+  void *out, *dq, *dk, *dv;
+  float* lse;
+  const int32_t* lengths;
+  const uint64_t* words;
+  int64_t qb, ql, qh, kb, kn, kh, vb, vn, vh, db, dl, dh; /* d: of dout */
+  int64_t B, L, N;
+  int H, HK, D, dtype;
+  float scale; /* > 0 */
+} moc_cross_args;
+int64_t moc_cross_rows(int64_t L, int H, int HK);
+size_t moc_cross_fwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D);
+int moc_cross_fwd(const moc_cross_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream);
+/* Gradients of the forward whose out and lse these are: dq (or NULL), dk and dv (both or neither NULL). */
+size_t moc_cross_bwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtype);
+int moc_cross_bwd(const moc_cross_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream);
+/* Packed key mask: mask one byte per key (0: does not count), element (b, n) at b * mb + n * mn. */
+int moc_key_words(const void* mask, int64_t mb, int64_t mn, const int32_t* lengths, int64_t B, int64_t N, uint64_t* words,
+                  hipStream_t stream);
+
+/* The same for few queries per sequence (single tokens), HBM-bound: K and V either as above (table NULL) or in pages of
+ * `page` tokens (a multiple of 16): row p of sequence b is row p % page of page table[b * tb + p / page], element (page,
+ * row, head, i) at page * kp + row * kn + head * kh + i.  n = lengths[b] (NULL: N) keys, at most max_pages * page;
+ * causal: query l sees the first n - L + l + 1.  Table entries outside [0, num_pages) are keys that do not count. */
+typedef struct {
+  const void *q, *k, *v;
+  void* out; /* [B][L][H][D] */
+  const int32_t *lengths, *table;
+  const uint64_t* words; /* not with a table */
+  int64_t qb, ql, qh, kb, kn, kh, vb, vn, vh, kp, vp, tb;
+  int64_t B, L, N, num_pages, max_pages;
+  int H, HK, D, dtype, page, causal;
+  float scale;
+} moc_kv_decode_args;
+size_t moc_kv_decode_workspace(int64_t B, int64_t L, int64_t n_max, int H, int HK, int D);
+int moc_kv_decode(const moc_kv_decode_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------- norms of heads with the rotation by position */
+
+/* Up to three sets of head rows of D elements (even, <= 512), each y = rotate(x / sqrt(mean(x^2) + eps) * w): element
+ * (b, l, h, i) at b * xb + l * xl + h * xh + i.  norm 0: no norm (and no weight); rotate 0: no rotation.  w f32 [D]
+ * (w_head 0) or [H][D] (w_head 1) or NULL.  Pair p < R / 2 of a head (elements p, p + R/2, or 2p, 2p + 1 with
+ * interleaved) turns by position * inv_freq[p] (f64, radians; reduced in f64); elements from R on stay.  The position is
+ * positions[b * pb + l * pl] (i64, or i32 with pos32; NULL: 0) + l * pstep.  With a table, y is a pool of pages as in
+ * moc_kv_decode_args and row (b, l) goes to that position's place, or nowhere if it has none. */
+typedef struct {
+  const void* x;
+  const float* w;
+  void* y;
+  const void* dy;
+  void* dx;
+  float* dw;
+  const void* positions;
+  const int32_t* table;
+  int64_t xb, xl, xh, yb, yl, yh; /* backward: y* are dy's; paged: yb is a page's */
+  int64_t pb, pl, pstep, tb;
+  int64_t B, L, num_pages, max_pages;
+  int H, w_head, norm, rotate, pos32, page;
+} moc_head_rows;
+typedef struct {
+  moc_head_rows seg[3];
+  const double* inv_freq;
+  int nseg, D, R, interleaved, dtype;
+  float eps;
+} moc_head_args;
+int moc_head_rotate_fwd(const moc_head_args* a, hipStream_t stream);
+/* dx [B][L][H][D] contiguous (or NULL) and dw f32 (as w, or NULL) of each set from dy. */
+size_t moc_head_rotate_bwd_workspace(const moc_head_args* a);
+int moc_head_rotate_bwd(const moc_head_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

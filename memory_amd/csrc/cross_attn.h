@@ -1,0 +1,108 @@
+// Shared parts of the attention over keys and values of another length (cross_attn_fwd.hip,
+// cross_attn_bwd.hip, kv_decode.hip):
+//   s_ij = scale q_i . k_j,   o_i = sum_j softmax_j(s_ij) v_j      over the live keys j of i's sequence.
+//
+// Rows: query l of head h = hk G + g is row r = l G + g of kv head hk, so the G heads that share a kv
+// head fill one block of rows whatever L is (a block of few queries would leave the matrix cores idle,
+// and heads of one query lie side by side in memory).  Keys come in tiles of 64; the live keys of a tile
+// are the bits of a 64-bit word, worked out from the sequence's length or read from packed mask words.
+#pragma once
+
+#include "moc_common.h"
+
+namespace moc {
+
+constexpr int kCaThreads = 256;
+constexpr int kCaRows = 128;     // rows of a workgroup (4 waves x 32)
+constexpr int kCaKeys = 64;      // keys of a tile
+constexpr uint32_t kCaOut = 0x80000000u;   // an offset behind every bounded buffer: reads as zeros
+
+typedef __attribute__((address_space(3))) void* ca_lds_ptr_t;
+// One 16-byte-per-lane LDS DMA: lane l's 16 bytes at voff of the buffer land at LDS address lds + 16 l;
+// offsets past the buffer's bound write zeros.  The wait is an explicit vmcnt(0).
+__device__ __forceinline__ void ca_dma16(__amdgpu_buffer_rsrc_t r, uint32_t voff, const char* lds) {
+  const uint32_t m0 = (uint32_t)(uintptr_t)(ca_lds_ptr_t)lds;
+  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(m0) : "memory");
+}
+__device__ __forceinline__ void ca_wait_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ float ca_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float ca_max3(float a, float b, float c) { return fmax_fast(fmax_fast(a, b), c); }
+
+// Rows of D elements, ROWS of them, moved global -> LDS (SwzTile<T, D>) by WAVES waves: an instruction
+// fills RPI rows of CH 16-byte chunks, wave w issues the IPW instructions from row (ROWS / WAVES) w.
+template <typename T, int D, int ROWS, int WAVES>
+struct CaStage {
+  static constexpr int CH = D * (int)sizeof(T) / 16;
+  static constexpr int RPI = 64 / CH;
+  static constexpr int RPW = ROWS / WAVES;       // rows per wave
+  static constexpr int IPW = RPW / RPI;
+  static_assert(CH >= 8 && 64 % CH == 0 && RPW % 8 == 0 && IPW * RPI == RPW, "staging geometry");
+  // row of the wave's block and byte offset in it that this lane moves with instruction i
+  static __device__ __forceinline__ int row(int i, int lane) { return RPI * i + lane / CH; }
+  static __device__ __forceinline__ uint32_t chunk(int i, int lane) {
+    return (uint32_t)(((lane % CH) ^ (row(i, lane) & 7)) * 16);
+  }
+};
+
+// A load from an address that is one for the whole wave, through the scalar cache: it does not queue behind the
+// DMAs in flight, as a vector load's wait would.  Nothing in the launch writes there.
+template <typename T>
+__device__ __forceinline__ T ca_scalar(const T* p) {
+  return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
+
+// A bounded buffer at an address that is one for the whole wave but may stand in vector registers
+__device__ __forceinline__ Buf ca_buf(const void* p, uint32_t bytes) {
+  const uint64_t a = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return Buf((const void*)(uintptr_t)((uint64_t)hi << 32 | lo), __builtin_amdgcn_readfirstlane(bytes));
+}
+
+// Live keys of a sequence's tile
+struct CaKeys {
+  const uint64_t* words;   // of the sequence, or null
+  int n;                   // keys before the sequence's end
+  __device__ __forceinline__ uint64_t word(int t) const {
+    if (words) return ca_scalar(words + t);
+    const int left = n - kCaKeys * t;
+    return left >= kCaKeys ? ~0ull : left <= 0 ? 0ull : ~0ull >> (kCaKeys - left);
+  }
+};
+
+// What a launch works on (moc_cross_args with the derived sizes)
+struct CaArgs {
+  const void *q, *k, *v, *dout, *out_in;
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta, *part, *part_lse;
+  const int32_t* lengths;
+  const uint64_t* words;
+  int64_t qb, ql, qh, kb, kn, kh, vb, vn, vh, db, dl, dh;   // element strides
+  int B, L, N, H, HK, G, rows, Lp, nt, nsplit;
+  float scale, scale_log2;
+};
+
+__device__ __forceinline__ int ca_keys_end(const CaArgs& a, int b) {
+  if (!a.lengths) return a.N;
+  const int n = ca_scalar(a.lengths + b);
+  return n < 0 ? 0 : n < a.N ? n : a.N;
+}
+
+// Scores of keys that do not count are set to `to`; lane (g, c16) holds keys 16 kb + 4 g + e.
+template <int QB>
+__device__ __forceinline__ void ca_mask(f32x4 (&st)[4][QB], uint64_t word, int g, float to) {
+  const uint32_t w[2] = {(uint32_t)word >> (4 * g), (uint32_t)(word >> 32) >> (4 * g)};
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool live = (w[kb >> 1] >> (16 * (kb & 1) + e)) & 1;
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) st[kb][qb][e] = live ? st[kb][qb][e] : to;
+    }
+}
+
+int ca_check(const char* who, const moc_cross_args* a, CaArgs* c);
+// out (and lse) of a.nsplit partial results a.part, a.part_lse over rows [B][HK][Lp]
+int ca_merge(int dtype, int D, const CaArgs& a, hipStream_t stream);
+
+}  // namespace moc

@@ -1,0 +1,489 @@
+// Attention over keys and values of another length, backward (notation of cross_attn.h).
+//   P_ij = 2^(scale log2(e) q_i . k_j - lse_i),  delta_i = dO_i . o_i,  dS_ij = P_ij (dO_i . v_j - delta_i)
+//   dq_i = scale sum_j dS_ij k_j,   dk_j = scale sum_i dS_ij q_i,   dv_j = sum_i P_ij dO_i
+// i over the rows (all queries of the G heads) of j's kv head.  dq runs over the keys of a block of rows and leaves
+// delta behind; dk and dv run over the rows of a block of keys, so nothing is summed by atomics and every result has
+// one order.  P and dS enter their products rounded to the operands' type; sums, P itself and delta are f32.
+#include "cross_attn.h"
+
+namespace moc {
+
+// dq: one workgroup = 128 rows of one (sequence, kv head) as in the forward, K and V tiles double-buffered; K^T for
+// dS K is read from the K tile with the transposing LDS read.  A tile's 64 keys go in two halves, which halves the
+// score registers.  With SPLIT each of nsplit workgroups takes a share of the keys and writes f32 rows.
+template <typename T, int D, bool SPLIT>
+__global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
+  typedef typename Frag<T>::type F8;
+  using Tile = SwzTile<T, D>;
+  using Stage = CaStage<T, D, kCaKeys, 4>;
+  constexpr int KS = D / 32, DB = D / 16, TB = kCaKeys * D * (int)sizeof(T);
+  __shared__ __attribute__((aligned(16))) char sK[2][TB];
+  __shared__ __attribute__((aligned(16))) char sV[2][TB];
+  const int nrb = a.Lp / kCaRows;
+  const int nsp = SPLIT ? a.nsplit : 1;
+  const int64_t t0 = xcd_tile((int64_t)a.B * a.HK * nsp * nrb);
+  if (t0 < 0) return;
+  const int64_t bh = t0 / ((int64_t)nsp * nrb);
+  const int b = (int)(bh / a.HK), hk = (int)(bh % a.HK);
+  const int sp = SPLIT ? (int)((t0 / nrb) % nsp) : 0;
+  const int r0 = (int)(t0 % nrb) * kCaRows;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, c16 = lane & 15;
+
+  const CaKeys keys{a.words ? a.words + (size_t)b * a.nt : nullptr, ca_keys_end(a, b)};
+  const int nt = (keys.n + kCaKeys - 1) / kCaKeys;
+  const int t_begin = SPLIT ? (int)((int64_t)nt * sp / nsp) : 0;
+  const int t_end = SPLIT ? (int)((int64_t)nt * (sp + 1) / nsp) : nt;
+
+  F8 qf[2][KS], dof[2][KS];
+  float lse[2], dl[2];
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    const int r = r0 + 32 * wave + 16 * qb + c16;
+    const bool ok = r < a.rows;
+    const int64_t l = r / a.G, h = hk * a.G + r % a.G;
+    const T* qp = (const T*)a.q + b * a.qb + l * a.ql + h * a.qh;
+    const T* dp = (const T*)a.dout + b * a.db + l * a.dl + h * a.dh;
+    const T* op = (const T*)a.out_in + (((size_t)b * a.L + l) * a.H + h) * D;
+    float sum = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[qb][ks] = ok ? Load8<T, T>::run(qp + 32 * ks + 8 * g) : zero_frag<T>();
+      dof[qb][ks] = ok ? Load8<T, T>::run(dp + 32 * ks + 8 * g) : zero_frag<T>();
+      if (ok) {
+        const F8 of = Load8<T, T>::run(op + 32 * ks + 8 * g);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) sum += to_f(dof[qb][ks][x]) * to_f(of[x]);
+      }
+    }
+    const size_t at = ((size_t)b * a.HK + hk) * a.Lp + r;
+    dl[qb] = quad_sum(sum);
+    lse[qb] = ok ? a.lse[at] : INFINITY;
+    if (g == 0 && sp == 0) a.delta[at] = dl[qb];
+  }
+  f32x4 acc[2][DB];
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[qb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const T* kbase = (const T*)a.k + b * a.kb + hk * a.kh;
+  const T* vbase = (const T*)a.v + b * a.vb + hk * a.vh;
+  auto fetch = [&](int t, uint64_t word, int buf) {
+    const int left = keys.n - kCaKeys * t, rows = left < kCaKeys ? left : kCaKeys;
+    const Buf kb = ca_buf(kbase + (int64_t)kCaKeys * t * a.kn, (uint32_t)(((rows - 1) * a.kn + D) * sizeof(T)));
+    const Buf vb = ca_buf(vbase + (int64_t)kCaKeys * t * a.vn, (uint32_t)(((rows - 1) * a.vn + D) * sizeof(T)));
+    const uint32_t live = (uint32_t)(word >> (16 * wave));
+#pragma unroll
+    for (int i = 0; i < Stage::IPW; ++i) {
+      const int row = Stage::row(i, lane);
+      const uint32_t ch = Stage::chunk(i, lane), r = 16 * wave + row;
+      uint32_t ko = r * (uint32_t)(a.kn * sizeof(T)) + ch, vo = r * (uint32_t)(a.vn * sizeof(T)) + ch;
+      if (word != ~0ull && !((live >> row) & 1)) ko = vo = kCaOut;
+      ca_dma16(kb.r, ko, sK[buf] + (TB / 4) * wave + 1024 * i);
+      ca_dma16(vb.r, vo, sV[buf] + (TB / 4) * wave + 1024 * i);
+    }
+  };
+  const float c = a.scale_log2;
+  int t = t_begin;
+  uint64_t word = 0;
+  while (t < t_end && !(word = keys.word(t))) ++t;
+  int buf = 0;
+  if (t < t_end) fetch(t, word, 0);
+  vm_wait_all();
+  __syncthreads();
+  while (t < t_end) {
+    int tn = t + 1;
+    uint64_t wn = 0;
+    while (tn < t_end && !(wn = keys.word(tn))) ++tn;
+    if (tn < t_end) fetch(tn, wn, buf ^ 1);
+    const char* Ks = sK[buf];
+    const char* Vs = sV[buf];
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh) {
+      f32x4 st[2][2], dp[2][2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+          st[kb][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+          dp[kb][qb] = f32x4{-dl[qb], -dl[qb], -dl[qb], -dl[qb]};
+        }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const F8 ak = Tile::frag(Ks, 32 * kh + 16 * kb + c16, 32 * ks + 8 * g);
+          const F8 av = Tile::frag(Vs, 32 * kh + 16 * kb + c16, 32 * ks + 8 * g);
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb) {
+            mma(st[kb][qb], ak, qf[qb][ks]);
+            mma(dp[kb][qb], av, dof[qb][ks]);
+          }
+        }
+      F8 dsf[2];
+      // (keys that do not count: P would be 2^-lse, which may be inf, of their zeroed logits)
+      const uint32_t live = (uint32_t)(word >> (32 * kh)) >> (4 * g);
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float ds = ca_exp2(st[kb][qb][e] * c - lse[qb]) * dp[kb][qb][e];
+            if (word != ~0ull) ds = (live >> (16 * kb + e)) & 1 ? ds : 0.f;
+            dsf[qb][4 * kb + e] = from_f<T>(ds);
+          }
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const F8 f = mk_frag<Tile, T>(Ks, 32 * kh, 16 * db, lane);
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) mma(acc[qb][db], dsf[qb], f);
+      }
+    }
+    if (tn < t_end) ca_wait_all();
+    t = tn;
+    word = wn;
+    buf ^= 1;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = r0 + 32 * wave + 16 * qb + 4 * g + e;
+      if constexpr (SPLIT) {
+        float* dst = a.part + ((((size_t)sp * a.B + b) * a.HK + hk) * a.Lp + r) * D;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) dst[16 * db + c16] = acc[qb][db][e];
+      } else if (r < a.rows) {
+        T* dst = (T*)a.dq + (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) dst[16 * db + c16] = from_f<T>(a.scale * acc[qb][db][e]);
+      }
+    }
+}
+
+// dq = scale * the sum of its splits, in their order
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cross_dq_sum_kernel(CaArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / (D / 4), nrow = (int64_t)a.B * a.HK * a.Lp;
+  const int d0 = (int)(i % (D / 4)) * 4;
+  if (row >= nrow) return;
+  const int r = (int)(row % a.Lp);
+  if (r >= a.rows) return;
+  const int64_t bh = row / a.Lp;
+  const int b = (int)(bh / a.HK), hk = (int)(bh % a.HK);
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int s = 0; s < a.nsplit; ++s) acc += *reinterpret_cast<const f32x4*>(a.part + (s * nrow + row) * D + d0);
+  T* dst = (T*)a.dq + (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + d0;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) dst[x] = from_f<T>(a.scale * acc[x]);
+}
+
+// dk, dv: one workgroup = 4 waves x 16 KB keys of one (sequence, kv head), whose K and V rows stay in registers as
+// matrix operands; the rows' Q and dO tiles of QS rows are double-buffered in LDS and shared by the waves, and read
+// from there both as they are and transposed.
+template <typename T, int D> struct DkvShape;
+template <> struct DkvShape<bf16, 64> { static constexpr int KB = 2, QS = 128; };
+template <> struct DkvShape<bf16, 128> { static constexpr int KB = 2, QS = 64; };
+template <> struct DkvShape<float, 64> { static constexpr int KB = 2, QS = 32; };
+template <> struct DkvShape<float, 128> { static constexpr int KB = 1, QS = 32; };
+
+template <typename T, int D, bool SPLIT>
+__global__ __launch_bounds__(kCaThreads) void cross_dkv_kernel(CaArgs a) {
+  typedef typename Frag<T>::type F8;
+  using Tile = SwzTile<T, D>;
+  constexpr int KB = DkvShape<T, D>::KB, QS = DkvShape<T, D>::QS, KEYS = 64 * KB;
+  using Stage = CaStage<T, D, QS, 4>;
+  constexpr int KS = D / 32, DB = D / 16, TB = QS * D * (int)sizeof(T);
+  __shared__ __attribute__((aligned(16))) char sQ[2][TB];
+  __shared__ __attribute__((aligned(16))) char sD[2][TB];
+  __shared__ float sL[2][QS], sDl[2][QS];
+  const int nkb = (a.N + KEYS - 1) / KEYS;
+  const int nsp = SPLIT ? a.nsplit : 1;
+  const int64_t t0 = xcd_tile((int64_t)a.B * a.HK * nsp * nkb);
+  if (t0 < 0) return;
+  const int64_t bh = t0 / ((int64_t)nsp * nkb);
+  const int b = (int)(bh / a.HK), hk = (int)(bh % a.HK);
+  const int sp = SPLIT ? (int)((t0 / nkb) % nsp) : 0;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, c16 = lane & 15;
+  const int k0 = (int)(t0 % nkb) * KEYS, kw = k0 + 16 * KB * wave;   // the workgroup's and the wave's first key
+
+  const CaKeys keys{a.words ? a.words + (size_t)b * a.nt : nullptr, ca_keys_end(a, b)};
+  uint64_t any = keys.word(k0 / kCaKeys);
+  if (KB == 2 && k0 + kCaKeys < a.N) any |= keys.word(k0 / kCaKeys + 1);
+  // bits of this wave's keys
+  const uint32_t live = kw < a.N ? (uint32_t)(keys.word(kw / kCaKeys) >> (kw % kCaKeys)) : 0u;
+
+  F8 kf[KB][KS], vf[KB][KS];
+  {
+    // bounded by the tensor's last row; what lies in keys that do not count stays in their own sums
+    const int left = a.N - kw;
+    const int rows = left < 0 ? 0 : left < 16 * KB ? left : 16 * KB;
+    const int64_t at = rows ? kw : 0;
+    const Buf kb = ca_buf((const T*)a.k + b * a.kb + hk * a.kh + at * a.kn,
+                          rows ? (uint32_t)(((rows - 1) * a.kn + D) * sizeof(T)) : 0u);
+    const Buf vb = ca_buf((const T*)a.v + b * a.vb + hk * a.vh + at * a.vn,
+                          rows ? (uint32_t)(((rows - 1) * a.vn + D) * sizeof(T)) : 0u);
+#pragma unroll
+    for (int kb2 = 0; kb2 < KB; ++kb2)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const uint32_t e = (32 * ks + 8 * g) * (uint32_t)sizeof(T), r = 16 * kb2 + c16;
+        const uint32_t ko = r * (uint32_t)(a.kn * sizeof(T)) + e, vo = r * (uint32_t)(a.vn * sizeof(T)) + e;
+        if constexpr (sizeof(T) == 2) {
+          kf[kb2][ks] = __builtin_bit_cast(F8, kb.load16(ko, 0));
+          vf[kb2][ks] = __builtin_bit_cast(F8, vb.load16(vo, 0));
+        } else {
+          const V16 w2[2] = {kb.load16(ko, 0), kb.load16(ko + 16, 0)}, x2[2] = {vb.load16(vo, 0), vb.load16(vo + 16, 0)};
+          kf[kb2][ks] = __builtin_bit_cast(F8, w2);
+          vf[kb2][ks] = __builtin_bit_cast(F8, x2);
+        }
+      }
+  }
+  f32x4 dk[KB][DB], dv[KB][DB];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      dk[kb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+      dv[kb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+  const int nstep = (a.rows + QS - 1) / QS;
+  const int s_begin = SPLIT ? (int)((int64_t)nstep * sp / nsp) : 0;
+  const int s_end = any == 0 ? s_begin : SPLIT ? (int)((int64_t)nstep * (sp + 1) / nsp) : nstep;
+  const float* lse = a.lse + bh * a.Lp;
+  const float* delta = a.delta + bh * a.Lp;
+  float preL = 0.f, preD = 0.f;
+  // rows of step s: 64-bit base of its first query, offsets from there (a step spans at most QS queries)
+  auto fetch = [&](int s, int buf) {
+    const int r0 = QS * s, l0 = r0 / a.G, q0 = r0 - l0 * a.G;
+    const int last = (r0 + QS < a.rows ? r0 + QS : a.rows) - 1;
+    const int span = last / a.G - l0;                // queries after the first
+    const Buf qb = ca_buf((const T*)a.q + b * a.qb + (int64_t)hk * a.G * a.qh + l0 * a.ql,
+                          (uint32_t)((span * a.ql + (a.G - 1) * a.qh + D) * sizeof(T)));
+    const Buf db = ca_buf((const T*)a.dout + b * a.db + (int64_t)hk * a.G * a.dh + l0 * a.dl,
+                          (uint32_t)((span * a.dl + (a.G - 1) * a.dh + D) * sizeof(T)));
+#pragma unroll
+    for (int i = 0; i < Stage::IPW; ++i) {
+      const int r = Stage::RPW * wave + Stage::row(i, lane);
+      const uint32_t x = (uint32_t)(q0 + r), l = x / (uint32_t)a.G, h = x - l * a.G, ch = Stage::chunk(i, lane);
+      uint32_t qo = (l * (uint32_t)a.ql + h * (uint32_t)a.qh) * (uint32_t)sizeof(T) + ch;
+      uint32_t od = (l * (uint32_t)a.dl + h * (uint32_t)a.dh) * (uint32_t)sizeof(T) + ch;
+      if (r0 + r >= a.rows) qo = od = kCaOut;
+      ca_dma16(qb.r, qo, sQ[buf] + (TB / 4) * wave + 1024 * i);
+      ca_dma16(db.r, od, sD[buf] + (TB / 4) * wave + 1024 * i);
+    }
+    if (tid < QS) {     // (padded to Lp, a multiple of QS: +inf and 0)
+      preL = lse[r0 + tid];
+      preD = delta[r0 + tid];
+    }
+  };
+  auto stash = [&](int buf) {
+    if (tid < QS) {
+      sL[buf][tid] = -preL;
+      sDl[buf][tid] = -preD;
+    }
+  };
+  const float c = a.scale_log2;
+  if (s_begin < s_end) {
+    fetch(s_begin, s_begin & 1);
+    stash(s_begin & 1);
+  }
+  ca_wait_all();
+  __syncthreads();
+  for (int s = s_begin; s < s_end; ++s) {
+    const int buf = s & 1;
+    if (s + 1 < s_end) fetch(s + 1, buf ^ 1);
+    const char* Qs = sQ[buf];
+    const char* Ds = sD[buf];
+#pragma unroll
+    for (int half = 0; half < QS / 32; ++half) {
+      const int r0 = 32 * half;
+      f32x4 st[2][KB], dp[2][KB], nl[2];
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        nl[qb] = *reinterpret_cast<const f32x4*>(&sL[buf][r0 + 16 * qb + 4 * g]);
+        const f32x4 nd = *reinterpret_cast<const f32x4*>(&sDl[buf][r0 + 16 * qb + 4 * g]);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          st[qb][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+          dp[qb][kb] = nd;
+        }
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+          const F8 qa = Tile::frag(Qs, r0 + 16 * qb + c16, 32 * ks + 8 * g);
+          const F8 da = Tile::frag(Ds, r0 + 16 * qb + c16, 32 * ks + 8 * g);
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            mma(st[qb][kb], qa, kf[kb][ks]);
+            mma(dp[qb][kb], da, vf[kb][ks]);
+          }
+        }
+      F8 pa[KB], sa[KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float pt = ca_exp2(st[qb][kb][e] * c + nl[qb][e]);
+            pa[kb][4 * qb + e] = from_f<T>(pt);
+            sa[kb][4 * qb + e] = from_f<T>(pt * dp[qb][kb][e]);
+          }
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const F8 fq = mk_frag<Tile, T>(Qs, r0, 16 * db, lane);
+        const F8 fd = mk_frag<Tile, T>(Ds, r0, 16 * db, lane);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          mma(dv[kb][db], pa[kb], fd);
+          mma(dk[kb][db], sa[kb], fq);
+        }
+      }
+    }
+    if (s + 1 < s_end) stash(buf ^ 1);
+    ca_wait_all();
+    __syncthreads();
+  }
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int key = kw + 16 * kb + 4 * g + e;
+      if (key >= a.N) continue;
+      const bool on = (live >> (16 * kb + 4 * g + e)) & 1;
+      const size_t row = ((size_t)b * a.N + key) * a.HK + hk;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const float x = on ? a.scale * dk[kb][db][e] : 0.f, y = on ? dv[kb][db][e] : 0.f;
+        if constexpr (SPLIT) {
+          float* dst = a.part + ((size_t)sp * a.B * a.N * a.HK + row) * (2 * D) + 16 * db + c16;
+          dst[0] = x;
+          dst[D] = y;
+        } else {
+          ((T*)a.dk)[row * D + 16 * db + c16] = from_f<T>(x);
+          ((T*)a.dv)[row * D + 16 * db + c16] = from_f<T>(y);
+        }
+      }
+    }
+}
+
+// dk, dv = the sums of their splits, in their order
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cross_dkv_sum_kernel(CaArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t nrow = (int64_t)a.B * a.N * a.HK, row = i / (D / 2);
+  const int d0 = (int)(i % (D / 2)) * 4;                  // of the 2 D columns dk | dv
+  if (row >= nrow) return;
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int s = 0; s < a.nsplit; ++s) acc += *reinterpret_cast<const f32x4*>(a.part + (s * nrow + row) * (2 * D) + d0);
+  T* dst = d0 < D ? (T*)a.dk + row * D + d0 : (T*)a.dv + row * D + d0 - D;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) dst[x] = from_f<T>(acc[x]);
+}
+
+constexpr int64_t kCaBwdWgs = 512;   // workgroups to aim at (two per CU)
+
+struct BwdPlan {
+  int dq_splits, dkv_splits;
+  size_t delta, dq_part, dkv_part;   // floats
+  size_t bytes() const { return 4 * (delta + (dq_part > dkv_part ? dq_part : dkv_part)); }
+};
+
+// Splits where there are few workgroups: of the keys for dq, of the rows for dk and dv.
+BwdPlan bwd_plan(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtype) {
+  BwdPlan p = {};
+  const int64_t rows = L * (H / HK), Lp = (rows + kCaRows - 1) / kCaRows * kCaRows;
+  auto splits = [](int64_t wgs, int64_t steps) {
+    if (wgs >= kCaBwdWgs / 2) return 1;
+    int64_t s = kCaBwdWgs / (wgs < 1 ? 1 : wgs);
+    if (s > steps / 2) s = steps / 2;
+    return s < 1 ? 1 : s > 32 ? 32 : (int)s;
+  };
+  const bool half = dtype == MOC_BF16;
+  const int KEYS = half || D == 64 ? 128 : 64, QS = !half ? 32 : D == 64 ? 128 : 64;
+  p.dq_splits = splits(B * HK * (Lp / kCaRows), (N + kCaKeys - 1) / kCaKeys);
+  p.dkv_splits = splits(B * HK * ((N + KEYS - 1) / KEYS), (rows + QS - 1) / QS);
+  p.delta = (size_t)B * HK * Lp;
+  p.dq_part = p.dq_splits > 1 ? (size_t)p.dq_splits * B * HK * Lp * D : 0;
+  p.dkv_part = p.dkv_splits > 1 ? (size_t)p.dkv_splits * B * N * HK * 2 * D : 0;
+  return p;
+}
+
+template <typename T, int D>
+static int bwd_launch(CaArgs& a, const BwdPlan& p, hipStream_t stream) {
+  const char* who = "moc_cross_bwd";
+  // (dq comes first: it leaves delta behind)
+  a.nsplit = p.dq_splits;
+  const int64_t tiles = (int64_t)a.B * a.HK * a.nsplit * (a.Lp / kCaRows);
+  MOC_REQUIRE(tiles < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "%s: too many row blocks", who);
+  if (a.nsplit > 1)
+    cross_dq_kernel<T, D, true><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
+  else
+    cross_dq_kernel<T, D, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
+  int rc = check_launch("moc_cross_bwd: dq");
+  if (rc != MOC_OK) return rc;
+  if (a.nsplit > 1) {
+    const int64_t lanes = (int64_t)a.B * a.HK * a.Lp * (D / 4);
+    cross_dq_sum_kernel<T, D><<<(unsigned)((lanes + 255) / 256), 256, 0, stream>>>(a);
+    rc = check_launch("moc_cross_bwd: dq sum");
+    if (rc != MOC_OK) return rc;
+  }
+  if (!a.dk) return MOC_OK;
+  constexpr int KEYS = 64 * DkvShape<T, D>::KB;
+  a.nsplit = p.dkv_splits;
+  const int64_t blocks = (int64_t)a.B * a.HK * a.nsplit * ((a.N + KEYS - 1) / KEYS);
+  MOC_REQUIRE(blocks < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "%s: too many key blocks", who);
+  if (a.nsplit > 1)
+    cross_dkv_kernel<T, D, true><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(a);
+  else
+    cross_dkv_kernel<T, D, false><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(a);
+  rc = check_launch("moc_cross_bwd: dk, dv");
+  if (rc != MOC_OK || a.nsplit == 1) return rc;
+  const int64_t lanes = (int64_t)a.B * a.N * a.HK * (D / 2);
+  cross_dkv_sum_kernel<T, D><<<(unsigned)((lanes + 255) / 256), 256, 0, stream>>>(a);
+  return check_launch("moc_cross_bwd: dk, dv sum");
+}
+
+}  // namespace moc
+
+using namespace moc;
+
+extern "C" {
+
+size_t moc_cross_bwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtype) {
+  return HK <= 0 ? 0 : bwd_plan(B, L, N, H, HK, D, dtype).bytes();
+}
+
+int moc_cross_bwd(const moc_cross_args* args, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  const char* who = "moc_cross_bwd";
+  CaArgs a;
+  int rc = ca_check(who, args, &a);
+  if (rc != MOC_OK) return rc;
+  MOC_REQUIRE(a.q && a.k && a.v && a.out && a.dout && a.lse && a.dq, MOC_ERR_ARG, "%s: null tensor", who);
+  MOC_REQUIRE(!a.dk == !a.dv, MOC_ERR_ARG, "%s: dk and dv together or neither", who);
+  // the rows of a step of dk, dv are read through one bounded buffer with 32-bit offsets
+  const int64_t es = dtype_size(args->dtype);
+  const int64_t far = 128 * (a.ql > a.dl ? a.ql : a.dl) + (int64_t)a.G * (a.qh > a.dh ? a.qh : a.dh) + args->D;
+  MOC_REQUIRE(far * es < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "%s: rows of Q and dO lie too far apart", who);
+  const BwdPlan p = bwd_plan(args->B, args->L, args->N, args->H, args->HK, args->D, args->dtype);
+  MOC_REQUIRE(workspace && workspace_bytes >= p.bytes(), MOC_ERR_ARG, "%s: workspace of %zu bytes, needs %zu", who,
+              workspace_bytes, p.bytes());
+  a.delta = (float*)workspace;
+  a.part = a.delta + p.delta;
+  if (args->dtype == MOC_BF16)
+    return args->D == 64 ? bwd_launch<bf16, 64>(a, p, stream) : bwd_launch<bf16, 128>(a, p, stream);
+  return args->D == 64 ? bwd_launch<float, 64>(a, p, stream) : bwd_launch<float, 128>(a, p, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,367 @@
+// Attention over keys and values of another length, forward (see cross_attn.h).
+//
+// One workgroup = 128 rows of one (sequence, kv head), four waves of 32; K and V tiles of 64 keys are
+// double-buffered in LDS, fetched by DMA.  Each wave computes S^T = K Q^T (a lane holds one row's logits of
+// 16 keys), keeps the running maximum, and accumulates O^T = V^T P^T, whose accumulator layout is again one
+// row per lane, so rescaling moves no data; the row sums come from a product with ones, so they are those of
+// the rounded P.  Keys that do not count are fetched as zeros (whatever their memory holds) and their logits
+// set to -inf; tiles without live keys are passed over.
+#include "cross_attn.h"
+
+namespace moc {
+
+// A row's reference maximum moves only when a tile's exceeds it by more than this (log2 units): most tiles skip
+// the rescale, and P stays <= 2^8.
+constexpr float kCaSlack = 8.f;
+
+template <typename T, int D, bool SPLIT>
+__global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
+  typedef typename Frag<T>::type F8;
+  using Tile = SwzTile<T, D>;
+  using Stage = CaStage<T, D, kCaKeys, 4>;
+  constexpr int KS = D / 32, DB = D / 16, TB = kCaKeys * D * (int)sizeof(T);
+  __shared__ __attribute__((aligned(16))) char sK[2][TB];
+  __shared__ __attribute__((aligned(16))) char sV[2][TB];
+
+  // (sequence, kv head) major, row block minor: blocks that read the same keys share an XCD's L2
+  const int nrb = a.Lp / kCaRows;
+  const int nsp = SPLIT ? a.nsplit : 1;
+  const int64_t t0 = xcd_tile((int64_t)a.B * a.HK * nsp * nrb);
+  if (t0 < 0) return;
+  const int64_t bh = t0 / ((int64_t)nsp * nrb);
+  const int b = (int)(bh / a.HK), hk = (int)(bh % a.HK);
+  const int sp = SPLIT ? (int)((t0 / nrb) % nsp) : 0;
+  const int r0 = (int)(t0 % nrb) * kCaRows;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, c16 = lane & 15;
+
+  const CaKeys keys{a.words ? a.words + (size_t)b * a.nt : nullptr, ca_keys_end(a, b)};
+  const int nt = (keys.n + kCaKeys - 1) / kCaKeys;
+  const int t_begin = SPLIT ? (int)((int64_t)nt * sp / nsp) : 0;
+  const int t_end = SPLIT ? (int)((int64_t)nt * (sp + 1) / nsp) : nt;
+
+  F8 qf[2][KS];
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    const int r = r0 + 32 * wave + 16 * qb + c16;
+    const T* qp = (const T*)a.q + b * a.qb + (int64_t)(r / a.G) * a.ql + (int64_t)(hk * a.G + r % a.G) * a.qh;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      qf[qb][ks] = r < a.rows ? Load8<T, T>::run(qp + 32 * ks + 8 * g) : zero_frag<T>();
+  }
+
+  const T* kbase = (const T*)a.k + b * a.kb + hk * a.kh;
+  const T* vbase = (const T*)a.v + b * a.vb + hk * a.vh;
+  auto fetch = [&](int t, uint64_t word, int buf) {
+    const int left = keys.n - kCaKeys * t, rows = left < kCaKeys ? left : kCaKeys;
+    const Buf kb = ca_buf(kbase + (int64_t)kCaKeys * t * a.kn, (uint32_t)(((rows - 1) * a.kn + D) * sizeof(T)));
+    const Buf vb = ca_buf(vbase + (int64_t)kCaKeys * t * a.vn, (uint32_t)(((rows - 1) * a.vn + D) * sizeof(T)));
+    const uint32_t live = (uint32_t)(word >> (16 * wave));
+#pragma unroll
+    for (int i = 0; i < Stage::IPW; ++i) {
+      const int row = Stage::row(i, lane);
+      const uint32_t ch = Stage::chunk(i, lane), r = 16 * wave + row;
+      uint32_t ko = r * (uint32_t)(a.kn * sizeof(T)) + ch, vo = r * (uint32_t)(a.vn * sizeof(T)) + ch;
+      if (word != ~0ull && !((live >> row) & 1)) ko = vo = kCaOut;
+      ca_dma16(kb.r, ko, sK[buf] + (TB / 4) * wave + 1024 * i);
+      ca_dma16(vb.r, vo, sV[buf] + (TB / 4) * wave + 1024 * i);
+    }
+  };
+
+  float m[2] = {-INFINITY, -INFINITY}, lsum[2] = {0.f, 0.f};
+  F8 ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones[j] = from_f<T>(1.f);
+  f32x4 o[DB][2];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) o[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float c = a.scale_log2;
+
+  int t = t_begin;
+  uint64_t word = 0;
+  while (t < t_end && !(word = keys.word(t))) ++t;
+  int buf = 0;
+  if (t < t_end) fetch(t, word, 0);
+  vm_wait_all();
+  __syncthreads();
+  while (t < t_end) {
+    int tn = t + 1;
+    uint64_t wn = 0;
+    while (tn < t_end && !(wn = keys.word(tn))) ++tn;
+    // (buffer buf ^ 1 was last read a tile ago, which every wave has finished)
+    if (tn < t_end) fetch(tn, wn, buf ^ 1);
+    const char* Ks = sK[buf];
+    const char* Vs = sV[buf];
+    f32x4 st[4][2];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) st[kb][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        const F8 f = Tile::frag(Ks, 16 * kb + c16, 32 * ks + 8 * g);
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) mma(st[kb][qb], f, qf[qb][ks]);
+      }
+    if (word != ~0ull) ca_mask(st, word, g, -INFINITY);
+    float cm[2];
+    bool grow = false;
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      float mx = ca_max3(st[0][qb][0], st[0][qb][1], st[0][qb][2]);
+      mx = ca_max3(mx, st[0][qb][3], st[1][qb][0]);
+      mx = ca_max3(mx, st[1][qb][1], st[1][qb][2]);
+      mx = ca_max3(mx, st[1][qb][3], st[2][qb][0]);
+      mx = ca_max3(mx, st[2][qb][1], st[2][qb][2]);
+      mx = ca_max3(mx, st[2][qb][3], st[3][qb][0]);
+      mx = ca_max3(mx, st[3][qb][1], st[3][qb][2]);
+      cm[qb] = quad_max_pl(fmax_fast(mx, st[3][qb][3])) * c;
+      grow |= cm[qb] > m[qb] + kCaSlack;
+    }
+    if (__any(grow)) {
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        const float mn = cm[qb] > m[qb] + kCaSlack ? cm[qb] : m[qb];
+        const float alpha = m[qb] == mn ? 1.f : ca_exp2(m[qb] - mn);
+        m[qb] = mn;
+        lsum[qb] *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db][qb] *= alpha;
+      }
+    }
+    F8 pf[2][2];
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      const float off = m[qb] == -INFINITY ? 0.f : m[qb];   // (a row whose logits so far are all -inf)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          pf[qb][h][e] = from_f<T>(ca_exp2(st[2 * h][qb][e] * c - off));
+          pf[qb][h][4 + e] = from_f<T>(ca_exp2(st[2 * h + 1][qb][e] * c - off));
+        }
+    }
+    f32x4 ls[2];
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      ls[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      mma(ls[qb], ones, pf[qb][0]);
+      mma(ls[qb], ones, pf[qb][1]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const F8 f = mk_frag<Tile, T>(Vs, 32 * h, 16 * db, lane);
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) mma(o[db][qb], f, pf[qb][h]);
+      }
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) lsum[qb] += ls[qb][0];
+    if (tn < t_end) ca_wait_all();
+    t = tn;
+    word = wn;
+    buf ^= 1;
+    __syncthreads();
+  }
+
+  // rows without live keys: 0, and +inf as the backward's log-sum-exp (its probabilities are 0 then), as in the
+  // padding rows up to Lp
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    const float l = lsum[qb];
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int r = r0 + 32 * wave + 16 * qb + c16;
+    if constexpr (SPLIT) {
+      const size_t row = (((size_t)sp * a.B + b) * a.HK + hk) * a.Lp + r;
+      float* pp = a.part + row * D + 4 * g;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(pp + 16 * db) = o[db][qb] * inv;
+      if (g == 0) a.part_lse[row] = l == 0.f ? -INFINITY : m[qb] + log2f(l);
+    } else {
+      if (r < a.rows) {
+        T* op = (T*)a.out + (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + 4 * g;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) op[16 * db + e] = from_f<T>(o[db][qb][e] * inv);
+      }
+      if (a.lse && g == 0)
+        a.lse[((size_t)b * a.HK + hk) * a.Lp + r] = r >= a.rows || l == 0.f ? INFINITY : m[qb] + log2f(l);
+    }
+  }
+}
+
+// out = sum_i 2^(lse_i - M) o_i / sum_i 2^(lse_i - M) over the splits of a row, and its log-sum-exp: D / 4 lanes
+// of four dims per row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cross_merge_kernel(CaArgs a) {
+  constexpr int LPR = D / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / LPR;                 // (b, hk, r)
+  const int ch = (int)(i % LPR);
+  const int64_t nrow = (int64_t)a.B * a.HK * a.Lp;
+  if (row >= nrow) return;
+  const int r = (int)(row % a.Lp);
+  const int64_t bh = row / a.Lp;
+  const int b = (int)(bh / a.HK), hk = (int)(bh % a.HK);
+  if (r >= a.rows) {
+    if (a.lse && ch == 0) a.lse[row] = INFINITY;
+    return;
+  }
+  float M = -INFINITY;
+#pragma unroll 8
+  for (int s = 0; s < a.nsplit; ++s) M = fmax_fast(M, a.part_lse[s * nrow + row]);
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  float den = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < a.nsplit; ++s) {
+    // (no weight for a split without live keys; a NaN goes through)
+    const float d = a.part_lse[s * nrow + row];
+    const float w = d == -INFINITY ? 0.f : ca_exp2(d - M);
+    acc += *reinterpret_cast<const f32x4*>(a.part + (s * nrow + row) * D + 4 * ch) * w;
+    den += w;
+  }
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  T* op = (T*)a.out + (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + 4 * ch;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) op[x] = from_f<T>(acc[x] * inv);
+  if (a.lse && ch == 0) a.lse[row] = den == 0.f ? INFINITY : M + log2f(den);
+}
+
+// words[b][t]: the live keys of tile t, from one byte per key and the sequence's length; a wave per word
+__global__ __launch_bounds__(256) void key_words_kernel(const uint8_t* __restrict__ mask, int64_t mb, int64_t mn,
+                                                        const int32_t* __restrict__ lengths, int64_t B, int N, int nt,
+                                                        uint64_t* __restrict__ words) {
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= B * nt) return;
+  const int64_t b = w / nt;
+  const int key = kCaKeys * (int)(w % nt) + (threadIdx.x & 63);
+  const bool live = key < N && (!lengths || key < lengths[b]) && mask[b * mb + key * mn] != 0;
+  const uint64_t bits = __ballot(live);
+  if ((threadIdx.x & 63) == 0) words[w] = bits;
+}
+
+// Workgroups of the forward from which on splitting the keys no longer pays (two to three per CU).
+constexpr int64_t kCaWgs = 512;
+
+// Splits of the keys: enough workgroups to fill the card, each with at least four tiles.
+int ca_fwd_splits(int64_t wgs, int64_t nt) {
+  if (wgs >= kCaWgs / 2) return 1;
+  int64_t s = kCaWgs / (wgs < 1 ? 1 : wgs);
+  if (s > nt / 4) s = nt / 4;
+  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+
+int ca_check(const char* who, const moc_cross_args* p, CaArgs* c) {
+  MOC_REQUIRE(p != nullptr, MOC_ERR_ARG, "%s: no arguments", who);
+  const moc_cross_args& a = *p;
+  MOC_REQUIRE(a.dtype == MOC_F32 || a.dtype == MOC_BF16, MOC_ERR_ARG, "%s: dtype %d", who, a.dtype);
+  MOC_REQUIRE(a.D == 64 || a.D == 128, MOC_ERR_UNSUPPORTED, "%s: head dim %d, expected 64 or 128", who, a.D);
+  MOC_REQUIRE(a.H > 0 && a.HK > 0 && a.H % a.HK == 0, MOC_ERR_ARG, "%s: %d query heads on %d kv heads", who, a.H, a.HK);
+  MOC_REQUIRE(a.B > 0 && a.L > 0 && a.N > 0, MOC_ERR_ARG, "%s: empty sizes", who);
+  const int64_t G = a.H / a.HK, es = dtype_size(a.dtype);
+  MOC_REQUIRE(a.L * G < (int64_t)1 << 30 && a.N < (int64_t)1 << 30 && a.B < (int64_t)1 << 24, MOC_ERR_UNSUPPORTED,
+              "%s: sizes B=%lld L=%lld N=%lld", who, (long long)a.B, (long long)a.L, (long long)a.N);
+  MOC_REQUIRE(a.scale > 0.f && a.scale <= 3.4028234e38f, MOC_ERR_ARG, "%s: scale must be positive and finite", who);
+  const int64_t st[] = {a.qb, a.ql, a.qh, a.kb, a.kn, a.kh, a.vb, a.vn, a.vh, a.db, a.dl, a.dh};
+  for (int64_t s : st)
+    MOC_REQUIRE(s >= 0 && s * es % 16 == 0, MOC_ERR_ARG, "%s: strides must be multiples of 16 bytes", who);
+  const void* ptrs[] = {a.q, a.k, a.v, a.out, a.dout, a.dq, a.dk, a.dv};
+  for (const void* x : ptrs)
+    MOC_REQUIRE(((uintptr_t)x & 15) == 0, MOC_ERR_ARG, "%s: tensors must be 16-byte aligned", who);
+  // a tile's rows are read through one bounded buffer with 32-bit offsets (the top bit marks keys left out)
+  MOC_REQUIRE((a.kn * es) < ((int64_t)1 << 24) && (a.vn * es) < ((int64_t)1 << 24), MOC_ERR_UNSUPPORTED,
+              "%s: rows of K and V must lie less than 16 MiB apart", who);
+  MOC_REQUIRE(a.N == 1 || (a.kn >= a.D && a.vn >= a.D), MOC_ERR_ARG, "%s: rows of K or V overlap", who);
+  CaArgs& o = *c;
+  o = CaArgs{};
+  o.q = a.q; o.k = a.k; o.v = a.v; o.out = a.out; o.out_in = a.out; o.dout = a.dout;
+  o.dq = a.dq; o.dk = a.dk; o.dv = a.dv; o.lse = a.lse; o.lengths = a.lengths; o.words = a.words;
+  o.qb = a.qb; o.ql = a.ql; o.qh = a.qh; o.kb = a.kb; o.kn = a.kn; o.kh = a.kh; o.vb = a.vb; o.vn = a.vn; o.vh = a.vh;
+  o.db = a.db; o.dl = a.dl; o.dh = a.dh;
+  o.B = (int)a.B; o.L = (int)a.L; o.N = (int)a.N; o.H = a.H; o.HK = a.HK; o.G = (int)G;
+  o.rows = (int)(a.L * G);
+  o.Lp = (o.rows + kCaRows - 1) / kCaRows * kCaRows;
+  o.nt = (o.N + kCaKeys - 1) / kCaKeys;
+  o.nsplit = 1;
+  o.scale = a.scale;
+  o.scale_log2 = a.scale * 1.4426950408889634f;
+  return MOC_OK;
+}
+
+template <typename T, int D>
+static int fwd_launch(CaArgs& a, hipStream_t stream) {
+  const int64_t tiles = (int64_t)a.B * a.HK * a.nsplit * (a.Lp / kCaRows);
+  MOC_REQUIRE(tiles < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "moc_cross_fwd: too many row blocks");
+  if (a.nsplit == 1) {
+    cross_fwd_kernel<T, D, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
+    return check_launch("moc_cross_fwd");
+  }
+  cross_fwd_kernel<T, D, true><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
+  int rc = check_launch("moc_cross_fwd");
+  if (rc != MOC_OK) return rc;
+  return ca_merge(sizeof(T) == 2 ? MOC_BF16 : MOC_F32, D, a, stream);
+}
+
+int ca_merge(int dtype, int D, const CaArgs& a, hipStream_t stream) {
+  const int64_t lanes = (int64_t)a.B * a.HK * a.Lp * (D / 4);
+  MOC_REQUIRE(lanes < (int64_t)1 << 39, MOC_ERR_UNSUPPORTED, "attention merge: too many rows");
+  const unsigned grid = (unsigned)((lanes + 255) / 256);
+  if (dtype == MOC_BF16)
+    D == 64 ? cross_merge_kernel<bf16, 64><<<grid, 256, 0, stream>>>(a)
+            : cross_merge_kernel<bf16, 128><<<grid, 256, 0, stream>>>(a);
+  else
+    D == 64 ? cross_merge_kernel<float, 64><<<grid, 256, 0, stream>>>(a)
+            : cross_merge_kernel<float, 128><<<grid, 256, 0, stream>>>(a);
+  return check_launch("attention merge");
+}
+
+}  // namespace moc
+
+using namespace moc;
+
+extern "C" {
+
+int64_t moc_cross_rows(int64_t L, int H, int HK) {
+  if (HK <= 0 || L <= 0) return 0;
+  return (L * (H / HK) + kCaRows - 1) / kCaRows * kCaRows;
+}
+
+size_t moc_cross_fwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D) {
+  const int64_t Lp = moc_cross_rows(L, H, HK);
+  const int s = ca_fwd_splits(B * HK * (Lp / kCaRows), (N + kCaKeys - 1) / kCaKeys);
+  return s == 1 ? 0 : (size_t)s * B * HK * Lp * (D + 1) * 4;
+}
+
+int moc_cross_fwd(const moc_cross_args* args, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  CaArgs a;
+  int rc = ca_check("moc_cross_fwd", args, &a);
+  if (rc != MOC_OK) return rc;
+  MOC_REQUIRE(a.q && a.k && a.v && a.out, MOC_ERR_ARG, "moc_cross_fwd: null tensor");
+  const int64_t bhl = (int64_t)a.B * a.HK * a.Lp;
+  a.nsplit = ca_fwd_splits((int64_t)a.B * a.HK * (a.Lp / kCaRows), a.nt);
+  const size_t need = moc_cross_fwd_workspace(args->B, args->L, args->N, args->H, args->HK, args->D);
+  MOC_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), MOC_ERR_ARG, "moc_cross_fwd: workspace of %zu bytes, needs %zu",
+              workspace_bytes, need);
+  a.part = (float*)workspace;
+  a.part_lse = a.part + (size_t)a.nsplit * bhl * args->D;
+  if (args->dtype == MOC_BF16) return args->D == 64 ? fwd_launch<bf16, 64>(a, stream) : fwd_launch<bf16, 128>(a, stream);
+  return args->D == 64 ? fwd_launch<float, 64>(a, stream) : fwd_launch<float, 128>(a, stream);
+}
+
+int moc_key_words(const void* mask, int64_t mb, int64_t mn, const int32_t* lengths, int64_t B, int64_t N, uint64_t* words,
+                  hipStream_t stream) {
+  MOC_REQUIRE(mask && words && B > 0 && N > 0 && N < (int64_t)1 << 30, MOC_ERR_ARG, "moc_key_words: bad arguments");
+  const int64_t nt = (N + kCaKeys - 1) / kCaKeys;
+  MOC_REQUIRE(B * nt < (int64_t)1 << 32, MOC_ERR_UNSUPPORTED, "moc_key_words: too many keys");
+  key_words_kernel<<<(unsigned)((B * nt + 3) / 4), 256, 0, stream>>>((const uint8_t*)mask, mb, mn, lengths, B, (int)N,
+                                                                    (int)nt, words);
+  return check_launch("moc_key_words");
+}
+
+}  // extern "C"

@@ -1,0 +1,290 @@
+// Attention of few queries per sequence over their keys and values, strided or in pages: bound by HBM, each key
+// and value is read once.
+//
+// A unit is one (sequence, kv head, 16 rows) with r = l G + g as in cross_attn.h; its tiles of 64 keys are split
+// over nsplit workgroups and there over four waves, each with a running maximum of its own, joined in LDS and
+// (nsplit > 1) by a second launch.  K goes straight to registers as the matrix operand, V through a tile of the
+// wave's own in LDS, from which it is read transposed.  A tile is four blocks of 16 keys, each within one page.
+#include "cross_attn.h"
+
+namespace moc {
+
+constexpr int kKdWaves = 4;
+
+struct KdArgs {
+  CaArgs c;
+  const int32_t* table;
+  int64_t kp, vp, tb, num_pages, max_pages;
+  int page, causal, nrb;
+};
+
+template <typename T, int D, bool PAGED, bool SPLIT>
+__global__ __launch_bounds__(64 * kKdWaves) void kv_decode_kernel(KdArgs p) {
+  typedef typename Frag<T>::type F8;
+  using Tile = SwzTile<T, D>;
+  using Stage = CaStage<T, D, 16, 1>;            // a block of 16 keys, by one wave
+  constexpr int KS = D / 32, DB = D / 16, TB = kCaKeys * D * (int)sizeof(T);
+  static_assert(TB >= 16 * D * 4, "a wave's V tile holds its 16 result rows");
+  __shared__ __attribute__((aligned(16))) char sV[kKdWaves][TB];
+  __shared__ float sM[kKdWaves][16], sL[kKdWaves][16];
+  const CaArgs& a = p.c;
+  const int nsp = SPLIT ? a.nsplit : 1;
+  const int64_t u = blockIdx.x;                  // ((b, hk), row block, split)
+  const int sp = (int)(u % nsp), rb = (int)(u / nsp % p.nrb);
+  const int64_t bh = u / nsp / p.nrb;
+  const int b = (int)(bh / a.HK), hk = (int)(bh % a.HK);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, c16 = lane & 15;
+
+  int n;
+  if constexpr (PAGED) {
+    const int64_t most = p.max_pages * p.page;
+    n = ca_scalar(a.lengths + b);
+    n = n < 0 ? 0 : (int64_t)n < most ? n : (int)most;
+  } else {
+    n = ca_keys_end(a, b);
+  }
+  const CaKeys keys{!PAGED && a.words ? a.words + (size_t)b * a.nt : nullptr, n};
+  const int nt = (n + kCaKeys - 1) / kCaKeys;
+  const int t_begin = (int)((int64_t)nt * sp / nsp), t_end = (int)((int64_t)nt * (sp + 1) / nsp);
+
+  const int r = 16 * rb + c16;
+  const bool row_ok = r < a.rows;
+  const int l = r / a.G, h = hk * a.G + r % a.G;
+  // keys that this lane's row sees, and those that every row does
+  const int limit = !row_ok ? 0 : p.causal ? n - a.L + l + 1 : n;
+  const int all_see = p.causal ? n - a.L + 1 : n;
+  F8 qf[KS];
+  const T* qp = (const T*)a.q + b * a.qb + (int64_t)l * a.ql + (int64_t)h * a.qh;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) qf[ks] = row_ok ? Load8<T, T>::run(qp + 32 * ks + 8 * g) : zero_frag<T>();
+
+  const T* kbase = (const T*)a.k + (PAGED ? 0 : b * a.kb) + hk * a.kh;
+  const T* vbase = (const T*)a.v + (PAGED ? 0 : b * a.vb) + hk * a.vh;
+  char* Vs = sV[wave];
+  F8 kf[4][KS];
+  uint64_t word = 0;
+  // requests a tile: K into kf, V into Vs; keys that do not count come as zeros
+  auto fetch = [&](int t) {
+    word = keys.word(t);
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      const int pos = kCaKeys * t + 16 * kb;
+      int rows = n - pos;
+      rows = rows < 0 ? 0 : rows < 16 ? rows : 16;
+      int64_t ko = (int64_t)pos * a.kn, vo = (int64_t)pos * a.vn;
+      if constexpr (PAGED) {
+        const int pg = rows > 0 ? ca_scalar(p.table + b * p.tb + pos / p.page) : -1;
+        if (pg < 0 || pg >= p.num_pages) {
+          rows = 0;
+          word &= ~(0xffffull << (16 * kb));
+        }
+        ko = (int64_t)pg * p.kp + (int64_t)(pos % p.page) * a.kn;
+        vo = (int64_t)pg * p.vp + (int64_t)(pos % p.page) * a.vn;
+      }
+      // (without rows the base stays within the tensor and the bound is 0)
+      const Buf kbuf = ca_buf(kbase + (rows ? ko : 0), rows ? (uint32_t)(((rows - 1) * a.kn + D) * sizeof(T)) : 0u);
+      const Buf vbuf = ca_buf(vbase + (rows ? vo : 0), rows ? (uint32_t)(((rows - 1) * a.vn + D) * sizeof(T)) : 0u);
+      const uint32_t live = (uint32_t)(word >> (16 * kb));
+#pragma unroll
+      for (int i = 0; i < Stage::IPW; ++i) {
+        const int row = Stage::row(i, lane);
+        uint32_t off = (uint32_t)row * (uint32_t)(a.vn * sizeof(T)) + Stage::chunk(i, lane);
+        if (!((live >> row) & 1)) off = kCaOut;
+        ca_dma16(vbuf.r, off, Vs + (TB / 4) * kb + 1024 * i);
+      }
+      const uint32_t ro = (live >> c16) & 1 ? (uint32_t)c16 * (uint32_t)(a.kn * sizeof(T)) : kCaOut;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const uint32_t off = ro + (32 * ks + 8 * g) * (int)sizeof(T);
+        if constexpr (sizeof(T) == 2) {
+          kf[kb][ks] = __builtin_bit_cast(F8, kbuf.load16(off, 0));
+        } else {
+          const V16 w2[2] = {kbuf.load16(off, 0), kbuf.load16(off + 16, 0)};
+          kf[kb][ks] = __builtin_bit_cast(F8, w2);
+        }
+      }
+    }
+  };
+
+  float m = -INFINITY, lsum = 0.f;
+  f32x4 o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float c = a.scale_log2;
+
+  for (int t = t_begin + wave; t < t_end; t += kKdWaves) {
+    fetch(t);
+    f32x4 st[4][1];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      st[kb][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) mma(st[kb][0], kf[kb][ks], qf[ks]);
+    }
+    if (word != ~0ull || kCaKeys * (t + 1) > all_see) {
+      const uint32_t w[2] = {(uint32_t)word >> (4 * g), (uint32_t)(word >> 32) >> (4 * g)};
+      const int left = limit - kCaKeys * t - 4 * g;
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!((w[kb >> 1] >> (16 * (kb & 1) + e)) & 1) || 16 * kb + e >= left) st[kb][0][e] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      mx = ca_max3(mx, st[kb][0][0], st[kb][0][1]);
+      mx = ca_max3(mx, st[kb][0][2], st[kb][0][3]);
+    }
+    const float cm = quad_max_pl(mx) * c;
+    if (__any(cm > m)) {
+      const float mn = cm > m ? cm : m;
+      const float alpha = m == mn ? 1.f : ca_exp2(m - mn);
+      m = mn;
+      lsum *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] *= alpha;
+    }
+    const float off = m == -INFINITY ? 0.f : m;
+    // the sums take the unrounded probabilities: a lane's 16 keys here, the four lanes of the row at the end
+    F8 pf[2];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = ca_exp2(st[2 * hh][0][e] * c - off), p1 = ca_exp2(st[2 * hh + 1][0][e] * c - off);
+        lsum += p0 + p1;
+        pf[hh][e] = from_f<T>(p0);
+        pf[hh][4 + e] = from_f<T>(p1);
+      }
+    ca_wait_all();   // V landed
+    wave_lds_sync();
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) mma(o[db], mk_frag<Tile, T>(Vs, 32 * hh, 16 * db, lane), pf[hh]);
+    wave_lds_sync();   // the next tile's V overwrites this one once it has been read
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  lsum = quad_sum(lsum);
+
+  // the waves' results in units of their common maximum
+  if (g == 0) {
+    sM[wave][c16] = m;
+    sL[wave][c16] = lsum;
+  }
+  __syncthreads();
+  float M = sM[0][c16];
+#pragma unroll
+  for (int w = 1; w < kKdWaves; ++w) M = fmax_fast(M, sM[w][c16]);
+  const float f = m == -INFINITY ? 0.f : ca_exp2(m - M);   // (a wave without live keys; its sums are 0 or NaN)
+  float* res = reinterpret_cast<float*>(Vs);               // [16 rows][D]
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+    *reinterpret_cast<f32x4*>(res + c16 * D + 16 * db + 4 * g) = m == -INFINITY ? o[db] : o[db] * f;
+  __syncthreads();
+#pragma unroll
+  for (int i = tid; i < 16 * D / 4; i += 64 * kKdWaves) {
+    const int row = i / (D / 4), d0 = i % (D / 4) * 4, rr = 16 * rb + row;
+    float Mr = sM[0][row], den = 0.f;
+#pragma unroll
+    for (int w = 1; w < kKdWaves; ++w) Mr = fmax_fast(Mr, sM[w][row]);
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kKdWaves; ++w) {
+      acc += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(sV[w]) + row * D + d0);
+      den += sM[w][row] == -INFINITY ? sL[w][row] : sL[w][row] * ca_exp2(sM[w][row] - Mr);
+    }
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    if constexpr (SPLIT) {
+      const size_t at = (((size_t)sp * a.B + b) * a.HK + hk) * a.Lp + rr;
+      *reinterpret_cast<f32x4*>(a.part + at * D + d0) = acc * inv;
+      if (d0 == 0) a.part_lse[at] = den == 0.f ? -INFINITY : Mr + log2f(den);
+    } else if (rr < a.rows) {
+      T* op = (T*)a.out + (((size_t)b * a.L + rr / a.G) * a.H + hk * a.G + rr % a.G) * D + d0;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) op[x] = from_f<T>(acc[x] * inv);
+    }
+  }
+}
+
+// Workgroups to aim at (four waves each): three per CU.
+constexpr int64_t kKdWgs = 768;
+
+int kd_splits(int64_t units, int64_t n_max) {
+  const int64_t most = ((n_max + kCaKeys - 1) / kCaKeys + kKdWaves - 1) / kKdWaves;   // a tile per wave
+  int64_t s = kKdWgs / (units < 1 ? 1 : units);
+  if (s > most) s = most;
+  return s < 1 ? 1 : s > 128 ? 128 : (int)s;
+}
+
+template <typename T, int D>
+static int kd_launch(KdArgs& p, bool paged, hipStream_t stream) {
+  const int64_t grid = (int64_t)p.c.B * p.c.HK * p.nrb * p.c.nsplit;
+  MOC_REQUIRE(grid < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "moc_kv_decode: too many rows");
+  const bool split = p.c.nsplit > 1;
+  const dim3 gr((unsigned)grid), bl(64 * kKdWaves);
+  if (paged)
+    split ? kv_decode_kernel<T, D, true, true><<<gr, bl, 0, stream>>>(p)
+          : kv_decode_kernel<T, D, true, false><<<gr, bl, 0, stream>>>(p);
+  else
+    split ? kv_decode_kernel<T, D, false, true><<<gr, bl, 0, stream>>>(p)
+          : kv_decode_kernel<T, D, false, false><<<gr, bl, 0, stream>>>(p);
+  int rc = check_launch("moc_kv_decode");
+  if (rc != MOC_OK || !split) return rc;
+  return ca_merge(sizeof(T) == 2 ? MOC_BF16 : MOC_F32, D, p.c, stream);
+}
+
+}  // namespace moc
+
+using namespace moc;
+
+extern "C" {
+
+size_t moc_kv_decode_workspace(int64_t B, int64_t L, int64_t n_max, int H, int HK, int D) {
+  if (HK <= 0) return 0;
+  const int64_t nrb = (L * (H / HK) + 15) / 16;
+  const int s = kd_splits(B * HK * nrb, n_max);
+  return s == 1 ? 0 : (size_t)s * B * HK * nrb * 16 * (D + 1) * 4;
+}
+
+int moc_kv_decode(const moc_kv_decode_args* d, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  const char* who = "moc_kv_decode";
+  MOC_REQUIRE(d != nullptr, MOC_ERR_ARG, "%s: no arguments", who);
+  const bool paged = d->table != nullptr;
+  moc_cross_args x = {};
+  x.q = d->q; x.k = d->k; x.v = d->v; x.out = d->out; x.lengths = d->lengths; x.words = d->words;
+  x.qb = d->qb; x.ql = d->ql; x.qh = d->qh;
+  x.kb = paged ? d->kp : d->kb; x.kn = d->kn; x.kh = d->kh;
+  x.vb = paged ? d->vp : d->vb; x.vn = d->vn; x.vh = d->vh;
+  x.B = d->B; x.L = d->L; x.H = d->H; x.HK = d->HK; x.D = d->D; x.dtype = d->dtype; x.scale = d->scale;
+  x.N = paged ? (d->max_pages > 0 && d->page > 0 ? d->max_pages * d->page : 0) : d->N;
+  KdArgs p = {};
+  int rc = ca_check(who, &x, &p.c);
+  if (rc != MOC_OK) return rc;
+  MOC_REQUIRE(d->q && d->k && d->v && d->out, MOC_ERR_ARG, "%s: null tensor", who);
+  if (paged) {
+    MOC_REQUIRE(d->lengths && !d->words, MOC_ERR_ARG, "%s: pages need lengths and take no key mask", who);
+    MOC_REQUIRE(d->page > 0 && d->page % 16 == 0, MOC_ERR_UNSUPPORTED, "%s: pages of %d tokens, expected a multiple of 16", who,
+                d->page);
+    MOC_REQUIRE(d->num_pages >= 0 && d->num_pages < (int64_t)1 << 31 && d->tb >= 0, MOC_ERR_ARG, "%s: bad page table", who);
+    p.table = d->table; p.kp = d->kp; p.vp = d->vp; p.tb = d->tb;
+    p.num_pages = d->num_pages; p.max_pages = d->max_pages; p.page = d->page;
+  }
+  p.causal = d->causal ? 1 : 0;
+  p.nrb = (p.c.rows + 15) / 16;
+  p.c.Lp = 16 * p.nrb;
+  p.c.lse = nullptr;
+  p.c.nsplit = kd_splits((int64_t)p.c.B * p.c.HK * p.nrb, p.c.N);
+  const size_t need = moc_kv_decode_workspace(x.B, x.L, x.N, x.H, x.HK, x.D);
+  MOC_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), MOC_ERR_ARG, "%s: workspace of %zu bytes, needs %zu", who,
+              workspace_bytes, need);
+  p.c.part = (float*)workspace;
+  p.c.part_lse = p.c.part + (size_t)p.c.nsplit * p.c.B * p.c.HK * p.c.Lp * x.D;
+  if (x.dtype == MOC_BF16)
+    return x.D == 64 ? kd_launch<bf16, 64>(p, paged, stream) : kd_launch<bf16, 128>(p, paged, stream);
+  return x.D == 64 ? kd_launch<float, 64>(p, paged, stream) : kd_launch<float, 128>(p, paged, stream);
+}
+
+}  // extern "C"

@@ -470,6 +470,179 @@ def decode_attention(q: torch.Tensor, cache: MemoryDecodeCache, routing: DecodeR
     return out
 
 
+class PagedKVCache:
+    """Keys and values of several sequences in pages of a pool, for tokens that attend to what came before them (or to
+    an encoder's states).  Inference only.
+
+    ``k_pages``, ``v_pages`` (pages, page size, kv heads, 64 or 128), float32 or bfloat16, the page size a multiple of 16;
+    they may be views with strides of their own (16-byte pieces).  ``block_table`` (sequences, pages of one) int32: token t
+    of sequence b lies in row t % page size of page block_table[b, t // page size]; entries outside the pool hold nothing:
+    what is written there is dropped, and keys there do not count.  ``lengths`` (sequences,) int32: tokens held.  The
+    server owns all four tensors and writes table and lengths as it hands out pages; the kernels read them on the device,
+    so a captured step stays right when they change."""
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor):
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+            raise ValueError(f"pages of shapes {tuple(k_pages.shape)}, {tuple(v_pages.shape)}: expected two equal (pages, page "
+                             "size, kv heads, head dim)")
+        if k_pages.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"pages must be float32 or bfloat16, got {k_pages.dtype}")
+        if k_pages.shape[1] == 0 or k_pages.shape[1] % 16 or k_pages.shape[2] == 0 or k_pages.shape[3] not in (64, 128):
+            raise ValueError(f"pages of {k_pages.shape[1]} tokens, {k_pages.shape[2]} kv heads, {k_pages.shape[3]} dims: expected "
+                             "a multiple of 16 tokens, heads of 64 or 128")
+        if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+            raise ValueError("block_table must be (sequences, pages) int32 with its rows in one piece")
+        if lengths.shape != block_table.shape[:1] or lengths.dtype != torch.int32 or not lengths.is_contiguous():
+            raise ValueError(f"lengths must be ({block_table.shape[0]},) int32, contiguous")
+        L.require_same_gpu(k_pages, v_pages, block_table, lengths)
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            es = t.element_size()
+            if t.stride(3) != 1 or t.data_ptr() % 16 or any(s * es % 16 for s in t.stride()[:3]):
+                raise ValueError(f"{name} must be rows in 16-byte pieces")
+            if t.stride(1) < t.shape[3] or t.stride(1) * es >= 1 << 24:
+                raise ValueError(f"{name}: rows that overlap, or lie 16 MiB or more apart")
+        self.k_pages, self.v_pages, self.block_table, self.lengths = k_pages, v_pages, block_table, lengths
+
+    @classmethod
+    def allocate(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, sequences: int, max_pages: int, *,
+                 dtype: torch.dtype = torch.bfloat16, device=None) -> "PagedKVCache":
+        """An empty cache: no sequence holds a page (table entries -1) or a token."""
+        dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+        shape = (num_pages, page_size, num_kv_heads, head_dim)
+        return cls(torch.zeros(shape, device=dev, dtype=dtype), torch.zeros(shape, device=dev, dtype=dtype),
+                   torch.full((sequences, max_pages), -1, device=dev, dtype=torch.int32),
+                   torch.zeros(sequences, device=dev, dtype=torch.int32))
+
+    @classmethod
+    @torch.no_grad()
+    def from_memory(cls, memory_attn, memory: torch.Tensor, memory_lengths: Optional[torch.Tensor] = None, *,
+                    page_size: int = 64, memory_positions: Optional[torch.Tensor] = None) -> "PagedKVCache":
+        """The keys and values of MemoryCrossAttention over an encoder's states (B, N, d), projected once for a
+        generation (``memory_decode_step``); pages lie in the order of the sequences.  ``memory_lengths`` (B,) as in its
+        forward; ``memory_positions`` as there."""
+        if memory.dim() != 3 or memory.shape[0] * memory.shape[1] == 0:
+            raise ValueError(f"memory must be (B, N, d) with states, got {tuple(memory.shape)}")
+        B, N, _ = memory.shape
+        k, v = memory_attn.project_memory(memory, memory_positions)
+        per = (N + page_size - 1) // page_size
+        self = cls.allocate(B * per, page_size, k.shape[2], k.shape[3], B, per, dtype=k.dtype, device=k.device)
+        self.block_table.copy_(torch.arange(B * per, device=k.device, dtype=torch.int32).view(B, per))
+        self.append(k, v)
+        if memory_lengths is not None:
+            if tuple(memory_lengths.shape) != (B,) or memory_lengths.dtype not in (torch.int32, torch.int64):
+                raise ValueError(f"memory_lengths of shape {tuple(memory_lengths.shape)}, expected ({B},) int32 or int64")
+            self.lengths.copy_(memory_lengths.clamp(0, N))
+        return self
+
+    @property
+    def page_size(self) -> int:
+        return self.k_pages.shape[1]
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.k_pages.dtype
+
+    @torch.no_grad()
+    def append(self, k: torch.Tensor, v: torch.Tensor, *, positions: Optional[torch.Tensor] = None,
+               q: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+               k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, norm: Optional[bool] = None,
+               inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False) -> Optional[torch.Tensor]:
+        """Writes new tokens' keys and values, k and v (sequences, tokens, kv heads, head dim), behind what the sequences
+        hold, and adds them to ``lengths``.  With ``positions`` (sequences,), int32 or int64, token i of sequence b goes to
+        place positions[b] + i instead and ``lengths`` stays the server's.  A token whose place has no page is dropped.
+
+        Keys may be normed and rotated on the way (``k_weight``, ``norm``, ``inv_freq``, ``interleaved`` as in
+        ``ops.qk_norm_rotate``, ``norm`` where a weight is given by default; the position is the token's place), and the
+        queries ``q`` of the same tokens with them: returns q so treated.  One launch."""
+        P, page, HK, D = self.k_pages.shape
+        B = self.lengths.shape[0]
+        if k.dim() != 4 or k.shape != v.shape or k.shape[0] != B or tuple(k.shape[2:]) != (HK, D):
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)}: expected ({B}, tokens, {HK}, {D})")
+        T = k.shape[1]
+        if q is not None and (q.dim() != 4 or tuple(q.shape[:2]) != (B, T) or q.shape[3] != D or q.shape[2] == 0):
+            raise ValueError(f"q {tuple(q.shape)}: expected ({B}, {T}, heads, {D})")
+        if positions is not None and (tuple(positions.shape) != (B,) or positions.dtype not in (torch.int32, torch.int64)):
+            raise ValueError(f"positions of shape {tuple(positions.shape)} {positions.dtype}, expected ({B},) int32 or int64")
+        if norm is None:
+            norm = q_weight is not None or k_weight is not None
+        if not norm and (q_weight is not None or k_weight is not None):
+            raise ValueError("a weight needs norm=True")
+        if q is None and q_weight is not None:
+            raise ValueError("q_weight without q")
+        if not (k.is_floating_point() and v.is_floating_point()) or (q is not None and not q.is_floating_point()):
+            raise ValueError("k, v and q must be floating-point")
+        L.require_same_gpu(self.k_pages, k, v, q, positions, q_weight, k_weight, inv_freq)
+        kw = ops._head_weight(k_weight, HK, D, "k_weight")
+        qw = None if q is None else ops._head_weight(q_weight, q.shape[2], D, "q_weight")
+        freq = ops._head_frequencies(inv_freq, D)
+        place = self.lengths if positions is None else positions
+        pos32 = int(place.dtype == torch.int32)
+
+        def rows(x):
+            x = x if x.dtype == self.dtype else x.to(self.dtype)
+            return x if x.stride(3) == 1 else x.contiguous()
+
+        def fields(x, w, y, strides, normed, turns, paged):
+            # (a page's stride in the batch stride's place)
+            xs = x.stride()
+            tab = (self.block_table.data_ptr(), self.block_table.stride(0), P, self.block_table.shape[1], page) if paged \
+                else (0, 0, 0, 0, 0)
+            return ops._pack_head_rows(x.data_ptr(), L.ptr0(w), y.data_ptr(), 0, 0, 0, place.data_ptr(), tab[0], *xs[:3],
+                                       *strides[:3], place.stride(0), 0, 1, tab[1], B, T, tab[2], tab[3], x.shape[2],
+                                       int(w is not None and w.dim() == 2), int(normed), int(turns), pos32, tab[4])
+
+        k, v = rows(k), rows(v)
+        turns = freq is not None
+        sets = [fields(k, kw, self.k_pages, self.k_pages.stride(), norm, turns, True),
+                fields(v, None, self.v_pages, self.v_pages.stride(), False, False, True)]
+        out = None
+        if q is not None:
+            q = rows(q)
+            out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+            sets.append(fields(q, qw, out, out.stride(), norm, turns, False))
+        dev = k.device
+        with L.on_device(dev):
+            call("moc_head_rotate_fwd", ops._head_args(sets, freq, D, interleaved, self.dtype, float(eps)), stream_ptr(dev))
+            if positions is None:
+                self.lengths.add_(T)
+        return out
+
+
+@torch.no_grad()
+def paged_attention(q: torch.Tensor, cache: PagedKVCache, *, causal: bool = False,
+                    softmax_scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of new tokens over their sequences' pages: q (B, H, D) or several tokens (B, L, H, D) -> the same shape
+    in the cache's type.  Each sees the ``cache.lengths`` first keys of its sequence; with ``causal`` token l of L the
+    first lengths - L + l + 1 (the tokens are the last ones appended).  A token that sees no key gets 0."""
+    _, page, HK, D = cache.k_pages.shape
+    B = cache.lengths.shape[0]
+    if q.dim() not in (3, 4) or q.shape[0] != B or q.shape[-1] != D or q.shape[-2] == 0 or q.shape[-2] % HK:
+        raise ValueError(f"queries of shape {tuple(q.shape)}: expected ({B}, [tokens,] heads, {D}) with heads a multiple of {HK}")
+    scale = float(D) ** -0.5 if softmax_scale is None else float(softmax_scale)
+    if not 0.0 < scale < 3e38:
+        raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
+    if not q.is_floating_point():
+        raise ValueError(f"queries of {q.dtype}")
+    L.require_same_gpu(cache.k_pages, q)
+    x = q.unsqueeze(1) if q.dim() == 3 else q
+    x = ops._attn_rows(x if x.dtype == cache.dtype else x.to(cache.dtype), False)
+    Lq, H, most = x.shape[1], x.shape[2], cache.block_table.shape[1]
+    if q.numel() == 0 or most == 0 or cache.k_pages.shape[0] == 0:
+        return torch.zeros(q.shape, device=q.device, dtype=cache.dtype)
+    out = torch.empty(q.shape, device=q.device, dtype=cache.dtype)
+    dev, ks, vs = q.device, cache.k_pages.stride(), cache.v_pages.stride()
+    nbytes = ops.kv_decode_workspace(B, Lq, most * page, H, HK, D)
+    with L.on_device(dev):
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        call("moc_kv_decode", ops.pack_kv_decode(x.data_ptr(), cache.k_pages.data_ptr(), cache.v_pages.data_ptr(),
+                                                 out.data_ptr(), cache.lengths.data_ptr(), cache.block_table.data_ptr(), 0,
+                                                 *ops._strides3(x), 0, ks[1], ks[2], 0, vs[1], vs[2], ks[0], vs[0],
+                                                 cache.block_table.stride(0), B, Lq, 0, cache.k_pages.shape[0], most, H, HK, D,
+                                                 L.dtype_code(cache.dtype), page, int(causal), scale),
+             ptr(ws), nbytes, stream_ptr(dev))
+    return out
+
+
 def _step_native(x, wq, wo, H: int, cache: MemoryDecodeCache, routing: DecodeRouting) -> bool:
     """Whether moc_decode_step takes the step (bf16 throughout, few rows; with the per-kernel timing armed
     the kernels run as separate entry points).  A re-routed step of 16 sequences: 172 to 182 us with a call
@@ -481,12 +654,39 @@ def _step_native(x, wq, wo, H: int, cache: MemoryDecodeCache, routing: DecodeRou
             and L.KERNEL_EVENTS is None)
 
 
-def memory_decode_step(memory_attn, hidden: torch.Tensor, cache: MemoryDecodeCache,
-                       routing: DecodeRouting) -> torch.Tensor:
+def _states_step(memory_attn, hidden: torch.Tensor, cache: PagedKVCache, positions) -> torch.Tensor:
+    """memory_decode_step over an encoder's states."""
+    B, Lx = hidden.shape[0], hidden.shape[1] if hidden.dim() == 3 else 1
+    H, D = memory_attn.num_heads, memory_attn.head_dim
+    wq, wo = memory_attn.q_proj.weight, memory_attn.o_proj.weight
+    if positions is not None and not memory_attn.rotary_dim:
+        raise ValueError("positions need rotary_dim")
+    if hidden.numel() == 0:
+        return torch.zeros(B, Lx, wo.shape[0], device=hidden.device, dtype=wo.dtype)
+    q = ops.linear(hidden.reshape(B, Lx, -1).to(wq.dtype), wq).view(B, Lx, H, D)
+    q = memory_attn.treat_queries(q, positions)
+    a = paged_attention(q, cache, softmax_scale=memory_attn.scale)
+    return ops.linear(a.reshape(B, Lx, H * D).to(wo.dtype), wo)
+
+
+def memory_decode_step(memory_attn, hidden: torch.Tensor, cache, routing: Optional[DecodeRouting] = None, *,
+                       positions: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One decode step of a memory sublayer: hidden (B, 1, d) -> (B, 1, d) (before the residual); or L tokens
-    of each sequence, (B, L, d) -> (B, L, d), over one routing (a prompt served from the cache)."""
+    of each sequence, (B, L, d) -> (B, L, d), over one routing (a prompt served from the cache).
+
+    Over an encoder's states: ``cache`` is a PagedKVCache (``PagedKVCache.from_memory``), there is no routing, and
+    ``positions`` (L,) or (B, L) are the tokens' for a module that rotates its heads (default 0, 1, ...)."""
     B = hidden.shape[0]
     H = memory_attn.num_heads
+    if isinstance(cache, PagedKVCache):
+        if routing is not None:
+            raise ValueError("a PagedKVCache takes no routing")
+        with torch.no_grad():
+            return _states_step(memory_attn, hidden, cache, positions)
+    if routing is None:
+        raise ValueError("a MemoryDecodeCache needs its routing")
+    if positions is not None or getattr(memory_attn, "treats_heads", False):
+        raise ValueError("positions, qk_norm and rotary_dim are for an encoder's states (PagedKVCache)")
     with torch.no_grad():
         wq, wo = memory_attn.q_proj.weight, memory_attn.o_proj.weight
         if hidden.dim() == 3 and hidden.shape[1] != 1:

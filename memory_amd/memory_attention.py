@@ -8,9 +8,13 @@ chapter, routed attention and its backward) runs in the HIP kernels.
 
 Three ways to call forward, all with the reference's return value
 ``(output (B, L, hidden_dim), None)``:
-  * ``memory=`` a (N, d) or (B, N, d) tensor, N a multiple of 64: dense
-    attention over it (memory_attention.py:402-478).  The rows are treated as
-    64-row chapters of weight 1; a 2-D memory is projected once for the batch.
+  * ``memory=`` a (N, d) or (B, N, d) tensor: dense attention over it
+    (memory_attention.py:402-478).  Where N is a multiple of 64 and nothing is
+    masked, normed or rotated, and heads have 64 dims, the rows are treated as
+    64-row chapters of weight 1; else (an encoder's states: any N,
+    ``memory_lengths`` or ``memory_mask``, heads of 64 or 128 dims) they are
+    projected and run through ops.cross_attention.  A 2-D memory is projected
+    once for the batch.
   * ``routed_memory_state=`` the fused sequence-level path: the bank, the
     selected chapters (shared prefix included) and their weights omega.  It
     computes exactly the reference's gather -> (normalise) -> x omega ->
@@ -40,12 +44,26 @@ except Exception:  # pragma: no cover
 CHAPTER_TOKENS = 64  # chapter tile height of the kernels
 
 
+class HeadNorm(nn.Module):
+    """Weight and eps of an RMS norm over the head dim, shared by the heads (ops.qk_norm_rotate applies it)."""
+
+    def __init__(self, head_dim: int, eps: float = 1e-6):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(head_dim))
+
+
 class MemoryCrossAttention(nn.Module):
     def __init__(self, hidden_dim: int, num_heads: int, num_kv_heads: Optional[int] = None,
                  memory_dim: Optional[int] = None, use_low_rank_projections: bool = False,
                  projection_rank: Optional[int] = None, reduced_dim_mode: bool = False,
                  reduced_dim: Optional[int] = None, wo_init_zero: bool = True, dropout: float = 0.0,
-                 use_flash_attention: bool = True, gradient_checkpointing: bool = False):
+                 use_flash_attention: bool = True, gradient_checkpointing: bool = False, qk_norm: bool = False,
+                 qk_norm_eps: float = 1e-6, rotary_dim: int = 0, rotary_base: float = 10000.0,
+                 rotary_interleaved: bool = False):
+        """The last five arguments have no reference counterpart and are for a dense ``memory``: ``qk_norm`` norms every
+        query and key head (parameters ``q_norm.weight``, ``k_norm.weight``), ``rotary_dim`` > 0 rotates that many dims of
+        each by position (``ops.qk_norm_rotate``)."""
         super().__init__()
         self.hidden_dim = hidden_dim
         self.memory_dim = memory_dim if memory_dim is not None else hidden_dim
@@ -81,6 +99,13 @@ class MemoryCrossAttention(nn.Module):
         if wo_init_zero:
             nn.init.zeros_(self.o_proj.weight)
         self._qnorm = None  # a caller's norm folded into q_proj for the duration of one call
+        if rotary_dim < 0 or rotary_dim % 2 or rotary_dim > self.head_dim:
+            raise ValueError(f"rotary_dim ({rotary_dim}) must be even and at most the head dim ({self.head_dim})")
+        if rotary_dim and not rotary_base > 0:
+            raise ValueError(f"rotary_base must be > 0, got {rotary_base}")
+        self.rotary_dim, self.rotary_base, self.rotary_interleaved = int(rotary_dim), float(rotary_base), bool(rotary_interleaved)
+        self.q_norm = HeadNorm(self.head_dim, qk_norm_eps) if qk_norm else None
+        self.k_norm = HeadNorm(self.head_dim, qk_norm_eps) if qk_norm else None
 
     # ------------------------------------------------------------------ helpers
     def _project_output(self, attn_output: torch.Tensor) -> torch.Tensor:
@@ -97,6 +122,69 @@ class MemoryCrossAttention(nn.Module):
         else:
             q = ops.linear(hidden_states, self.q_proj.weight)
         return q.view(B, L, self.num_heads, self.head_dim)
+
+    @property
+    def treats_heads(self) -> bool:
+        """Whether query and key heads are normed or rotated."""
+        return self.q_norm is not None or self.rotary_dim > 0
+
+    def _head_options(self, device) -> Dict[str, Any]:
+        freq = ops.rope_frequencies(self.rotary_dim, self.rotary_base, device) if self.rotary_dim else None
+        return dict(norm=self.q_norm is not None, eps=1e-6 if self.q_norm is None else self.q_norm.eps, inv_freq=freq,
+                    interleaved=self.rotary_interleaved)
+
+    def treat_queries(self, q: torch.Tensor, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Projected queries (B, L, H, Dh) normed and rotated as this module does, by ``positions`` (default 0, 1, ...)."""
+        if not self.treats_heads:
+            return q
+        w = None if self.q_norm is None else self.q_norm.weight
+        return ops.head_norm_rotate(q, w, positions=positions if self.rotary_dim else None, **self._head_options(q.device))
+
+    def _project_kv(self, memory: torch.Tensor):
+        """(k, v) of a dense memory, (B, N, kv heads, Dh), of batch 1 for a 2-D one."""
+        if memory.dim() not in (2, 3):
+            raise ValueError(f"memory must be (N, d) or (B, N, d), got {tuple(memory.shape)}")
+        opt = getattr(memory, "_moc_bank_opt", None)
+        if opt is not None:
+            opt.flush()     # every row is read
+        wk, wv = self.k_proj.weight, self.v_proj.weight
+        x = (memory if memory.dim() == 3 else memory.unsqueeze(0)).to(wk.dtype)
+        shape = (*x.shape[:2], self.num_kv_heads, self.head_dim)
+        return ops.linear(x, wk).view(shape), ops.linear(x, wv).view(shape)
+
+    def project_memory(self, memory: torch.Tensor, memory_positions: Optional[torch.Tensor] = None):
+        """Keys (normed and rotated as this module does) and values of an encoder's states (B, N, d), each
+        (B, N, kv heads, Dh): what a generation keeps of them (PagedKVCache.from_memory)."""
+        k, v = self._project_kv(memory)
+        if self.treats_heads:
+            w = None if self.k_norm is None else self.k_norm.weight
+            k = ops.head_norm_rotate(k, w, positions=memory_positions if self.rotary_dim else None,
+                                     **self._head_options(k.device))
+        return k, v
+
+    def _attend_states(self, hidden_states: torch.Tensor, memory: torch.Tensor, lengths, mask, query_positions,
+                       memory_positions) -> torch.Tensor:
+        """Attention over an encoder's states of any length, before o_proj."""
+        B, Lq, _ = hidden_states.shape
+        if memory.dim() == 3 and memory.shape[0] != B:
+            raise ValueError("batched memory must have the batch size of hidden_states")
+        qnorm = self._qnorm
+
+        def attend(h, m):
+            q = self._queries(h, qnorm)
+            k, v = self._project_kv(m)
+            if self.treats_heads:
+                wq, wk = (None, None) if self.q_norm is None else (self.q_norm.weight, self.k_norm.weight)
+                at = dict(q_positions=query_positions, k_positions=memory_positions) if self.rotary_dim else {}
+                q, k = ops.qk_norm_rotate(q, k, wq, wk, **at, **self._head_options(q.device))
+            if m.dim() == 2:
+                k, v = k[0], v[0]
+            a = ops.cross_attention(q, k, v, kv_lengths=lengths, key_mask=mask, softmax_scale=self.scale)
+            return a.reshape(B, Lq, self.hidden_dim)
+
+        if self._checkpointing():
+            return torch_checkpoint(attend, hidden_states, memory, use_reentrant=False)
+        return attend(hidden_states, memory)
 
     def _checkpointing(self) -> bool:
         return bool(self.gradient_checkpointing and self.training and torch.is_grad_enabled() and torch_checkpoint)
@@ -157,6 +245,8 @@ class MemoryCrossAttention(nn.Module):
         the forward): N = the memory rows, or the selected chapters' rows (slot-major, omega-weighted
         keys) for ``routed_memory_state``.  Computed by moc_xattn_weights from the forward's row
         log-sum-exp; no autograd."""
+        if self.treats_heads or self.head_dim != CHAPTER_TOKENS:
+            raise NotImplementedError("attention weights are formed of heads of 64 dims that are not normed or rotated")
         if routed_memory_state is not None:
             st = routed_memory_state
             norm_type = st.get("norm_type") if st.get("normalize", False) else None
@@ -177,11 +267,20 @@ class MemoryCrossAttention(nn.Module):
     def forward(self, hidden_states: torch.Tensor, memory: Optional[torch.Tensor] = None,
                 token_routing_state: Optional[Dict[str, Any]] = None, token_routing_kernel_version: str = "v2",
                 return_attn_weights: bool = False,
-                routed_memory_state: Optional[Dict[str, Any]] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+                routed_memory_state: Optional[Dict[str, Any]] = None, *, memory_lengths: Optional[torch.Tensor] = None,
+                memory_mask: Optional[torch.Tensor] = None, query_positions: Optional[torch.Tensor] = None,
+                memory_positions: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+        """Of a dense ``memory``: ``memory_lengths`` (B,) states of each sequence, ``memory_mask`` (B, N) which of them count
+        (True: it does), and with ``rotary_dim`` the positions of queries and states (default 0, 1, ...)."""
         if return_attn_weights and token_routing_state is not None:
             raise ValueError("return_attn_weights=True is not supported for token_routing_state path.")
+        if return_attn_weights and (memory_lengths is not None or memory_mask is not None):
+            raise ValueError("return_attn_weights=True is not supported with memory_lengths or memory_mask")
         out = self._project_output(self.attention_preproj(hidden_states, memory, token_routing_state,
-                                                          token_routing_kernel_version, routed_memory_state))
+                                                          token_routing_kernel_version, routed_memory_state,
+                                                          memory_lengths=memory_lengths, memory_mask=memory_mask,
+                                                          query_positions=query_positions,
+                                                          memory_positions=memory_positions))
         if return_attn_weights:
             return out, self.attention_weights(hidden_states, memory, routed_memory_state)
         return out, None
@@ -190,7 +289,9 @@ class MemoryCrossAttention(nn.Module):
                           token_routing_state: Optional[Dict[str, Any]] = None,
                           token_routing_kernel_version: str = "v2",
                           routed_memory_state: Optional[Dict[str, Any]] = None,
-                          query_norm=None) -> torch.Tensor:
+                          query_norm=None, *, memory_lengths: Optional[torch.Tensor] = None,
+                          memory_mask: Optional[torch.Tensor] = None, query_positions: Optional[torch.Tensor] = None,
+                          memory_positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """forward's attention output before o_proj, (B, L, hidden_dim).  ``query_norm`` =
         (weight, bias, eps, "rms" | "layer"): hidden_states are the un-normalised rows and the norm
         is applied inside the q projection (only the queries read the normalised rows)."""
@@ -200,9 +301,16 @@ class MemoryCrossAttention(nn.Module):
             prev, self._qnorm = self._qnorm, query_norm
             try:
                 return self.attention_preproj(hidden_states, memory, token_routing_state, token_routing_kernel_version,
-                                              routed_memory_state)
+                                              routed_memory_state, memory_lengths=memory_lengths, memory_mask=memory_mask,
+                                              query_positions=query_positions, memory_positions=memory_positions)
             finally:
                 self._qnorm = prev
+        states = (memory_lengths, memory_mask, query_positions, memory_positions)
+        if token_routing_state is not None or routed_memory_state is not None:
+            if self.treats_heads or any(t is not None for t in states):
+                raise ValueError("qk_norm, rotary_dim, memory_lengths, memory_mask and positions are for a dense memory")
+        if not self.rotary_dim and (query_positions is not None or memory_positions is not None):
+            raise ValueError("positions need rotary_dim")
         if token_routing_state is not None:
             return self._forward_token_routed_attention(hidden_states, token_routing_state,
                                                         token_routing_kernel_version)
@@ -214,6 +322,9 @@ class MemoryCrossAttention(nn.Module):
                                 float(st.get("eps", 1e-6)))
         if memory is None:
             raise ValueError("memory must be provided when token_routing_state is None.")
+        if (self.treats_heads or self.head_dim != CHAPTER_TOKENS or memory.dim() in (2, 3) and memory.shape[-2] % CHAPTER_TOKENS
+                or any(t is not None for t in states)):
+            return self._attend_states(hidden_states, memory, *states)
         return self._dense_as_chapters(hidden_states, memory)
 
     def _forward_token_routed_attention(self, hidden_states: torch.Tensor, token_routing_state: Dict[str, Any],

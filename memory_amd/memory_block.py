@@ -59,12 +59,16 @@ class MemorySublayer(nn.Module):
     ``residual_scale`` scales the stream it is added to: hidden = residual_scale * hidden + gate * norm(attention).
     ``forward(..., next_norm=module)`` also returns the next sublayer's norm of the new hidden states, (hidden, normed),
     from the same pass; ``normed=`` takes such rows in place of this sublayer's own norm, and ``gate=`` a gate of
-    the caller's own, one per row (..., 1) or per element, in place of the parameter."""
+    the caller's own, one per row (..., 1) or per element, in place of the parameter.
+
+    A dense ``memory`` may be an encoder's states of any length (``memory_lengths``, ``memory_mask``, ``query_positions``,
+    ``memory_positions`` as in MemoryCrossAttention.forward; ``qk_norm`` and ``rotary_*`` as in its constructor)."""
 
     def __init__(self, hidden_dim: int, num_heads: int, num_kv_heads: Optional[int] = None,
                  use_rms_norm: bool = True, norm_eps: float = 1e-6, memory_dim: Optional[int] = None,
                  wo_init_zero: bool = True, gradient_checkpointing: bool = False, post_norm: bool = False,
-                 gate: Optional[str] = None, gate_init: float = 1.0, residual_scale: float = 1.0):
+                 gate: Optional[str] = None, gate_init: float = 1.0, residual_scale: float = 1.0, qk_norm: bool = False,
+                 rotary_dim: int = 0, rotary_base: float = 10000.0, rotary_interleaved: bool = False):
         super().__init__()
         if gate not in (None, "scalar", "channel"):
             raise ValueError(f"gate must be None, 'scalar' or 'channel', got {gate!r}")
@@ -80,7 +84,9 @@ class MemorySublayer(nn.Module):
                                                                                                   eps=norm_eps)
         self.memory_attn = MemoryCrossAttention(hidden_dim, num_heads, num_kv_heads, memory_dim=memory_dim,
                                                 wo_init_zero=wo_init_zero,
-                                                gradient_checkpointing=gradient_checkpointing)
+                                                gradient_checkpointing=gradient_checkpointing, qk_norm=qk_norm,
+                                                qk_norm_eps=norm_eps, rotary_dim=rotary_dim, rotary_base=rotary_base,
+                                                rotary_interleaved=rotary_interleaved)
         # memory_layernorm folded into the q projection's GEMM where the shapes allow it
         # (ops.norm_linear_supported); False runs the norm kernel ahead of the projection
         self.fuse_norm = True
@@ -89,7 +95,9 @@ class MemorySublayer(nn.Module):
     def forward(self, hidden_states: torch.Tensor, memory: Optional[torch.Tensor] = None,
                 token_routing_state: Optional[Dict[str, Any]] = None, token_routing_kernel_version: str = "v2",
                 routed_memory_state: Optional[Dict[str, Any]] = None, *, normed: Optional[torch.Tensor] = None,
-                next_norm: Optional[nn.Module] = None, gate: Optional[torch.Tensor] = None):
+                next_norm: Optional[nn.Module] = None, gate: Optional[torch.Tensor] = None,
+                memory_lengths: Optional[torch.Tensor] = None, memory_mask: Optional[torch.Tensor] = None,
+                query_positions: Optional[torch.Tensor] = None, memory_positions: Optional[torch.Tensor] = None):
         attn = self.memory_attn
         cdt = attn.q_proj.weight.dtype
         if cdt not in (torch.float32, torch.bfloat16):
@@ -97,17 +105,19 @@ class MemorySublayer(nn.Module):
         ln = self.memory_layernorm
         kind = "rms" if self.use_rms_norm else "layer"
         bias = None if self.use_rms_norm else ln.bias
+        states = dict(memory_lengths=memory_lengths, memory_mask=memory_mask, query_positions=query_positions,
+                      memory_positions=memory_positions)
         if normed is not None:
             pre = attn.attention_preproj(normed.to(cdt), memory, token_routing_state, token_routing_kernel_version,
-                                         routed_memory_state)
+                                         routed_memory_state, **states)
         elif self.fuse_norm and ops.norm_linear_supported(hidden_states, attn.q_proj.weight):
             # only the q projection reads the normalised rows: the norm runs inside its GEMM
             pre = attn.attention_preproj(hidden_states, memory, token_routing_state, token_routing_kernel_version,
-                                         routed_memory_state, query_norm=(ln.weight, bias, ln.eps, kind))
+                                         routed_memory_state, query_norm=(ln.weight, bias, ln.eps, kind), **states)
         else:
             x = ops.row_norm(hidden_states, ln.weight, bias, ln.eps, kind, cdt)
             pre = attn.attention_preproj(x, memory, token_routing_state, token_routing_kernel_version,
-                                         routed_memory_state)
+                                         routed_memory_state, **states)
         gate = self.gate if gate is None else gate
         if self.post_layernorm is None and gate is None and next_norm is None and self.residual_scale == 1.0:
             return ops.linear_residual(pre, attn.o_proj.weight, hidden_states)

@@ -1574,3 +1574,416 @@ def token_routed_attention(q, routed_memory, wk, wv, idx, chapter_weights, *, to
     from .sparse_attention import token_routed_attention as _tra
     return _tra(q, routed_memory, wk, wv, idx, chapter_weights, tokens_per_chapter=tokens_per_chapter,
                 version=version, num_kv_heads=num_kv_heads)
+
+
+# --------------------------------------------------------------------------- heads: norm and rotation
+
+class _HeadRows(ctypes.Structure):
+    """moc_head_rows."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "w", "y", "dy", "dx", "dw", "positions", "table")]
+                + [(n, ctypes.c_int64) for n in ("xb", "xl", "xh", "yb", "yl", "yh", "pb", "pl", "pstep", "tb", "B", "L",
+                                                 "num_pages", "max_pages")]
+                + [(n, ctypes.c_int) for n in ("H", "w_head", "norm", "rotate", "pos32", "page")])
+
+
+class _HeadTail(ctypes.Structure):
+    """moc_head_args behind its sets."""
+    _fields_ = ([("inv_freq", ctypes.c_void_p)] + [(n, ctypes.c_int) for n in ("nseg", "D", "R", "interleaved", "dtype")]
+                + [("eps", ctypes.c_float)])
+
+
+_pack_head_rows = L.packer(_HeadRows)
+_pack_head_tail = L.packer(_HeadTail)
+_NO_ROWS = bytes(ctypes.sizeof(_HeadRows))
+
+
+def _head_args(sets, inv_freq, D: int, interleaved: bool, dtype: torch.dtype, eps: float) -> bytes:
+    """moc_head_args of packed sets of rows."""
+    R = 0 if inv_freq is None else 2 * inv_freq.shape[0]
+    return b"".join(sets) + _NO_ROWS * (3 - len(sets)) + _pack_head_tail(ptr0(inv_freq), len(sets), D, R, int(interleaved),
+                                                                         L.dtype_code(dtype), eps)
+
+
+def _position_fields(positions, count: int):
+    """(pointer, batch stride, row stride, step, 32-bit) of positions (L,), (B, L) or (B, 1); None: 0, 1, ..."""
+    if positions is None:
+        return 0, 0, 0, 1, 0
+    st = positions.stride()
+    if positions.dim() == 1:
+        return positions.data_ptr(), 0, st[0], 0, int(positions.dtype == torch.int32)
+    return (positions.data_ptr(), st[0] if positions.shape[0] > 1 else 0, st[1] if positions.shape[1] == count else 0, 0,
+            int(positions.dtype == torch.int32))
+
+
+def _check_positions(positions, B: int, count: int, name: str):
+    if positions is None:
+        return
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be int32 or int64, got {positions.dtype}")
+    if tuple(positions.shape) not in ((count,), (B, count), (1, count)):
+        raise ValueError(f"{name} of shape {tuple(positions.shape)}, expected ({count},) or ({B}, {count})")
+
+
+def _rope_fresh(rotary_dim: int, base: float, device: torch.device) -> torch.Tensor:
+    p = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device)
+    return torch.pow(torch.full_like(p, base), -p / rotary_dim)
+
+
+@functools.lru_cache(maxsize=64)
+def _rope_table(rotary_dim: int, base: float, device: torch.device) -> torch.Tensor:
+    with torch.inference_mode(False):
+        table = _rope_fresh(rotary_dim, base, device)
+    if table.is_cuda:
+        torch.cuda.current_stream(device).synchronize()     # callers on any stream find it there
+    return table
+
+
+def rope_frequencies(rotary_dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """Angle per position of each of the rotary_dim / 2 pairs of a head, base^(-2 p / rotary_dim), float64.  One tensor
+    per device, worked out at the first call (outside of a graph's capture) and not to be written to."""
+    if rotary_dim <= 0 or rotary_dim % 2 or not base > 0:
+        raise ValueError(f"rotary_dim must be even and positive, base positive; got {rotary_dim}, {base}")
+    device = torch.device("cpu" if device is None else device)
+    if device.type == "cuda":
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        if torch.cuda.is_current_stream_capturing():    # memory of a graph's own is not kept
+            return _rope_fresh(int(rotary_dim), float(base), device)
+    return _rope_table(int(rotary_dim), float(base), device)
+
+
+def _head_set(x, w, y, dy, dx, dw, norm: bool, rotate: bool, positions, out=None) -> bytes:
+    """moc_head_rows of x (B, L, H, D); ``out``: the tensor whose strides are y's or dy's."""
+    B, count, H, _ = x.shape
+    xs, ys = x.stride(), (x if out is None else out).stride()
+    pos, pb, pl, step, pos32 = _position_fields(positions, count) if rotate else (0, 0, 0, 0, 0)
+    return _pack_head_rows(x.data_ptr(), ptr0(w), ptr0(y), ptr0(dy), ptr0(dx), ptr0(dw), pos, 0, xs[0], xs[1], xs[2], ys[0],
+                           ys[1], ys[2], pb, pl, step, 0, B, count, 0, 0, H, int(w is not None and w.dim() == 2), int(norm),
+                           int(rotate), pos32, 0)
+
+
+def _head_rotate_forward(rows, weights, positions, inv_freq, cfg):
+    norm, interleaved, eps = cfg
+    out = [torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in rows]
+    sets = [_head_set(x, w, y, None, None, None, norm, inv_freq is not None, p, y)
+            for x, w, y, p in zip(rows, weights, out, positions)]
+    dev = rows[0].device
+    with L.on_device(dev):
+        call("moc_head_rotate_fwd", _head_args(sets, inv_freq, rows[0].shape[-1], interleaved, rows[0].dtype, eps),
+             stream_ptr(dev))
+    return out
+
+
+class _HeadRotate(torch.autograd.Function):
+    """qk_norm_rotate on rows whose last dim is contiguous (moc_head_rotate_fwd / _bwd).  The backward reads the rows
+    again and works their norms and angles out again: nothing is kept but the inputs."""
+
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, pq, pk, inv_freq, cfg):
+        rows, weights, pos = [q], [wq], [pq]
+        if k is not None:
+            rows, weights, pos = [q, k], [wq, wk], [pq, pk]
+        out = _head_rotate_forward(rows, weights, pos, inv_freq, cfg)
+        ctx.save_for_backward(q, k, wq, wk, pq, pk, inv_freq)
+        ctx.cfg = cfg
+        ctx.set_materialize_grads(False)
+        return tuple(out) if k is not None else out[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk=None):
+        q, k, wq, wk, pq, pk, inv_freq = ctx.saved_tensors
+        norm, interleaved, eps = ctx.cfg
+        need = ctx.needs_input_grad
+        grads = [None] * 8
+        sets, keep = [], []
+        for x, w, p, dy, ix, iw in ((q, wq, pq, dq, 0, 2), (k, wk, pk, dk, 1, 3)):
+            if x is None or dy is None or not (need[ix] or need[iw]):
+                continue
+            if dy.stride(-1) != 1:
+                dy = dy.contiguous()
+            dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[ix] else None
+            # (the gradients outlive the call, as .grad: they share nothing with its workspace)
+            dw = torch.empty(w.shape, device=x.device, dtype=torch.float32) if w is not None and need[iw] else None
+            sets.append(_head_set(x, w, None, dy, dx, dw, norm, inv_freq is not None, p, dy))
+            keep.append(dy)
+            grads[ix], grads[iw] = dx, dw
+        if sets:
+            dev = q.device
+            args = _head_args(sets, inv_freq, q.shape[-1], interleaved, q.dtype, eps)
+            with L.on_device(dev):
+                nbytes = L.query("moc_head_rotate_bwd_workspace", args)
+                ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+                call("moc_head_rotate_bwd", args, ptr(ws), nbytes, stream_ptr(dev))
+        return tuple(grads)
+
+
+def _head_weight(w, H: int, D: int, name: str):
+    if w is None:
+        return None
+    if tuple(w.shape) not in ((D,), (H, D)):
+        raise ValueError(f"{name} of shape {tuple(w.shape)}, expected ({D},) or ({H}, {D})")
+    return w.float().contiguous()
+
+
+def _head_frequencies(inv_freq, D: int):
+    if inv_freq is None:
+        return None
+    if inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= D or not inv_freq.is_floating_point():
+        raise ValueError(f"inv_freq: up to {D // 2} frequencies (one per pair), got {tuple(inv_freq.shape)} {inv_freq.dtype}")
+    return inv_freq.detach().double().contiguous()
+
+
+def _head_dim(x, name: str) -> int:
+    if x.dim() != 4 or x.shape[3] % 2 or not 0 < x.shape[3] <= 512 or x.shape[2] == 0:
+        raise ValueError(f"{name} of shape {tuple(x.shape)}: expected (batch, rows, heads, head dim), head dim even and at "
+                         "most 512")
+    return x.shape[3]
+
+
+def _heads(q, k, wq, wk, eps, norm, pq, pk, inv_freq, interleaved):
+    D = _head_dim(q, "q")
+    if k is not None and (_head_dim(k, "k") != D or k.dtype != q.dtype):
+        raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype}: one head dim and type")
+    if not norm and (wq is not None or wk is not None):
+        raise ValueError("a weight needs norm=True")
+    if inv_freq is None and not norm:
+        raise ValueError("neither a norm nor frequencies to rotate by: nothing to do")
+    if inv_freq is None and (pq is not None or pk is not None):
+        raise ValueError("positions need inv_freq")
+    if not q.is_floating_point():
+        raise ValueError(f"heads of {q.dtype}")
+    L.require_same_gpu(q, k, wq, wk, pq, pk, inv_freq)
+    _check_positions(pq, q.shape[0], q.shape[1], "q_positions")
+    wq = _head_weight(wq, q.shape[2], D, "q_weight")
+    if k is not None:
+        _check_positions(pk, k.shape[0], k.shape[1], "k_positions")
+        wk = _head_weight(wk, k.shape[2], D, "k_weight")
+    inv_freq = _head_frequencies(inv_freq, D)
+    dt = q.dtype
+    kt = dt if dt in _ROWS else torch.float32
+
+    def rows(x):
+        if x is None:
+            return None
+        x = x if x.dtype == kt else x.to(kt)
+        return x if x.stride(3) == 1 else x.contiguous()
+
+    q, k = rows(q), rows(k)
+    cfg = (bool(norm), bool(interleaved), float(eps))
+    if q.numel() == 0 and (k is None or k.numel() == 0) and not _differentiated(q, k, wq, wk):
+        out = (torch.empty_like(q), None if k is None else torch.empty_like(k))
+    elif _differentiated(q, k, wq, wk):
+        out = _HeadRotate.apply(q, k, wq, wk, pq, pk, inv_freq, cfg)
+        out = out if k is not None else (out, None)
+    elif k is None:
+        out = (_head_rotate_forward([q], [wq], [pq], inv_freq, cfg)[0], None)
+    else:
+        out = _head_rotate_forward([q, k], [wq, wk], [pq, pk], inv_freq, cfg)
+    return tuple(t if t is None or t.dtype == dt else t.to(dt) for t in out)
+
+
+def head_norm_rotate(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, eps: float = 1e-6, norm: bool = True,
+                     positions: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None,
+                     interleaved: bool = False) -> torch.Tensor:
+    """RMS norm of every head and its rotation by position, in one pass over x (batch, rows, heads, head dim).
+
+        u = x / sqrt(mean(x^2) + eps) * weight                       (``norm=False``: u = x)
+        (a, b) -> (a cos t - b sin t, b cos t + a sin t)             t = position * inv_freq[p], pair p of u
+
+    ``weight``: (head dim,), or one per head (heads, head dim).  ``inv_freq``: radians per position of the rotated pairs
+    (``rope_frequencies``; without it nothing turns), at most head dim / 2, as float64 (other types are converted).  Of
+    n frequencies pair p is elements (p, n + p), with ``interleaved`` (2 p, 2 p + 1); elements from 2 n on stay.
+    ``positions``: int32 or int64, (rows,) or (batch, rows); default 0, 1, ...  Angles are formed and reduced in float64.
+    x is float32 or bfloat16 (float16 runs as float32), with any strides; everything in between is float32, the result is
+    rounded once.  Differentiable once in x and weight."""
+    return _heads(x, None, weight, None, eps, norm, positions, None, inv_freq, interleaved)[0]
+
+
+def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                   k_weight: Optional[torch.Tensor] = None, *, eps: float = 1e-6, norm: bool = True,
+                   q_positions: Optional[torch.Tensor] = None, k_positions: Optional[torch.Tensor] = None,
+                   inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False):
+    """``head_norm_rotate`` of queries and keys (of other numbers of rows and heads, one head dim and type) in one
+    launch, forward and backward: (q, k)."""
+    return _heads(q, k, q_weight, k_weight, eps, norm, q_positions, k_positions, inv_freq, interleaved)
+
+
+# --------------------------------------------------------------------------- attention over another length
+
+class _CrossArgs(ctypes.Structure):
+    """moc_cross_args."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout", "out", "dq", "dk", "dv", "lse", "lengths", "words")]
+                + [(n, ctypes.c_int64) for n in ("qb", "ql", "qh", "kb", "kn", "kh", "vb", "vn", "vh", "db", "dl", "dh", "B",
+                                                 "L", "N")]
+                + [(n, ctypes.c_int) for n in ("H", "HK", "D", "dtype")] + [("scale", ctypes.c_float)])
+
+
+class _KvDecodeArgs(ctypes.Structure):
+    """moc_kv_decode_args."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lengths", "table", "words")]
+                + [(n, ctypes.c_int64) for n in ("qb", "ql", "qh", "kb", "kn", "kh", "vb", "vn", "vh", "kp", "vp", "tb", "B",
+                                                 "L", "N", "num_pages", "max_pages")]
+                + [(n, ctypes.c_int) for n in ("H", "HK", "D", "dtype", "page", "causal")] + [("scale", ctypes.c_float)])
+
+
+_pack_cross = L.packer(_CrossArgs)
+pack_kv_decode = L.packer(_KvDecodeArgs)
+_FEW_ROWS = 16      # rows per kv head up to which single tokens' attention is the faster forward
+
+
+def _attn_rows(t: torch.Tensor, rows_apart: bool) -> torch.Tensor:
+    """t (B, rows, heads, D) as the attention kernels read it: 16-byte pieces at strides of 16 bytes, and for keys
+    and values rows that do not overlap and lie less than 16 MiB apart.  Copied otherwise."""
+    es, sizes, st = t.element_size(), t.shape, t.stride()
+    ok = st[3] == 1 and t.data_ptr() % 16 == 0
+    for i in range(3):
+        ok = ok and (sizes[i] == 1 or st[i] * es % 16 == 0)
+    if ok and sizes[1] > 1:
+        ok = sizes[3] <= st[1] and st[1] * es < 1 << 24 if rows_apart else st[1] * es < 1 << 23
+    if ok and not rows_apart and sizes[2] > 1:
+        ok = st[2] * es * sizes[2] < 1 << 29
+    if ok:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides3(t: torch.Tensor):
+    """Batch, row and head strides; 0 where there is one of them."""
+    st, sizes = t.stride(), t.shape
+    return (st[0] if sizes[0] > 1 else 0, st[1] if sizes[1] > 1 else 0, st[2] if sizes[2] > 1 else 0)
+
+
+@functools.lru_cache(maxsize=1024)
+def _cross_sizes(B: int, Lq: int, N: int, H: int, HK: int, D: int):
+    """(bytes of the forward's workspace, rows of its log-sum-exp)"""
+    return L.query("moc_cross_fwd_workspace", B, Lq, N, H, HK, D), L.query("moc_cross_rows", Lq, H, HK)
+
+
+@functools.lru_cache(maxsize=1024)
+def _cross_bwd_workspace(B: int, Lq: int, N: int, H: int, HK: int, D: int, dt: int) -> int:
+    return L.query("moc_cross_bwd_workspace", B, Lq, N, H, HK, D, dt)
+
+
+@functools.lru_cache(maxsize=1024)
+def kv_decode_workspace(B: int, Lq: int, n_max: int, H: int, HK: int, D: int) -> int:
+    return L.query("moc_kv_decode_workspace", B, Lq, n_max, H, HK, D)
+
+
+def _cross_forward(q, k, v, lengths, words, scale: float, trains: bool):
+    """(out, lse) of checked operands; lse None where nothing trains."""
+    B, Lq, H, D = q.shape
+    N, HK = k.shape[1], k.shape[2]
+    dev, dt = q.device, L.dtype_code(q.dtype)
+    if B * Lq * N == 0:
+        return torch.zeros(B, Lq, H, D, device=dev, dtype=q.dtype), None
+    out = torch.empty(B, Lq, H, D, device=dev, dtype=q.dtype)
+    with L.on_device(dev):
+        if not trains and Lq * (H // HK) <= _FEW_ROWS:
+            nbytes = kv_decode_workspace(B, Lq, N, H, HK, D)
+            ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+            call("moc_kv_decode", pack_kv_decode(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr0(lengths), 0,
+                                                 ptr0(words), *_strides3(q), *_strides3(k), *_strides3(v), 0, 0, 0, B, Lq, N,
+                                                 0, 0, H, HK, D, dt, 0, 0, scale), ptr(ws), nbytes, stream_ptr(dev))
+            return out, None
+        nbytes, Lp = _cross_sizes(B, Lq, N, H, HK, D)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        lse = torch.empty(B, HK, Lp, device=dev, dtype=torch.float32) if trains else None
+        call("moc_cross_fwd", _pack_cross(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), 0, 0, 0, ptr0(lse),
+                                          ptr0(lengths), ptr0(words), *_strides3(q), *_strides3(k), *_strides3(v), 0, 0, 0, B,
+                                          Lq, N, H, HK, D, dt, scale), ptr(ws), nbytes, stream_ptr(dev))
+    return out, lse
+
+
+class _CrossAttention(torch.autograd.Function):
+    """cross_attention on checked operands (moc_cross_fwd / _bwd)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, words, scale):
+        out, lse = _cross_forward(q, k, v, lengths, words, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, lengths, words)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, lengths, words = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        B, Lq, H, D = q.shape
+        N, HK = k.shape[1], k.shape[2]
+        dev, dt = q.device, L.dtype_code(q.dtype)
+        if lse is None:     # no keys or no queries
+            return (*(torch.zeros(t.shape, device=dev, dtype=t.dtype) if n else None for t, n in zip((q, k, v), need)), None,
+                    None, None)
+        dout = _attn_rows(dout, False)
+        dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        dk = dv = None
+        if need[1] or need[2]:
+            dk, dv = torch.empty(k.shape, device=dev, dtype=q.dtype), torch.empty(v.shape, device=dev, dtype=q.dtype)
+        with L.on_device(dev):
+            nbytes = _cross_bwd_workspace(B, Lq, N, H, HK, D, dt)
+            ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+            call("moc_cross_bwd", _pack_cross(q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(),
+                                              dq.data_ptr(), ptr0(dk), ptr0(dv), lse.data_ptr(), ptr0(lengths), ptr0(words),
+                                              *_strides3(q), *_strides3(k), *_strides3(v), *_strides3(dout), B, Lq, N, H, HK,
+                                              D, dt, ctx.scale), ptr(ws), nbytes, stream_ptr(dev))
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None
+
+
+def _key_words(key_mask, lengths, B: int, N: int):
+    words = torch.empty(B, (N + 63) // 64, device=key_mask.device, dtype=torch.int64)
+    with L.on_device(key_mask.device):
+        call("moc_key_words", key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1), ptr(lengths), B, N,
+             words.data_ptr(), stream_ptr(key_mask.device))
+    return words
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lengths: Optional[torch.Tensor] = None,
+                    key_mask: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None) -> torch.Tensor:
+    """softmax(softmax_scale q k^T) v of queries q (B, L, H, D) over keys and values of another length, (B, N, HK, D), or
+    (N, HK, D) shared by the batch; query head h reads kv head h // (H / HK).  Result (B, L, H, D).
+
+    ``kv_lengths`` (B,) integers: keys of sequence b from kv_lengths[b] on do not count.  ``key_mask`` (B, N) truth
+    values: keys where it is False do not.  Keys that do not count may hold anything (NaN too) and get gradient 0; a
+    sequence none of whose keys counts has result 0 and gives no gradient.  D is 64 or 128, L and N any; float32 or
+    bfloat16 of one type (float16 runs as float32), with any strides (rows that are not 16-byte pieces are copied).
+    ``softmax_scale`` > 0, default D^-0.5.  Logits, sums and the running maximum are float32; in bfloat16 the
+    probabilities enter their products rounded to it.  Differentiable once in q, k and v."""
+    if k.dim() == 3 and v.dim() == 3:
+        k, v = k.expand(q.shape[0], *k.shape), v.expand(q.shape[0], *v.shape)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: expected (B, L, H, D), (B, N, HK, D) "
+                         "and k's shape")
+    B, Lq, H, D = q.shape
+    N, HK = k.shape[1], k.shape[2]
+    if D not in (64, 128):
+        raise ValueError(f"cross_attention takes heads of 64 or 128 dims, got {D}")
+    if HK == 0 or H == 0 or H % HK:
+        raise ValueError(f"{H} query heads on {HK} kv heads")
+    if q.dtype != k.dtype or q.dtype != v.dtype or not q.is_floating_point():
+        raise ValueError(f"q, k and v of one floating-point type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    scale = float(D) ** -0.5 if softmax_scale is None else float(softmax_scale)
+    if not 0.0 < scale < 3e38:
+        raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
+    L.require_same_gpu(q, k, v, kv_lengths, key_mask)
+    lengths = words = None
+    if kv_lengths is not None:
+        if tuple(kv_lengths.shape) != (B,) or kv_lengths.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"kv_lengths of shape {tuple(kv_lengths.shape)} {kv_lengths.dtype}, expected ({B},) int32 or int64")
+        lengths = (kv_lengths if kv_lengths.dtype == torch.int32 else kv_lengths.clamp(0, N).int()).contiguous()
+    if key_mask is not None:
+        if tuple(key_mask.shape) != (B, N) or key_mask.dtype != torch.bool:
+            raise ValueError(f"key_mask of shape {tuple(key_mask.shape)} {key_mask.dtype}, expected ({B}, {N}) bool")
+    dt = q.dtype
+    if dt not in _ROWS:
+        q, k, v = q.float(), k.float(), v.float()
+    if key_mask is not None and B * N:
+        words = _key_words(key_mask, lengths, B, N)
+    q, k, v = _attn_rows(q, False), _attn_rows(k, True), _attn_rows(v, True)
+    if _differentiated(q, k, v):
+        out = _CrossAttention.apply(q, k, v, lengths, words, scale)
+    else:
+        out = _cross_forward(q, k, v, lengths, words, scale, False)[0]
+    return out if out.dtype == dt else out.to(dt)
