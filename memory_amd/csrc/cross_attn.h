@@ -28,6 +28,18 @@ __device__ __forceinline__ void ca_wait_all() { asm volatile("s_waitcnt vmcnt(0)
 __device__ __forceinline__ float ca_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float ca_max3(float a, float b, float c) { return fmax_fast(fmax_fast(a, b), c); }
 
+// s c - off; EXACT rounds the product by itself, so that a row's largest logit has exactly 2^0
+template <bool EXACT>
+__device__ __forceinline__ float ca_logit(float s, float c, float off) {
+  if constexpr (EXACT) {
+#pragma clang fp contract(off)
+    const float x = s * c;
+    return x - off;
+  } else {
+    return __builtin_fmaf(s, c, -off);
+  }
+}
+
 // Rows of D elements, ROWS of them, moved global -> LDS (SwzTile<T, D>) by WAVES waves: an instruction
 // fills RPI rows of CH 16-byte chunks, wave w issues the IPW instructions from row (ROWS / WAVES) w.
 template <typename T, int D, int ROWS, int WAVES>
@@ -69,10 +81,16 @@ struct CaKeys {
   }
 };
 
+// bf16 probabilities and logit gradients enter their products rounded to 8 bits, which adds to a result about as much
+// error as its own rounding has (1.4 times in all) where many keys and rows share it, and more where few do.  There (up
+// to this many keys, or rows of a kv head) they go in two pieces, 16 bits, at half as many products again: those calls
+// are launches and loads, not products.
+constexpr int kCaFew = 128;
+
 // What a launch works on (moc_cross_args with the derived sizes)
 struct CaArgs {
-  const void *q, *k, *v, *dout, *out_in;
-  void *out, *dq, *dk, *dv;
+  const void *q, *k, *v, *dout;
+  void *out, *out_low, *dq, *dk, *dv;
   float *lse, *delta, *part, *part_lse;
   const int32_t* lengths;
   const uint64_t* words;
@@ -100,6 +118,23 @@ __device__ __forceinline__ void ca_mask(f32x4 (&st)[4][QB], uint64_t word, int g
       for (int qb = 0; qb < QB; ++qb) st[kb][qb][e] = live ? st[kb][qb][e] : to;
     }
 }
+
+// Stores 4 consecutive results, and with `low` what their rounding left over
+template <typename T>
+__device__ __forceinline__ void ca_store4(T* out, T* low, const f32x4& x) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const T y = from_f<T>(x[e]);
+    out[e] = y;
+    if (low) low[e] = from_f<T>(x[e] - to_f(y));
+  }
+}
+
+// The piece of x that its rounding to T leaves over
+template <typename T>
+__device__ __forceinline__ T ca_low(float x, T rounded) { return from_f<T>(x - to_f(rounded)); }
+
+inline bool ca_few(const CaArgs& a) { return a.N <= kCaFew || a.rows <= kCaFew; }
 
 int ca_check(const char* who, const moc_cross_args* a, CaArgs* c);
 // out (and lse) of a.nsplit partial results a.part, a.part_lse over rows [B][HK][Lp]

@@ -1,6 +1,8 @@
 // Attention over keys and values of another length, backward (notation of cross_attn.h).
 //   P_ij = 2^(scale log2(e) q_i . k_j - lse_i),  delta_i = dO_i . o_i,  dS_ij = P_ij (dO_i . v_j - delta_i)
 //   dq_i = scale sum_j dS_ij k_j,   dk_j = scale sum_i dS_ij q_i,   dv_j = sum_i P_ij dO_i
+// delta takes the result before its rounding (out + out_low): where few keys share a row's weight, dO . v_j and delta
+// nearly cancel, and out's 2^-9 alone made dq and dk twice as inexact as everything else.
 // i over the rows (all queries of the G heads) of j's kv head.  dq runs over the keys of a block of rows and leaves
 // delta behind; dk and dv run over the rows of a block of keys, so nothing is summed by atomics and every result has
 // one order.  P and dS enter their products rounded to the operands' type; sums, P itself and delta are f32.
@@ -11,12 +13,14 @@ namespace moc {
 // dq: one workgroup = 128 rows of one (sequence, kv head) as in the forward, K and V tiles double-buffered; K^T for
 // dS K is read from the K tile with the transposing LDS read.  A tile's 64 keys go in two halves, which halves the
 // score registers.  With SPLIT each of nsplit workgroups takes a share of the keys and writes f32 rows.
-template <typename T, int D, bool SPLIT>
+template <typename T, int D, bool SPLIT, bool TWO>
 __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
   typedef typename Frag<T>::type F8;
   using Tile = SwzTile<T, D>;
   using Stage = CaStage<T, D, kCaKeys, 4>;
   constexpr int KS = D / 32, DB = D / 16, TB = kCaKeys * D * (int)sizeof(T);
+  // dP - delta: from -delta as the product's start, which saves a subtraction, or, where exact, from the whole dP
+  constexpr bool kSub = TWO || sizeof(T) == 4;
   __shared__ __attribute__((aligned(16))) char sK[2][TB];
   __shared__ __attribute__((aligned(16))) char sV[2][TB];
   const int nrb = a.Lp / kCaRows;
@@ -44,20 +48,27 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
     const int64_t l = r / a.G, h = hk * a.G + r % a.G;
     const T* qp = (const T*)a.q + b * a.qb + l * a.ql + h * a.qh;
     const T* dp = (const T*)a.dout + b * a.db + l * a.dl + h * a.dh;
-    const T* op = (const T*)a.out_in + (((size_t)b * a.L + l) * a.H + h) * D;
-    float sum = 0.f;
+    const size_t oat = (((size_t)b * a.L + l) * a.H + h) * D;
+    // delta is formed as dP is, by the matrix cores and in their order: the diagonal of dO o^T.  A row that one key
+    // takes whole (o = v) then has dP = delta to the bit, and no gradient.
+    f32x4 dd = f32x4{0.f, 0.f, 0.f, 0.f}, dlow = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       qf[qb][ks] = ok ? Load8<T, T>::run(qp + 32 * ks + 8 * g) : zero_frag<T>();
       dof[qb][ks] = ok ? Load8<T, T>::run(dp + 32 * ks + 8 * g) : zero_frag<T>();
-      if (ok) {
-        const F8 of = Load8<T, T>::run(op + 32 * ks + 8 * g);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) sum += to_f(dof[qb][ks][x]) * to_f(of[x]);
+      const F8 of = ok ? Load8<T, T>::run((const T*)a.out + oat + 32 * ks + 8 * g) : zero_frag<T>();
+      mma(dd, of, dof[qb][ks]);
+      if (a.out_low) {
+        const F8 ol = ok ? Load8<T, T>::run((const T*)a.out_low + oat + 32 * ks + 8 * g) : zero_frag<T>();
+        mma(dlow, ol, dof[qb][ks]);
       }
     }
+    // the lane of group c16 / 4 holds row c16 of column c16
+    dd += dlow;
+    const float mine = (c16 & 2) ? ((c16 & 1) ? dd[3] : dd[2]) : ((c16 & 1) ? dd[1] : dd[0]);
+    const float del = __shfl(mine, 16 * (c16 >> 2) + c16, 64);
     const size_t at = ((size_t)b * a.HK + hk) * a.Lp + r;
-    dl[qb] = quad_sum(sum);
+    dl[qb] = del;
     lse[qb] = ok ? a.lse[at] : INFINITY;
     if (g == 0 && sp == 0) a.delta[at] = dl[qb];
   }
@@ -107,7 +118,8 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
           st[kb][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
-          dp[kb][qb] = f32x4{-dl[qb], -dl[qb], -dl[qb], -dl[qb]};
+          const float d0 = kSub ? 0.f : -dl[qb];
+          dp[kb][qb] = f32x4{d0, d0, d0, d0};
         }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
@@ -121,7 +133,7 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
             mma(dp[kb][qb], av, dof[qb][ks]);
           }
         }
-      F8 dsf[2];
+      F8 dsf[2], dsl[2];
       // (keys that do not count: P would be 2^-lse, which may be inf, of their zeroed logits)
       const uint32_t live = (uint32_t)(word >> (32 * kh)) >> (4 * g);
 #pragma unroll
@@ -130,15 +142,19 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float ds = ca_exp2(st[kb][qb][e] * c - lse[qb]) * dp[kb][qb][e];
+            float ds = ca_exp2(st[kb][qb][e] * c - lse[qb]) * (kSub ? dp[kb][qb][e] - dl[qb] : dp[kb][qb][e]);
             if (word != ~0ull) ds = (live >> (16 * kb + e)) & 1 ? ds : 0.f;
             dsf[qb][4 * kb + e] = from_f<T>(ds);
+            if constexpr (TWO) dsl[qb][4 * kb + e] = ca_low<T>(ds, dsf[qb][4 * kb + e]);
           }
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
         const F8 f = mk_frag<Tile, T>(Ks, 32 * kh, 16 * db, lane);
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb) mma(acc[qb][db], dsf[qb], f);
+        for (int qb = 0; qb < 2; ++qb) {
+          mma(acc[qb][db], dsf[qb], f);
+          if constexpr (TWO) mma(acc[qb][db], dsl[qb], f);
+        }
       }
     }
     if (tn < t_end) ca_wait_all();
@@ -192,13 +208,14 @@ template <> struct DkvShape<bf16, 128> { static constexpr int KB = 2, QS = 64; }
 template <> struct DkvShape<float, 64> { static constexpr int KB = 2, QS = 32; };
 template <> struct DkvShape<float, 128> { static constexpr int KB = 1, QS = 32; };
 
-template <typename T, int D, bool SPLIT>
+template <typename T, int D, bool SPLIT, bool TWO>
 __global__ __launch_bounds__(kCaThreads) void cross_dkv_kernel(CaArgs a) {
   typedef typename Frag<T>::type F8;
   using Tile = SwzTile<T, D>;
   constexpr int KB = DkvShape<T, D>::KB, QS = DkvShape<T, D>::QS, KEYS = 64 * KB;
   using Stage = CaStage<T, D, QS, 4>;
   constexpr int KS = D / 32, DB = D / 16, TB = QS * D * (int)sizeof(T);
+  constexpr bool kSub = TWO || sizeof(T) == 4;   // as in dq
   __shared__ __attribute__((aligned(16))) char sQ[2][TB];
   __shared__ __attribute__((aligned(16))) char sD[2][TB];
   __shared__ float sL[2][QS], sDl[2][QS];
@@ -305,15 +322,15 @@ __global__ __launch_bounds__(kCaThreads) void cross_dkv_kernel(CaArgs a) {
 #pragma unroll
     for (int half = 0; half < QS / 32; ++half) {
       const int r0 = 32 * half;
-      f32x4 st[2][KB], dp[2][KB], nl[2];
+      f32x4 st[2][KB], dp[2][KB], nl[2], nd[2];
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
         nl[qb] = *reinterpret_cast<const f32x4*>(&sL[buf][r0 + 16 * qb + 4 * g]);
-        const f32x4 nd = *reinterpret_cast<const f32x4*>(&sDl[buf][r0 + 16 * qb + 4 * g]);
+        nd[qb] = *reinterpret_cast<const f32x4*>(&sDl[buf][r0 + 16 * qb + 4 * g]);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           st[qb][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-          dp[qb][kb] = nd;
+          dp[qb][kb] = kSub ? f32x4{0.f, 0.f, 0.f, 0.f} : nd[qb];
         }
       }
 #pragma unroll
@@ -328,7 +345,7 @@ __global__ __launch_bounds__(kCaThreads) void cross_dkv_kernel(CaArgs a) {
             mma(dp[qb][kb], da, vf[kb][ks]);
           }
         }
-      F8 pa[KB], sa[KB];
+      F8 pa[KB], sa[KB], pb[KB], sb[KB];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -336,8 +353,13 @@ __global__ __launch_bounds__(kCaThreads) void cross_dkv_kernel(CaArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float pt = ca_exp2(st[qb][kb][e] * c + nl[qb][e]);
+            const float ds = pt * (kSub ? dp[qb][kb][e] + nd[qb][e] : dp[qb][kb][e]);
             pa[kb][4 * qb + e] = from_f<T>(pt);
-            sa[kb][4 * qb + e] = from_f<T>(pt * dp[qb][kb][e]);
+            sa[kb][4 * qb + e] = from_f<T>(ds);
+            if constexpr (TWO) {
+              pb[kb][4 * qb + e] = ca_low<T>(pt, pa[kb][4 * qb + e]);
+              sb[kb][4 * qb + e] = ca_low<T>(ds, sa[kb][4 * qb + e]);
+            }
           }
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
@@ -347,6 +369,10 @@ __global__ __launch_bounds__(kCaThreads) void cross_dkv_kernel(CaArgs a) {
         for (int kb = 0; kb < KB; ++kb) {
           mma(dv[kb][db], pa[kb], fd);
           mma(dk[kb][db], sa[kb], fq);
+          if constexpr (TWO) {
+            mma(dv[kb][db], pb[kb], fd);
+            mma(dk[kb][db], sb[kb], fq);
+          }
         }
       }
     }
@@ -423,14 +449,18 @@ BwdPlan bwd_plan(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtyp
 template <typename T, int D>
 static int bwd_launch(CaArgs& a, const BwdPlan& p, hipStream_t stream) {
   const char* who = "moc_cross_bwd";
+  constexpr bool kHalf = sizeof(T) == 2;
+  const bool few = kHalf && ca_few(a);
   // (dq comes first: it leaves delta behind)
   a.nsplit = p.dq_splits;
   const int64_t tiles = (int64_t)a.B * a.HK * a.nsplit * (a.Lp / kCaRows);
   MOC_REQUIRE(tiles < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "%s: too many row blocks", who);
   if (a.nsplit > 1)
-    cross_dq_kernel<T, D, true><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
+    few ? cross_dq_kernel<T, D, true, kHalf><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a)
+        : cross_dq_kernel<T, D, true, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
   else
-    cross_dq_kernel<T, D, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
+    few ? cross_dq_kernel<T, D, false, kHalf><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a)
+        : cross_dq_kernel<T, D, false, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
   int rc = check_launch("moc_cross_bwd: dq");
   if (rc != MOC_OK) return rc;
   if (a.nsplit > 1) {
@@ -445,9 +475,11 @@ static int bwd_launch(CaArgs& a, const BwdPlan& p, hipStream_t stream) {
   const int64_t blocks = (int64_t)a.B * a.HK * a.nsplit * ((a.N + KEYS - 1) / KEYS);
   MOC_REQUIRE(blocks < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "%s: too many key blocks", who);
   if (a.nsplit > 1)
-    cross_dkv_kernel<T, D, true><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(a);
+    few ? cross_dkv_kernel<T, D, true, kHalf><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(a)
+        : cross_dkv_kernel<T, D, true, false><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(a);
   else
-    cross_dkv_kernel<T, D, false><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(a);
+    few ? cross_dkv_kernel<T, D, false, kHalf><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(a)
+        : cross_dkv_kernel<T, D, false, false><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(a);
   rc = check_launch("moc_cross_bwd: dk, dv");
   if (rc != MOC_OK || a.nsplit == 1) return rc;
   const int64_t lanes = (int64_t)a.B * a.N * a.HK * (D / 2);

@@ -14,7 +14,7 @@ namespace moc {
 // the rescale, and P stays <= 2^8.
 constexpr float kCaSlack = 8.f;
 
-template <typename T, int D, bool SPLIT>
+template <typename T, int D, bool SPLIT, bool TWO>
 __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
   typedef typename Frag<T>::type F8;
   using Tile = SwzTile<T, D>;
@@ -133,24 +133,28 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
         for (int db = 0; db < DB; ++db) o[db][qb] *= alpha;
       }
     }
-    F8 pf[2][2];
+    F8 pf[2][2], pl[2][2];
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
       const float off = m[qb] == -INFINITY ? 0.f : m[qb];   // (a row whose logits so far are all -inf)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          pf[qb][h][e] = from_f<T>(ca_exp2(st[2 * h][qb][e] * c - off));
-          pf[qb][h][4 + e] = from_f<T>(ca_exp2(st[2 * h + 1][qb][e] * c - off));
+        for (int x = 0; x < 8; ++x) {
+          const float p = ca_exp2(ca_logit<TWO || sizeof(T) == 4>(st[2 * h + (x >> 2)][qb][x & 3], c, off));
+          pf[qb][h][x] = from_f<T>(p);
+          if constexpr (TWO) pl[qb][h][x] = ca_low<T>(p, pf[qb][h][x]);
         }
     }
     f32x4 ls[2];
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
       ls[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
-      mma(ls[qb], ones, pf[qb][0]);
-      mma(ls[qb], ones, pf[qb][1]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mma(ls[qb], ones, pf[qb][h]);
+        if constexpr (TWO) mma(ls[qb], ones, pl[qb][h]);
+      }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -158,7 +162,10 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
       for (int db = 0; db < DB; ++db) {
         const F8 f = mk_frag<Tile, T>(Vs, 32 * h, 16 * db, lane);
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb) mma(o[db][qb], f, pf[qb][h]);
+        for (int qb = 0; qb < 2; ++qb) {
+          mma(o[db][qb], f, pf[qb][h]);
+          if constexpr (TWO) mma(o[db][qb], f, pl[qb][h]);
+        }
       }
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) lsum[qb] += ls[qb][0];
@@ -184,11 +191,11 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
       if (g == 0) a.part_lse[row] = l == 0.f ? -INFINITY : m[qb] + log2f(l);
     } else {
       if (r < a.rows) {
-        T* op = (T*)a.out + (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + 4 * g;
+        const size_t at = (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + 4 * g;
+        T* op = (T*)a.out + at;
+        T* lp = a.out_low ? (T*)a.out_low + at : nullptr;
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) op[16 * db + e] = from_f<T>(o[db][qb][e] * inv);
+        for (int db = 0; db < DB; ++db) ca_store4<T>(op + 16 * db, lp ? lp + 16 * db : nullptr, o[db][qb] * inv);
       }
       if (a.lse && g == 0)
         a.lse[((size_t)b * a.HK + hk) * a.Lp + r] = r >= a.rows || l == 0.f ? INFINITY : m[qb] + log2f(l);
@@ -227,9 +234,8 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(CaArgs a) {
     den += w;
   }
   const float inv = den == 0.f ? 0.f : 1.f / den;
-  T* op = (T*)a.out + (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + 4 * ch;
-#pragma unroll
-  for (int x = 0; x < 4; ++x) op[x] = from_f<T>(acc[x] * inv);
+  const size_t at = (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + 4 * ch;
+  ca_store4<T>((T*)a.out + at, a.out_low ? (T*)a.out_low + at : nullptr, acc * inv);
   if (a.lse && ch == 0) a.lse[row] = den == 0.f ? INFINITY : M + log2f(den);
 }
 
@@ -271,7 +277,7 @@ int ca_check(const char* who, const moc_cross_args* p, CaArgs* c) {
   const int64_t st[] = {a.qb, a.ql, a.qh, a.kb, a.kn, a.kh, a.vb, a.vn, a.vh, a.db, a.dl, a.dh};
   for (int64_t s : st)
     MOC_REQUIRE(s >= 0 && s * es % 16 == 0, MOC_ERR_ARG, "%s: strides must be multiples of 16 bytes", who);
-  const void* ptrs[] = {a.q, a.k, a.v, a.out, a.dout, a.dq, a.dk, a.dv};
+  const void* ptrs[] = {a.q, a.k, a.v, a.out, a.out_low, a.dout, a.dq, a.dk, a.dv};
   for (const void* x : ptrs)
     MOC_REQUIRE(((uintptr_t)x & 15) == 0, MOC_ERR_ARG, "%s: tensors must be 16-byte aligned", who);
   // a tile's rows are read through one bounded buffer with 32-bit offsets (the top bit marks keys left out)
@@ -280,7 +286,7 @@ int ca_check(const char* who, const moc_cross_args* p, CaArgs* c) {
   MOC_REQUIRE(a.N == 1 || (a.kn >= a.D && a.vn >= a.D), MOC_ERR_ARG, "%s: rows of K or V overlap", who);
   CaArgs& o = *c;
   o = CaArgs{};
-  o.q = a.q; o.k = a.k; o.v = a.v; o.out = a.out; o.out_in = a.out; o.dout = a.dout;
+  o.q = a.q; o.k = a.k; o.v = a.v; o.out = a.out; o.out_low = a.dtype == MOC_BF16 ? a.out_low : nullptr; o.dout = a.dout;
   o.dq = a.dq; o.dk = a.dk; o.dv = a.dv; o.lse = a.lse; o.lengths = a.lengths; o.words = a.words;
   o.qb = a.qb; o.ql = a.ql; o.qh = a.qh; o.kb = a.kb; o.kn = a.kn; o.kh = a.kh; o.vb = a.vb; o.vn = a.vn; o.vh = a.vh;
   o.db = a.db; o.dl = a.dl; o.dh = a.dh;
@@ -298,11 +304,15 @@ template <typename T, int D>
 static int fwd_launch(CaArgs& a, hipStream_t stream) {
   const int64_t tiles = (int64_t)a.B * a.HK * a.nsplit * (a.Lp / kCaRows);
   MOC_REQUIRE(tiles < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "moc_cross_fwd: too many row blocks");
+  constexpr bool kHalf = sizeof(T) == 2;
+  const bool few = kHalf && ca_few(a);
   if (a.nsplit == 1) {
-    cross_fwd_kernel<T, D, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
+    few ? cross_fwd_kernel<T, D, false, kHalf><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a)
+        : cross_fwd_kernel<T, D, false, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
     return check_launch("moc_cross_fwd");
   }
-  cross_fwd_kernel<T, D, true><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
+  few ? cross_fwd_kernel<T, D, true, kHalf><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a)
+      : cross_fwd_kernel<T, D, true, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
   int rc = check_launch("moc_cross_fwd");
   if (rc != MOC_OK) return rc;
   return ca_merge(sizeof(T) == 2 ? MOC_BF16 : MOC_F32, D, a, stream);

@@ -24,6 +24,7 @@ __global__ __launch_bounds__(64 * kKdWaves) void kv_decode_kernel(KdArgs p) {
   using Tile = SwzTile<T, D>;
   using Stage = CaStage<T, D, 16, 1>;            // a block of 16 keys, by one wave
   constexpr int KS = D / 32, DB = D / 16, TB = kCaKeys * D * (int)sizeof(T);
+  constexpr bool kTwo = sizeof(T) == 2;
   static_assert(TB >= 16 * D * 4, "a wave's V tile holds its 16 result rows");
   __shared__ __attribute__((aligned(16))) char sV[kKdWaves][TB];
   __shared__ float sM[kKdWaves][16], sL[kKdWaves][16];
@@ -147,23 +148,29 @@ __global__ __launch_bounds__(64 * kKdWaves) void kv_decode_kernel(KdArgs p) {
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
     }
     const float off = m == -INFINITY ? 0.f : m;
-    // the sums take the unrounded probabilities: a lane's 16 keys here, the four lanes of the row at the end
-    F8 pf[2];
+    // the sums: a lane's 16 keys here, the four lanes of the row at the end.  In bf16 the probabilities enter their
+    // product in two pieces, 16 bits of them: the second product costs nothing under the loads, and one piece alone would
+    // add as much error again as the result's rounding has.
+    F8 pf[2], pl[2];
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p0 = ca_exp2(st[2 * hh][0][e] * c - off), p1 = ca_exp2(st[2 * hh + 1][0][e] * c - off);
-        lsum += p0 + p1;
-        pf[hh][e] = from_f<T>(p0);
-        pf[hh][4 + e] = from_f<T>(p1);
+      for (int x = 0; x < 8; ++x) {
+        const float p = ca_exp2(ca_logit<true>(st[2 * hh + (x >> 2)][0][x & 3], c, off));
+        lsum += p;
+        pf[hh][x] = from_f<T>(p);
+        if constexpr (kTwo) pl[hh][x] = ca_low<T>(p, pf[hh][x]);
       }
     ca_wait_all();   // V landed
     wave_lds_sync();
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-      for (int db = 0; db < DB; ++db) mma(o[db], mk_frag<Tile, T>(Vs, 32 * hh, 16 * db, lane), pf[hh]);
+      for (int db = 0; db < DB; ++db) {
+        const F8 f = mk_frag<Tile, T>(Vs, 32 * hh, 16 * db, lane);
+        mma(o[db], f, pf[hh]);
+        if constexpr (kTwo) mma(o[db], f, pl[hh]);
+      }
     wave_lds_sync();   // the next tile's V overwrites this one once it has been read
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }

@@ -1813,7 +1813,8 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
 
 class _CrossArgs(ctypes.Structure):
     """moc_cross_args."""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout", "out", "dq", "dk", "dv", "lse", "lengths", "words")]
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout", "out", "out_low", "dq", "dk", "dv", "lse", "lengths",
+                                                "words")]
                 + [(n, ctypes.c_int64) for n in ("qb", "ql", "qh", "kb", "kn", "kh", "vb", "vn", "vh", "db", "dl", "dh", "B",
                                                  "L", "N")]
                 + [(n, ctypes.c_int) for n in ("H", "HK", "D", "dtype")] + [("scale", ctypes.c_float)])
@@ -1872,12 +1873,12 @@ def kv_decode_workspace(B: int, Lq: int, n_max: int, H: int, HK: int, D: int) ->
 
 
 def _cross_forward(q, k, v, lengths, words, scale: float, trains: bool):
-    """(out, lse) of checked operands; lse None where nothing trains."""
+    """(out, what its rounding left over, lse) of checked operands; the last two None where nothing trains."""
     B, Lq, H, D = q.shape
     N, HK = k.shape[1], k.shape[2]
     dev, dt = q.device, L.dtype_code(q.dtype)
     if B * Lq * N == 0:
-        return torch.zeros(B, Lq, H, D, device=dev, dtype=q.dtype), None
+        return torch.zeros(B, Lq, H, D, device=dev, dtype=q.dtype), None, None
     out = torch.empty(B, Lq, H, D, device=dev, dtype=q.dtype)
     with L.on_device(dev):
         if not trains and Lq * (H // HK) <= _FEW_ROWS:
@@ -1886,14 +1887,15 @@ def _cross_forward(q, k, v, lengths, words, scale: float, trains: bool):
             call("moc_kv_decode", pack_kv_decode(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr0(lengths), 0,
                                                  ptr0(words), *_strides3(q), *_strides3(k), *_strides3(v), 0, 0, 0, B, Lq, N,
                                                  0, 0, H, HK, D, dt, 0, 0, scale), ptr(ws), nbytes, stream_ptr(dev))
-            return out, None
+            return out, None, None
         nbytes, Lp = _cross_sizes(B, Lq, N, H, HK, D)
         ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
         lse = torch.empty(B, HK, Lp, device=dev, dtype=torch.float32) if trains else None
-        call("moc_cross_fwd", _pack_cross(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), 0, 0, 0, ptr0(lse),
-                                          ptr0(lengths), ptr0(words), *_strides3(q), *_strides3(k), *_strides3(v), 0, 0, 0, B,
-                                          Lq, N, H, HK, D, dt, scale), ptr(ws), nbytes, stream_ptr(dev))
-    return out, lse
+        low = torch.empty_like(out) if trains and q.dtype == torch.bfloat16 else None
+        call("moc_cross_fwd", _pack_cross(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), ptr0(low), 0, 0, 0,
+                                          ptr0(lse), ptr0(lengths), ptr0(words), *_strides3(q), *_strides3(k), *_strides3(v),
+                                          0, 0, 0, B, Lq, N, H, HK, D, dt, scale), ptr(ws), nbytes, stream_ptr(dev))
+    return out, low, lse
 
 
 class _CrossAttention(torch.autograd.Function):
@@ -1901,15 +1903,15 @@ class _CrossAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lengths, words, scale):
-        out, lse = _cross_forward(q, k, v, lengths, words, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths, words)
+        out, low, lse = _cross_forward(q, k, v, lengths, words, scale, True)
+        ctx.save_for_backward(q, k, v, out, low, lse, lengths, words)
         ctx.scale = scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, lengths, words = ctx.saved_tensors
+        q, k, v, out, low, lse, lengths, words = ctx.saved_tensors
         need = ctx.needs_input_grad
         B, Lq, H, D = q.shape
         N, HK = k.shape[1], k.shape[2]
@@ -1926,9 +1928,9 @@ class _CrossAttention(torch.autograd.Function):
             nbytes = _cross_bwd_workspace(B, Lq, N, H, HK, D, dt)
             ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
             call("moc_cross_bwd", _pack_cross(q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(),
-                                              dq.data_ptr(), ptr0(dk), ptr0(dv), lse.data_ptr(), ptr0(lengths), ptr0(words),
-                                              *_strides3(q), *_strides3(k), *_strides3(v), *_strides3(dout), B, Lq, N, H, HK,
-                                              D, dt, ctx.scale), ptr(ws), nbytes, stream_ptr(dev))
+                                              ptr0(low), dq.data_ptr(), ptr0(dk), ptr0(dv), lse.data_ptr(), ptr0(lengths),
+                                              ptr0(words), *_strides3(q), *_strides3(k), *_strides3(v), *_strides3(dout), B,
+                                              Lq, N, H, HK, D, dt, ctx.scale), ptr(ws), nbytes, stream_ptr(dev))
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None
 
 
