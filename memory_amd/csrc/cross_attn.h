@@ -24,6 +24,11 @@ __device__ __forceinline__ void ca_dma16(__amdgpu_buffer_rsrc_t r, uint32_t voff
   const uint32_t m0 = (uint32_t)(uintptr_t)(ca_lds_ptr_t)lds;
   asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(m0) : "memory");
 }
+// The same with 4 bytes per lane
+__device__ __forceinline__ void ca_dma4(__amdgpu_buffer_rsrc_t r, uint32_t voff, const void* lds) {
+  const uint32_t m0 = (uint32_t)(uintptr_t)(ca_lds_ptr_t)lds;
+  asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(m0) : "memory");
+}
 __device__ __forceinline__ void ca_wait_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ float ca_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float ca_max3(float a, float b, float c) { return fmax_fast(fmax_fast(a, b), c); }
@@ -53,6 +58,47 @@ struct CaStage {
   static __device__ __forceinline__ int row(int i, int lane) { return RPI * i + lane / CH; }
   static __device__ __forceinline__ uint32_t chunk(int i, int lane) {
     return (uint32_t)(((lane % CH) ^ (row(i, lane) & 7)) * 16);
+  }
+};
+
+// The operand reads of a lane from SwzTile<T, D> tiles, with what a lane adds to their addresses worked out once (bf16:
+// two registers for rows as they are, four for rows transposed; a row block, a further 64 dims and the tile itself are
+// constants in the instructions).  R, rb: first row, multiples of 16 and of 32.
+template <typename T, int D>
+struct CaFrag {
+  using Tile = SwzTile<T, D>;
+  typedef typename Frag<T>::type F8;
+  int lane;
+  uint32_t s[2], t[4];
+  __device__ __forceinline__ explicit CaFrag(int ln) : lane(ln) {
+    if constexpr (sizeof(T) == 2) {
+      const int g = ln >> 4, q = ln & 15, row = 4 * g + (q >> 2);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s[i] = (uint32_t)(q * 2 * D + (((4 * i + g) ^ (q & 7)) << 4));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        t[i] = (uint32_t)(row * 2 * D + (((2 * i + ((q & 3) >> 1)) ^ (row & 7)) << 4) + 8 * (q & 1));
+    }
+  }
+  // rows R + c16, dims 32 ks + 8 g ..
+  __device__ __forceinline__ F8 row(const char* tile, int R, int ks) const {
+    if constexpr (sizeof(T) == 2)
+      return *reinterpret_cast<const bf16x8*>(tile + s[ks & 1] + (R * 2 * D + 128 * (ks >> 1)));
+    else
+      return Tile::frag(tile, R + (lane & 15), 32 * ks + 8 * (lane >> 4));
+  }
+  // dim 16 db + c16 of rows rb + 4 g + e and rb + 16 + 4 g + e
+  __device__ __forceinline__ F8 col(const char* tile, int rb, int db) const {
+    if constexpr (sizeof(T) == 2) {
+      typedef short v4s __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) v4s* lds_v4s;
+      const char* p = tile + t[db & 3] + (rb * 2 * D + 128 * (db >> 2));
+      const v4s v[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)p),
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(p + 16 * 2 * D))};
+      return __builtin_bit_cast(F8, v);
+    } else {
+      return mk_frag<Tile, T>(tile, rb, 16 * db, lane);
+    }
   }
 };
 
@@ -99,6 +145,13 @@ struct CaArgs {
   float scale, scale_log2;
 };
 
+// Pair i of a launch's (sequence, kv head) pairs, the sequences innermost: the eight XCDs each take a run of pairs,
+// and with ragged sequences those of one head are as much work as those of another.
+__device__ __forceinline__ void ca_pair(const CaArgs& a, int64_t i, int& b, int& hk) {
+  b = (int)((uint32_t)i % (uint32_t)a.B);
+  hk = (int)((uint32_t)i / (uint32_t)a.B);
+}
+
 __device__ __forceinline__ int ca_keys_end(const CaArgs& a, int b) {
   if (!a.lengths) return a.N;
   const int n = ca_scalar(a.lengths + b);
@@ -120,14 +173,19 @@ __device__ __forceinline__ void ca_mask(f32x4 (&st)[4][QB], uint64_t word, int g
 }
 
 // Stores 4 consecutive results, and with `low` what their rounding left over
+template <typename T> struct Vec4;
+template <> struct Vec4<bf16> { typedef bf16x4 type; };
+template <> struct Vec4<float> { typedef f32x4 type; };
 template <typename T>
 __device__ __forceinline__ void ca_store4(T* out, T* low, const f32x4& x) {
+  typename Vec4<T>::type y, z;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const T y = from_f<T>(x[e]);
-    out[e] = y;
-    if (low) low[e] = from_f<T>(x[e] - to_f(y));
+    y[e] = from_f<T>(x[e]);
+    z[e] = from_f<T>(x[e] - to_f(y[e]));
   }
+  *reinterpret_cast<typename Vec4<T>::type*>(out) = y;
+  if (low) *reinterpret_cast<typename Vec4<T>::type*>(low) = z;
 }
 
 // The piece of x that its rounding to T leaves over

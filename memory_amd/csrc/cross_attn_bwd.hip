@@ -27,8 +27,8 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
   const int nsp = SPLIT ? a.nsplit : 1;
   const int64_t t0 = xcd_tile((int64_t)a.B * a.HK * nsp * nrb);
   if (t0 < 0) return;
-  const int64_t bh = t0 / ((int64_t)nsp * nrb);
-  const int b = (int)(bh / a.HK), hk = (int)(bh % a.HK);
+  int b, hk;
+  ca_pair(a, t0 / ((int64_t)nsp * nrb), b, hk);
   const int sp = SPLIT ? (int)((t0 / nrb) % nsp) : 0;
   const int r0 = (int)(t0 % nrb) * kCaRows;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -202,29 +202,35 @@ __global__ __launch_bounds__(256) void cross_dq_sum_kernel(CaArgs a) {
 // dk, dv: one workgroup = 4 waves x 16 KB keys of one (sequence, kv head), whose K and V rows stay in registers as
 // matrix operands; the rows' Q and dO tiles of QS rows are double-buffered in LDS and shared by the waves, and read
 // from there both as they are and transposed.
+// VL: V stays in LDS, each wave reading its own rows, where with it the registers of two waves per SIMD do not hold.
 template <typename T, int D> struct DkvShape;
-template <> struct DkvShape<bf16, 64> { static constexpr int KB = 2, QS = 128; };
-template <> struct DkvShape<bf16, 128> { static constexpr int KB = 2, QS = 64; };
-template <> struct DkvShape<float, 64> { static constexpr int KB = 2, QS = 32; };
-template <> struct DkvShape<float, 128> { static constexpr int KB = 1, QS = 32; };
+template <> struct DkvShape<bf16, 64> { static constexpr int KB = 2, QS = 128, VL = 0, WAVES = 2; };
+template <> struct DkvShape<bf16, 128> { static constexpr int KB = 2, QS = 32, VL = 1, WAVES = 2; };
+template <> struct DkvShape<float, 64> { static constexpr int KB = 2, QS = 32, VL = 0, WAVES = 1; };
+template <> struct DkvShape<float, 128> { static constexpr int KB = 1, QS = 32, VL = 0, WAVES = 1; };
 
 template <typename T, int D, bool SPLIT, bool TWO>
-__global__ __launch_bounds__(kCaThreads) void cross_dkv_kernel(CaArgs a) {
+__global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv_kernel(CaArgs a) {
   typedef typename Frag<T>::type F8;
   using Tile = SwzTile<T, D>;
   constexpr int KB = DkvShape<T, D>::KB, QS = DkvShape<T, D>::QS, KEYS = 64 * KB;
   using Stage = CaStage<T, D, QS, 4>;
   constexpr int KS = D / 32, DB = D / 16, TB = QS * D * (int)sizeof(T);
   constexpr bool kSub = TWO || sizeof(T) == 4;   // as in dq
-  __shared__ __attribute__((aligned(16))) char sQ[2][TB];
-  __shared__ __attribute__((aligned(16))) char sD[2][TB];
-  __shared__ float sL[2][QS], sDl[2][QS];
+  constexpr bool kVL = DkvShape<T, D>::VL;
+  using StageV = CaStage<T, D, KEYS, 4>;
+  constexpr int VB = kVL ? KEYS * D * (int)sizeof(T) : 16;
+  __shared__ __attribute__((aligned(16))) char sQ[2][TB], sD[2][TB], sV[VB];
+  __shared__ __attribute__((aligned(16))) float sL[2][QS], sDl[2][QS];
+  // what a lane's DMAs of a step need: offsets of its rows in Q and dO, and the rows' heads (out of registers meanwhile)
+  __shared__ uint32_t sAt[3 * Stage::IPW][kCaThreads];
   const int nkb = (a.N + KEYS - 1) / KEYS;
   const int nsp = SPLIT ? a.nsplit : 1;
   const int64_t t0 = xcd_tile((int64_t)a.B * a.HK * nsp * nkb);
   if (t0 < 0) return;
-  const int64_t bh = t0 / ((int64_t)nsp * nkb);
-  const int b = (int)(bh / a.HK), hk = (int)(bh % a.HK);
+  int b, hk;
+  ca_pair(a, t0 / ((int64_t)nsp * nkb), b, hk);
+  const int64_t bh = (int64_t)b * a.HK + hk;
   const int sp = SPLIT ? (int)((t0 / nkb) % nsp) : 0;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c16 = lane & 15;
@@ -236,7 +242,7 @@ __global__ __launch_bounds__(kCaThreads) void cross_dkv_kernel(CaArgs a) {
   // bits of this wave's keys
   const uint32_t live = kw < a.N ? (uint32_t)(keys.word(kw / kCaKeys) >> (kw % kCaKeys)) : 0u;
 
-  F8 kf[KB][KS], vf[KB][KS];
+  F8 kf[KB][KS], vf[kVL ? 1 : KB][KS];
   {
     // bounded by the tensor's last row; what lies in keys that do not count stays in their own sums
     const int left = a.N - kw;
@@ -254,13 +260,19 @@ __global__ __launch_bounds__(kCaThreads) void cross_dkv_kernel(CaArgs a) {
         const uint32_t ko = r * (uint32_t)(a.kn * sizeof(T)) + e, vo = r * (uint32_t)(a.vn * sizeof(T)) + e;
         if constexpr (sizeof(T) == 2) {
           kf[kb2][ks] = __builtin_bit_cast(F8, kb.load16(ko, 0));
-          vf[kb2][ks] = __builtin_bit_cast(F8, vb.load16(vo, 0));
+          if constexpr (!kVL) vf[kb2][ks] = __builtin_bit_cast(F8, vb.load16(vo, 0));
         } else {
           const V16 w2[2] = {kb.load16(ko, 0), kb.load16(ko + 16, 0)}, x2[2] = {vb.load16(vo, 0), vb.load16(vo + 16, 0)};
           kf[kb2][ks] = __builtin_bit_cast(F8, w2);
           vf[kb2][ks] = __builtin_bit_cast(F8, x2);
         }
       }
+    if constexpr (kVL) {
+#pragma unroll
+      for (int i = 0; i < StageV::IPW; ++i)
+        ca_dma16(vb.r, (uint32_t)StageV::row(i, lane) * (uint32_t)(a.vn * sizeof(T)) + StageV::chunk(i, lane),
+                 sV + (VB / 4) * wave + 1024 * i);
+    }
   }
   f32x4 dk[KB][DB], dv[KB][DB];
 #pragma unroll
@@ -276,84 +288,98 @@ __global__ __launch_bounds__(kCaThreads) void cross_dkv_kernel(CaArgs a) {
   const int s_end = any == 0 ? s_begin : SPLIT ? (int)((int64_t)nstep * (sp + 1) / nsp) : nstep;
   const float* lse = a.lse + bh * a.Lp;
   const float* delta = a.delta + bh * a.Lp;
-  float preL = 0.f, preD = 0.f;
-  // rows of step s: 64-bit base of its first query, offsets from there (a step spans at most QS queries)
+  // Rows of step s: row QS s + r is query l0 + (q0 + r) / G, head (q0 + r) % G of the group, with r = lr G + hr a
+  // constant of the lane; so its offset from query l0 is that of (lr, hr), q0 heads on, and a query on where q0 + hr
+  // passes G.  (The buffers' bases are 64-bit, a step spans at most QS queries.)
+#pragma unroll
+  for (int i = 0; i < Stage::IPW; ++i) {
+    const int r = Stage::RPW * wave + Stage::row(i, lane), lr = r / a.G, hr = r - lr * a.G;
+    sAt[3 * i][tid] = (uint32_t)(lr * (uint32_t)a.ql + hr * (uint32_t)a.qh) * (uint32_t)sizeof(T) + Stage::chunk(i, lane);
+    sAt[3 * i + 1][tid] = (uint32_t)(lr * (uint32_t)a.dl + hr * (uint32_t)a.dh) * (uint32_t)sizeof(T) + Stage::chunk(i, lane);
+    sAt[3 * i + 2][tid] = (uint32_t)hr;
+  }
+  const uint32_t q_on = (uint32_t)((a.ql - a.G * a.qh) * (int64_t)sizeof(T)), d_on = (uint32_t)((a.dl - a.G * a.dh) * (int64_t)sizeof(T));
+  const int l_step = QS / a.G, q_step = QS - l_step * a.G;
+  int l0 = (int)((int64_t)QS * s_begin / a.G), q0 = QS * s_begin - l0 * a.G;   // of the step to be fetched next
   auto fetch = [&](int s, int buf) {
-    const int r0 = QS * s, l0 = r0 / a.G, q0 = r0 - l0 * a.G;
-    const int last = (r0 + QS < a.rows ? r0 + QS : a.rows) - 1;
-    const int span = last / a.G - l0;                // queries after the first
+    const int r0 = QS * s, rows = a.rows - r0 < QS ? a.rows - r0 : QS;
+    const int span = (q0 + rows - 1) / a.G;          // queries after the first
     const Buf qb = ca_buf((const T*)a.q + b * a.qb + (int64_t)hk * a.G * a.qh + l0 * a.ql,
                           (uint32_t)((span * a.ql + (a.G - 1) * a.qh + D) * sizeof(T)));
     const Buf db = ca_buf((const T*)a.dout + b * a.db + (int64_t)hk * a.G * a.dh + l0 * a.dl,
                           (uint32_t)((span * a.dl + (a.G - 1) * a.dh + D) * sizeof(T)));
+    const uint32_t qs = q0 * (uint32_t)(a.qh * sizeof(T)), ds = q0 * (uint32_t)(a.dh * sizeof(T));
 #pragma unroll
     for (int i = 0; i < Stage::IPW; ++i) {
       const int r = Stage::RPW * wave + Stage::row(i, lane);
-      const uint32_t x = (uint32_t)(q0 + r), l = x / (uint32_t)a.G, h = x - l * a.G, ch = Stage::chunk(i, lane);
-      uint32_t qo = (l * (uint32_t)a.ql + h * (uint32_t)a.qh) * (uint32_t)sizeof(T) + ch;
-      uint32_t od = (l * (uint32_t)a.dl + h * (uint32_t)a.dh) * (uint32_t)sizeof(T) + ch;
-      if (r0 + r >= a.rows) qo = od = kCaOut;
+      const bool on = q0 + (int)sAt[3 * i + 2][tid] >= a.G;
+      uint32_t qo = sAt[3 * i][tid] + qs + (on ? q_on : 0u), od = sAt[3 * i + 1][tid] + ds + (on ? d_on : 0u);
+      if (r >= rows) qo = od = kCaOut;
       ca_dma16(qb.r, qo, sQ[buf] + (TB / 4) * wave + 1024 * i);
       ca_dma16(db.r, od, sD[buf] + (TB / 4) * wave + 1024 * i);
     }
-    if (tid < QS) {     // (padded to Lp, a multiple of QS: +inf and 0)
-      preL = lse[r0 + tid];
-      preD = delta[r0 + tid];
+    l0 += l_step;
+    q0 += q_step;
+    if (q0 >= a.G) {
+      q0 -= a.G;
+      ++l0;
     }
-  };
-  auto stash = [&](int buf) {
-    if (tid < QS) {
-      sL[buf][tid] = -preL;
-      sDl[buf][tid] = -preD;
+    // lse and delta of the rows, padded to Lp, a multiple of QS, with +inf and 0
+    if (64 * wave < QS) {
+      const bool in = 64 * wave + lane < QS;
+      const uint32_t o = in ? 4u * (64 * wave + lane) : kCaOut;
+      const Buf lb = ca_buf(lse + r0, 4 * QS), eb = ca_buf(delta + r0, 4 * QS);
+      if (in) {
+        ca_dma4(lb.r, o, &sL[buf][64 * wave]);
+        ca_dma4(eb.r, o, &sDl[buf][64 * wave]);
+      }
     }
   };
   const float c = a.scale_log2;
-  if (s_begin < s_end) {
-    fetch(s_begin, s_begin & 1);
-    stash(s_begin & 1);
-  }
+  const CaFrag<T, D> fr(lane);
+  const char* Vw = sV + 16 * KB * wave * D * (int)sizeof(T);
+  if (s_begin < s_end) fetch(s_begin, 0);
   ca_wait_all();
   __syncthreads();
-  for (int s = s_begin; s < s_end; ++s) {
-    const int buf = s & 1;
+  // A step goes in halves of 32 rows, a half's logits in two blocks of 16: the products over the rows take 32, the
+  // scores of 16 are all that is held at a time.
+  auto step = [&](const int s, auto which) {
+    constexpr int buf = decltype(which)::value;
     if (s + 1 < s_end) fetch(s + 1, buf ^ 1);
     const char* Qs = sQ[buf];
     const char* Ds = sD[buf];
 #pragma unroll
     for (int half = 0; half < QS / 32; ++half) {
       const int r0 = 32 * half;
-      f32x4 st[2][KB], dp[2][KB], nl[2], nd[2];
-#pragma unroll
-      for (int qb = 0; qb < 2; ++qb) {
-        nl[qb] = *reinterpret_cast<const f32x4*>(&sL[buf][r0 + 16 * qb + 4 * g]);
-        nd[qb] = *reinterpret_cast<const f32x4*>(&sDl[buf][r0 + 16 * qb + 4 * g]);
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          st[qb][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-          dp[qb][kb] = kSub ? f32x4{0.f, 0.f, 0.f, 0.f} : nd[qb];
-        }
-      }
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int qb = 0; qb < 2; ++qb) {
-          const F8 qa = Tile::frag(Qs, r0 + 16 * qb + c16, 32 * ks + 8 * g);
-          const F8 da = Tile::frag(Ds, r0 + 16 * qb + c16, 32 * ks + 8 * g);
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
-            mma(st[qb][kb], qa, kf[kb][ks]);
-            mma(dp[qb][kb], da, vf[kb][ks]);
-          }
-        }
       F8 pa[KB], sa[KB], pb[KB], sb[KB];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+      for (int qb = 0; qb < 2; ++qb) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(&sL[buf][r0 + 16 * qb + 4 * g]);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(&sDl[buf][r0 + 16 * qb + 4 * g]);
+        f32x4 st[KB], dp[KB];
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb)
+        for (int kb = 0; kb < KB; ++kb) {
+          st[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+          dp[kb] = kSub ? f32x4{0.f, 0.f, 0.f, 0.f} : -de;
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const F8 qa = fr.row(Qs, r0 + 16 * qb, ks), da = fr.row(Ds, r0 + 16 * qb, ks);
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            mma(st[kb], qa, kf[kb][ks]);
+            if constexpr (kVL)
+              mma(dp[kb], da, fr.row(Vw, 16 * kb, ks));
+            else
+              mma(dp[kb], da, vf[kb][ks]);
+          }
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float pt = ca_exp2(st[qb][kb][e] * c + nl[qb][e]);
-            const float ds = pt * (kSub ? dp[qb][kb][e] + nd[qb][e] : dp[qb][kb][e]);
+            const float pt = ca_exp2(st[kb][e] * c - ls[e]);
+            const float ds = pt * (kSub ? dp[kb][e] - de[e] : dp[kb][e]);
             pa[kb][4 * qb + e] = from_f<T>(pt);
             sa[kb][4 * qb + e] = from_f<T>(ds);
             if constexpr (TWO) {
@@ -361,10 +387,10 @@ __global__ __launch_bounds__(kCaThreads) void cross_dkv_kernel(CaArgs a) {
               sb[kb][4 * qb + e] = ca_low<T>(ds, sa[kb][4 * qb + e]);
             }
           }
+      }
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        const F8 fq = mk_frag<Tile, T>(Qs, r0, 16 * db, lane);
-        const F8 fd = mk_frag<Tile, T>(Ds, r0, 16 * db, lane);
+        const F8 fq = fr.col(Qs, r0, db), fd = fr.col(Ds, r0, db);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           mma(dv[kb][db], pa[kb], fd);
@@ -376,9 +402,12 @@ __global__ __launch_bounds__(kCaThreads) void cross_dkv_kernel(CaArgs a) {
         }
       }
     }
-    if (s + 1 < s_end) stash(buf ^ 1);
-    ca_wait_all();
+    ca_wait_all();   // the next step's rows landed
     __syncthreads();
+  };
+  for (int s = s_begin; s < s_end; s += 2) {
+    step(s, std::integral_constant<int, 0>());
+    if (s + 1 < s_end) step(s + 1, std::integral_constant<int, 1>());
   }
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
@@ -436,8 +465,15 @@ BwdPlan bwd_plan(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtyp
     if (s > steps / 2) s = steps / 2;
     return s < 1 ? 1 : s > 32 ? 32 : (int)s;
   };
-  const bool half = dtype == MOC_BF16;
-  const int KEYS = half || D == 64 ? 128 : 64, QS = !half ? 32 : D == 64 ? 128 : 64;
+  int KEYS = 0, QS = 0;
+  auto shape = [&](auto s) {
+    KEYS = 64 * decltype(s)::KB;
+    QS = decltype(s)::QS;
+  };
+  if (dtype == MOC_BF16)
+    D == 64 ? shape(DkvShape<bf16, 64>()) : shape(DkvShape<bf16, 128>());
+  else
+    D == 64 ? shape(DkvShape<float, 64>()) : shape(DkvShape<float, 128>());
   p.dq_splits = splits(B * HK * (Lp / kCaRows), (N + kCaKeys - 1) / kCaKeys);
   p.dkv_splits = splits(B * HK * ((N + KEYS - 1) / KEYS), (rows + QS - 1) / QS);
   p.delta = (size_t)B * HK * Lp;

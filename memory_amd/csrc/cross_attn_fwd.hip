@@ -28,8 +28,8 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
   const int nsp = SPLIT ? a.nsplit : 1;
   const int64_t t0 = xcd_tile((int64_t)a.B * a.HK * nsp * nrb);
   if (t0 < 0) return;
-  const int64_t bh = t0 / ((int64_t)nsp * nrb);
-  const int b = (int)(bh / a.HK), hk = (int)(bh % a.HK);
+  int b, hk;
+  ca_pair(a, t0 / ((int64_t)nsp * nrb), b, hk);
   const int sp = SPLIT ? (int)((t0 / nrb) % nsp) : 0;
   const int r0 = (int)(t0 % nrb) * kCaRows;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);

@@ -210,8 +210,7 @@ __global__ __launch_bounds__(64 * kKdWaves) void kv_decode_kernel(KdArgs p) {
       if (d0 == 0) a.part_lse[at] = den == 0.f ? -INFINITY : Mr + log2f(den);
     } else if (rr < a.rows) {
       T* op = (T*)a.out + (((size_t)b * a.L + rr / a.G) * a.H + hk * a.G + rr % a.G) * D + d0;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) op[x] = from_f<T>(acc[x] * inv);
+      ca_store4<T>(op, nullptr, acc * inv);
     }
   }
 }
