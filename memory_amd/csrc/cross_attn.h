@@ -33,6 +33,23 @@ __device__ __forceinline__ void ca_wait_all() { asm volatile("s_waitcnt vmcnt(0)
 __device__ __forceinline__ float ca_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float ca_max3(float a, float b, float c) { return fmax_fast(fmax_fast(a, b), c); }
 
+// Four zeros that the compiler takes for unknown: products that start from them read these registers instead of having
+// their own cleared first (a tenth of the forward's vector instructions).
+__device__ __forceinline__ f32x4 ca_zeros() {
+  f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
+  asm volatile("" : "+v"(z));
+  return z;
+}
+// a b + c as a new accumulator
+__device__ __forceinline__ f32x4 ca_mma(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 ca_mma(const f32x8& a, const f32x8& b, const f32x4& c) {
+  f32x4 x = c;
+  mma(x, a, b);
+  return x;
+}
+
 // s c - off; EXACT rounds the product by itself, so that a row's largest logit has exactly 2^0
 template <bool EXACT>
 __device__ __forceinline__ float ca_logit(float s, float c, float off) {
@@ -158,18 +175,11 @@ __device__ __forceinline__ int ca_keys_end(const CaArgs& a, int b) {
   return n < 0 ? 0 : n < a.N ? n : a.N;
 }
 
-// Scores of keys that do not count are set to `to`; lane (g, c16) holds keys 16 kb + 4 g + e.
-template <int QB>
-__device__ __forceinline__ void ca_mask(f32x4 (&st)[4][QB], uint64_t word, int g, float to) {
-  const uint32_t w[2] = {(uint32_t)word >> (4 * g), (uint32_t)(word >> 32) >> (4 * g)};
-#pragma unroll
-  for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool live = (w[kb >> 1] >> (16 * (kb & 1) + e)) & 1;
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) st[kb][qb][e] = live ? st[kb][qb][e] : to;
-    }
+// What a tile's logits start from: 0, or -inf for keys that do not count (whose rows of K are fetched as zeros), as the
+// first operand of their product.  Written with the tile by one wave; lane (g, c16) reads keys 16 kb + 4 g + e.  (Setting
+// the logits afterwards took two vector instructions for each of them.)
+__device__ __forceinline__ void ca_bias_put(float* bias, uint64_t word, int lane) {
+  bias[lane] = (word >> lane) & 1 ? 0.f : -INFINITY;
 }
 
 // Stores 4 consecutive results, and with `low` what their rounding left over

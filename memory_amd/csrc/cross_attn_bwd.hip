@@ -16,13 +16,13 @@ namespace moc {
 template <typename T, int D, bool SPLIT, bool TWO>
 __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
   typedef typename Frag<T>::type F8;
-  using Tile = SwzTile<T, D>;
   using Stage = CaStage<T, D, kCaKeys, 4>;
   constexpr int KS = D / 32, DB = D / 16, TB = kCaKeys * D * (int)sizeof(T);
   // dP - delta: from -delta as the product's start, which saves a subtraction, or, where exact, from the whole dP
   constexpr bool kSub = TWO || sizeof(T) == 4;
   __shared__ __attribute__((aligned(16))) char sK[2][TB];
   __shared__ __attribute__((aligned(16))) char sV[2][TB];
+  __shared__ __attribute__((aligned(16))) float sB[2][kCaKeys];
   const int nrb = a.Lp / kCaRows;
   const int nsp = SPLIT ? a.nsplit : 1;
   const int64_t t0 = xcd_tile((int64_t)a.B * a.HK * nsp * nrb);
@@ -84,6 +84,7 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
     const int left = keys.n - kCaKeys * t, rows = left < kCaKeys ? left : kCaKeys;
     const Buf kb = ca_buf(kbase + (int64_t)kCaKeys * t * a.kn, (uint32_t)(((rows - 1) * a.kn + D) * sizeof(T)));
     const Buf vb = ca_buf(vbase + (int64_t)kCaKeys * t * a.vn, (uint32_t)(((rows - 1) * a.vn + D) * sizeof(T)));
+    if (wave == 0) ca_bias_put(sB[buf], word, lane);
     const uint32_t live = (uint32_t)(word >> (16 * wave));
 #pragma unroll
     for (int i = 0; i < Stage::IPW; ++i) {
@@ -95,15 +96,18 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
       ca_dma16(vb.r, vo, sV[buf] + (TB / 4) * wave + 1024 * i);
     }
   };
+  const f32x4 dinit[2] = {f32x4{-dl[0], -dl[0], -dl[0], -dl[0]}, f32x4{-dl[1], -dl[1], -dl[1], -dl[1]}};
   const float c = a.scale_log2;
   int t = t_begin;
   uint64_t word = 0;
   while (t < t_end && !(word = keys.word(t))) ++t;
-  int buf = 0;
   if (t < t_end) fetch(t, word, 0);
   vm_wait_all();
   __syncthreads();
-  while (t < t_end) {
+  const CaFrag<T, D> fr(lane);
+  const f32x4 zeros = ca_zeros();
+  auto step = [&](auto which) {
+    constexpr int buf = decltype(which)::value;
     int tn = t + 1;
     uint64_t wn = 0;
     while (tn < t_end && !(wn = keys.word(tn))) ++tn;
@@ -114,42 +118,32 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
     for (int kh = 0; kh < 2; ++kh) {
       f32x4 st[2][2], dp[2][2];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int qb = 0; qb < 2; ++qb) {
-          st[kb][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
-          const float d0 = kSub ? 0.f : -dl[qb];
-          dp[kb][qb] = f32x4{d0, d0, d0, d0};
-        }
-#pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          const F8 ak = Tile::frag(Ks, 32 * kh + 16 * kb + c16, 32 * ks + 8 * g);
-          const F8 av = Tile::frag(Vs, 32 * kh + 16 * kb + c16, 32 * ks + 8 * g);
+          const F8 ak = fr.row(Ks, 32 * kh + 16 * kb, ks);
+          const F8 av = fr.row(Vs, 32 * kh + 16 * kb, ks);
+          const f32x4 from = *reinterpret_cast<const f32x4*>(&sB[buf][32 * kh + 16 * kb + 4 * g]);
 #pragma unroll
           for (int qb = 0; qb < 2; ++qb) {
-            mma(st[kb][qb], ak, qf[qb][ks]);
-            mma(dp[kb][qb], av, dof[qb][ks]);
+            st[kb][qb] = ca_mma(ak, qf[qb][ks], ks == 0 ? from : st[kb][qb]);
+            dp[kb][qb] = ca_mma(av, dof[qb][ks], ks != 0 ? dp[kb][qb] : kSub ? zeros : dinit[qb]);
           }
         }
       F8 dsf[2], dsl[2];
-      // (keys that do not count: P would be 2^-lse, which may be inf, of their zeroed logits)
-      const uint32_t live = (uint32_t)(word >> (32 * kh)) >> (4 * g);
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float ds = ca_exp2(st[kb][qb][e] * c - lse[qb]) * (kSub ? dp[kb][qb][e] - dl[qb] : dp[kb][qb][e]);
-            if (word != ~0ull) ds = (live >> (16 * kb + e)) & 1 ? ds : 0.f;
+            const float ds = ca_exp2(st[kb][qb][e] * c - lse[qb]) * (kSub ? dp[kb][qb][e] - dl[qb] : dp[kb][qb][e]);
             dsf[qb][4 * kb + e] = from_f<T>(ds);
             if constexpr (TWO) dsl[qb][4 * kb + e] = ca_low<T>(ds, dsf[qb][4 * kb + e]);
           }
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        const F8 f = mk_frag<Tile, T>(Ks, 32 * kh, 16 * db, lane);
+        const F8 f = fr.col(Ks, 32 * kh, db);
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
           mma(acc[qb][db], dsf[qb], f);
@@ -160,8 +154,11 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
     if (tn < t_end) ca_wait_all();
     t = tn;
     word = wn;
-    buf ^= 1;
     __syncthreads();
+  };
+  while (t < t_end) {
+    step(std::integral_constant<int, 0>());
+    if (t < t_end) step(std::integral_constant<int, 1>());
   }
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb)
@@ -212,7 +209,6 @@ template <> struct DkvShape<float, 128> { static constexpr int KB = 1, QS = 32, 
 template <typename T, int D, bool SPLIT, bool TWO>
 __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv_kernel(CaArgs a) {
   typedef typename Frag<T>::type F8;
-  using Tile = SwzTile<T, D>;
   constexpr int KB = DkvShape<T, D>::KB, QS = DkvShape<T, D>::QS, KEYS = 64 * KB;
   using Stage = CaStage<T, D, QS, 4>;
   constexpr int KS = D / 32, DB = D / 16, TB = QS * D * (int)sizeof(T);
@@ -337,6 +333,7 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
   };
   const float c = a.scale_log2;
   const CaFrag<T, D> fr(lane);
+  const f32x4 zeros = ca_zeros();
   const char* Vw = sV + 16 * KB * wave * D * (int)sizeof(T);
   if (s_begin < s_end) fetch(s_begin, 0);
   ca_wait_all();
@@ -357,21 +354,18 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
         const f32x4 ls = *reinterpret_cast<const f32x4*>(&sL[buf][r0 + 16 * qb + 4 * g]);
         const f32x4 de = *reinterpret_cast<const f32x4*>(&sDl[buf][r0 + 16 * qb + 4 * g]);
         f32x4 st[KB], dp[KB];
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          st[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-          dp[kb] = kSub ? f32x4{0.f, 0.f, 0.f, 0.f} : -de;
-        }
+        const f32x4 nd = -de;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           const F8 qa = fr.row(Qs, r0 + 16 * qb, ks), da = fr.row(Ds, r0 + 16 * qb, ks);
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) {
-            mma(st[kb], qa, kf[kb][ks]);
+            st[kb] = ca_mma(qa, kf[kb][ks], ks == 0 ? zeros : st[kb]);
+            const f32x4 d0 = ks != 0 ? dp[kb] : kSub ? zeros : nd;
             if constexpr (kVL)
-              mma(dp[kb], da, fr.row(Vw, 16 * kb, ks));
+              dp[kb] = ca_mma(da, fr.row(Vw, 16 * kb, ks), d0);
             else
-              mma(dp[kb], da, vf[kb][ks]);
+              dp[kb] = ca_mma(da, vf[kb][ks], d0);
           }
         }
 #pragma unroll

@@ -17,11 +17,11 @@ constexpr float kCaSlack = 8.f;
 template <typename T, int D, bool SPLIT, bool TWO>
 __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
   typedef typename Frag<T>::type F8;
-  using Tile = SwzTile<T, D>;
   using Stage = CaStage<T, D, kCaKeys, 4>;
   constexpr int KS = D / 32, DB = D / 16, TB = kCaKeys * D * (int)sizeof(T);
   __shared__ __attribute__((aligned(16))) char sK[2][TB];
   __shared__ __attribute__((aligned(16))) char sV[2][TB];
+  __shared__ __attribute__((aligned(16))) float sB[2][kCaKeys];
 
   // (sequence, kv head) major, row block minor: blocks that read the same keys share an XCD's L2
   const int nrb = a.Lp / kCaRows;
@@ -56,6 +56,7 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
     const int left = keys.n - kCaKeys * t, rows = left < kCaKeys ? left : kCaKeys;
     const Buf kb = ca_buf(kbase + (int64_t)kCaKeys * t * a.kn, (uint32_t)(((rows - 1) * a.kn + D) * sizeof(T)));
     const Buf vb = ca_buf(vbase + (int64_t)kCaKeys * t * a.vn, (uint32_t)(((rows - 1) * a.vn + D) * sizeof(T)));
+    if (wave == 0) ca_bias_put(sB[buf], word, lane);
     const uint32_t live = (uint32_t)(word >> (16 * wave));
 #pragma unroll
     for (int i = 0; i < Stage::IPW; ++i) {
@@ -82,11 +83,13 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
   int t = t_begin;
   uint64_t word = 0;
   while (t < t_end && !(word = keys.word(t))) ++t;
-  int buf = 0;
   if (t < t_end) fetch(t, word, 0);
   vm_wait_all();
   __syncthreads();
-  while (t < t_end) {
+  const CaFrag<T, D> fr(lane);
+  const f32x4 zeros = ca_zeros();
+  auto step = [&](auto which) {
+    constexpr int buf = decltype(which)::value;
     int tn = t + 1;
     uint64_t wn = 0;
     while (tn < t_end && !(wn = keys.word(tn))) ++tn;
@@ -96,18 +99,14 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
     const char* Vs = sV[buf];
     f32x4 st[4][2];
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-      for (int qb = 0; qb < 2; ++qb) st[kb][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) {
-        const F8 f = Tile::frag(Ks, 16 * kb + c16, 32 * ks + 8 * g);
+        const F8 f = fr.row(Ks, 16 * kb, ks);
+        const f32x4 from = *reinterpret_cast<const f32x4*>(&sB[buf][16 * kb + 4 * g]);
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb) mma(st[kb][qb], f, qf[qb][ks]);
+        for (int qb = 0; qb < 2; ++qb) st[kb][qb] = ca_mma(f, qf[qb][ks], ks == 0 ? from : st[kb][qb]);
       }
-    if (word != ~0ull) ca_mask(st, word, g, -INFINITY);
     float cm[2];
     bool grow = false;
 #pragma unroll
@@ -149,10 +148,9 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
     f32x4 ls[2];
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
-      ls[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        mma(ls[qb], ones, pf[qb][h]);
+        ls[qb] = ca_mma(ones, pf[qb][h], h == 0 ? zeros : ls[qb]);
         if constexpr (TWO) mma(ls[qb], ones, pl[qb][h]);
       }
     }
@@ -160,7 +158,7 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        const F8 f = mk_frag<Tile, T>(Vs, 32 * h, 16 * db, lane);
+        const F8 f = fr.col(Vs, 32 * h, db);
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
           mma(o[db][qb], f, pf[qb][h]);
@@ -172,8 +170,11 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
     if (tn < t_end) ca_wait_all();
     t = tn;
     word = wn;
-    buf ^= 1;
     __syncthreads();
+  };
+  while (t < t_end) {
+    step(std::integral_constant<int, 0>());
+    if (t < t_end) step(std::integral_constant<int, 1>());
   }
 
   // rows without live keys: 0, and +inf as the backward's log-sum-exp (its probabilities are 0 then), as in the
