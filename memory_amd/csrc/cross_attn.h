@@ -154,7 +154,7 @@ constexpr int kCaFew = 128;
 struct CaArgs {
   const void *q, *k, *v, *dout;
   void *out, *out_low, *dq, *dk, *dv;
-  float *lse, *delta, *part, *part_lse;
+  float *lse, *ndelta, *part, *part_lse;
   const int32_t* lengths;
   const uint64_t* words;
   int64_t qb, ql, qh, kb, kn, kh, vb, vn, vh, db, dl, dh;   // element strides

@@ -4,7 +4,7 @@
 // delta takes the result before its rounding (out + out_low): where few keys share a row's weight, dO . v_j and delta
 // nearly cancel, and out's 2^-9 alone made dq and dk twice as inexact as everything else.
 // i over the rows (all queries of the G heads) of j's kv head.  dq runs over the keys of a block of rows and leaves
-// delta behind; dk and dv run over the rows of a block of keys, so nothing is summed by atomics and every result has
+// -delta behind; dk and dv run over the rows of a block of keys, so nothing is summed by atomics and every result has
 // one order.  P and dS enter their products rounded to the operands' type; sums, P itself and delta are f32.
 #include "cross_attn.h"
 
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
     const size_t at = ((size_t)b * a.HK + hk) * a.Lp + r;
     dl[qb] = del;
     lse[qb] = ok ? a.lse[at] : INFINITY;
-    if (g == 0 && sp == 0) a.delta[at] = dl[qb];
+    if (g == 0 && sp == 0) a.ndelta[at] = -dl[qb];
   }
   f32x4 acc[2][DB];
 #pragma unroll
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
   const int s_begin = SPLIT ? (int)((int64_t)nstep * sp / nsp) : 0;
   const int s_end = any == 0 ? s_begin : SPLIT ? (int)((int64_t)nstep * (sp + 1) / nsp) : nstep;
   const float* lse = a.lse + bh * a.Lp;
-  const float* delta = a.delta + bh * a.Lp;
+  const float* ndelta = a.ndelta + bh * a.Lp;
   // Rows of step s: row QS s + r is query l0 + (q0 + r) / G, head (q0 + r) % G of the group, with r = lr G + hr a
   // constant of the lane; so its offset from query l0 is that of (lr, hr), q0 heads on, and a query on where q0 + hr
   // passes G.  (The buffers' bases are 64-bit, a step spans at most QS queries.)
@@ -320,11 +320,11 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
       q0 -= a.G;
       ++l0;
     }
-    // lse and delta of the rows, padded to Lp, a multiple of QS, with +inf and 0
+    // lse and -delta of the rows, padded to Lp, a multiple of QS, with +inf and 0
     if (64 * wave < QS) {
       const bool in = 64 * wave + lane < QS;
       const uint32_t o = in ? 4u * (64 * wave + lane) : kCaOut;
-      const Buf lb = ca_buf(lse + r0, 4 * QS), eb = ca_buf(delta + r0, 4 * QS);
+      const Buf lb = ca_buf(lse + r0, 4 * QS), eb = ca_buf(ndelta + r0, 4 * QS);
       if (in) {
         ca_dma4(lb.r, o, &sL[buf][64 * wave]);
         ca_dma4(eb.r, o, &sDl[buf][64 * wave]);
@@ -352,9 +352,8 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
         const f32x4 ls = *reinterpret_cast<const f32x4*>(&sL[buf][r0 + 16 * qb + 4 * g]);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(&sDl[buf][r0 + 16 * qb + 4 * g]);
+        const f32x4 nd = *reinterpret_cast<const f32x4*>(&sDl[buf][r0 + 16 * qb + 4 * g]);
         f32x4 st[KB], dp[KB];
-        const f32x4 nd = -de;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           const F8 qa = fr.row(Qs, r0 + 16 * qb, ks), da = fr.row(Ds, r0 + 16 * qb, ks);
@@ -373,7 +372,7 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float pt = ca_exp2(st[kb][e] * c - ls[e]);
-            const float ds = pt * (kSub ? dp[kb][e] - de[e] : dp[kb][e]);
+            const float ds = pt * (kSub ? dp[kb][e] + nd[e] : dp[kb][e]);
             pa[kb][4 * qb + e] = from_f<T>(pt);
             sa[kb][4 * qb + e] = from_f<T>(ds);
             if constexpr (TWO) {
@@ -541,8 +540,8 @@ int moc_cross_bwd(const moc_cross_args* args, void* workspace, size_t workspace_
   const BwdPlan p = bwd_plan(args->B, args->L, args->N, args->H, args->HK, args->D, args->dtype);
   MOC_REQUIRE(workspace && workspace_bytes >= p.bytes(), MOC_ERR_ARG, "%s: workspace of %zu bytes, needs %zu", who,
               workspace_bytes, p.bytes());
-  a.delta = (float*)workspace;
-  a.part = a.delta + p.delta;
+  a.ndelta = (float*)workspace;
+  a.part = a.ndelta + p.delta;
   if (args->dtype == MOC_BF16)
     return args->D == 64 ? bwd_launch<bf16, 64>(a, p, stream) : bwd_launch<bf16, 128>(a, p, stream);
   return args->D == 64 ? bwd_launch<float, 64>(a, p, stream) : bwd_launch<float, 128>(a, p, stream);

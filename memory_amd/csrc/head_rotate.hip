@@ -331,9 +331,9 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_bwd_kernel(HrArgs a, i
   }
 }
 
-// dw of each set: sums over the slices, in their order: 16 columns per workgroup, 16 threads each
-__global__ __launch_bounds__(256) void head_rotate_dw_kernel(HrArgs a, int n0, int n1, int n2) {
-  __shared__ float red[16][17];
+// dw of each set: sums over the slices, in their order: 16 columns per workgroup, 64 threads each
+__global__ __launch_bounds__(1024) void head_rotate_dw_kernel(HrArgs a, int n0, int n1, int n2) {
+  __shared__ float red[64][17];
   int blk = blockIdx.x, si = 0, cols = 0;
   for (; si < a.nseg; ++si) {
     const moc_head_rows& r = a.seg[si].r;
@@ -346,13 +346,16 @@ __global__ __launch_bounds__(256) void head_rotate_dw_kernel(HrArgs a, int n0, i
   const int n = si == 0 ? n0 : si == 1 ? n1 : n2;
   const int c = 16 * blk + (threadIdx.x & 15), q = threadIdx.x >> 4;
   float sum = 0.f;
-  if (c < cols)
-    for (int i = q; i < n; i += 16) sum += s.part[(int64_t)i * cols + c];
+  if (c < cols) {
+#pragma unroll 8
+    for (int i = q; i < n; i += 64) sum += s.part[(int64_t)i * cols + c];
+  }
   red[q][threadIdx.x & 15] = sum;
   __syncthreads();
   if (q == 0 && c < cols) {
     float t = 0.f;
-    for (int i = 0; i < 16; ++i) t += red[i][threadIdx.x & 15];
+#pragma unroll
+    for (int i = 0; i < 64; ++i) t += red[i][threadIdx.x & 15];
     s.r.dw[c] = t;
   }
 }
@@ -488,7 +491,7 @@ int moc_head_rotate_bwd(const moc_head_args* args, void* workspace, size_t works
     head_rotate_bwd_kernel<float><<<grid, kHrThreads, 0, stream>>>(a, wgs[0], wgs[1], wgs[2]);
   rc = check_launch("moc_head_rotate_bwd");
   if (rc != MOC_OK || cols == 0) return rc;
-  head_rotate_dw_kernel<<<cols, 256, 0, stream>>>(a, slices[0], slices[1], slices[2]);
+  head_rotate_dw_kernel<<<cols, 1024, 0, stream>>>(a, slices[0], slices[1], slices[2]);
   return check_launch("moc_head_rotate_bwd: weights");
 }
 
