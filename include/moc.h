@@ -857,7 +857,7 @@ typedef struct {
   float scale; /* > 0 */
 } moc_cross_args;
 int64_t moc_cross_rows(int64_t L, int H, int HK);
-size_t moc_cross_fwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D);
+size_t moc_cross_fwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtype);
 int moc_cross_fwd(const moc_cross_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream);
 /* Gradients of the forward whose out and lse these are: dq (or NULL), dk and dv (both or neither NULL). */
 size_t moc_cross_bwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtype);
@@ -880,7 +880,7 @@ typedef struct {
   int H, HK, D, dtype, page, causal;
   float scale;
 } moc_kv_decode_args;
-size_t moc_kv_decode_workspace(int64_t B, int64_t L, int64_t n_max, int H, int HK, int D);
+size_t moc_kv_decode_workspace(int64_t B, int64_t L, int64_t n_max, int H, int HK, int D, int dtype);
 int moc_kv_decode(const moc_kv_decode_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* ---------------------------- norms of heads with the rotation by position */

@@ -166,12 +166,12 @@ _SIGS = {
     "moc_router_select_bwd": (_I, [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I, _I, _I, _I, _F, _P, _P]),
     "moc_router_balance": (_I, [_P, _I64, _I64, _I, _F, _P, _P, _P]),
     "moc_cross_rows": (_I64, [_I64, _I, _I]),
-    "moc_cross_fwd_workspace": (_SZ, [_I64, _I64, _I64, _I, _I, _I]),
+    "moc_cross_fwd_workspace": (_SZ, [_I64, _I64, _I64, _I, _I, _I, _I]),
     "moc_cross_fwd": (_I, [_P, _P, _SZ, _P]),
     "moc_cross_bwd_workspace": (_SZ, [_I64, _I64, _I64, _I, _I, _I, _I]),
     "moc_cross_bwd": (_I, [_P, _P, _SZ, _P]),
     "moc_key_words": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _P]),
-    "moc_kv_decode_workspace": (_SZ, [_I64, _I64, _I64, _I, _I, _I]),
+    "moc_kv_decode_workspace": (_SZ, [_I64, _I64, _I64, _I, _I, _I, _I]),
     "moc_kv_decode": (_I, [_P, _P, _SZ, _P]),
     "moc_head_rotate_fwd": (_I, [_P, _P]),
     "moc_head_rotate_bwd_workspace": (_SZ, [_P]),

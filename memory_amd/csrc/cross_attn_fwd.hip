@@ -204,35 +204,49 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
   }
 }
 
-// out = sum_i 2^(lse_i - M) o_i / sum_i 2^(lse_i - M) over the splits of a row, and its log-sum-exp: D / 4 lanes
-// of four dims per row.
+// out = sum_i 2^(lse_i - M) o_i / sum_i 2^(lse_i - M) over the splits of a row, and its log-sum-exp.  A workgroup per
+// row: D / 4 lanes of four dims in each of 1024 / D groups, a group taking every so many splits, joined in LDS (a
+// chain of two loads whatever the number of splits; with all of a row's splits in one lane 32 of them took 7 us).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void cross_merge_kernel(CaArgs a) {
-  constexpr int LPR = D / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / LPR;                 // (b, hk, r)
-  const int ch = (int)(i % LPR);
-  const int64_t nrow = (int64_t)a.B * a.HK * a.Lp;
-  if (row >= nrow) return;
-  const int r = (int)(row % a.Lp);
-  const int64_t bh = row / a.Lp;
-  const int b = (int)(bh / a.HK), hk = (int)(bh % a.HK);
+  constexpr int LPR = D / 4, GR = 256 / LPR;
+  __shared__ float sM[GR], sS[GR];
+  __shared__ __attribute__((aligned(16))) float sO[GR][D];
+  const int64_t row = blockIdx.x, nrow = gridDim.x;         // (b, hk, r)
+  const int ch = threadIdx.x % LPR, gr = threadIdx.x / LPR;
+  const int r = (int)((uint32_t)row % (uint32_t)a.Lp);
+  const uint32_t bh = (uint32_t)row / (uint32_t)a.Lp, b = bh / (uint32_t)a.HK, hk = bh - b * a.HK;
   if (r >= a.rows) {
-    if (a.lse && ch == 0) a.lse[row] = INFINITY;
+    if (a.lse && threadIdx.x == 0) a.lse[row] = INFINITY;
     return;
   }
-  float M = -INFINITY;
-#pragma unroll 8
-  for (int s = 0; s < a.nsplit; ++s) M = fmax_fast(M, a.part_lse[s * nrow + row]);
+  float M = -INFINITY, den = 0.f;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-  float den = 0.f;
-#pragma unroll 8
-  for (int s = 0; s < a.nsplit; ++s) {
-    // (no weight for a split without live keys; a NaN goes through)
+#pragma unroll 4
+  for (int s = gr; s < a.nsplit; s += GR) {
     const float d = a.part_lse[s * nrow + row];
-    const float w = d == -INFINITY ? 0.f : ca_exp2(d - M);
-    acc += *reinterpret_cast<const f32x4*>(a.part + (s * nrow + row) * D + 4 * ch) * w;
-    den += w;
+    const f32x4 o = *reinterpret_cast<const f32x4*>(a.part + (s * nrow + row) * D + 4 * ch);
+    // (no weight for a split without live keys; a NaN goes through)
+    const float m = fmax_fast(M, d);
+    const float w = d == -INFINITY ? 0.f : ca_exp2(d - m), f = M == -INFINITY ? 0.f : ca_exp2(M - m);
+    acc = acc * f + o * w;
+    den = den * f + w;
+    M = m;
+  }
+  if (ch == 0) {
+    sM[gr] = M;
+    sS[gr] = den;
+  }
+  *reinterpret_cast<f32x4*>(&sO[gr][4 * ch]) = acc;
+  __syncthreads();
+  if (gr != 0) return;
+  const int used = a.nsplit < GR ? a.nsplit : GR;
+  for (int q = 1; q < used; ++q) {
+    const float d = sM[q], m = fmax_fast(M, d);
+    const float w = d == -INFINITY ? 0.f : ca_exp2(d - m), f = M == -INFINITY ? 0.f : ca_exp2(M - m);
+    acc = acc * f + *reinterpret_cast<const f32x4*>(&sO[q][4 * ch]) * w;
+    den = den * f + sS[q] * w;
+    M = m;
   }
   const float inv = den == 0.f ? 0.f : 1.f / den;
   const size_t at = (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + 4 * ch;
@@ -256,11 +270,13 @@ __global__ __launch_bounds__(256) void key_words_kernel(const uint8_t* __restric
 // Workgroups of the forward from which on splitting the keys no longer pays (two to three per CU).
 constexpr int64_t kCaWgs = 512;
 
-// Splits of the keys: enough workgroups to fill the card, each with at least four tiles.
-int ca_fwd_splits(int64_t wgs, int64_t nt) {
+// Splits of the keys: enough workgroups to fill the card, each with a few tiles (float32: one; a tile costs a workgroup
+// on its own about 5 us there and 1.2 in bf16, the join 4).
+int ca_fwd_splits(int64_t wgs, int64_t nt, int dtype) {
   if (wgs >= kCaWgs / 2) return 1;
   int64_t s = kCaWgs / (wgs < 1 ? 1 : wgs);
-  if (s > nt / 4) s = nt / 4;
+  const int64_t most = dtype == MOC_F32 ? nt : nt / 4;
+  if (s > most) s = most;
   return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 
@@ -320,9 +336,9 @@ static int fwd_launch(CaArgs& a, hipStream_t stream) {
 }
 
 int ca_merge(int dtype, int D, const CaArgs& a, hipStream_t stream) {
-  const int64_t lanes = (int64_t)a.B * a.HK * a.Lp * (D / 4);
-  MOC_REQUIRE(lanes < (int64_t)1 << 39, MOC_ERR_UNSUPPORTED, "attention merge: too many rows");
-  const unsigned grid = (unsigned)((lanes + 255) / 256);
+  const int64_t rows = (int64_t)a.B * a.HK * a.Lp;
+  MOC_REQUIRE(rows < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "attention merge: too many rows");
+  const unsigned grid = (unsigned)rows;
   if (dtype == MOC_BF16)
     D == 64 ? cross_merge_kernel<bf16, 64><<<grid, 256, 0, stream>>>(a)
             : cross_merge_kernel<bf16, 128><<<grid, 256, 0, stream>>>(a);
@@ -343,9 +359,9 @@ int64_t moc_cross_rows(int64_t L, int H, int HK) {
   return (L * (H / HK) + kCaRows - 1) / kCaRows * kCaRows;
 }
 
-size_t moc_cross_fwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D) {
+size_t moc_cross_fwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtype) {
   const int64_t Lp = moc_cross_rows(L, H, HK);
-  const int s = ca_fwd_splits(B * HK * (Lp / kCaRows), (N + kCaKeys - 1) / kCaKeys);
+  const int s = ca_fwd_splits(B * HK * (Lp / kCaRows), (N + kCaKeys - 1) / kCaKeys, dtype);
   return s == 1 ? 0 : (size_t)s * B * HK * Lp * (D + 1) * 4;
 }
 
@@ -355,8 +371,8 @@ int moc_cross_fwd(const moc_cross_args* args, void* workspace, size_t workspace_
   if (rc != MOC_OK) return rc;
   MOC_REQUIRE(a.q && a.k && a.v && a.out, MOC_ERR_ARG, "moc_cross_fwd: null tensor");
   const int64_t bhl = (int64_t)a.B * a.HK * a.Lp;
-  a.nsplit = ca_fwd_splits((int64_t)a.B * a.HK * (a.Lp / kCaRows), a.nt);
-  const size_t need = moc_cross_fwd_workspace(args->B, args->L, args->N, args->H, args->HK, args->D);
+  a.nsplit = ca_fwd_splits((int64_t)a.B * a.HK * (a.Lp / kCaRows), a.nt, args->dtype);
+  const size_t need = moc_cross_fwd_workspace(args->B, args->L, args->N, args->H, args->HK, args->D, args->dtype);
   MOC_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), MOC_ERR_ARG, "moc_cross_fwd: workspace of %zu bytes, needs %zu",
               workspace_bytes, need);
   a.part = (float*)workspace;

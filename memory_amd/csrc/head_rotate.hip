@@ -19,12 +19,12 @@ struct HrSeg {
   int64_t tokens;          // B * L
   int first;               // first workgroup of the set
   float* part;             // backward: [workgroups][columns] of dw, columns D or H * D
-  int vec;                 // rows in 16-byte pieces
 };
 struct HrArgs {
   HrSeg seg[3];
   const double* inv_freq;
-  int nseg, D, R, R2, interleaved, lph, toks, groups;   // R2 = pairs, lph: lanes per head, toks: tokens per step
+  int nseg, D, R, R2, interleaved, lph, toks, vec;   // R2: pairs, lph: lanes per head, toks: tokens per step,
+                                                         // vec: all rows in 16-byte pieces
   float eps;
 };
 
@@ -42,9 +42,9 @@ __device__ __forceinline__ float hr_sum(float v, int lph) {
 }
 
 // The lane's elements: a = first eight (or even places), b = the others, as a row's two runs of eight
-template <typename T>
-__device__ __forceinline__ void hr_load(const T* p, int e0, int e1, int D, bool vec, float (&x)[16]) {
-  if (vec) {
+template <typename T, bool VEC>
+__device__ __forceinline__ void hr_load(const T* p, int e0, int e1, int D, float (&x)[16]) {
+  if constexpr (VEC) {
     ChunkLoadF<T>::run(p + e0, x);
     ChunkLoadF<T>::run(p + e1, x + 8);
   } else {
@@ -100,9 +100,9 @@ __device__ __forceinline__ void hr_pair(const HrArgs& a, int p, int& e0, int& e1
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void hr_read(const HrArgs& a, const HrLane& l, const T* p, bool vec, float (&x)[16]) {
-  if (l.mixed) {
+template <typename T, bool VEC>
+__device__ __forceinline__ void hr_read(const HrArgs& a, const HrLane& l, const T* p, float (&x)[16]) {
+  if (!VEC && l.mixed) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       int e0, e1;
@@ -111,12 +111,12 @@ __device__ __forceinline__ void hr_read(const HrArgs& a, const HrLane& l, const 
       x[8 + i] = e1 < a.D ? to_f(p[e1]) : 0.f;
     }
   } else {
-    hr_load<T>(p, l.e0, l.e1, a.D, vec, x);
+    hr_load<T, VEC>(p, l.e0, l.e1, a.D, x);
   }
 }
-template <typename T>
-__device__ __forceinline__ void hr_write(const HrArgs& a, const HrLane& l, T* p, bool vec, const float (&y)[16]) {
-  if (l.mixed) {
+template <typename T, bool VEC>
+__device__ __forceinline__ void hr_write(const HrArgs& a, const HrLane& l, T* p, const float (&y)[16]) {
+  if (!VEC && l.mixed) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       int e0, e1;
@@ -124,7 +124,7 @@ __device__ __forceinline__ void hr_write(const HrArgs& a, const HrLane& l, T* p,
       if (e0 < a.D) p[e0] = from_f<T>(y[i]);
       if (e1 < a.D) p[e1] = from_f<T>(y[8 + i]);
     }
-  } else if (vec) {
+  } else if constexpr (VEC) {
     HrStore<T>::run(p + l.e0, y);
     HrStore<T>::run(p + l.e1, y + 8);
   } else {
@@ -137,11 +137,12 @@ __device__ __forceinline__ void hr_write(const HrArgs& a, const HrLane& l, T* p,
 }
 
 // Turns the lane's pairs by +-angle (dir): pairs lie (i, 8 + i) in halves and mixed lanes, (2 i, 2 i + 1) interleaved.
+template <bool VEC>
 __device__ __forceinline__ void hr_turn(const HrArgs& a, const HrLane& l, const float2* cs, float dir, float (&x)[16]) {
   if (!l.turns) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const bool in = l.p0 + i < a.R2;
+    const bool in = VEC || l.p0 + i < a.R2;     // (with 16-byte pieces eight pairs turn together or not at all)
     const float2 t = in ? cs[l.p0 + i] : float2{1.f, 0.f};
     const float s = t.y * dir;
     if (a.interleaved) {
@@ -182,9 +183,9 @@ __device__ __forceinline__ int hr_segment(const HrArgs& a) {
   return s;
 }
 
-template <typename T>
+template <typename T, bool VEC>
 __global__ __launch_bounds__(kHrThreads) void head_rotate_fwd_kernel(HrArgs a) {
-  __shared__ float2 cs[kHrAngles];
+  extern __shared__ float2 cs[];
   const int si = hr_segment(a);
   const HrSeg& s = a.seg[si];
   const moc_head_rows& r = s.r;
@@ -194,32 +195,43 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_fwd_kernel(HrArgs a) {
   const int j = lane % a.lph, sub = lane / a.lph, hpw = 64 / a.lph;
   const HrLane ln = hr_lane(a, j);
   const bool lane_on = 16 * j < a.D;
+  const int rows = n * r.H;
+  auto read = [&](int row, float (&x)[16]) {
+    const uint32_t tk = (uint32_t)row / (uint32_t)r.H, h = row - tk * r.H;
+    const uint32_t t = (uint32_t)t0 + tk, b = t / (uint32_t)r.L, l = t - b * (uint32_t)r.L;
+    hr_read<T, VEC>(a, ln, (const T*)r.x + b * r.xb + l * r.xl + h * r.xh, x);
+  };
+  // (a row is requested before the angles are worked out, and then a row ahead of the one in hand)
+  float next[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) next[i] = 0.f;
+  int row = wave * hpw + sub;
+  if (lane_on && row < rows) read(row, next);
+  float w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = 1.f;
+  if (r.w && !r.w_head && lane_on) hr_read<float, VEC>(a, ln, r.w, w);
   if (r.rotate) {
     hr_angles(a, s, t0, n, cs);
     __syncthreads();
   }
-  float w[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = 1.f;
-  if (r.w && !r.w_head && lane_on) hr_read<float>(a, ln, r.w, s.vec, w);
-  const int rows = n * r.H;
-  for (int row = wave * hpw + sub; row < rows; row += 4 * hpw) {
-    const int tk = row / r.H, h = row % r.H;
-    const int64_t t = t0 + tk, b = t / r.L, l = t % r.L;
+  for (; row < rows; row += 4 * hpw) {
     float x[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = 0.f;
-    if (lane_on) hr_read<T>(a, ln, (const T*)r.x + b * r.xb + l * r.xl + h * r.xh, s.vec, x);
+    for (int i = 0; i < 16; ++i) x[i] = next[i];
+    if (lane_on && row + 4 * hpw < rows) read(row + 4 * hpw, next);
+    const uint32_t tk = (uint32_t)row / (uint32_t)r.H, h = row - tk * r.H;
+    const uint32_t t = (uint32_t)t0 + tk, b = t / (uint32_t)r.L, l = t - b * (uint32_t)r.L;
     if (r.norm) {
       float sq = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) sq += x[i] * x[i];
       const float rstd = 1.f / sqrtf(hr_sum(sq, a.lph) / (float)a.D + a.eps);
-      if (r.w_head && lane_on) hr_read<float>(a, ln, r.w + (int64_t)h * a.D, s.vec, w);
+      if (r.w_head && lane_on) hr_read<float, VEC>(a, ln, r.w + (int64_t)h * a.D, w);
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = x[i] * rstd * w[i];
     }
-    if (r.rotate) hr_turn(a, ln, cs + tk * a.R2, 1.f, x);
+    if (r.rotate) hr_turn<VEC>(a, ln, cs + tk * a.R2, 1.f, x);
     int64_t at = b * r.yb + l * r.yl;
     if (r.table) {
       const int64_t p = hr_position(r, b, l), pg = p < 0 ? r.max_pages : p / r.page;
@@ -227,16 +239,16 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_fwd_kernel(HrArgs a) {
       if (id < 0 || id >= r.num_pages) continue;     // (the whole head's lanes)
       at = id * r.yb + (p % r.page) * r.yl;
     }
-    if (lane_on) hr_write<T>(a, ln, (T*)r.y + at + h * r.yh, s.vec, x);
+    if (lane_on) hr_write<T, VEC>(a, ln, (T*)r.y + at + h * r.yh, x);
   }
 }
 
 // Backward: a workgroup goes over its share of the tokens, `toks` at a time, for one group of heads (those of a wave's
 // lanes, so that a lane's sums for dw belong to one head); its sums of dw go to its row of `part`.
-template <typename T>
+template <typename T, bool VEC>
 __global__ __launch_bounds__(kHrThreads) void head_rotate_bwd_kernel(HrArgs a, int wgs0, int wgs1, int wgs2) {
-  __shared__ float2 cs[kHrAngles];
-  __shared__ float red[4][64 * 16];
+  extern __shared__ float2 cs[];                      // the angles, and at the end
+  float (*red)[64 * 16] = reinterpret_cast<float (*)[64 * 16]>(cs);   // the waves' sums of dw
   const int si = hr_segment(a);
   const HrSeg& s = a.seg[si];
   const moc_head_rows& r = s.r;
@@ -256,29 +268,48 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_bwd_kernel(HrArgs a, i
     dw[i] = 0.f;
   }
   if (r.w && lane_on && (!r.w_head || h_lane < r.H))
-    hr_read<float>(a, ln, r.w + (r.w_head ? (int64_t)h_lane * a.D : 0), s.vec, w);
+    hr_read<float, VEC>(a, ln, r.w + (r.w_head ? (int64_t)h_lane * a.D : 0), w);
   const int64_t steps = (s.tokens + a.toks - 1) / a.toks;
+  const int per = r.w_head ? hpw : r.H;               // rows of a token that the workgroup takes
   for (int64_t st = slice; st < steps; st += nslice) {
     const int64_t t0 = st * a.toks;
-    const int n = (int)(s.tokens - t0 < a.toks ? s.tokens - t0 : a.toks);
+    const int n = (int)(s.tokens - t0 < a.toks ? s.tokens - t0 : a.toks), rows = n * per;
+    auto at = [&](int row, uint32_t& tk, uint32_t& h, uint32_t& b, uint32_t& l) {
+      tk = (uint32_t)row / (uint32_t)per;
+      h = r.w_head ? (uint32_t)h_lane : row - tk * per;
+      const uint32_t t = (uint32_t)t0 + tk;
+      b = t / (uint32_t)r.L;
+      l = t - b * (uint32_t)r.L;
+    };
+    auto read = [&](int row, float (&g)[16], float (&x)[16]) {
+      uint32_t tk, h, b, l;
+      at(row, tk, h, b, l);
+      if (!lane_on || h >= (uint32_t)r.H) return;
+      hr_read<T, VEC>(a, ln, (const T*)r.dy + b * r.yb + l * r.yl + h * r.yh, g);
+      if (r.norm) hr_read<T, VEC>(a, ln, (const T*)r.x + b * r.xb + l * r.xl + h * r.xh, x);
+    };
+    float gn[16], xn[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) gn[i] = xn[i] = 0.f;
+    int row = wave * hpw + sub;
+    if (row < rows) read(row, gn, xn);
     if (r.rotate) {
       __syncthreads();
       hr_angles(a, s, t0, n, cs);
       __syncthreads();
     }
-    const int per = r.w_head ? hpw : r.H, rows = n * per;
-    for (int row = wave * hpw + sub; row < rows; row += 4 * hpw) {
-      const int tk = row / per, h = r.w_head ? h_lane : row % per;
-      if (h >= r.H) continue;
-      const int64_t t = t0 + tk, b = t / r.L, l = t % r.L;
+    for (; row < rows; row += 4 * hpw) {
       float g[16], x[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) g[i] = x[i] = 0.f;
-      if (lane_on) {
-        hr_read<T>(a, ln, (const T*)r.dy + b * r.yb + l * r.yl + h * r.yh, s.vec, g);
-        if (r.norm) hr_read<T>(a, ln, (const T*)r.x + b * r.xb + l * r.xl + h * r.xh, s.vec, x);
+      for (int i = 0; i < 16; ++i) {
+        g[i] = gn[i];
+        x[i] = xn[i];
       }
-      if (r.rotate) hr_turn(a, ln, cs + tk * a.R2, -1.f, g);
+      if (row + 4 * hpw < rows) read(row + 4 * hpw, gn, xn);
+      uint32_t tk, h, b, l;
+      at(row, tk, h, b, l);
+      if (h >= (uint32_t)r.H) continue;
+      if (r.rotate) hr_turn<VEC>(a, ln, cs + tk * a.R2, -1.f, g);
       if (r.norm) {
         float sq = 0.f;
 #pragma unroll
@@ -296,11 +327,12 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_bwd_kernel(HrArgs a, i
 #pragma unroll
         for (int i = 0; i < 16; ++i) g[i] = rstd * (g[i] - x[i] * mean);
       }
-      if (r.dx && lane_on) hr_write<T>(a, ln, (T*)r.dx + ((t * r.H) + h) * a.D, s.vec, g);
+      if (r.dx && lane_on) hr_write<T, VEC>(a, ln, (T*)r.dx + ((t0 + tk) * r.H + h) * a.D, g);
     }
   }
   if (!s.part) return;
   // this workgroup's sums: over its waves, and over the heads where they share the weight
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < 16; ++i) red[wave][lane * 16 + i] = dw[i];
   __syncthreads();
@@ -373,6 +405,7 @@ static int hr_check(const char* who, const moc_head_args* p, bool bwd, HrArgs* o
   h.inv_freq = a.inv_freq;
   h.nseg = a.nseg; h.D = a.D; h.R = a.R; h.R2 = a.R / 2; h.interleaved = a.interleaved ? 1 : 0; h.eps = a.eps;
   h.lph = 1;
+  h.vec = 1;
   while (16 * h.lph < a.D) h.lph *= 2;
   for (int i = 0; i < a.nseg; ++i) {
     const moc_head_rows& r = a.seg[i];
@@ -393,7 +426,7 @@ static int hr_check(const char* who, const moc_head_args* p, bool bwd, HrArgs* o
     for (int64_t x : st) vec = vec && x * es % 16 == 0;
     const void* ps[] = {r.x, r.y, r.dy, r.dx, r.w};
     for (const void* x : ps) vec = vec && ((uintptr_t)x & 15) == 0;
-    s.vec = vec ? 1 : 0;
+    if (!vec) h.vec = 0;
   }
   return MOC_OK;
 }
@@ -447,10 +480,12 @@ int moc_head_rotate_fwd(const moc_head_args* args, hipStream_t stream) {
   }
   MOC_REQUIRE(grid < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "moc_head_rotate_fwd: too many tokens");
   if (grid == 0) return MOC_OK;
+  const size_t lds = (size_t)a.toks * a.R2 * 8;
+  const dim3 gr((unsigned)grid), bl(kHrThreads);
   if (args->dtype == MOC_BF16)
-    head_rotate_fwd_kernel<bf16><<<(unsigned)grid, kHrThreads, 0, stream>>>(a);
+    a.vec ? head_rotate_fwd_kernel<bf16, true><<<gr, bl, lds, stream>>>(a) : head_rotate_fwd_kernel<bf16, false><<<gr, bl, lds, stream>>>(a);
   else
-    head_rotate_fwd_kernel<float><<<(unsigned)grid, kHrThreads, 0, stream>>>(a);
+    a.vec ? head_rotate_fwd_kernel<float, true><<<gr, bl, lds, stream>>>(a) : head_rotate_fwd_kernel<float, false><<<gr, bl, lds, stream>>>(a);
   return check_launch("moc_head_rotate_fwd");
 }
 
@@ -485,10 +520,14 @@ int moc_head_rotate_bwd(const moc_head_args* args, void* workspace, size_t works
     ws += part[i];
     if (part[i]) cols += ((s.r.w_head ? s.r.H * a.D : a.D) + 15) / 16;
   }
+  size_t lds = (size_t)a.toks * a.R2 * 8;
+  if (cols && lds < 4 * 64 * 16 * 4) lds = 4 * 64 * 16 * 4;
   if (args->dtype == MOC_BF16)
-    head_rotate_bwd_kernel<bf16><<<grid, kHrThreads, 0, stream>>>(a, wgs[0], wgs[1], wgs[2]);
+    a.vec ? head_rotate_bwd_kernel<bf16, true><<<grid, kHrThreads, lds, stream>>>(a, wgs[0], wgs[1], wgs[2])
+          : head_rotate_bwd_kernel<bf16, false><<<grid, kHrThreads, lds, stream>>>(a, wgs[0], wgs[1], wgs[2]);
   else
-    head_rotate_bwd_kernel<float><<<grid, kHrThreads, 0, stream>>>(a, wgs[0], wgs[1], wgs[2]);
+    a.vec ? head_rotate_bwd_kernel<float, true><<<grid, kHrThreads, lds, stream>>>(a, wgs[0], wgs[1], wgs[2])
+          : head_rotate_bwd_kernel<float, false><<<grid, kHrThreads, lds, stream>>>(a, wgs[0], wgs[1], wgs[2]);
   rc = check_launch("moc_head_rotate_bwd");
   if (rc != MOC_OK || cols == 0) return rc;
   head_rotate_dw_kernel<<<cols, 1024, 0, stream>>>(a, slices[0], slices[1], slices[2]);

@@ -502,6 +502,12 @@ class PagedKVCache:
             if t.stride(1) < t.shape[3] or t.stride(1) * es >= 1 << 24:
                 raise ValueError(f"{name}: rows that overlap, or lie 16 MiB or more apart")
         self.k_pages, self.v_pages, self.block_table, self.lengths = k_pages, v_pages, block_table, lengths
+        # what every call hands to the kernels of them, worked out once (a step is two launches: its host time counts)
+        P, page, HK, D = k_pages.shape
+        self._sizes = (P, page, HK, D, block_table.shape[0], block_table.shape[1])
+        self._k_strides, self._v_strides = k_pages.stride()[:3], v_pages.stride()[:3]
+        self._table = (block_table.stride(0), P, block_table.shape[1], page)
+        self._code = L.dtype_code(k_pages.dtype)
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, sequences: int, max_pages: int, *,
@@ -542,7 +548,6 @@ class PagedKVCache:
     def dtype(self) -> torch.dtype:
         return self.k_pages.dtype
 
-    @torch.no_grad()
     def append(self, k: torch.Tensor, v: torch.Tensor, *, positions: Optional[torch.Tensor] = None,
                q: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
                k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, norm: Optional[bool] = None,
@@ -554,18 +559,19 @@ class PagedKVCache:
         Keys may be normed and rotated on the way (``k_weight``, ``norm``, ``inv_freq``, ``interleaved`` as in
         ``ops.qk_norm_rotate``, ``norm`` where a weight is given by default; the position is the token's place), and the
         queries ``q`` of the same tokens with them: returns q so treated.  One launch."""
-        P, page, HK, D = self.k_pages.shape
-        B = self.lengths.shape[0]
-        if k.dim() != 4 or k.shape != v.shape or k.shape[0] != B or tuple(k.shape[2:]) != (HK, D):
+        _, _, HK, D, B, _ = self._sizes
+        shape = k.shape
+        if len(shape) != 4 or shape != v.shape or shape[0] != B or shape[2] != HK or shape[3] != D:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)}: expected ({B}, tokens, {HK}, {D})")
-        T = k.shape[1]
-        if q is not None and (q.dim() != 4 or tuple(q.shape[:2]) != (B, T) or q.shape[3] != D or q.shape[2] == 0):
+        T = shape[1]
+        if q is not None and (q.dim() != 4 or q.shape[0] != B or q.shape[1] != T or q.shape[3] != D or q.shape[2] == 0):
             raise ValueError(f"q {tuple(q.shape)}: expected ({B}, {T}, heads, {D})")
         if positions is not None and (tuple(positions.shape) != (B,) or positions.dtype not in (torch.int32, torch.int64)):
             raise ValueError(f"positions of shape {tuple(positions.shape)} {positions.dtype}, expected ({B},) int32 or int64")
+        weighed = q_weight is not None or k_weight is not None
         if norm is None:
-            norm = q_weight is not None or k_weight is not None
-        if not norm and (q_weight is not None or k_weight is not None):
+            norm = weighed
+        if weighed and not norm:
             raise ValueError("a weight needs norm=True")
         if q is None and q_weight is not None:
             raise ValueError("q_weight without q")
@@ -576,30 +582,24 @@ class PagedKVCache:
         qw = None if q is None else ops._head_weight(q_weight, q.shape[2], D, "q_weight")
         freq = ops._head_frequencies(inv_freq, D)
         place = self.lengths if positions is None else positions
-        pos32 = int(place.dtype == torch.int32)
-
-        def rows(x):
-            x = x if x.dtype == self.dtype else x.to(self.dtype)
-            return x if x.stride(3) == 1 else x.contiguous()
-
-        def fields(x, w, y, strides, normed, turns, paged):
-            # (a page's stride in the batch stride's place)
-            xs = x.stride()
-            tab = (self.block_table.data_ptr(), self.block_table.stride(0), P, self.block_table.shape[1], page) if paged \
-                else (0, 0, 0, 0, 0)
-            return ops._pack_head_rows(x.data_ptr(), L.ptr0(w), y.data_ptr(), 0, 0, 0, place.data_ptr(), tab[0], *xs[:3],
-                                       *strides[:3], place.stride(0), 0, 1, tab[1], B, T, tab[2], tab[3], x.shape[2],
-                                       int(w is not None and w.dim() == 2), int(normed), int(turns), pos32, tab[4])
-
-        k, v = rows(k), rows(v)
+        # (pointer, batch stride, row stride, step) of the places; the page table
+        at, pos32 = (place.stride(0), 0, 1), int(place.dtype == torch.int32)
+        tb, P, most, page = self._table
+        where, table = place.data_ptr(), self.block_table.data_ptr()
         turns = freq is not None
-        sets = [fields(k, kw, self.k_pages, self.k_pages.stride(), norm, turns, True),
-                fields(v, None, self.v_pages, self.v_pages.stride(), False, False, True)]
+        k, v = self._rows(k), self._rows(v)
+        pack = ops._pack_head_rows
+        sets = [pack(k.data_ptr(), L.ptr0(kw), self.k_pages.data_ptr(), 0, 0, 0, where, table, *k.stride()[:3], *self._k_strides,
+                     *at, tb, B, T, P, most, HK, int(kw is not None and kw.dim() == 2), int(norm), int(turns), pos32, page),
+                pack(v.data_ptr(), 0, self.v_pages.data_ptr(), 0, 0, 0, where, table, *v.stride()[:3], *self._v_strides, *at, tb,
+                     B, T, P, most, HK, 0, 0, 0, pos32, page)]
         out = None
         if q is not None:
-            q = rows(q)
-            out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-            sets.append(fields(q, qw, out, out.stride(), norm, turns, False))
+            q = self._rows(q)
+            H = q.shape[2]
+            out = torch.empty(B, T, H, D, device=q.device, dtype=q.dtype)
+            sets.append(pack(q.data_ptr(), L.ptr0(qw), out.data_ptr(), 0, 0, 0, where, 0, *q.stride()[:3], T * H * D, H * D, D, *at,
+                             0, B, T, 0, 0, H, int(qw is not None and qw.dim() == 2), int(norm), int(turns), pos32, 0))
         dev = k.device
         with L.on_device(dev):
             call("moc_head_rotate_fwd", ops._head_args(sets, freq, D, interleaved, self.dtype, float(eps)), stream_ptr(dev))
@@ -607,16 +607,21 @@ class PagedKVCache:
                 self.lengths.add_(T)
         return out
 
+    def _rows(self, x: torch.Tensor) -> torch.Tensor:
+        x = x.detach()
+        if x.dtype != self.k_pages.dtype:
+            x = x.to(self.k_pages.dtype)
+        return x if x.stride(3) == 1 else x.contiguous()
 
-@torch.no_grad()
+
 def paged_attention(q: torch.Tensor, cache: PagedKVCache, *, causal: bool = False,
                     softmax_scale: Optional[float] = None) -> torch.Tensor:
     """Attention of new tokens over their sequences' pages: q (B, H, D) or several tokens (B, L, H, D) -> the same shape
     in the cache's type.  Each sees the ``cache.lengths`` first keys of its sequence; with ``causal`` token l of L the
     first lengths - L + l + 1 (the tokens are the last ones appended).  A token that sees no key gets 0."""
-    _, page, HK, D = cache.k_pages.shape
-    B = cache.lengths.shape[0]
-    if q.dim() not in (3, 4) or q.shape[0] != B or q.shape[-1] != D or q.shape[-2] == 0 or q.shape[-2] % HK:
+    P, page, HK, D, B, most = cache._sizes
+    shape = q.shape
+    if len(shape) not in (3, 4) or shape[0] != B or shape[-1] != D or shape[-2] == 0 or shape[-2] % HK:
         raise ValueError(f"queries of shape {tuple(q.shape)}: expected ({B}, [tokens,] heads, {D}) with heads a multiple of {HK}")
     scale = float(D) ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not 0.0 < scale < 3e38:
@@ -624,22 +629,25 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, *, causal: bool = Fals
     if not q.is_floating_point():
         raise ValueError(f"queries of {q.dtype}")
     L.require_same_gpu(cache.k_pages, q)
-    x = q.unsqueeze(1) if q.dim() == 3 else q
+    q = q.detach()
+    x = q.unsqueeze(1) if len(shape) == 3 else q
     x = ops._attn_rows(x if x.dtype == cache.dtype else x.to(cache.dtype), False)
-    Lq, H, most = x.shape[1], x.shape[2], cache.block_table.shape[1]
-    if q.numel() == 0 or most == 0 or cache.k_pages.shape[0] == 0:
-        return torch.zeros(q.shape, device=q.device, dtype=cache.dtype)
-    out = torch.empty(q.shape, device=q.device, dtype=cache.dtype)
-    dev, ks, vs = q.device, cache.k_pages.stride(), cache.v_pages.stride()
-    nbytes = ops.kv_decode_workspace(B, Lq, most * page, H, HK, D)
+    Lq, H = x.shape[1], x.shape[2]
+    if B == 0 or Lq == 0 or most == 0 or P == 0:
+        return torch.zeros(shape, device=q.device, dtype=cache.dtype)
+    dev = q.device
+    out = torch.empty(shape, device=dev, dtype=cache.dtype)
+    nbytes = ops.kv_decode_workspace(B, Lq, most * page, H, HK, D, cache._code)
+    (kp, kn, kh), (vp, vn, vh) = cache._k_strides, cache._v_strides
+    args = ops.pack_kv_decode(x.data_ptr(), cache.k_pages.data_ptr(), cache.v_pages.data_ptr(), out.data_ptr(),
+                              cache.lengths.data_ptr(), cache.block_table.data_ptr(), 0, *ops._strides3(x), 0, kn, kh, 0, vn, vh,
+                              kp, vp, cache._table[0], B, Lq, 0, P, most, H, HK, D, cache._code, page, int(causal), scale)
     with L.on_device(dev):
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        call("moc_kv_decode", ops.pack_kv_decode(x.data_ptr(), cache.k_pages.data_ptr(), cache.v_pages.data_ptr(),
-                                                 out.data_ptr(), cache.lengths.data_ptr(), cache.block_table.data_ptr(), 0,
-                                                 *ops._strides3(x), 0, ks[1], ks[2], 0, vs[1], vs[2], ks[0], vs[0],
-                                                 cache.block_table.stride(0), B, Lq, 0, cache.k_pages.shape[0], most, H, HK, D,
-                                                 L.dtype_code(cache.dtype), page, int(causal), scale),
-             ptr(ws), nbytes, stream_ptr(dev))
+        if nbytes:
+            ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+            call("moc_kv_decode", args, ws.data_ptr(), nbytes, stream_ptr(dev))
+        else:
+            call("moc_kv_decode", args, None, 0, stream_ptr(dev))
     return out
 
 

@@ -1723,7 +1723,9 @@ def _head_weight(w, H: int, D: int, name: str):
         return None
     if tuple(w.shape) not in ((D,), (H, D)):
         raise ValueError(f"{name} of shape {tuple(w.shape)}, expected ({D},) or ({H}, {D})")
-    return w.float().contiguous()
+    if w.dtype != torch.float32:
+        w = w.float()
+    return w if w.is_contiguous() else w.contiguous()
 
 
 def _head_frequencies(inv_freq, D: int):
@@ -1731,7 +1733,9 @@ def _head_frequencies(inv_freq, D: int):
         return None
     if inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= D or not inv_freq.is_floating_point():
         raise ValueError(f"inv_freq: up to {D // 2} frequencies (one per pair), got {tuple(inv_freq.shape)} {inv_freq.dtype}")
-    return inv_freq.detach().double().contiguous()
+    if inv_freq.dtype != torch.float64 or inv_freq.requires_grad:
+        inv_freq = inv_freq.detach().double()
+    return inv_freq if inv_freq.is_contiguous() else inv_freq.contiguous()
 
 
 def _head_dim(x, name: str) -> int:
@@ -1763,24 +1767,21 @@ def _heads(q, k, wq, wk, eps, norm, pq, pk, inv_freq, interleaved):
     dt = q.dtype
     kt = dt if dt in _ROWS else torch.float32
 
-    def rows(x):
-        if x is None:
-            return None
-        x = x if x.dtype == kt else x.to(kt)
-        return x if x.stride(3) == 1 else x.contiguous()
-
-    q, k = rows(q), rows(k)
+    if kt != dt:
+        q, k = q.to(kt), None if k is None else k.to(kt)
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if k is not None and k.stride(3) != 1:
+        k = k.contiguous()
     cfg = (bool(norm), bool(interleaved), float(eps))
-    if q.numel() == 0 and (k is None or k.numel() == 0) and not _differentiated(q, k, wq, wk):
-        out = (torch.empty_like(q), None if k is None else torch.empty_like(k))
-    elif _differentiated(q, k, wq, wk):
+    if _differentiated(q, k, wq, wk):
         out = _HeadRotate.apply(q, k, wq, wk, pq, pk, inv_freq, cfg)
         out = out if k is not None else (out, None)
     elif k is None:
         out = (_head_rotate_forward([q], [wq], [pq], inv_freq, cfg)[0], None)
     else:
-        out = _head_rotate_forward([q, k], [wq, wk], [pq, pk], inv_freq, cfg)
-    return tuple(t if t is None or t.dtype == dt else t.to(dt) for t in out)
+        out = tuple(_head_rotate_forward([q, k], [wq, wk], [pq, pk], inv_freq, cfg))
+    return out if kt == dt else tuple(None if t is None else t.to(dt) for t in out)
 
 
 def head_norm_rotate(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, eps: float = 1e-6, norm: bool = True,
@@ -1830,12 +1831,15 @@ class _KvDecodeArgs(ctypes.Structure):
 
 _pack_cross = L.packer(_CrossArgs)
 pack_kv_decode = L.packer(_KvDecodeArgs)
-_FEW_ROWS = 16      # rows per kv head up to which single tokens' attention is the faster forward
+_FEW_ROWS = 32      # rows per kv head up to which single tokens' attention is the faster forward
 
 
 def _attn_rows(t: torch.Tensor, rows_apart: bool) -> torch.Tensor:
     """t (B, rows, heads, D) as the attention kernels read it: 16-byte pieces at strides of 16 bytes, and for keys
     and values rows that do not overlap and lie less than 16 MiB apart.  Copied otherwise."""
+    if t.is_contiguous():
+        if t.data_ptr() % 16 == 0 and (t.shape[2] * t.shape[3] < 1 << 20):
+            return t
     es, sizes, st = t.element_size(), t.shape, t.stride()
     ok = st[3] == 1 and t.data_ptr() % 16 == 0
     for i in range(3):
@@ -1851,15 +1855,17 @@ def _attn_rows(t: torch.Tensor, rows_apart: bool) -> torch.Tensor:
 
 
 def _strides3(t: torch.Tensor):
-    """Batch, row and head strides; 0 where there is one of them."""
+    """Batch, row and head strides; 0 where there is one of them (which may have any in torch)."""
     st, sizes = t.stride(), t.shape
+    if sizes[0] > 1 and sizes[1] > 1 and sizes[2] > 1:
+        return st[:3]
     return (st[0] if sizes[0] > 1 else 0, st[1] if sizes[1] > 1 else 0, st[2] if sizes[2] > 1 else 0)
 
 
 @functools.lru_cache(maxsize=1024)
-def _cross_sizes(B: int, Lq: int, N: int, H: int, HK: int, D: int):
+def _cross_sizes(B: int, Lq: int, N: int, H: int, HK: int, D: int, dt: int):
     """(bytes of the forward's workspace, rows of its log-sum-exp)"""
-    return L.query("moc_cross_fwd_workspace", B, Lq, N, H, HK, D), L.query("moc_cross_rows", Lq, H, HK)
+    return L.query("moc_cross_fwd_workspace", B, Lq, N, H, HK, D, dt), L.query("moc_cross_rows", Lq, H, HK)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1868,8 +1874,8 @@ def _cross_bwd_workspace(B: int, Lq: int, N: int, H: int, HK: int, D: int, dt: i
 
 
 @functools.lru_cache(maxsize=1024)
-def kv_decode_workspace(B: int, Lq: int, n_max: int, H: int, HK: int, D: int) -> int:
-    return L.query("moc_kv_decode_workspace", B, Lq, n_max, H, HK, D)
+def kv_decode_workspace(B: int, Lq: int, n_max: int, H: int, HK: int, D: int, dt: int) -> int:
+    return L.query("moc_kv_decode_workspace", B, Lq, n_max, H, HK, D, dt)
 
 
 def _cross_forward(q, k, v, lengths, words, scale: float, trains: bool):
@@ -1882,14 +1888,14 @@ def _cross_forward(q, k, v, lengths, words, scale: float, trains: bool):
     out = torch.empty(B, Lq, H, D, device=dev, dtype=q.dtype)
     with L.on_device(dev):
         if not trains and Lq * (H // HK) <= _FEW_ROWS:
-            nbytes = kv_decode_workspace(B, Lq, N, H, HK, D)
+            nbytes = kv_decode_workspace(B, Lq, N, H, HK, D, dt)
             ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
             call("moc_kv_decode", pack_kv_decode(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr0(lengths), 0,
                                                  ptr0(words), *_strides3(q), *_strides3(k), *_strides3(v), 0, 0, 0, B, Lq, N,
                                                  0, 0, H, HK, D, dt, 0, 0, scale), ptr(ws), nbytes, stream_ptr(dev))
             return out, None, None
-        nbytes, Lp = _cross_sizes(B, Lq, N, H, HK, D)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        nbytes, Lp = _cross_sizes(B, Lq, N, H, HK, D, dt)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
         lse = torch.empty(B, HK, Lp, device=dev, dtype=torch.float32) if trains else None
         low = torch.empty_like(out) if trains and q.dtype == torch.bfloat16 else None
         call("moc_cross_fwd", _pack_cross(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), ptr0(low), 0, 0, 0,
