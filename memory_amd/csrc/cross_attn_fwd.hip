@@ -204,49 +204,47 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
   }
 }
 
-// out = sum_i 2^(lse_i - M) o_i / sum_i 2^(lse_i - M) over the splits of a row, and its log-sum-exp.  A workgroup per
-// row: D / 4 lanes of four dims in each of 1024 / D groups, a group taking every so many splits, joined in LDS (a
-// chain of two loads whatever the number of splits; with all of a row's splits in one lane 32 of them took 7 us).
-template <typename T, int D>
-__global__ __launch_bounds__(256) void cross_merge_kernel(CaArgs a) {
+// out = sum_i 2^(lse_i - M) o_i / sum_i 2^(lse_i - M) over the splits of a row, and its log-sum-exp: D / 4 lanes of four
+// dims in each of 1024 / D groups.  With few rows all groups of a workgroup share one, each taking every so many
+// splits, joined in LDS: a chain of two loads whatever the number of splits (32 of them one after the other took 7 us,
+// this 3).  With many rows (ALONE) each group has its own, which keeps more loads in flight.
+template <typename T, int D, bool ALONE>
+__global__ __launch_bounds__(256) void cross_merge_kernel(CaArgs a, int64_t nrow) {
   constexpr int LPR = D / 4, GR = 256 / LPR;
   __shared__ float sM[GR], sS[GR];
-  __shared__ __attribute__((aligned(16))) float sO[GR][D];
-  const int64_t row = blockIdx.x, nrow = gridDim.x;         // (b, hk, r)
+  __shared__ __attribute__((aligned(16))) float sO[ALONE ? 1 : GR][D];
   const int ch = threadIdx.x % LPR, gr = threadIdx.x / LPR;
+  const int64_t row = ALONE ? (int64_t)blockIdx.x * GR + gr : blockIdx.x;   // (b, hk, r)
+  if (row >= nrow) return;
   const int r = (int)((uint32_t)row % (uint32_t)a.Lp);
   const uint32_t bh = (uint32_t)row / (uint32_t)a.Lp, b = bh / (uint32_t)a.HK, hk = bh - b * a.HK;
   if (r >= a.rows) {
-    if (a.lse && threadIdx.x == 0) a.lse[row] = INFINITY;
+    if (a.lse && ch == 0) a.lse[row] = INFINITY;
     return;
   }
   float M = -INFINITY, den = 0.f;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = gr; s < a.nsplit; s += GR) {
-    const float d = a.part_lse[s * nrow + row];
-    const f32x4 o = *reinterpret_cast<const f32x4*>(a.part + (s * nrow + row) * D + 4 * ch);
+  auto take = [&](float d, const f32x4& o, float s) {
     // (no weight for a split without live keys; a NaN goes through)
     const float m = fmax_fast(M, d);
     const float w = d == -INFINITY ? 0.f : ca_exp2(d - m), f = M == -INFINITY ? 0.f : ca_exp2(M - m);
     acc = acc * f + o * w;
-    den = den * f + w;
+    den = den * f + s * w;
     M = m;
-  }
-  if (ch == 0) {
-    sM[gr] = M;
-    sS[gr] = den;
-  }
-  *reinterpret_cast<f32x4*>(&sO[gr][4 * ch]) = acc;
-  __syncthreads();
-  if (gr != 0) return;
-  const int used = a.nsplit < GR ? a.nsplit : GR;
-  for (int q = 1; q < used; ++q) {
-    const float d = sM[q], m = fmax_fast(M, d);
-    const float w = d == -INFINITY ? 0.f : ca_exp2(d - m), f = M == -INFINITY ? 0.f : ca_exp2(M - m);
-    acc = acc * f + *reinterpret_cast<const f32x4*>(&sO[q][4 * ch]) * w;
-    den = den * f + sS[q] * w;
-    M = m;
+  };
+#pragma unroll 4
+  for (int s = ALONE ? 0 : gr; s < a.nsplit; s += ALONE ? 1 : GR)
+    take(a.part_lse[s * nrow + row], *reinterpret_cast<const f32x4*>(a.part + (s * nrow + row) * D + 4 * ch), 1.f);
+  if constexpr (!ALONE) {
+    if (ch == 0) {
+      sM[gr] = M;
+      sS[gr] = den;
+    }
+    *reinterpret_cast<f32x4*>(&sO[gr][4 * ch]) = acc;
+    __syncthreads();
+    if (gr != 0) return;
+    const int used = a.nsplit < GR ? a.nsplit : GR;
+    for (int q = 1; q < used; ++q) take(sM[q], *reinterpret_cast<const f32x4*>(&sO[q][4 * ch]), sS[q]);
   }
   const float inv = den == 0.f ? 0.f : 1.f / den;
   const size_t at = (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + 4 * ch;
@@ -335,16 +333,22 @@ static int fwd_launch(CaArgs& a, hipStream_t stream) {
   return ca_merge(sizeof(T) == 2 ? MOC_BF16 : MOC_F32, D, a, stream);
 }
 
+template <typename T, int D>
+static void merge_launch(const CaArgs& a, int64_t rows, hipStream_t stream) {
+  constexpr int GR = 1024 / D;
+  if (rows >= 2048)
+    cross_merge_kernel<T, D, true><<<(unsigned)((rows + GR - 1) / GR), 256, 0, stream>>>(a, rows);
+  else
+    cross_merge_kernel<T, D, false><<<(unsigned)rows, 256, 0, stream>>>(a, rows);
+}
+
 int ca_merge(int dtype, int D, const CaArgs& a, hipStream_t stream) {
   const int64_t rows = (int64_t)a.B * a.HK * a.Lp;
   MOC_REQUIRE(rows < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "attention merge: too many rows");
-  const unsigned grid = (unsigned)rows;
   if (dtype == MOC_BF16)
-    D == 64 ? cross_merge_kernel<bf16, 64><<<grid, 256, 0, stream>>>(a)
-            : cross_merge_kernel<bf16, 128><<<grid, 256, 0, stream>>>(a);
+    D == 64 ? merge_launch<bf16, 64>(a, rows, stream) : merge_launch<bf16, 128>(a, rows, stream);
   else
-    D == 64 ? cross_merge_kernel<float, 64><<<grid, 256, 0, stream>>>(a)
-            : cross_merge_kernel<float, 128><<<grid, 256, 0, stream>>>(a);
+    D == 64 ? merge_launch<float, 64>(a, rows, stream) : merge_launch<float, 128>(a, rows, stream);
   return check_launch("attention merge");
 }
 

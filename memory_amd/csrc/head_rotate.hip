@@ -17,13 +17,14 @@ constexpr int kHrAngles = 4096;    // angles of a workgroup's tokens (32 KB)
 struct HrSeg {
   moc_head_rows r;
   int64_t tokens;          // B * L
+  int toks;                // of a workgroup's step
   int first;               // first workgroup of the set
   float* part;             // backward: [workgroups][columns] of dw, columns D or H * D
 };
 struct HrArgs {
   HrSeg seg[3];
   const double* inv_freq;
-  int nseg, D, R, R2, interleaved, lph, toks, vec;   // R2: pairs, lph: lanes per head, toks: tokens per step,
+  int nseg, D, R, R2, interleaved, lph, vec;   // R2: pairs, lph: lanes per head,
                                                          // vec: all rows in 16-byte pieces
   float eps;
 };
@@ -189,8 +190,8 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_fwd_kernel(HrArgs a) {
   const int si = hr_segment(a);
   const HrSeg& s = a.seg[si];
   const moc_head_rows& r = s.r;
-  const int64_t t0 = (int64_t)(blockIdx.x - s.first) * a.toks;
-  const int n = (int)(s.tokens - t0 < a.toks ? s.tokens - t0 : a.toks);
+  const int64_t t0 = (int64_t)(blockIdx.x - s.first) * s.toks;
+  const int n = (int)(s.tokens - t0 < s.toks ? s.tokens - t0 : s.toks);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int j = lane % a.lph, sub = lane / a.lph, hpw = 64 / a.lph;
   const HrLane ln = hr_lane(a, j);
@@ -269,11 +270,11 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_bwd_kernel(HrArgs a, i
   }
   if (r.w && lane_on && (!r.w_head || h_lane < r.H))
     hr_read<float, VEC>(a, ln, r.w + (r.w_head ? (int64_t)h_lane * a.D : 0), w);
-  const int64_t steps = (s.tokens + a.toks - 1) / a.toks;
+  const int64_t steps = (s.tokens + s.toks - 1) / s.toks;
   const int per = r.w_head ? hpw : r.H;               // rows of a token that the workgroup takes
   for (int64_t st = slice; st < steps; st += nslice) {
-    const int64_t t0 = st * a.toks;
-    const int n = (int)(s.tokens - t0 < a.toks ? s.tokens - t0 : a.toks), rows = n * per;
+    const int64_t t0 = st * s.toks;
+    const int n = (int)(s.tokens - t0 < s.toks ? s.tokens - t0 : s.toks), rows = n * per;
     auto at = [&](int row, uint32_t& tk, uint32_t& h, uint32_t& b, uint32_t& l) {
       tk = (uint32_t)row / (uint32_t)per;
       h = r.w_head ? (uint32_t)h_lane : row - tk * per;
@@ -431,27 +432,31 @@ static int hr_check(const char* who, const moc_head_args* p, bool bwd, HrArgs* o
   return MOC_OK;
 }
 
-// Tokens of a workgroup's step: their angles fit LDS, and a large launch has a few rows per lane, a small one
+// Tokens of a workgroup's step: their angles fit LDS, their rows (`per` of a token) keep each lane busy for about four
+// rows, behind which the start of a workgroup and its angles disappear (8,192 + 12,000 rows of 12 heads of 64 in 8, 16 and
+// 32 tokens: forward 17.4, 15.6, 19.0 us; 8,156 of 32 + 8 heads of 128: 31.8, 35.3, 56), and a small launch has
 // workgroups on every CU.
-static int hr_tokens(const HrArgs& h) {
+static int hr_tokens(const HrArgs& h, const HrSeg& s, int per) {
   int64_t total = 0;
   for (int i = 0; i < h.nseg; ++i) total += h.seg[i].tokens;
-  int64_t t = total / 512;
-  const int most = h.R2 ? kHrAngles / h.R2 : 16;
+  int64_t t = 4 * kHrThreads / ((int64_t)per * h.lph);
+  const int64_t most = h.R2 ? kHrAngles / h.R2 : 16;
   if (t > 16) t = 16;
   if (t > most) t = most;
+  if (t > total / 512) t = total / 512;
   return t < 1 ? 1 : (int)t;
 }
 
 // Workgroups of each set's backward: up to 512 slices of its tokens, times the head groups of weights per head.
-static void hr_bwd_plan(const HrArgs& h, int (&slices)[3], int (&wgs)[3], size_t (&part)[3]) {
+static void hr_bwd_plan(HrArgs& h, int (&slices)[3], int (&wgs)[3], size_t (&part)[3]) {
   for (int i = 0; i < 3; ++i) {
     slices[i] = wgs[i] = 0;
     part[i] = 0;
     if (i >= h.nseg) continue;
-    const HrSeg& s = h.seg[i];
+    HrSeg& s = h.seg[i];
     const int hpw = 64 / h.lph, ngrp = s.r.w_head ? (s.r.H + hpw - 1) / hpw : 1;
-    const int64_t steps = (s.tokens + h.toks - 1) / h.toks;
+    s.toks = hr_tokens(h, s, s.r.w_head ? hpw : s.r.H);
+    const int64_t steps = (s.tokens + s.toks - 1) / s.toks;
     int64_t n = 512 / ngrp;
     if (n < 64) n = 64;
     if (n > steps) n = steps;
@@ -472,15 +477,17 @@ int moc_head_rotate_fwd(const moc_head_args* args, hipStream_t stream) {
   HrArgs a;
   int rc = hr_check("moc_head_rotate_fwd", args, false, &a);
   if (rc != MOC_OK) return rc;
-  a.toks = hr_tokens(a);
   int64_t grid = 0;
+  size_t lds = 0;
   for (int i = 0; i < a.nseg; ++i) {
-    a.seg[i].first = (int)grid;
-    grid += (a.seg[i].tokens + a.toks - 1) / a.toks;
+    HrSeg& s = a.seg[i];
+    s.toks = hr_tokens(a, s, s.r.H);
+    s.first = (int)grid;
+    grid += (s.tokens + s.toks - 1) / s.toks;
+    if (lds < (size_t)s.toks * a.R2 * 8) lds = (size_t)s.toks * a.R2 * 8;
   }
   MOC_REQUIRE(grid < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "moc_head_rotate_fwd: too many tokens");
   if (grid == 0) return MOC_OK;
-  const size_t lds = (size_t)a.toks * a.R2 * 8;
   const dim3 gr((unsigned)grid), bl(kHrThreads);
   if (args->dtype == MOC_BF16)
     a.vec ? head_rotate_fwd_kernel<bf16, true><<<gr, bl, lds, stream>>>(a) : head_rotate_fwd_kernel<bf16, false><<<gr, bl, lds, stream>>>(a);
@@ -492,7 +499,6 @@ int moc_head_rotate_fwd(const moc_head_args* args, hipStream_t stream) {
 size_t moc_head_rotate_bwd_workspace(const moc_head_args* args) {
   HrArgs a;
   if (hr_check("moc_head_rotate_bwd", args, true, &a) != MOC_OK) return 0;
-  a.toks = hr_tokens(a);
   int slices[3], wgs[3];
   size_t part[3];
   hr_bwd_plan(a, slices, wgs, part);
@@ -503,7 +509,6 @@ int moc_head_rotate_bwd(const moc_head_args* args, void* workspace, size_t works
   HrArgs a;
   int rc = hr_check("moc_head_rotate_bwd", args, true, &a);
   if (rc != MOC_OK) return rc;
-  a.toks = hr_tokens(a);
   int slices[3], wgs[3];
   size_t part[3];
   hr_bwd_plan(a, slices, wgs, part);
@@ -512,15 +517,16 @@ int moc_head_rotate_bwd(const moc_head_args* args, void* workspace, size_t works
               workspace_bytes, need);
   float* ws = (float*)workspace;
   int grid = 0, cols = 0;
+  size_t lds = 0;
   for (int i = 0; i < a.nseg; ++i) {
     HrSeg& s = a.seg[i];
     s.first = grid;
     grid += wgs[i];
+    if (lds < (size_t)s.toks * a.R2 * 8) lds = (size_t)s.toks * a.R2 * 8;
     s.part = part[i] ? ws : nullptr;
     ws += part[i];
     if (part[i]) cols += ((s.r.w_head ? s.r.H * a.D : a.D) + 15) / 16;
   }
-  size_t lds = (size_t)a.toks * a.R2 * 8;
   if (cols && lds < 4 * 64 * 16 * 4) lds = 4 * 64 * 16 * 4;
   if (args->dtype == MOC_BF16)
     a.vec ? head_rotate_bwd_kernel<bf16, true><<<grid, kHrThreads, lds, stream>>>(a, wgs[0], wgs[1], wgs[2])
