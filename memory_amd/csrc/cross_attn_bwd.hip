@@ -340,57 +340,59 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
   __syncthreads();
   // A step goes in halves of 32 rows, a half's logits in two blocks of 16: the products over the rows take 32, the
   // scores of 16 are all that is held at a time.
-  auto step = [&](const int s, auto which) {
+  auto step = [&](const int s, auto which, auto works) {
     constexpr int buf = decltype(which)::value;
     if (s + 1 < s_end) fetch(s + 1, buf ^ 1);
     const char* Qs = sQ[buf];
     const char* Ds = sD[buf];
+    if constexpr (decltype(works)::value) {
 #pragma unroll
-    for (int half = 0; half < QS / 32; ++half) {
-      const int r0 = 32 * half;
-      F8 pa[KB], sa[KB], pb[KB], sb[KB];
+      for (int half = 0; half < QS / 32; ++half) {
+        const int r0 = 32 * half;
+        F8 pa[KB], sa[KB], pb[KB], sb[KB];
 #pragma unroll
-      for (int qb = 0; qb < 2; ++qb) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(&sL[buf][r0 + 16 * qb + 4 * g]);
-        const f32x4 nd = *reinterpret_cast<const f32x4*>(&sDl[buf][r0 + 16 * qb + 4 * g]);
-        f32x4 st[KB], dp[KB];
+        for (int qb = 0; qb < 2; ++qb) {
+          const f32x4 ls = *reinterpret_cast<const f32x4*>(&sL[buf][r0 + 16 * qb + 4 * g]);
+          const f32x4 nd = *reinterpret_cast<const f32x4*>(&sDl[buf][r0 + 16 * qb + 4 * g]);
+          f32x4 st[KB], dp[KB];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const F8 qa = fr.row(Qs, r0 + 16 * qb, ks), da = fr.row(Ds, r0 + 16 * qb, ks);
+          for (int ks = 0; ks < KS; ++ks) {
+            const F8 qa = fr.row(Qs, r0 + 16 * qb, ks), da = fr.row(Ds, r0 + 16 * qb, ks);
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
-            st[kb] = ca_mma(qa, kf[kb][ks], ks == 0 ? zeros : st[kb]);
-            const f32x4 d0 = ks != 0 ? dp[kb] : kSub ? zeros : nd;
-            if constexpr (kVL)
-              dp[kb] = ca_mma(da, fr.row(Vw, 16 * kb, ks), d0);
-            else
-              dp[kb] = ca_mma(da, vf[kb][ks], d0);
-          }
-        }
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float pt = ca_exp2(st[kb][e] * c - ls[e]);
-            const float ds = pt * (kSub ? dp[kb][e] + nd[e] : dp[kb][e]);
-            pa[kb][4 * qb + e] = from_f<T>(pt);
-            sa[kb][4 * qb + e] = from_f<T>(ds);
-            if constexpr (TWO) {
-              pb[kb][4 * qb + e] = ca_low<T>(pt, pa[kb][4 * qb + e]);
-              sb[kb][4 * qb + e] = ca_low<T>(ds, sa[kb][4 * qb + e]);
+            for (int kb = 0; kb < KB; ++kb) {
+              st[kb] = ca_mma(qa, kf[kb][ks], ks == 0 ? zeros : st[kb]);
+              const f32x4 d0 = ks != 0 ? dp[kb] : kSub ? zeros : nd;
+              if constexpr (kVL)
+                dp[kb] = ca_mma(da, fr.row(Vw, 16 * kb, ks), d0);
+              else
+                dp[kb] = ca_mma(da, vf[kb][ks], d0);
             }
           }
-      }
 #pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const F8 fq = fr.col(Qs, r0, db), fd = fr.col(Ds, r0, db);
+          for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          mma(dv[kb][db], pa[kb], fd);
-          mma(dk[kb][db], sa[kb], fq);
-          if constexpr (TWO) {
-            mma(dv[kb][db], pb[kb], fd);
-            mma(dk[kb][db], sb[kb], fq);
+            for (int e = 0; e < 4; ++e) {
+              const float pt = ca_exp2(st[kb][e] * c - ls[e]);
+              const float ds = pt * (kSub ? dp[kb][e] + nd[e] : dp[kb][e]);
+              pa[kb][4 * qb + e] = from_f<T>(pt);
+              sa[kb][4 * qb + e] = from_f<T>(ds);
+              if constexpr (TWO) {
+                pb[kb][4 * qb + e] = ca_low<T>(pt, pa[kb][4 * qb + e]);
+                sb[kb][4 * qb + e] = ca_low<T>(ds, sa[kb][4 * qb + e]);
+              }
+            }
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const F8 fq = fr.col(Qs, r0, db), fd = fr.col(Ds, r0, db);
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            mma(dv[kb][db], pa[kb], fd);
+            mma(dk[kb][db], sa[kb], fq);
+            if constexpr (TWO) {
+              mma(dv[kb][db], pb[kb], fd);
+              mma(dk[kb][db], sb[kb], fq);
+            }
           }
         }
       }
@@ -398,10 +400,17 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
     ca_wait_all();   // the next step's rows landed
     __syncthreads();
   };
-  for (int s = s_begin; s < s_end; s += 2) {
-    step(s, std::integral_constant<int, 0>());
-    if (s + 1 < s_end) step(s + 1, std::integral_constant<int, 1>());
-  }
+  auto walk = [&](auto works) {
+    for (int s = s_begin; s < s_end; s += 2) {
+      step(s, std::integral_constant<int, 0>(), works);
+      if (s + 1 < s_end) step(s + 1, std::integral_constant<int, 1>(), works);
+    }
+  };
+  // (a wave none of whose keys counts fetches with the others and leaves its SIMD to them)
+  if (live)
+    walk(std::true_type());
+  else
+    walk(std::false_type());
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll

@@ -1831,7 +1831,14 @@ class _KvDecodeArgs(ctypes.Structure):
 
 _pack_cross = L.packer(_CrossArgs)
 pack_kv_decode = L.packer(_KvDecodeArgs)
-_FEW_ROWS = 32      # rows per kv head up to which single tokens' attention is the faster forward
+
+
+def _few_rows_attend(rows: int, D: int, dtype: torch.dtype) -> bool:
+    """Whether a forward of so many rows per kv head is faster on the kernels of single tokens, which read keys and values
+    once per 32 rows and split them finer.  16 sequences of 1,500 keys, 12 heads of 64, in us there / on the kernels of many
+    rows: bfloat16 16 rows 20 / 37, 32 rows 26 / 37, 48 rows 39 / 36; float32 16 rows 38 / 121, 96 rows 104 / 121.  4 of
+    4,000, 8 kv heads of 128, float32: 32 rows 74 / 99, 64 rows 110 / 100."""
+    return rows <= (96 if dtype == torch.float32 and D == 64 else 32)
 
 
 def _attn_rows(t: torch.Tensor, rows_apart: bool) -> torch.Tensor:
@@ -1887,7 +1894,7 @@ def _cross_forward(q, k, v, lengths, words, scale: float, trains: bool):
         return torch.zeros(B, Lq, H, D, device=dev, dtype=q.dtype), None, None
     out = torch.empty(B, Lq, H, D, device=dev, dtype=q.dtype)
     with L.on_device(dev):
-        if not trains and Lq * (H // HK) <= _FEW_ROWS:
+        if not trains and _few_rows_attend(Lq * (H // HK), D, q.dtype):
             nbytes = kv_decode_workspace(B, Lq, N, H, HK, D, dt)
             ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
             call("moc_kv_decode", pack_kv_decode(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr0(lengths), 0,
