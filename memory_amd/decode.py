@@ -558,7 +558,8 @@ class PagedKVCache:
 
         Keys may be normed and rotated on the way (``k_weight``, ``norm``, ``inv_freq``, ``interleaved`` as in
         ``ops.qk_norm_rotate``, ``norm`` where a weight is given by default; the position is the token's place), and the
-        queries ``q`` of the same tokens with them: returns q so treated.  One launch."""
+        queries ``q`` of the same tokens with them: returns q so treated.  One launch.  k, v and q of another type than
+        the cache's are rounded to it first."""
         _, _, HK, D, B, _ = self._sizes
         shape = k.shape
         if len(shape) != 4 or shape != v.shape or shape[0] != B or shape[2] != HK or shape[3] != D:
@@ -667,8 +668,8 @@ def _states_step(memory_attn, hidden: torch.Tensor, cache: PagedKVCache, positio
     B, Lx = hidden.shape[0], hidden.shape[1] if hidden.dim() == 3 else 1
     H, D = memory_attn.num_heads, memory_attn.head_dim
     wq, wo = memory_attn.q_proj.weight, memory_attn.o_proj.weight
-    if positions is not None and not memory_attn.rotary_dim:
-        raise ValueError("positions need rotary_dim")
+    if (positions is not None) != (memory_attn.rotary_dim > 0):
+        raise ValueError("positions are given for a module that rotates its heads (rotary_dim), and only then")
     if hidden.numel() == 0:
         return torch.zeros(B, Lx, wo.shape[0], device=hidden.device, dtype=wo.dtype)
     q = ops.linear(hidden.reshape(B, Lx, -1).to(wq.dtype), wq).view(B, Lx, H, D)
@@ -682,8 +683,8 @@ def memory_decode_step(memory_attn, hidden: torch.Tensor, cache, routing: Option
     """One decode step of a memory sublayer: hidden (B, 1, d) -> (B, 1, d) (before the residual); or L tokens
     of each sequence, (B, L, d) -> (B, L, d), over one routing (a prompt served from the cache).
 
-    Over an encoder's states: ``cache`` is a PagedKVCache (``PagedKVCache.from_memory``), there is no routing, and
-    ``positions`` (L,) or (B, L) are the tokens' for a module that rotates its heads (default 0, 1, ...)."""
+    Over an encoder's states: ``cache`` is a PagedKVCache (``PagedKVCache.from_memory``), there is no routing, and a
+    module that rotates its heads needs the tokens' ``positions``, (L,) or (B, L)."""
     B = hidden.shape[0]
     H = memory_attn.num_heads
     if isinstance(cache, PagedKVCache):
@@ -733,6 +734,8 @@ def _group_native(layers, inputs) -> bool:
     step, of one shape, with the slot counts its combine kernel takes."""
     shapes = set()
     for (attn, cache, routing), h in zip(layers, inputs):
+        if isinstance(cache, PagedKVCache) or getattr(attn, "treats_heads", False):
+            return False
         wq, wo, H = attn.q_proj.weight, attn.o_proj.weight, attn.num_heads
         if h.dtype != wq.dtype or not (h.is_contiguous() and wq.is_contiguous() and wo.is_contiguous()):
             return False

@@ -125,7 +125,7 @@ class MemoryCrossAttention(nn.Module):
 
     @property
     def treats_heads(self) -> bool:
-        """Whether query and key heads are normed or rotated."""
+        """Whether query and key heads are normed or rotated (for a dense memory alone)."""
         return self.q_norm is not None or self.rotary_dim > 0
 
     def _head_options(self, device) -> Dict[str, Any]:
@@ -245,8 +245,8 @@ class MemoryCrossAttention(nn.Module):
         the forward): N = the memory rows, or the selected chapters' rows (slot-major, omega-weighted
         keys) for ``routed_memory_state``.  Computed by moc_xattn_weights from the forward's row
         log-sum-exp; no autograd."""
-        if self.treats_heads or self.head_dim != CHAPTER_TOKENS:
-            raise NotImplementedError("attention weights are formed of heads of 64 dims that are not normed or rotated")
+        if self.treats_heads:
+            raise NotImplementedError("attention weights are formed of heads that are not normed or rotated")
         if routed_memory_state is not None:
             st = routed_memory_state
             norm_type = st.get("norm_type") if st.get("normalize", False) else None

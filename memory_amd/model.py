@@ -196,6 +196,8 @@ class RoutedMemoryLayer(nn.Module):
         if not self.fused or not getattr(self.router, "plain_selection", True):
             return None
         attn = self.memory_attn
+        if getattr(attn, "treats_heads", False):
+            return None     # (the module refuses routed memory then)
         strategy = self.router.routing_strategy
         S = self.num_shared_chapters
         C = self.num_chapters

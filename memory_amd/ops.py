@@ -1605,14 +1605,13 @@ def _head_args(sets, inv_freq, D: int, interleaved: bool, dtype: torch.dtype, ep
 
 
 def _position_fields(positions, count: int):
-    """(pointer, batch stride, row stride, step, 32-bit) of positions (L,), (B, L) or (B, 1); None: 0, 1, ..."""
+    """(pointer, batch stride, row stride, step, 32-bit) of positions (L,), (B, L) or (1, L); None: 0, 1, ..."""
     if positions is None:
         return 0, 0, 0, 1, 0
     st = positions.stride()
     if positions.dim() == 1:
         return positions.data_ptr(), 0, st[0], 0, int(positions.dtype == torch.int32)
-    return (positions.data_ptr(), st[0] if positions.shape[0] > 1 else 0, st[1] if positions.shape[1] == count else 0, 0,
-            int(positions.dtype == torch.int32))
+    return positions.data_ptr(), st[0] if positions.shape[0] > 1 else 0, st[1], 0, int(positions.dtype == torch.int32)
 
 
 def _check_positions(positions, B: int, count: int, name: str):

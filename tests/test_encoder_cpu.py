@@ -156,3 +156,28 @@ def test_entry_points_refuse():
         with pytest.raises(ValueError, match=match):
             heads(**kw)
     assert ctypes.sizeof(ops._HeadRows) == 200
+
+
+def test_decode_step_arguments():
+    """A cache of pages takes no routing, a module that rotates needs positions, another takes none; a routed layer
+    refuses an attention module that norms or rotates its heads."""
+    from memory_amd.decode import PagedKVCache, _group_native, memory_decode_step
+    from memory_amd.memory_attention import MemoryCrossAttention
+    from memory_amd.model import RoutedMemoryLayer
+    cache = PagedKVCache.__new__(PagedKVCache)
+    plain, turning = MemoryCrossAttention(256, 4, 2), MemoryCrossAttention(256, 4, 2, rotary_dim=64)
+    h = rnd(2, 1, 256)
+    with pytest.raises(ValueError, match="no routing"):
+        memory_decode_step(plain, h, cache, object())
+    with pytest.raises(ValueError, match="positions are given"):
+        memory_decode_step(plain, h, cache, positions=torch.zeros(1, dtype=torch.int64))
+    with pytest.raises(ValueError, match="positions are given"):
+        memory_decode_step(turning, h, cache)
+    with pytest.raises(ValueError, match="needs its routing"):
+        memory_decode_step(plain, h, object())
+    with pytest.raises(ValueError, match="PagedKVCache"):
+        memory_decode_step(turning, h, object(), object())
+    assert not _group_native([(plain, cache, None)] * 2, [h, h])
+    layer = RoutedMemoryLayer(256, 4, num_chapters=4, tokens_per_chapter=64, top_k=2)
+    layer.memory_attn = MemoryCrossAttention(256, 4, qk_norm=True)
+    assert layer._fused(h, rnd(256, 256)) is None
