@@ -348,10 +348,12 @@ def require_gpu(*tensors: torch.Tensor) -> None:
 
 def require_same_gpu(first: torch.Tensor, *tensors: torch.Tensor) -> None:
     """require_gpu, and all on the first one's device."""
-    require_gpu(first, *tensors)
     dev = first.device
+    if dev.type != "cuda":
+        require_gpu(first)
     for t in tensors:
         if t is not None and t.device != dev:
+            require_gpu(t)
             raise ValueError(f"expected tensors on one device, got {dev} and {t.device}")
 
 

@@ -35,7 +35,11 @@ def _differentiated(*tensors: Optional[torch.Tensor]) -> bool:
     forward-mode level is open, where the function refuses a tangent that the kernels would drop."""
     if forward_ad._current_level >= 0:
         return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def recorded_backward(fn, inputs, needs, grad_outputs):
@@ -1604,23 +1608,19 @@ def _head_args(sets, inv_freq, D: int, interleaved: bool, dtype: torch.dtype, ep
                                                                          L.dtype_code(dtype), eps)
 
 
-def _position_fields(positions, count: int):
+def _position_fields(positions, B: int, count: int, name: str):
     """(pointer, batch stride, row stride, step, 32-bit) of positions (L,), (B, L) or (1, L); None: 0, 1, ..."""
     if positions is None:
         return 0, 0, 0, 1, 0
+    dt, shape = positions.dtype, positions.shape
+    if dt != torch.int64 and dt != torch.int32:
+        raise ValueError(f"{name} must be int32 or int64, got {dt}")
+    if len(shape) == 1 and shape[0] == count:
+        return positions.data_ptr(), 0, positions.stride(0), 0, int(dt == torch.int32)
+    if len(shape) != 2 or shape[1] != count or shape[0] not in (1, B):
+        raise ValueError(f"{name} of shape {tuple(shape)}, expected ({count},) or ({B}, {count})")
     st = positions.stride()
-    if positions.dim() == 1:
-        return positions.data_ptr(), 0, st[0], 0, int(positions.dtype == torch.int32)
-    return positions.data_ptr(), st[0] if positions.shape[0] > 1 else 0, st[1], 0, int(positions.dtype == torch.int32)
-
-
-def _check_positions(positions, B: int, count: int, name: str):
-    if positions is None:
-        return
-    if positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{name} must be int32 or int64, got {positions.dtype}")
-    if tuple(positions.shape) not in ((count,), (B, count), (1, count)):
-        raise ValueError(f"{name} of shape {tuple(positions.shape)}, expected ({count},) or ({B}, {count})")
+    return positions.data_ptr(), st[0] if shape[0] > 1 else 0, st[1], 0, int(dt == torch.int32)
 
 
 def _rope_fresh(rotary_dim: int, base: float, device: torch.device) -> torch.Tensor:
@@ -1651,25 +1651,33 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, device=None) -> tor
     return _rope_table(int(rotary_dim), float(base), device)
 
 
-def _head_set(x, w, y, dy, dx, dw, norm: bool, rotate: bool, positions, out=None) -> bytes:
-    """moc_head_rows of x (B, L, H, D); ``out``: the tensor whose strides are y's or dy's."""
-    B, count, H, _ = x.shape
-    xs, ys = x.stride(), (x if out is None else out).stride()
-    pos, pb, pl, step, pos32 = _position_fields(positions, count) if rotate else (0, 0, 0, 0, 0)
-    return _pack_head_rows(x.data_ptr(), ptr0(w), ptr0(y), ptr0(dy), ptr0(dx), ptr0(dw), pos, 0, xs[0], xs[1], xs[2], ys[0],
-                           ys[1], ys[2], pb, pl, step, 0, B, count, 0, 0, H, int(w is not None and w.dim() == 2), int(norm),
-                           int(rotate), pos32, 0)
+_NO_POSITIONS = (0, 0, 0, 0, 0)
+
+
+def _head_set(x, shape, w, y, dy, dx, dw, norm: bool, rotate: bool, pos, ys) -> bytes:
+    """moc_head_rows of x (B, L, H, D); ``ys``: the strides of y or dy."""
+    xs = x.stride()
+    where, pb, pl, step, pos32 = pos
+    return _pack_head_rows(x.data_ptr(), 0 if w is None else w.data_ptr(), y, dy, dx, dw, where, 0, xs[0], xs[1], xs[2], ys[0],
+                           ys[1], ys[2], pb, pl, step, 0, shape[0], shape[1], 0, 0, shape[2],
+                           int(w is not None and w.dim() == 2), norm, rotate, pos32, 0)
 
 
 def _head_rotate_forward(rows, weights, positions, inv_freq, cfg):
     norm, interleaved, eps = cfg
-    out = [torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in rows]
-    sets = [_head_set(x, w, y, None, None, None, norm, inv_freq is not None, p, y)
-            for x, w, y, p in zip(rows, weights, out, positions)]
-    dev = rows[0].device
+    first = rows[0]
+    dev, dt, rotate = first.device, first.dtype, int(inv_freq is not None)
+    out, sets = [], []
+    for x, w, p, name in zip(rows, weights, positions, ("q_positions", "k_positions")):
+        shape = x.shape
+        y = torch.empty(shape, device=dev, dtype=dt)
+        B, count, H, D = shape
+        out.append(y)
+        sets.append(_head_set(x, shape, w, y.data_ptr(), 0, 0, 0, norm, rotate,
+                              _position_fields(p, B, count, name) if rotate else _NO_POSITIONS, (count * H * D, H * D, D)))
+    args = _head_args(sets, inv_freq, D, interleaved, dt, eps)
     with L.on_device(dev):
-        call("moc_head_rotate_fwd", _head_args(sets, inv_freq, rows[0].shape[-1], interleaved, rows[0].dtype, eps),
-             stream_ptr(dev))
+        call("moc_head_rotate_fwd", args, stream_ptr(dev))
     return out
 
 
@@ -1696,6 +1704,7 @@ class _HeadRotate(torch.autograd.Function):
         need = ctx.needs_input_grad
         grads = [None] * 8
         sets, keep = [], []
+        rotate = int(inv_freq is not None)
         for x, w, p, dy, ix, iw in ((q, wq, pq, dq, 0, 2), (k, wk, pk, dk, 1, 3)):
             if x is None or dy is None or not (need[ix] or need[iw]):
                 continue
@@ -1704,7 +1713,9 @@ class _HeadRotate(torch.autograd.Function):
             dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[ix] else None
             # (the gradients outlive the call, as .grad: they share nothing with its workspace)
             dw = torch.empty(w.shape, device=x.device, dtype=torch.float32) if w is not None and need[iw] else None
-            sets.append(_head_set(x, w, None, dy, dx, dw, norm, inv_freq is not None, p, dy))
+            shape = x.shape
+            sets.append(_head_set(x, shape, w, 0, dy.data_ptr(), ptr0(dx), ptr0(dw), norm, rotate,
+                                  _position_fields(p, shape[0], shape[1], "positions") if rotate else _NO_POSITIONS, dy.stride()))
             keep.append(dy)
             grads[ix], grads[iw] = dx, dw
         if sets:
@@ -1720,8 +1731,9 @@ class _HeadRotate(torch.autograd.Function):
 def _head_weight(w, H: int, D: int, name: str):
     if w is None:
         return None
-    if tuple(w.shape) not in ((D,), (H, D)):
-        raise ValueError(f"{name} of shape {tuple(w.shape)}, expected ({D},) or ({H}, {D})")
+    shape = w.shape
+    if shape[-1:] != (D,) or not (len(shape) == 1 or len(shape) == 2 and shape[0] == H):
+        raise ValueError(f"{name} of shape {tuple(shape)}, expected ({D},) or ({H}, {D})")
     if w.dtype != torch.float32:
         w = w.float()
     return w if w.is_contiguous() else w.contiguous()
@@ -1737,50 +1749,52 @@ def _head_frequencies(inv_freq, D: int):
     return inv_freq if inv_freq.is_contiguous() else inv_freq.contiguous()
 
 
-def _head_dim(x, name: str) -> int:
-    if x.dim() != 4 or x.shape[3] % 2 or not 0 < x.shape[3] <= 512 or x.shape[2] == 0:
-        raise ValueError(f"{name} of shape {tuple(x.shape)}: expected (batch, rows, heads, head dim), head dim even and at "
+def _head_dims(x, name: str):
+    shape = x.shape
+    if len(shape) != 4 or shape[3] % 2 or not 0 < shape[3] <= 512 or shape[2] == 0:
+        raise ValueError(f"{name} of shape {tuple(shape)}: expected (batch, rows, heads, head dim), head dim even and at "
                          "most 512")
-    return x.shape[3]
+    return shape[2], shape[3]
 
 
 def _heads(q, k, wq, wk, eps, norm, pq, pk, inv_freq, interleaved):
-    D = _head_dim(q, "q")
-    if k is not None and (_head_dim(k, "k") != D or k.dtype != q.dtype):
-        raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype}: one head dim and type")
+    H, D = _head_dims(q, "q")
+    dt = q.dtype
+    if k is not None:
+        HK, DK = _head_dims(k, "k")
+        if DK != D or k.dtype != dt:
+            raise ValueError(f"q {tuple(q.shape)} {dt} and k {tuple(k.shape)} {k.dtype}: one head dim and type")
     if not norm and (wq is not None or wk is not None):
         raise ValueError("a weight needs norm=True")
-    if inv_freq is None and not norm:
-        raise ValueError("neither a norm nor frequencies to rotate by: nothing to do")
-    if inv_freq is None and (pq is not None or pk is not None):
-        raise ValueError("positions need inv_freq")
-    if not q.is_floating_point():
-        raise ValueError(f"heads of {q.dtype}")
+    if inv_freq is None:
+        if not norm:
+            raise ValueError("neither a norm nor frequencies to rotate by: nothing to do")
+        if pq is not None or pk is not None:
+            raise ValueError("positions need inv_freq")
+    else:
+        inv_freq = _head_frequencies(inv_freq, D)
+    if not dt.is_floating_point:
+        raise ValueError(f"heads of {dt}")
     L.require_same_gpu(q, k, wq, wk, pq, pk, inv_freq)
-    _check_positions(pq, q.shape[0], q.shape[1], "q_positions")
-    wq = _head_weight(wq, q.shape[2], D, "q_weight")
+    wq = _head_weight(wq, H, D, "q_weight")
     if k is not None:
-        _check_positions(pk, k.shape[0], k.shape[1], "k_positions")
-        wk = _head_weight(wk, k.shape[2], D, "k_weight")
-    inv_freq = _head_frequencies(inv_freq, D)
-    dt = q.dtype
-    kt = dt if dt in _ROWS else torch.float32
-
-    if kt != dt:
-        q, k = q.to(kt), None if k is None else k.to(kt)
+        wk = _head_weight(wk, HK, D, "k_weight")
+    half = dt not in _ROWS
+    if half:
+        q, k = q.float(), None if k is None else k.float()
     if q.stride(3) != 1:
         q = q.contiguous()
     if k is not None and k.stride(3) != 1:
         k = k.contiguous()
-    cfg = (bool(norm), bool(interleaved), float(eps))
+    cfg = (int(norm), int(interleaved), float(eps))
     if _differentiated(q, k, wq, wk):
         out = _HeadRotate.apply(q, k, wq, wk, pq, pk, inv_freq, cfg)
         out = out if k is not None else (out, None)
     elif k is None:
-        out = (_head_rotate_forward([q], [wq], [pq], inv_freq, cfg)[0], None)
+        out = (_head_rotate_forward((q,), (wq,), (pq,), inv_freq, cfg)[0], None)
     else:
-        out = tuple(_head_rotate_forward([q, k], [wq, wk], [pq, pk], inv_freq, cfg))
-    return out if kt == dt else tuple(None if t is None else t.to(dt) for t in out)
+        out = tuple(_head_rotate_forward((q, k), (wq, wk), (pq, pk), inv_freq, cfg))
+    return tuple(None if t is None else t.to(dt) for t in out) if half else out
 
 
 def head_norm_rotate(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, eps: float = 1e-6, norm: bool = True,
@@ -1843,29 +1857,25 @@ def _few_rows_attend(rows: int, D: int, dtype: torch.dtype) -> bool:
 def _attn_rows(t: torch.Tensor, rows_apart: bool) -> torch.Tensor:
     """t (B, rows, heads, D) as the attention kernels read it: 16-byte pieces at strides of 16 bytes, and for keys
     and values rows that do not overlap and lie less than 16 MiB apart.  Copied otherwise."""
-    if t.is_contiguous():
-        if t.data_ptr() % 16 == 0 and (t.shape[2] * t.shape[3] < 1 << 20):
+    if t.data_ptr() % 16 == 0:
+        st, sizes = t.stride(), t.shape
+        es = 4 if t.dtype == torch.float32 else 2
+        sb, sr, sh, sd = st
+        B, R, H, D = sizes
+        piece = 16 // es
+        if (sd == 1 and (B == 1 or sb % piece == 0) and (R == 1 or sr % piece == 0) and (H == 1 or sh % piece == 0)
+                and (R == 1 or (D <= sr and sr * es < 1 << 24 if rows_apart else sr * es < 1 << 23))
+                and (rows_apart or H == 1 or sh * es * H < 1 << 29)):
             return t
-    es, sizes, st = t.element_size(), t.shape, t.stride()
-    ok = st[3] == 1 and t.data_ptr() % 16 == 0
-    for i in range(3):
-        ok = ok and (sizes[i] == 1 or st[i] * es % 16 == 0)
-    if ok and sizes[1] > 1:
-        ok = sizes[3] <= st[1] and st[1] * es < 1 << 24 if rows_apart else st[1] * es < 1 << 23
-    if ok and not rows_apart and sizes[2] > 1:
-        ok = st[2] * es * sizes[2] < 1 << 29
-    if ok:
-        return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides3(t: torch.Tensor):
     """Batch, row and head strides; 0 where there is one of them (which may have any in torch)."""
-    st, sizes = t.stride(), t.shape
-    if sizes[0] > 1 and sizes[1] > 1 and sizes[2] > 1:
-        return st[:3]
-    return (st[0] if sizes[0] > 1 else 0, st[1] if sizes[1] > 1 else 0, st[2] if sizes[2] > 1 else 0)
+    sb, sr, sh, _ = t.stride()
+    B, R, H, _ = t.shape
+    return (sb if B > 1 else 0, sr if R > 1 else 0, sh if H > 1 else 0)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1982,6 +1992,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     if not 0.0 < scale < 3e38:
         raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
     L.require_same_gpu(q, k, v, kv_lengths, key_mask)
+    if H * D >= 1 << 20 or HK * D >= 1 << 20:
+        raise ValueError(f"{H} heads of {D}: rows of a million elements or more are not taken")
     lengths = words = None
     if kv_lengths is not None:
         if tuple(kv_lengths.shape) != (B,) or kv_lengths.dtype not in (torch.int32, torch.int64):
