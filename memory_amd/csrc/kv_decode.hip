@@ -5,6 +5,10 @@
 // over nsplit workgroups and there over four waves, each with a running maximum of its own, joined in LDS and
 // (nsplit > 1) by a second launch.  K goes straight to registers as the matrix operand, V through a tile of the
 // wave's own in LDS, from which it is read transposed.  A tile is four blocks of 16 keys, each within one page.
+//
+// Measured: 123 us for 64 sequences of up to 4,096 keys, 12 heads of 64 (608 MB: 4.9 TB/s, a copy runs at 5.2), 111 + 4
+// for 37 of up to 5,001 keys, 8 kv heads of 128 in pages of 16 (575 MB: 5.0), 9 + 3 for one of 8,191 keys (34 MB), where
+// the chain length -> page -> keys -> products -> join of a few loads each is what is left.
 #include "cross_attn.h"
 
 namespace moc {
