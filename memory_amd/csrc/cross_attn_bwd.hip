@@ -473,7 +473,7 @@ BwdPlan bwd_plan(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtyp
     if (wgs >= kCaBwdWgs / 2) return 1;
     int64_t s = kCaBwdWgs / (wgs < 1 ? 1 : wgs);
     if (s > steps / 2) s = steps / 2;
-    return s < 1 ? 1 : s > 32 ? 32 : (int)s;
+    return s < 1 ? 1 : s > 128 ? 128 : (int)s;
   };
   int KEYS = 0, QS = 0;
   auto shape = [&](auto s) {

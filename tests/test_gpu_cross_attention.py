@@ -100,7 +100,8 @@ def check(q, k, v, do, live=None, scale=None, **kw):
 
 SHAPES = [(1, 1, 1, 1, 1, 64), (2, 3, 5, 4, 2, 64), (1, 16, 64, 2, 2, 128), (2, 17, 65, 4, 1, 64), (1, 129, 63, 2, 2, 64),
           (2, 128, 130, 3, 3, 128), (1, 300, 333, 4, 2, 64), (1, 131, 257, 8, 1, 128), (3, 40, 700, 6, 2, 64),
-          (1, 5, 1999, 2, 1, 64), (1, 260, 129, 1, 1, 128)]
+          (1, 5, 1999, 2, 1, 64), (1, 260, 129, 1, 1, 128), (1, 2100, 5, 8, 1, 64), (1, 700, 200, 4, 1, 128),
+          (2, 50, 60, 30, 2, 64)]
 
 
 @pytest.mark.gpu

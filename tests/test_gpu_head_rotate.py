@@ -249,3 +249,24 @@ def test_captured(gpu_device):
         got = [o.clone() for o in out]
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, step())), f"replay {rep}"
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(gpu_device):
+    """2.3 G elements: the last token's rows, and their gradient."""
+    from memory_amd import ops
+    x = torch.zeros(1, 70001, 256, 128, device=gpu_device, dtype=BF)
+    g = torch.Generator(device=gpu_device).manual_seed(11)
+    x[:, -1].normal_(generator=g)
+    dy = torch.zeros_like(x)
+    dy[:, -1].normal_(generator=g)
+    x.requires_grad_(True)
+    w = torch.ones(128, device=gpu_device, requires_grad=True)
+    freq = ops.rope_frequencies(128, 10000.0, gpu_device)
+    y = ops.head_norm_rotate(x, w, inv_freq=freq)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    pos = torch.tensor([[70000]], device=gpu_device)
+    ref, bound = reference(x[:, -1:].detach(), w, 1e-6, True, pos, freq, False, dy[:, -1:])
+    close(y[:, -1:].detach(), ref[0], bound[0], "y")
+    close(dx[:, -1:], ref[1], bound[1], "dx")
+    close(dw, ref[2], bound[2], "dw")

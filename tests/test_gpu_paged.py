@@ -93,6 +93,20 @@ def test_long(gpu_device, B):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("L", [1, 6])
+def test_roomy_table(gpu_device, L):
+    """A table with room for many times the tokens held: most workgroups find none."""
+    from memory_amd.decode import PagedKVCache, paged_attention
+    cache, dense = pool(gpu_device, BF, [90, 0, 7], 16, 2, 128)
+    table = torch.full((3, 5000), -1, dtype=torch.int32, device=gpu_device)
+    table[:, :cache.block_table.shape[1]] = cache.block_table
+    roomy = PagedKVCache(cache.k_pages, cache.v_pages, table, cache.lengths)
+    q = torch.randn(3, L, 8, 128, generator=gen(13)).to(BF).to(gpu_device)
+    ref, bound = expect(q, dense, True)
+    ca.close(paged_attention(q, roomy, causal=True), ref, bound, "out")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bad", [-1, -2 ** 31, 10 ** 6, 2 ** 31 - 1])
 def test_entries_outside_the_pool(gpu_device, bad):
     """Keys of a page that is none do not count, and what is written there is dropped."""
