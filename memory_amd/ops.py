@@ -1654,6 +1654,11 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, device=None) -> tor
 _NO_POSITIONS = (0, 0, 0, 0, 0)
 
 
+def _contiguous_like(t: torch.Tensor) -> torch.Tensor:
+    """An empty contiguous tensor of t's shape and type (empty_like takes half of empty's host time)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
 def _head_set(x, shape, w, y, dy, dx, dw, norm: bool, rotate: bool, pos, ys) -> bytes:
     """moc_head_rows of x (B, L, H, D); ``ys``: the strides of y or dy."""
     xs = x.stride()
@@ -1670,7 +1675,7 @@ def _head_rotate_forward(rows, weights, positions, inv_freq, cfg):
     out, sets = [], []
     for x, w, p, name in zip(rows, weights, positions, ("q_positions", "k_positions")):
         shape = x.shape
-        y = torch.empty(shape, device=dev, dtype=dt)
+        y = _contiguous_like(x)
         B, count, H, D = shape
         out.append(y)
         sets.append(_head_set(x, shape, w, y.data_ptr(), 0, 0, 0, norm, rotate,
@@ -1710,9 +1715,9 @@ class _HeadRotate(torch.autograd.Function):
                 continue
             if dy.stride(-1) != 1:
                 dy = dy.contiguous()
-            dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[ix] else None
+            dx = _contiguous_like(x) if need[ix] else None
             # (the gradients outlive the call, as .grad: they share nothing with its workspace)
-            dw = torch.empty(w.shape, device=x.device, dtype=torch.float32) if w is not None and need[iw] else None
+            dw = torch.empty_like(w) if w is not None and need[iw] else None     # (w is float32, contiguous)
             shape = x.shape
             sets.append(_head_set(x, shape, w, 0, dy.data_ptr(), ptr0(dx), ptr0(dw), norm, rotate,
                                   _position_fields(p, shape[0], shape[1], "positions") if rotate else _NO_POSITIONS, dy.stride()))
@@ -1721,9 +1726,9 @@ class _HeadRotate(torch.autograd.Function):
         if sets:
             dev = q.device
             args = _head_args(sets, inv_freq, q.shape[-1], interleaved, q.dtype, eps)
+            nbytes = L.query("moc_head_rotate_bwd_workspace", args)
             with L.on_device(dev):
-                nbytes = L.query("moc_head_rotate_bwd_workspace", args)
-                ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+                ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
                 call("moc_head_rotate_bwd", args, ptr(ws), nbytes, stream_ptr(dev))
         return tuple(grads)
 
@@ -1901,7 +1906,7 @@ def _cross_forward(q, k, v, lengths, words, scale: float, trains: bool):
     dev, dt = q.device, L.dtype_code(q.dtype)
     if B * Lq * N == 0:
         return torch.zeros(B, Lq, H, D, device=dev, dtype=q.dtype), None, None
-    out = torch.empty(B, Lq, H, D, device=dev, dtype=q.dtype)
+    out = _contiguous_like(q)
     with L.on_device(dev):
         if not trains and _few_rows_attend(Lq * (H // HK), D, q.dtype):
             nbytes = kv_decode_workspace(B, Lq, N, H, HK, D, dt)
@@ -1942,10 +1947,9 @@ class _CrossAttention(torch.autograd.Function):
             return (*(torch.zeros(t.shape, device=dev, dtype=t.dtype) if n else None for t, n in zip((q, k, v), need)), None,
                     None, None)
         dout = _attn_rows(dout, False)
-        dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        dk = dv = None
+        dq, dk, dv = _contiguous_like(q), None, None
         if need[1] or need[2]:
-            dk, dv = torch.empty(k.shape, device=dev, dtype=q.dtype), torch.empty(v.shape, device=dev, dtype=q.dtype)
+            dk, dv = _contiguous_like(k), _contiguous_like(v)
         with L.on_device(dev):
             nbytes = _cross_bwd_workspace(B, Lq, N, H, HK, D, dt)
             ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
