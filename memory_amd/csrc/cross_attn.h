@@ -33,8 +33,8 @@ __device__ __forceinline__ void ca_wait_all() { asm volatile("s_waitcnt vmcnt(0)
 __device__ __forceinline__ float ca_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float ca_max3(float a, float b, float c) { return fmax_fast(fmax_fast(a, b), c); }
 
-// Four zeros that the compiler takes for unknown: products that start from them read these registers instead of having
-// their own cleared first (a tenth of the forward's vector instructions).
+// Four zeros that the compiler takes for unknown, so that a product that starts from them reads these registers instead
+// of having its own cleared first (the row sums of the forward: 57.6 -> 55.3 us at 64 dims).
 __device__ __forceinline__ f32x4 ca_zeros() {
   f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
   asm volatile("" : "+v"(z));

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
   vm_wait_all();
   __syncthreads();
   const CaFrag<T, D> fr(lane);
-  const f32x4 zeros = ca_zeros();
+  const f32x4 zeros = f32x4{0.f, 0.f, 0.f, 0.f};
   auto step = [&](auto which) {
     constexpr int buf = decltype(which)::value;
     int tn = t + 1;
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
   };
   const float c = a.scale_log2;
   const CaFrag<T, D> fr(lane);
-  const f32x4 zeros = ca_zeros();
+  const f32x4 zeros = f32x4{0.f, 0.f, 0.f, 0.f};
   const char* Vw = sV + 16 * KB * wave * D * (int)sizeof(T);
   if (s_begin < s_end) fetch(s_begin, 0);
   ca_wait_all();
