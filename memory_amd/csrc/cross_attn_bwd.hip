@@ -181,10 +181,9 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
     }
 }
 
-// dq = scale * the sum of its splits, in their order
+// dq = scale * the sum of its splits, in their order: four elements per thread
 template <typename T, int D>
-__global__ __launch_bounds__(256) void cross_dq_sum_kernel(CaArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__device__ __forceinline__ void dq_sum(const CaArgs& a, int64_t i) {
   const int64_t row = i / (D / 4), nrow = (int64_t)a.B * a.HK * a.Lp;
   const int d0 = (int)(i % (D / 4)) * 4;
   if (row >= nrow) return;
@@ -195,9 +194,7 @@ __global__ __launch_bounds__(256) void cross_dq_sum_kernel(CaArgs a) {
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
   for (int s = 0; s < a.nsplit; ++s) acc += *reinterpret_cast<const f32x4*>(a.part + (s * nrow + row) * D + d0);
-  T* dst = (T*)a.dq + (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + d0;
-#pragma unroll
-  for (int x = 0; x < 4; ++x) dst[x] = from_f<T>(a.scale * acc[x]);
+  ca_store4<T>((T*)a.dq + (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + d0, nullptr, acc * a.scale);
 }
 
 // dk, dv: one workgroup = 4 waves x 16 KB keys of one (sequence, kv head), whose K and V rows stay in registers as
@@ -444,17 +441,23 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
 
 // dk, dv = the sums of their splits, in their order
 template <typename T, int D>
-__global__ __launch_bounds__(256) void cross_dkv_sum_kernel(CaArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__device__ __forceinline__ void dkv_sum(const CaArgs& a, int64_t i) {
   const int64_t nrow = (int64_t)a.B * a.N * a.HK, row = i / (D / 2);
   const int d0 = (int)(i % (D / 2)) * 4;                  // of the 2 D columns dk | dv
   if (row >= nrow) return;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
   for (int s = 0; s < a.nsplit; ++s) acc += *reinterpret_cast<const f32x4*>(a.part + (s * nrow + row) * (2 * D) + d0);
-  T* dst = d0 < D ? (T*)a.dk + row * D + d0 : (T*)a.dv + row * D + d0 - D;
-#pragma unroll
-  for (int x = 0; x < 4; ++x) dst[x] = from_f<T>(acc[x]);
+  ca_store4<T>(d0 < D ? (T*)a.dk + row * D + d0 : (T*)a.dv + row * D + d0 - D, nullptr, acc);
+}
+
+// The sums of the splits, where there are any: the first `dq_blocks` workgroups dq's, the others dk's and dv's
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cross_bwd_sum_kernel(CaArgs dq, CaArgs dkv, int64_t dq_blocks) {
+  if (blockIdx.x < dq_blocks)
+    dq_sum<T, D>(dq, (int64_t)blockIdx.x * 256 + threadIdx.x);
+  else
+    dkv_sum<T, D>(dkv, ((int64_t)blockIdx.x - dq_blocks) * 256 + threadIdx.x);
 }
 
 constexpr int64_t kCaBwdWgs = 512;   // workgroups to aim at (two per CU)
@@ -462,7 +465,7 @@ constexpr int64_t kCaBwdWgs = 512;   // workgroups to aim at (two per CU)
 struct BwdPlan {
   int dq_splits, dkv_splits;
   size_t delta, dq_part, dkv_part;   // floats
-  size_t bytes() const { return 4 * (delta + (dq_part > dkv_part ? dq_part : dkv_part)); }
+  size_t bytes() const { return 4 * (delta + dq_part + dkv_part); }
 };
 
 // Splits where there are few workgroups: of the keys for dq, of the rows for dk and dv.
@@ -496,41 +499,40 @@ template <typename T, int D>
 static int bwd_launch(CaArgs& a, const BwdPlan& p, hipStream_t stream) {
   const char* who = "moc_cross_bwd";
   constexpr bool kHalf = sizeof(T) == 2;
+  constexpr int KEYS = 64 * DkvShape<T, D>::KB;
   const bool few = kHalf && ca_few(a);
-  // (dq comes first: it leaves delta behind)
-  a.nsplit = p.dq_splits;
-  const int64_t tiles = (int64_t)a.B * a.HK * a.nsplit * (a.Lp / kCaRows);
-  MOC_REQUIRE(tiles < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "%s: too many row blocks", who);
-  if (a.nsplit > 1)
-    few ? cross_dq_kernel<T, D, true, kHalf><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a)
-        : cross_dq_kernel<T, D, true, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
+  CaArgs q = a, kv = a;
+  q.nsplit = p.dq_splits;
+  kv.nsplit = p.dkv_splits;
+  kv.part = a.part + p.dq_part;
+  const int64_t tiles = (int64_t)a.B * a.HK * q.nsplit * (a.Lp / kCaRows);
+  const int64_t blocks = (int64_t)a.B * a.HK * kv.nsplit * ((a.N + KEYS - 1) / KEYS);
+  MOC_REQUIRE(tiles < (int64_t)1 << 31 && blocks < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "%s: too many row or key blocks", who);
+  // (dq comes first: it leaves -delta behind)
+  if (q.nsplit > 1)
+    few ? cross_dq_kernel<T, D, true, kHalf><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(q)
+        : cross_dq_kernel<T, D, true, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(q);
   else
-    few ? cross_dq_kernel<T, D, false, kHalf><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a)
-        : cross_dq_kernel<T, D, false, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
+    few ? cross_dq_kernel<T, D, false, kHalf><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(q)
+        : cross_dq_kernel<T, D, false, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(q);
   int rc = check_launch("moc_cross_bwd: dq");
   if (rc != MOC_OK) return rc;
-  if (a.nsplit > 1) {
-    const int64_t lanes = (int64_t)a.B * a.HK * a.Lp * (D / 4);
-    cross_dq_sum_kernel<T, D><<<(unsigned)((lanes + 255) / 256), 256, 0, stream>>>(a);
-    rc = check_launch("moc_cross_bwd: dq sum");
+  if (a.dk) {
+    if (kv.nsplit > 1)
+      few ? cross_dkv_kernel<T, D, true, kHalf><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(kv)
+          : cross_dkv_kernel<T, D, true, false><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(kv);
+    else
+      few ? cross_dkv_kernel<T, D, false, kHalf><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(kv)
+          : cross_dkv_kernel<T, D, false, false><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(kv);
+    rc = check_launch("moc_cross_bwd: dk, dv");
     if (rc != MOC_OK) return rc;
   }
-  if (!a.dk) return MOC_OK;
-  constexpr int KEYS = 64 * DkvShape<T, D>::KB;
-  a.nsplit = p.dkv_splits;
-  const int64_t blocks = (int64_t)a.B * a.HK * a.nsplit * ((a.N + KEYS - 1) / KEYS);
-  MOC_REQUIRE(blocks < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "%s: too many key blocks", who);
-  if (a.nsplit > 1)
-    few ? cross_dkv_kernel<T, D, true, kHalf><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(a)
-        : cross_dkv_kernel<T, D, true, false><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(a);
-  else
-    few ? cross_dkv_kernel<T, D, false, kHalf><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(a)
-        : cross_dkv_kernel<T, D, false, false><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(a);
-  rc = check_launch("moc_cross_bwd: dk, dv");
-  if (rc != MOC_OK || a.nsplit == 1) return rc;
-  const int64_t lanes = (int64_t)a.B * a.N * a.HK * (D / 2);
-  cross_dkv_sum_kernel<T, D><<<(unsigned)((lanes + 255) / 256), 256, 0, stream>>>(a);
-  return check_launch("moc_cross_bwd: dk, dv sum");
+  const int64_t nq = q.nsplit > 1 ? ((int64_t)a.B * a.HK * a.Lp * (D / 4) + 255) / 256 : 0;
+  const int64_t nk = a.dk && kv.nsplit > 1 ? ((int64_t)a.B * a.N * a.HK * (D / 2) + 255) / 256 : 0;
+  if (nq + nk == 0) return MOC_OK;
+  MOC_REQUIRE(nq + nk < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "%s: too many rows to sum", who);
+  cross_bwd_sum_kernel<T, D><<<(unsigned)(nq + nk), 256, 0, stream>>>(q, kv, nq);
+  return check_launch("moc_cross_bwd: sums");
 }
 
 }  // namespace moc
