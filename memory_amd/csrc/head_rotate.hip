@@ -28,8 +28,7 @@ struct HrSeg {
 struct HrArgs {
   HrSeg seg[3];
   const double* inv_freq;
-  int nseg, D, R, R2, interleaved, lph, vec;   // R2: pairs, lph: lanes per head,
-                                                         // vec: all rows in 16-byte pieces
+  int nseg, D, R, R2, interleaved, lph, form;   // R2: pairs, lph: lanes per head, form: HrForm of all rows
   float eps;
 };
 
@@ -46,12 +45,33 @@ __device__ __forceinline__ float hr_sum(float v, int lph) {
   return v;
 }
 
+// How rows are read and written: in 16-byte pieces (kWide: every run of eight starts on one, and eight pairs turn
+// together or not at all), in the same vectors at 4-byte boundaries (kLoose: any number of rotated dims and odd strides;
+// a lane that straddles the rotated part's end still goes one by one), or element by element.  Measured, 16,384 rows of
+// 16 bf16 heads of 128 (forward, backward): 31 and 57 us with 128 rotated, 72 rotated 65 and 109 us loose against 118 and
+// 196 one by one, 72 rotated in pairs 36 and 64 against 129 and 213.
+enum HrForm { kByOne, kLoose, kWide };
+typedef uint32_t hr_u32x4 __attribute__((ext_vector_type(4)));
+typedef hr_u32x4 hr_loose4 __attribute__((aligned(4)));
+
 // The lane's elements: a = first eight (or even places), b = the others, as a row's two runs of eight
-template <typename T, bool VEC>
+template <typename T, int FORM>
 __device__ __forceinline__ void hr_load(const T* p, int e0, int e1, int D, float (&x)[16]) {
-  if constexpr (VEC) {
+  if constexpr (FORM == kWide) {
     ChunkLoadF<T>::run(p + e0, x);
     ChunkLoadF<T>::run(p + e1, x + 8);
+  } else if constexpr (FORM == kLoose) {
+    constexpr int N = 8 * (int)sizeof(T) / 16;       // vectors of a run
+    hr_u32x4 v[2 * N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = reinterpret_cast<const hr_loose4*>(p + e0)[i];
+      v[N + i] = reinterpret_cast<const hr_loose4*>(p + e1)[i];
+    }
+    T t[16];
+    __builtin_memcpy(t, v, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = to_f(t[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -105,9 +125,9 @@ __device__ __forceinline__ void hr_pair(const HrArgs& a, int p, int& e0, int& e1
   }
 }
 
-template <typename T, bool VEC>
+template <typename T, int FORM>
 __device__ __forceinline__ void hr_read(const HrArgs& a, const HrLane& l, const T* p, float (&x)[16]) {
-  if (!VEC && l.mixed) {
+  if (FORM != kWide && l.mixed) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       int e0, e1;
@@ -116,12 +136,12 @@ __device__ __forceinline__ void hr_read(const HrArgs& a, const HrLane& l, const 
       x[8 + i] = e1 < a.D ? to_f(p[e1]) : 0.f;
     }
   } else {
-    hr_load<T, VEC>(p, l.e0, l.e1, a.D, x);
+    hr_load<T, FORM>(p, l.e0, l.e1, a.D, x);
   }
 }
-template <typename T, bool VEC>
+template <typename T, int FORM>
 __device__ __forceinline__ void hr_write(const HrArgs& a, const HrLane& l, T* p, const float (&y)[16]) {
-  if (!VEC && l.mixed) {
+  if (FORM != kWide && l.mixed) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       int e0, e1;
@@ -129,9 +149,21 @@ __device__ __forceinline__ void hr_write(const HrArgs& a, const HrLane& l, T* p,
       if (e0 < a.D) p[e0] = from_f<T>(y[i]);
       if (e1 < a.D) p[e1] = from_f<T>(y[8 + i]);
     }
-  } else if constexpr (VEC) {
+  } else if constexpr (FORM == kWide) {
     HrStore<T>::run(p + l.e0, y);
     HrStore<T>::run(p + l.e1, y + 8);
+  } else if constexpr (FORM == kLoose) {
+    constexpr int N = 8 * (int)sizeof(T) / 16;
+    T t[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[i] = from_f<T>(y[i]);
+    hr_u32x4 v[2 * N];
+    __builtin_memcpy(v, t, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      reinterpret_cast<hr_loose4*>(p + l.e0)[i] = v[i];
+      reinterpret_cast<hr_loose4*>(p + l.e1)[i] = v[N + i];
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -142,12 +174,12 @@ __device__ __forceinline__ void hr_write(const HrArgs& a, const HrLane& l, T* p,
 }
 
 // Turns the lane's pairs by +-angle (dir): pairs lie (i, 8 + i) in halves and mixed lanes, (2 i, 2 i + 1) interleaved.
-template <bool VEC>
+template <int FORM>
 __device__ __forceinline__ void hr_turn(const HrArgs& a, const HrLane& l, const float2* cs, float dir, float (&x)[16]) {
   if (!l.turns) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const bool in = VEC || l.p0 + i < a.R2;     // (with 16-byte pieces eight pairs turn together or not at all)
+    const bool in = FORM == kWide || l.p0 + i < a.R2;
     const float2 t = in ? cs[l.p0 + i] : float2{1.f, 0.f};
     const float s = t.y * dir;
     if (a.interleaved) {
@@ -188,7 +220,7 @@ __device__ __forceinline__ int hr_segment(const HrArgs& a) {
   return s;
 }
 
-template <typename T, bool VEC>
+template <typename T, int FORM>
 __global__ __launch_bounds__(kHrThreads) void head_rotate_fwd_kernel(HrArgs a) {
   extern __shared__ float2 cs[];
   const int si = hr_segment(a);
@@ -204,7 +236,7 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_fwd_kernel(HrArgs a) {
   auto read = [&](int row, float (&x)[16]) {
     const uint32_t tk = (uint32_t)row / (uint32_t)r.H, h = row - tk * r.H;
     const uint32_t t = (uint32_t)t0 + tk, b = t / (uint32_t)r.L, l = t - b * (uint32_t)r.L;
-    hr_read<T, VEC>(a, ln, (const T*)r.x + b * r.xb + l * r.xl + h * r.xh, x);
+    hr_read<T, FORM>(a, ln, (const T*)r.x + b * r.xb + l * r.xl + h * r.xh, x);
   };
   // (a row is requested before the angles are worked out, and then a row ahead of the one in hand)
   float next[16];
@@ -215,7 +247,7 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_fwd_kernel(HrArgs a) {
   float w[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = 1.f;
-  if (r.w && !r.w_head && lane_on) hr_read<float, VEC>(a, ln, r.w, w);
+  if (r.w && !r.w_head && lane_on) hr_read<float, FORM>(a, ln, r.w, w);
   if (r.rotate) {
     hr_angles(a, s, t0, n, cs);
     __syncthreads();
@@ -232,11 +264,11 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_fwd_kernel(HrArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) sq += x[i] * x[i];
       const float rstd = 1.f / sqrtf(hr_sum(sq, a.lph) / (float)a.D + a.eps);
-      if (r.w_head && lane_on) hr_read<float, VEC>(a, ln, r.w + (int64_t)h * a.D, w);
+      if (r.w_head && lane_on) hr_read<float, FORM>(a, ln, r.w + (int64_t)h * a.D, w);
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = x[i] * rstd * w[i];
     }
-    if (r.rotate) hr_turn<VEC>(a, ln, cs + tk * a.R2, 1.f, x);
+    if (r.rotate) hr_turn<FORM>(a, ln, cs + tk * a.R2, 1.f, x);
     int64_t at = b * r.yb + l * r.yl;
     if (r.table) {
       const int64_t p = hr_position(r, b, l), pg = p < 0 ? r.max_pages : p / r.page;
@@ -244,13 +276,13 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_fwd_kernel(HrArgs a) {
       if (id < 0 || id >= r.num_pages) continue;     // (the whole head's lanes)
       at = id * r.yb + (p % r.page) * r.yl;
     }
-    if (lane_on) hr_write<T, VEC>(a, ln, (T*)r.y + at + h * r.yh, x);
+    if (lane_on) hr_write<T, FORM>(a, ln, (T*)r.y + at + h * r.yh, x);
   }
 }
 
 // Backward: a workgroup goes over its share of the tokens, `toks` at a time, for one group of heads (those of a wave's
 // lanes, so that a lane's sums for dw belong to one head); its sums of dw go to its row of `part`.
-template <typename T, bool VEC>
+template <typename T, int FORM>
 __global__ __launch_bounds__(kHrThreads) void head_rotate_bwd_kernel(HrArgs a, int wgs0, int wgs1, int wgs2) {
   extern __shared__ float2 cs[];                      // the angles, and at the end
   float (*red)[64 * 16] = reinterpret_cast<float (*)[64 * 16]>(cs);   // the waves' sums of dw
@@ -273,7 +305,7 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_bwd_kernel(HrArgs a, i
     dw[i] = 0.f;
   }
   if (r.w && lane_on && (!r.w_head || h_lane < r.H))
-    hr_read<float, VEC>(a, ln, r.w + (r.w_head ? (int64_t)h_lane * a.D : 0), w);
+    hr_read<float, FORM>(a, ln, r.w + (r.w_head ? (int64_t)h_lane * a.D : 0), w);
   const int64_t steps = (s.tokens + s.toks - 1) / s.toks;
   const int per = r.w_head ? hpw : r.H;               // rows of a token that the workgroup takes
   for (int64_t st = slice; st < steps; st += nslice) {
@@ -290,8 +322,8 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_bwd_kernel(HrArgs a, i
       uint32_t tk, h, b, l;
       at(row, tk, h, b, l);
       if (!lane_on || h >= (uint32_t)r.H) return;
-      hr_read<T, VEC>(a, ln, (const T*)r.dy + b * r.yb + l * r.yl + h * r.yh, g);
-      if (r.norm) hr_read<T, VEC>(a, ln, (const T*)r.x + b * r.xb + l * r.xl + h * r.xh, x);
+      hr_read<T, FORM>(a, ln, (const T*)r.dy + b * r.yb + l * r.yl + h * r.yh, g);
+      if (r.norm) hr_read<T, FORM>(a, ln, (const T*)r.x + b * r.xb + l * r.xl + h * r.xh, x);
     };
     float gn[16], xn[16];
 #pragma unroll
@@ -314,7 +346,7 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_bwd_kernel(HrArgs a, i
       uint32_t tk, h, b, l;
       at(row, tk, h, b, l);
       if (h >= (uint32_t)r.H) continue;
-      if (r.rotate) hr_turn<VEC>(a, ln, cs + tk * a.R2, -1.f, g);
+      if (r.rotate) hr_turn<FORM>(a, ln, cs + tk * a.R2, -1.f, g);
       if (r.norm) {
         float sq = 0.f;
 #pragma unroll
@@ -332,7 +364,7 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_bwd_kernel(HrArgs a, i
 #pragma unroll
         for (int i = 0; i < 16; ++i) g[i] = rstd * (g[i] - x[i] * mean);
       }
-      if (r.dx && lane_on) hr_write<T, VEC>(a, ln, (T*)r.dx + ((t0 + tk) * r.H + h) * a.D, g);
+      if (r.dx && lane_on) hr_write<T, FORM>(a, ln, (T*)r.dx + ((t0 + tk) * r.H + h) * a.D, g);
     }
   }
   if (!s.part) return;
@@ -410,7 +442,7 @@ static int hr_check(const char* who, const moc_head_args* p, bool bwd, HrArgs* o
   h.inv_freq = a.inv_freq;
   h.nseg = a.nseg; h.D = a.D; h.R = a.R; h.R2 = a.R / 2; h.interleaved = a.interleaved ? 1 : 0; h.eps = a.eps;
   h.lph = 1;
-  h.vec = 1;
+  h.form = kWide;
   while (16 * h.lph < a.D) h.lph *= 2;
   for (int i = 0; i < a.nseg; ++i) {
     const moc_head_rows& r = a.seg[i];
@@ -427,11 +459,18 @@ static int hr_check(const char* who, const moc_head_args* p, bool bwd, HrArgs* o
     s.r.rotate = r.rotate && a.R > 0 ? 1 : 0;
     s.tokens = r.B * r.L;
     const int64_t st[] = {r.xb, r.xl, r.xh, r.yb, r.yl, r.yh};
-    bool vec = a.D % 16 == 0 && a.R % 16 == 0;
-    for (int64_t x : st) vec = vec && x * es % 16 == 0;
+    bool wide = a.D % 16 == 0 && a.R % 16 == 0, loose = a.D % 16 == 0 && (h.interleaved || es == 4 || a.R % 4 == 0);
+    for (int64_t x : st) {
+      wide = wide && x * es % 16 == 0;
+      loose = loose && x * es % 4 == 0;
+    }
     const void* ps[] = {r.x, r.y, r.dy, r.dx, r.w};
-    for (const void* x : ps) vec = vec && ((uintptr_t)x & 15) == 0;
-    if (!vec) h.vec = 0;
+    for (const void* x : ps) {
+      wide = wide && ((uintptr_t)x & 15) == 0;
+      loose = loose && ((uintptr_t)x & 3) == 0;
+    }
+    const int form = wide ? kWide : loose ? kLoose : kByOne;
+    if (form < h.form) h.form = form;
   }
   return MOC_OK;
 }
@@ -449,6 +488,25 @@ static int hr_tokens(const HrArgs& h, const HrSeg& s, int per) {
   if (t > most) t = most;
   if (t > total / 512) t = total / 512;
   return t < 1 ? 1 : (int)t;
+}
+
+template <typename T>
+static void hr_fwd_launch(const HrArgs& a, unsigned grid, size_t lds, hipStream_t stream) {
+  if (a.form == kWide)
+    head_rotate_fwd_kernel<T, kWide><<<grid, kHrThreads, lds, stream>>>(a);
+  else if (a.form == kLoose)
+    head_rotate_fwd_kernel<T, kLoose><<<grid, kHrThreads, lds, stream>>>(a);
+  else
+    head_rotate_fwd_kernel<T, kByOne><<<grid, kHrThreads, lds, stream>>>(a);
+}
+template <typename T>
+static void hr_bwd_launch(const HrArgs& a, int grid, size_t lds, const int (&wgs)[3], hipStream_t stream) {
+  if (a.form == kWide)
+    head_rotate_bwd_kernel<T, kWide><<<grid, kHrThreads, lds, stream>>>(a, wgs[0], wgs[1], wgs[2]);
+  else if (a.form == kLoose)
+    head_rotate_bwd_kernel<T, kLoose><<<grid, kHrThreads, lds, stream>>>(a, wgs[0], wgs[1], wgs[2]);
+  else
+    head_rotate_bwd_kernel<T, kByOne><<<grid, kHrThreads, lds, stream>>>(a, wgs[0], wgs[1], wgs[2]);
 }
 
 // Workgroups of each set's backward: up to 512 slices of its tokens, times the head groups of weights per head.
@@ -492,11 +550,10 @@ int moc_head_rotate_fwd(const moc_head_args* args, hipStream_t stream) {
   }
   MOC_REQUIRE(grid < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "moc_head_rotate_fwd: too many tokens");
   if (grid == 0) return MOC_OK;
-  const dim3 gr((unsigned)grid), bl(kHrThreads);
   if (args->dtype == MOC_BF16)
-    a.vec ? head_rotate_fwd_kernel<bf16, true><<<gr, bl, lds, stream>>>(a) : head_rotate_fwd_kernel<bf16, false><<<gr, bl, lds, stream>>>(a);
+    hr_fwd_launch<bf16>(a, (unsigned)grid, lds, stream);
   else
-    a.vec ? head_rotate_fwd_kernel<float, true><<<gr, bl, lds, stream>>>(a) : head_rotate_fwd_kernel<float, false><<<gr, bl, lds, stream>>>(a);
+    hr_fwd_launch<float>(a, (unsigned)grid, lds, stream);
   return check_launch("moc_head_rotate_fwd");
 }
 
@@ -533,11 +590,9 @@ int moc_head_rotate_bwd(const moc_head_args* args, void* workspace, size_t works
   }
   if (cols && lds < 4 * 64 * 16 * 4) lds = 4 * 64 * 16 * 4;
   if (args->dtype == MOC_BF16)
-    a.vec ? head_rotate_bwd_kernel<bf16, true><<<grid, kHrThreads, lds, stream>>>(a, wgs[0], wgs[1], wgs[2])
-          : head_rotate_bwd_kernel<bf16, false><<<grid, kHrThreads, lds, stream>>>(a, wgs[0], wgs[1], wgs[2]);
+    hr_bwd_launch<bf16>(a, grid, lds, wgs, stream);
   else
-    a.vec ? head_rotate_bwd_kernel<float, true><<<grid, kHrThreads, lds, stream>>>(a, wgs[0], wgs[1], wgs[2])
-          : head_rotate_bwd_kernel<float, false><<<grid, kHrThreads, lds, stream>>>(a, wgs[0], wgs[1], wgs[2]);
+    hr_bwd_launch<float>(a, grid, lds, wgs, stream);
   rc = check_launch("moc_head_rotate_bwd");
   if (rc != MOC_OK || cols == 0) return rc;
   head_rotate_dw_kernel<<<cols, 1024, 0, stream>>>(a, slices[0], slices[1], slices[2]);

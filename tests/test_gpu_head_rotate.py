@@ -171,6 +171,34 @@ def test_strides(gpu_device, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("off,step", [(0, 0), (2, 0), (1, 0), (2, 6), (3, 5)])
+@pytest.mark.parametrize("D,R,inter", [(64, 20, False), (128, 72, False), (96, 56, False), (64, 22, False), (128, 40, True), (48, 2, True),
+                                       (256, 4, False), (64, 64, False)])
+def test_parts_and_bases(gpu_device, D, R, inter, off, step, dt):
+    """Rotated parts that end inside a run of eight, and rows that start at 2, 4, 6 bytes past a 16-byte piece."""
+    from memory_amd import ops
+    B, L, H = 2, 19, 3
+    g = gen(D + R + off)
+
+    def rows():
+        n = B * L * H * (D + step)
+        flat = torch.full((n + off,), float("nan"), dtype=dt, device=gpu_device)
+        x = flat[off:].view(B, L, H, D + step)[..., :D]
+        x.copy_(torch.randn(B, L, H, D, generator=g))
+        return x
+    x, dy = rows().requires_grad_(True), rows()
+    w = (1 + 0.1 * torch.randn(H, D, generator=g)).to(gpu_device).requires_grad_(True)
+    freq = ops.rope_frequencies(R, 1000.0, gpu_device)
+    pos = (torch.arange(L) * 3 + 1)[None].expand(B, L).to(gpu_device)
+    y = ops.head_norm_rotate(x, w, positions=pos, inv_freq=freq, interleaved=inter)
+    got = (y.detach(), *torch.autograd.grad(y, [x, w], dy))
+    ref, bound = reference(x, w, 1e-6, True, pos, freq, inter, dy)
+    for name, a, b, c in zip(("y", "dx", "dw"), got, ref, bound):
+        close(a, b, c, name)
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences(gpu_device):
     from memory_amd import ops
     x, w, dy = data(gpu_device, F32, 2, 9, 3, 64, "head", seed=6)
