@@ -17,11 +17,12 @@ namespace moc {
 // dq (bound as the forward is): one workgroup = 128 rows of one (sequence, kv head) as in the forward, K and V tiles double-buffered; K^T for
 // dS K is read from the K tile with the transposing LDS read.  A tile's 64 keys go in two halves, which halves the
 // score registers.  With SPLIT each of nsplit workgroups takes a share of the keys and writes f32 rows.
-template <typename T, int D, bool SPLIT, bool TWO>
+template <typename T, int D, bool SPLIT, bool FEW>
 __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
   typedef typename Frag<T>::type F8;
   using Stage = CaStage<T, D, kCaKeys, 4>;
   constexpr int KS = D / 32, DB = D / 16, TB = kCaKeys * D * (int)sizeof(T);
+  constexpr bool TWO = FEW && sizeof(T) == 2;
   // dP - delta: from -delta as the product's start, which saves a subtraction, or, where exact, from the whole dP
   constexpr bool kSub = TWO || sizeof(T) == 4;
   __shared__ __attribute__((aligned(16))) char sK[2][TB];
@@ -116,44 +117,51 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
     uint64_t wn = 0;
     while (tn < t_end && !(wn = keys.word(tn))) ++tn;
     if (tn < t_end) fetch(tn, wn, buf ^ 1);
-    const char* Ks = sK[buf];
-    const char* Vs = sV[buf];
+    auto attend = [&] {
+      const char* Ks = sK[buf];
+      const char* Vs = sV[buf];
 #pragma unroll
-    for (int kh = 0; kh < 2; ++kh) {
-      f32x4 st[2][2], dp[2][2];
+      for (int kh = 0; kh < 2; ++kh) {
+        f32x4 st[2][2], dp[2][2];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const F8 ak = fr.row(Ks, 32 * kh + 16 * kb, ks);
-          const F8 av = fr.row(Vs, 32 * kh + 16 * kb, ks);
-          const f32x4 from = *reinterpret_cast<const f32x4*>(&sB[buf][32 * kh + 16 * kb + 4 * g]);
+          for (int kb = 0; kb < 2; ++kb) {
+            const F8 ak = fr.row(Ks, 32 * kh + 16 * kb, ks);
+            const F8 av = fr.row(Vs, 32 * kh + 16 * kb, ks);
+            const f32x4 from = *reinterpret_cast<const f32x4*>(&sB[buf][32 * kh + 16 * kb + 4 * g]);
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb) {
+              st[kb][qb] = ca_mma(ak, qf[qb][ks], ks == 0 ? from : st[kb][qb]);
+              dp[kb][qb] = ca_mma(av, dof[qb][ks], ks != 0 ? dp[kb][qb] : kSub ? zeros : dinit[qb]);
+            }
+          }
+        F8 dsf[2], dsl[2];
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float ds = ca_exp2(st[kb][qb][e] * c - lse[qb]) * (kSub ? dp[kb][qb][e] - dl[qb] : dp[kb][qb][e]);
+              dsf[qb][4 * kb + e] = from_f<T>(ds);
+              if constexpr (TWO) dsl[qb][4 * kb + e] = ca_low<T>(ds, dsf[qb][4 * kb + e]);
+            }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const F8 f = fr.col(Ks, 32 * kh, db);
 #pragma unroll
           for (int qb = 0; qb < 2; ++qb) {
-            st[kb][qb] = ca_mma(ak, qf[qb][ks], ks == 0 ? from : st[kb][qb]);
-            dp[kb][qb] = ca_mma(av, dof[qb][ks], ks != 0 ? dp[kb][qb] : kSub ? zeros : dinit[qb]);
+            mma(acc[qb][db], dsf[qb], f);
+            if constexpr (TWO) mma(acc[qb][db], dsl[qb], f);
           }
-        }
-      F8 dsf[2], dsl[2];
-#pragma unroll
-      for (int qb = 0; qb < 2; ++qb)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float ds = ca_exp2(st[kb][qb][e] * c - lse[qb]) * (kSub ? dp[kb][qb][e] - dl[qb] : dp[kb][qb][e]);
-            dsf[qb][4 * kb + e] = from_f<T>(ds);
-            if constexpr (TWO) dsl[qb][4 * kb + e] = ca_low<T>(ds, dsf[qb][4 * kb + e]);
-          }
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const F8 f = fr.col(Ks, 32 * kh, db);
-#pragma unroll
-        for (int qb = 0; qb < 2; ++qb) {
-          mma(acc[qb][db], dsf[qb], f);
-          if constexpr (TWO) mma(acc[qb][db], dsl[qb], f);
         }
       }
+    };
+    if constexpr (FEW) {      // (a wave without rows leaves its SIMD to the others)
+      if (r0 + 32 * wave < a.rows) attend();
+    } else {
+      attend();
     }
     if (tn < t_end) ca_wait_all();
     t = tn;
@@ -211,12 +219,13 @@ template <> struct DkvShape<bf16, 128> { static constexpr int KB = 2, QS = 32, V
 template <> struct DkvShape<float, 64> { static constexpr int KB = 2, QS = 32, VL = 0, WAVES = 1; };
 template <> struct DkvShape<float, 128> { static constexpr int KB = 1, QS = 32, VL = 0, WAVES = 1; };
 
-template <typename T, int D, bool SPLIT, bool TWO>
+template <typename T, int D, bool SPLIT, bool FEW>
 __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv_kernel(CaArgs a) {
   typedef typename Frag<T>::type F8;
   constexpr int KB = DkvShape<T, D>::KB, QS = DkvShape<T, D>::QS, KEYS = 64 * KB;
   using Stage = CaStage<T, D, QS, 4>;
   constexpr int KS = D / 32, DB = D / 16, TB = QS * D * (int)sizeof(T);
+  constexpr bool TWO = FEW && sizeof(T) == 2;
   constexpr bool kSub = TWO || sizeof(T) == 4;   // as in dq
   constexpr bool kVL = DkvShape<T, D>::VL;
   using StageV = CaStage<T, D, KEYS, 4>;
@@ -354,6 +363,8 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
 #pragma unroll
       for (int half = 0; half < QS / 32; ++half) {
         const int r0 = 32 * half;
+        if constexpr (FEW)
+          if (QS * s + r0 >= a.rows) break;      // (no rows there)
         F8 pa[KB], sa[KB], pb[KB], sb[KB];
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
@@ -498,9 +509,8 @@ BwdPlan bwd_plan(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtyp
 template <typename T, int D>
 static int bwd_launch(CaArgs& a, const BwdPlan& p, hipStream_t stream) {
   const char* who = "moc_cross_bwd";
-  constexpr bool kHalf = sizeof(T) == 2;
   constexpr int KEYS = 64 * DkvShape<T, D>::KB;
-  const bool few = kHalf && ca_few(a);
+  const bool few = ca_few(a);
   CaArgs q = a, kv = a;
   q.nsplit = p.dq_splits;
   kv.nsplit = p.dkv_splits;
@@ -510,19 +520,19 @@ static int bwd_launch(CaArgs& a, const BwdPlan& p, hipStream_t stream) {
   MOC_REQUIRE(tiles < (int64_t)1 << 31 && blocks < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "%s: too many row or key blocks", who);
   // (dq comes first: it leaves -delta behind)
   if (q.nsplit > 1)
-    few ? cross_dq_kernel<T, D, true, kHalf><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(q)
+    few ? cross_dq_kernel<T, D, true, true><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(q)
         : cross_dq_kernel<T, D, true, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(q);
   else
-    few ? cross_dq_kernel<T, D, false, kHalf><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(q)
+    few ? cross_dq_kernel<T, D, false, true><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(q)
         : cross_dq_kernel<T, D, false, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(q);
   int rc = check_launch("moc_cross_bwd: dq");
   if (rc != MOC_OK) return rc;
   if (a.dk) {
     if (kv.nsplit > 1)
-      few ? cross_dkv_kernel<T, D, true, kHalf><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(kv)
+      few ? cross_dkv_kernel<T, D, true, true><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(kv)
           : cross_dkv_kernel<T, D, true, false><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(kv);
     else
-      few ? cross_dkv_kernel<T, D, false, kHalf><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(kv)
+      few ? cross_dkv_kernel<T, D, false, true><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(kv)
           : cross_dkv_kernel<T, D, false, false><<<xcd_grid(blocks), kCaThreads, 0, stream>>>(kv);
     rc = check_launch("moc_cross_bwd: dk, dv");
     if (rc != MOC_OK) return rc;

@@ -23,11 +23,13 @@ namespace moc {
 // the rescale, and P stays <= 2^8.
 constexpr float kCaSlack = 8.f;
 
-template <typename T, int D, bool SPLIT, bool TWO>
+// FEW (see kCaFew): bf16 probabilities in two pieces, and waves without rows leave their SIMD to the others.
+template <typename T, int D, bool SPLIT, bool FEW>
 __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
   typedef typename Frag<T>::type F8;
   using Stage = CaStage<T, D, kCaKeys, 4>;
   constexpr int KS = D / 32, DB = D / 16, TB = kCaKeys * D * (int)sizeof(T);
+  constexpr bool TWO = FEW && sizeof(T) == 2;
   __shared__ __attribute__((aligned(16))) char sK[2][TB];
   __shared__ __attribute__((aligned(16))) char sV[2][TB];
   __shared__ __attribute__((aligned(16))) float sB[2][kCaKeys];
@@ -104,78 +106,85 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
     while (tn < t_end && !(wn = keys.word(tn))) ++tn;
     // (buffer buf ^ 1 was last read a tile ago, which every wave has finished)
     if (tn < t_end) fetch(tn, wn, buf ^ 1);
-    const char* Ks = sK[buf];
-    const char* Vs = sV[buf];
-    f32x4 st[4][2];
+    auto attend = [&] {
+      const char* Ks = sK[buf];
+      const char* Vs = sV[buf];
+      f32x4 st[4][2];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb) {
-        const F8 f = fr.row(Ks, 16 * kb, ks);
-        const f32x4 from = *reinterpret_cast<const f32x4*>(&sB[buf][16 * kb + 4 * g]);
+        for (int kb = 0; kb < 4; ++kb) {
+          const F8 f = fr.row(Ks, 16 * kb, ks);
+          const f32x4 from = *reinterpret_cast<const f32x4*>(&sB[buf][16 * kb + 4 * g]);
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb) st[kb][qb] = ca_mma(f, qf[qb][ks], ks == 0 ? from : st[kb][qb]);
-      }
-    float cm[2];
-    bool grow = false;
-#pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
-      float mx = ca_max3(st[0][qb][0], st[0][qb][1], st[0][qb][2]);
-      mx = ca_max3(mx, st[0][qb][3], st[1][qb][0]);
-      mx = ca_max3(mx, st[1][qb][1], st[1][qb][2]);
-      mx = ca_max3(mx, st[1][qb][3], st[2][qb][0]);
-      mx = ca_max3(mx, st[2][qb][1], st[2][qb][2]);
-      mx = ca_max3(mx, st[2][qb][3], st[3][qb][0]);
-      mx = ca_max3(mx, st[3][qb][1], st[3][qb][2]);
-      cm[qb] = quad_max_pl(fmax_fast(mx, st[3][qb][3])) * c;
-      grow |= cm[qb] > m[qb] + kCaSlack;
-    }
-    if (__any(grow)) {
+          for (int qb = 0; qb < 2; ++qb) st[kb][qb] = ca_mma(f, qf[qb][ks], ks == 0 ? from : st[kb][qb]);
+        }
+      float cm[2];
+      bool grow = false;
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
-        const float mn = cm[qb] > m[qb] + kCaSlack ? cm[qb] : m[qb];
-        const float alpha = m[qb] == mn ? 1.f : ca_exp2(m[qb] - mn);
-        m[qb] = mn;
-        lsum[qb] *= alpha;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[db][qb] *= alpha;
+        float mx = ca_max3(st[0][qb][0], st[0][qb][1], st[0][qb][2]);
+        mx = ca_max3(mx, st[0][qb][3], st[1][qb][0]);
+        mx = ca_max3(mx, st[1][qb][1], st[1][qb][2]);
+        mx = ca_max3(mx, st[1][qb][3], st[2][qb][0]);
+        mx = ca_max3(mx, st[2][qb][1], st[2][qb][2]);
+        mx = ca_max3(mx, st[2][qb][3], st[3][qb][0]);
+        mx = ca_max3(mx, st[3][qb][1], st[3][qb][2]);
+        cm[qb] = quad_max_pl(fmax_fast(mx, st[3][qb][3])) * c;
+        grow |= cm[qb] > m[qb] + kCaSlack;
       }
-    }
-    F8 pf[2][2], pl[2][2];
+      if (__any(grow)) {
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
-      const float off = m[qb] == -INFINITY ? 0.f : m[qb];   // (a row whose logits so far are all -inf)
+        for (int qb = 0; qb < 2; ++qb) {
+          const float mn = cm[qb] > m[qb] + kCaSlack ? cm[qb] : m[qb];
+          const float alpha = m[qb] == mn ? 1.f : ca_exp2(m[qb] - mn);
+          m[qb] = mn;
+          lsum[qb] *= alpha;
+#pragma unroll
+          for (int db = 0; db < DB; ++db) o[db][qb] *= alpha;
+        }
+      }
+      F8 pf[2][2], pl[2][2];
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        const float off = m[qb] == -INFINITY ? 0.f : m[qb];   // (a row whose logits so far are all -inf)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const float p = ca_exp2(ca_logit<TWO || sizeof(T) == 4>(st[2 * h + (x >> 2)][qb][x & 3], c, off));
+            pf[qb][h][x] = from_f<T>(p);
+            if constexpr (TWO) pl[qb][h][x] = ca_low<T>(p, pf[qb][h][x]);
+          }
+      }
+      f32x4 ls[2];
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          ls[qb] = ca_mma(ones, pf[qb][h], h == 0 ? zeros : ls[qb]);
+          if constexpr (TWO) mma(ls[qb], ones, pl[qb][h]);
+        }
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const float p = ca_exp2(ca_logit<TWO || sizeof(T) == 4>(st[2 * h + (x >> 2)][qb][x & 3], c, off));
-          pf[qb][h][x] = from_f<T>(p);
-          if constexpr (TWO) pl[qb][h][x] = ca_low<T>(p, pf[qb][h][x]);
+        for (int db = 0; db < DB; ++db) {
+          const F8 f = fr.col(Vs, 32 * h, db);
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb) {
+            mma(o[db][qb], f, pf[qb][h]);
+            if constexpr (TWO) mma(o[db][qb], f, pl[qb][h]);
+          }
         }
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) lsum[qb] += ls[qb][0];
+    };
+    if constexpr (FEW) {
+      if (r0 + 32 * wave < a.rows) attend();
+    } else {
+      attend();
     }
-    f32x4 ls[2];
-#pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        ls[qb] = ca_mma(ones, pf[qb][h], h == 0 ? zeros : ls[qb]);
-        if constexpr (TWO) mma(ls[qb], ones, pl[qb][h]);
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const F8 f = fr.col(Vs, 32 * h, db);
-#pragma unroll
-        for (int qb = 0; qb < 2; ++qb) {
-          mma(o[db][qb], f, pf[qb][h]);
-          if constexpr (TWO) mma(o[db][qb], f, pl[qb][h]);
-        }
-      }
-#pragma unroll
-    for (int qb = 0; qb < 2; ++qb) lsum[qb] += ls[qb][0];
     if (tn < t_end) ca_wait_all();
     t = tn;
     word = wn;
@@ -328,14 +337,13 @@ template <typename T, int D>
 static int fwd_launch(CaArgs& a, hipStream_t stream) {
   const int64_t tiles = (int64_t)a.B * a.HK * a.nsplit * (a.Lp / kCaRows);
   MOC_REQUIRE(tiles < (int64_t)1 << 31, MOC_ERR_UNSUPPORTED, "moc_cross_fwd: too many row blocks");
-  constexpr bool kHalf = sizeof(T) == 2;
-  const bool few = kHalf && ca_few(a);
+  const bool few = ca_few(a);
   if (a.nsplit == 1) {
-    few ? cross_fwd_kernel<T, D, false, kHalf><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a)
+    few ? cross_fwd_kernel<T, D, false, true><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a)
         : cross_fwd_kernel<T, D, false, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
     return check_launch("moc_cross_fwd");
   }
-  few ? cross_fwd_kernel<T, D, true, kHalf><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a)
+  few ? cross_fwd_kernel<T, D, true, true><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a)
       : cross_fwd_kernel<T, D, true, false><<<xcd_grid(tiles), kCaThreads, 0, stream>>>(a);
   int rc = check_launch("moc_cross_fwd");
   if (rc != MOC_OK) return rc;
