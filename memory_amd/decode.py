@@ -478,8 +478,8 @@ class PagedKVCache:
     they may be views with strides of their own (16-byte pieces).  ``block_table`` (sequences, pages of one) int32: token t
     of sequence b lies in row t % page size of page block_table[b, t // page size]; entries outside the pool hold nothing:
     what is written there is dropped, and keys there do not count.  ``lengths`` (sequences,) int32: tokens held.  The
-    server owns all four tensors and writes table and lengths as it hands out pages; the kernels read them on the device,
-    so a captured step stays right when they change."""
+    server owns all four tensors and writes table and lengths as it hands out pages (in place: another tensor needs another
+    PagedKVCache); the kernels read them on the device, so a captured step stays right when they change."""
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor):
         if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
@@ -508,6 +508,11 @@ class PagedKVCache:
         self._k_strides, self._v_strides = k_pages.stride()[:3], v_pages.stride()[:3]
         self._table = (block_table.stride(0), P, block_table.shape[1], page)
         self._code = L.dtype_code(k_pages.dtype)
+
+    def __setattr__(self, name, value):
+        if name in ("k_pages", "v_pages", "block_table", "lengths") and name in self.__dict__ and value is not self.__dict__[name]:
+            raise AttributeError(f"{name} is written to in place: its checks and strides are those of the cache's construction")
+        super().__setattr__(name, value)
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, sequences: int, max_pages: int, *,

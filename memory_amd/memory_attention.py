@@ -271,7 +271,8 @@ class MemoryCrossAttention(nn.Module):
                 memory_mask: Optional[torch.Tensor] = None, query_positions: Optional[torch.Tensor] = None,
                 memory_positions: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         """Of a dense ``memory``: ``memory_lengths`` (B,) states of each sequence, ``memory_mask`` (B, N) which of them count
-        (True: it does), and with ``rotary_dim`` the positions of queries and states (default 0, 1, ...)."""
+        (True: it does), and with ``rotary_dim`` the positions of queries and states (default 0, 1, ...).  States that do
+        not count change nothing, but in training they must be finite: they meet gradients of 0 in the projections'."""
         if return_attn_weights and token_routing_state is not None:
             raise ValueError("return_attn_weights=True is not supported for token_routing_state path.")
         if return_attn_weights and (memory_lengths is not None or memory_mask is not None):

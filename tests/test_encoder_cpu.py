@@ -92,6 +92,21 @@ def test_paged_cache_device():
         PagedKVCache(rnd(4, 16, 2, 64), rnd(4, 16, 2, 64), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
 
 
+def test_paged_cache_tensors_stay():
+    """Another tensor of another shape or type would be read with the strides of the first."""
+    from memory_amd.decode import PagedKVCache
+    cache = PagedKVCache.__new__(PagedKVCache)
+    for name in ("k_pages", "v_pages", "block_table", "lengths"):
+        t = torch.zeros(4, dtype=torch.int32)
+        setattr(cache, name, t)
+        with pytest.raises(AttributeError, match="in place"):
+            setattr(cache, name, torch.zeros(2, dtype=torch.int64))
+        cache.__dict__[name].add_(1)
+        setattr(cache, name, getattr(cache, name))     # (what `cache.lengths += 1` does)
+        assert getattr(cache, name) is t
+    cache.owner = 1
+
+
 def test_module_options():
     from memory_amd.memory_attention import MemoryCrossAttention
     for kw in (dict(rotary_dim=63), dict(rotary_dim=128), dict(rotary_dim=-2), dict(rotary_dim=64, rotary_base=0.0)):
