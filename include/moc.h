@@ -889,8 +889,9 @@ int moc_kv_decode(const moc_kv_decode_args* a, void* workspace, size_t workspace
  * (b, l, h, i) at b * xb + l * xl + h * xh + i.  norm 0: no norm (and no weight); rotate 0: no rotation.  w f32 [D]
  * (w_head 0) or [H][D] (w_head 1) or NULL.  Pair p < R / 2 of a head (elements p, p + R/2, or 2p, 2p + 1 with
  * interleaved) turns by position * inv_freq[p] (f64, radians; reduced in f64); elements from R on stay.  The position is
- * positions[b * pb + l * pl] (i64, or i32 with pos32; NULL: 0) + l * pstep.  With a table, y is a pool of pages as in
- * moc_kv_decode_args and row (b, l) goes to that position's place, or nowhere if it has none. */
+ * positions[b * pb + l * pl] (i64, or i32 with pos32; NULL: 0) + l * pstep.  With page > 0, y is a pool of pages as in
+ * moc_kv_decode_args and row (b, l) goes to that position's place, or nowhere if it has none (table may be NULL where
+ * max_pages is 0, y where max_pages or num_pages is: all rows go nowhere).  page 0: rows, and no table. */
 typedef struct {
   const void* x;
   const float* w;

@@ -270,7 +270,7 @@ __global__ __launch_bounds__(kHrThreads) void head_rotate_fwd_kernel(HrArgs a) {
     }
     if (r.rotate) hr_turn<FORM>(a, ln, cs + tk * a.R2, 1.f, x);
     int64_t at = b * r.yb + l * r.yl;
-    if (r.table) {
+    if (r.page) {       // (a table without columns has no address: it is the page that says where rows go)
       const int64_t p = hr_position(r, b, l), pg = p < 0 ? r.max_pages : p / r.page;
       const int id = pg < r.max_pages ? r.table[b * r.tb + pg] : -1;
       if (id < 0 || id >= r.num_pages) continue;     // (the whole head's lanes)
@@ -449,10 +449,13 @@ static int hr_check(const char* who, const moc_head_args* p, bool bwd, HrArgs* o
     MOC_REQUIRE(r.B >= 0 && r.L >= 0 && r.H > 0 && r.H <= 1 << 16, MOC_ERR_ARG, "%s: bad sizes", who);
     MOC_REQUIRE(r.B == 0 || r.L < ((int64_t)1 << 31) / r.B, MOC_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 tokens", who);
     const bool empty = r.B * r.L == 0;
-    MOC_REQUIRE(empty || (bwd ? (r.dy && (r.x || !r.norm)) : (r.x && r.y)), MOC_ERR_ARG, "%s: null tensor", who);
+    MOC_REQUIRE(r.page >= 0 && (r.page > 0 ? !bwd && r.max_pages >= 0 && r.num_pages >= 0 && (r.table || r.max_pages == 0 || empty)
+                                           : !r.table),
+                MOC_ERR_ARG, "%s: bad pages", who);
+    const bool nowhere = r.page > 0 && (r.max_pages == 0 || r.num_pages == 0);     // (no row has a place)
+    MOC_REQUIRE(empty || (bwd ? (r.dy && (r.x || !r.norm)) : (r.x && (r.y || nowhere))), MOC_ERR_ARG, "%s: null tensor", who);
     MOC_REQUIRE(!r.rotate || a.R == 0 || a.inv_freq, MOC_ERR_ARG, "%s: a rotation needs its frequencies", who);
     MOC_REQUIRE(r.norm || !r.w, MOC_ERR_ARG, "%s: a weight without a norm", who);
-    MOC_REQUIRE(!r.table || (!bwd && r.page > 0 && r.max_pages >= 0 && r.num_pages >= 0), MOC_ERR_ARG, "%s: bad pages", who);
     HrSeg& s = h.seg[i];
     s.r = r;
     s.r.w_head = r.w && r.w_head ? 1 : 0;

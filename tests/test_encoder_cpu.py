@@ -196,3 +196,26 @@ def test_decode_step_arguments():
     layer = RoutedMemoryLayer(256, 4, num_chapters=4, tokens_per_chapter=64, top_k=2)
     layer.memory_attn = MemoryCrossAttention(256, 4, qk_norm=True)
     assert layer._fused(h, rnd(256, 256)) is None
+
+
+def test_pages_without_a_table():
+    """Rows of pages never become rows in a piece: a page size without a table is taken only where the table has no
+    columns (whose tensor has no address), and a table without a page size is refused."""
+    from memory_amd import _lib as L
+    from memory_amd import ops
+    assert torch.empty(2, 0, dtype=torch.int32).data_ptr() == 0
+
+    def heads(*, y=16, table=16, page=16, pages=4, most=3, B=1, name="moc_head_rotate_fwd"):
+        f = ops._pack_head_rows(16, 0, y, 16, 16, 0, 16, table, 256, 64, 64, 2048, 128, 64, 0, 0, 1, most, B, 2, pages, most, 2, 0,
+                                1, 0, 0, page)
+        a = f + ops._NO_ROWS * 2 + ops._pack_head_tail(0, 1, 64, 0, 0, L.MOC_BF16, 1e-6)
+        L.call(name, a, *(() if name.endswith("fwd") else (None, 0)), None)
+
+    for kw in (dict(table=0), dict(table=0, pages=0), dict(page=0), dict(page=-16), dict(most=-1), dict(pages=-1),
+               dict(name="moc_head_rotate_bwd")):
+        with pytest.raises(ValueError, match="pages"):
+            heads(**kw)
+    for kw in (dict(y=0), dict(y=0, page=0, table=0)):
+        with pytest.raises(ValueError, match="null"):
+            heads(**kw)
+    heads(B=0, table=0)     # (no sequences: nothing is launched)

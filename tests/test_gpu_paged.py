@@ -308,3 +308,25 @@ def test_trained_and_served(gpu_device):
         out = h[:, 5:6] + memory_decode_step(s.memory_attn, x, cache, positions=torch.tensor([5], device=gpu_device))
         # (two bfloat16 paths with their own roundings of queries, attention, projection and sum: 6 half steps)
         assert (out.float() - ref[:, 5:6].float()).abs().max() <= 6 * 2.0 ** -8 * ref.float().abs().max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("positions", [False, True])
+@pytest.mark.parametrize("pages,most", [(4, 0), (0, 0), (0, 2)])
+def test_append_without_places(gpu_device, pages, most, positions, dt):
+    """A table without columns, a pool without pages: every token is dropped (three sequences of two tokens, so that rows
+    in a piece would stay within the four pages), the queries are treated and lengths grow."""
+    from memory_amd.decode import PagedKVCache, paged_attention
+    g = gen(50)
+    k, v = (torch.full((pages, 16, 2, 64), 7.0, device=gpu_device, dtype=dt) for _ in range(2))
+    cache = PagedKVCache(k, v, torch.zeros(3, most, device=gpu_device, dtype=torch.int32),
+                         torch.tensor([0, 1, 5], device=gpu_device, dtype=torch.int32))
+    new = torch.randn(3, 2, 8, 64, generator=g).to(dt).to(gpu_device)
+    q = cache.append(new[:, :, 4:6], new[:, :, 6:], q=new[:, :, :4],
+                     positions=torch.zeros(3, device=gpu_device, dtype=torch.int64) if positions else None)
+    assert torch.equal(q, new[:, :, :4]) and (k == 7).all() and (v == 7).all()
+    assert cache.lengths.tolist() == ([0, 1, 5] if positions else [2, 3, 7])
+    assert cache.append(new[:, :, 4:6], new[:, :, 6:], positions=cache.lengths) is None and (k == 7).all() and (v == 7).all()
+    o = paged_attention(q, cache, causal=True)
+    assert o.shape == q.shape and (o == 0).all()
