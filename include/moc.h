@@ -868,8 +868,9 @@ int moc_key_words(const void* mask, int64_t mb, int64_t mn, const int32_t* lengt
 
 /* The same for few queries per sequence (single tokens), HBM-bound: K and V either as above (table NULL) or in pages of
  * `page` tokens (a multiple of 16): row p of sequence b is row p % page of page table[b * tb + p / page], element (page,
- * row, head, i) at page * kp + row * kn + head * kh + i.  n = lengths[b] (NULL: N) keys, at most max_pages * page;
- * causal: query l sees the first n - L + l + 1.  Table entries outside [0, num_pages) are keys that do not count. */
+ * row, head, i) at page * kp + row * kn + head * kh + i.  The keys are the first lengths[b] (NULL: N), of which those
+ * past N, or max_pages * page, do not exist; causal: query l sees the first lengths[b] - L + l + 1 of them.  Table entries
+ * outside [0, num_pages) are keys that do not count. */
 typedef struct {
   const void *q, *k, *v;
   void* out; /* [B][L][H][D] */

@@ -43,27 +43,25 @@ __global__ __launch_bounds__(64 * kKdWaves) void kv_decode_kernel(KdArgs p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c16 = lane & 15;
 
-  int n;
-  if constexpr (PAGED) {
-    const int64_t most = p.max_pages * p.page;
-    n = ca_scalar(a.lengths + b);
-    n = n < 0 ? 0 : (int64_t)n < most ? n : (int)most;
-  } else {
-    n = ca_keys_end(a, b);
-  }
+  // tokens of the sequence, and those of them that have a place (the first n): what a causal row sees is counted from
+  // the former, since the tokens of the call are the sequence's last ones whether they found a place or not
+  int len = a.lengths ? ca_scalar(a.lengths + b) : a.N;
+  len = len < 0 ? 0 : len;
+  const int n = len < a.N ? len : a.N;
   const CaKeys keys{!PAGED && a.words ? a.words + (size_t)b * a.nt : nullptr, n};
   const int nt = (n + kCaKeys - 1) / kCaKeys;
   const int t_begin = (int)((int64_t)nt * sp / nsp), t_end = (int)((int64_t)nt * (sp + 1) / nsp);
 
   // keys that this lane's rows see, and those that every row does
   int limit[RB];
-  const int all_see = p.causal ? n - a.L + 1 : n;
+  const int all_see = p.causal && len - (a.L - 1) < n ? len - (a.L - 1) : n;
   F8 qf[RB][KS];
 #pragma unroll
   for (int x = 0; x < RB; ++x) {
     const int r = ROWS * rb + 16 * x + c16, l = r / a.G, h = hk * a.G + r % a.G;
     const bool ok = r < a.rows;
-    limit[x] = !ok ? 0 : p.causal ? n - a.L + l + 1 : n;
+    const int see = len - (ok ? a.L - l - 1 : 0);       // (never past len, which may be 2^31 - 1)
+    limit[x] = !ok ? 0 : p.causal && see < n ? see : n;
     const T* qp = (const T*)a.q + b * a.qb + (int64_t)l * a.ql + (int64_t)h * a.qh;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[x][ks] = ok ? Load8<T, T>::run(qp + 32 * ks + 8 * g) : zero_frag<T>();

@@ -330,3 +330,52 @@ def test_append_without_places(gpu_device, pages, most, positions, dt):
     assert cache.append(new[:, :, 4:6], new[:, :, 6:], positions=cache.lengths) is None and (k == 7).all() and (v == 7).all()
     o = paged_attention(q, cache, causal=True)
     assert o.shape == q.shape and (o == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("L", [1, 5, 20])
+@pytest.mark.parametrize("page,pages", [(16, 4), (48, 3)])
+def test_causal_past_the_table(gpu_device, page, pages, L, dt):
+    """Lengths past the table's end, as an append leaves them that dropped tokens: token l of L sees the places below
+    lengths - L + l + 1 that there are, the same with room left in the table as without."""
+    from memory_amd.decode import PagedKVCache, paged_attention
+    room = page * pages
+    lens = [room + n for n in (3, L, L + 7, -1, 0)] + [2 ** 31 - 1]
+    cache, dense = pool(gpu_device, dt, [room] * len(lens), page, 2, 64)
+    cache.lengths.copy_(torch.tensor(lens, dtype=torch.int32))
+    q = torch.randn(len(lens), L, 8, 64, generator=gen(51)).to(dt).to(gpu_device)
+    o = paged_attention(q, cache, causal=True)
+    for b, n in enumerate(lens):
+        k, v = dense[b]
+        for l in range(L):
+            see = min(room, n - L + l + 1)
+            ref, bound = ca.reference(q[b:b + 1, l:l + 1], k[None, :see], v[None, :see])
+            ca.close(o[b:b + 1, l:l + 1], ref, bound, f"length {n}, token {l}")
+    roomy = torch.full((len(lens), pages + 3), -1, dtype=torch.int32, device=gpu_device)
+    roomy[:, :pages] = cache.block_table
+    cache.lengths[-1] = room + 40
+    same = PagedKVCache(cache.k_pages, cache.v_pages, roomy, cache.lengths)
+    # (other splits of the keys: the sums differ by their order)
+    for b, n in enumerate(cache.lengths.tolist()):
+        for l in range(L):
+            see = min(room, n - L + l + 1)
+            ref, bound = ca.reference(q[b:b + 1, l:l + 1], dense[b][0][None, :see], dense[b][1][None, :see])
+            ca.close(paged_attention(q, same, causal=True)[b:b + 1, l:l + 1], ref, bound, f"with room, length {n}, token {l}")
+
+
+@pytest.mark.gpu
+def test_append_past_the_table(gpu_device):
+    """A sequence of 62 tokens with room for 64 takes five more: two find a place, and each of the five sees itself where
+    it has one and everything before it."""
+    from memory_amd.decode import paged_attention
+    cache, dense = pool(gpu_device, BF, [62], 16, 2, 64)
+    new = torch.randn(1, 5, 12, 64, generator=gen(52)).to(BF).to(gpu_device)
+    q = cache.append(new[:, :, 8:10], new[:, :, 10:], q=new[:, :, :8])
+    assert cache.lengths.tolist() == [67]
+    o = paged_attention(q, cache, causal=True)
+    k, v = (torch.cat([d, x[0, :2]]) for d, x in zip(dense[0], (new[:, :, 8:10], new[:, :, 10:])))
+    for l in range(5):
+        see = min(64, 63 + l)
+        ref, bound = ca.reference(q[:, l:l + 1], k[None, :see], v[None, :see])
+        ca.close(o[:, l:l + 1], ref, bound, f"token {l}")
