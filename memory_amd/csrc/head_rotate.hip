@@ -174,6 +174,7 @@ __device__ __forceinline__ void hr_write(const HrArgs& a, const HrLane& l, T* p,
 }
 
 // Turns the lane's pairs by +-angle (dir): pairs lie (i, 8 + i) in halves and mixed lanes, (2 i, 2 i + 1) interleaved.
+// Pairs behind the rotated part are left alone: turned by 0, an infinity or NaN in one element would reach the other.
 template <int FORM>
 __device__ __forceinline__ void hr_turn(const HrArgs& a, const HrLane& l, const float2* cs, float dir, float (&x)[16]) {
   if (!l.turns) return;
@@ -182,15 +183,15 @@ __device__ __forceinline__ void hr_turn(const HrArgs& a, const HrLane& l, const 
     const bool in = FORM == kWide || l.p0 + i < a.R2;
     const float2 t = in ? cs[l.p0 + i] : float2{1.f, 0.f};
     const float s = t.y * dir;
-    if (a.interleaved) {
-      const float u = x[2 * i], v = x[2 * i + 1];
-      x[2 * i] = u * t.x - v * s;
-      x[2 * i + 1] = v * t.x + u * s;
-    } else {
-      const float u = x[i], v = x[8 + i];
-      x[i] = u * t.x - v * s;
-      x[8 + i] = v * t.x + u * s;
-    }
+    auto turn = [&](float& u, float& v) {
+      const float y = u * t.x - v * s, z = v * t.x + u * s;
+      u = in ? y : u;
+      v = in ? z : v;
+    };
+    if (a.interleaved)
+      turn(x[2 * i], x[2 * i + 1]);
+    else
+      turn(x[i], x[8 + i]);
   }
 }
 

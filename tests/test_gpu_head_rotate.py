@@ -298,3 +298,36 @@ def test_offsets_past_32_bits(gpu_device):
     close(y[:, -1:].detach(), ref[0], bound[0], "y")
     close(dx[:, -1:], ref[1], bound[1], "dx")
     close(dw, ref[2], bound[2], "dw")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("pairs", [False, True])
+@pytest.mark.parametrize("D,R", [(128, 72), (128, 64), (64, 20), (50, 6), (64, 2), (62, 62), (64, 34)])
+def test_dims_that_do_not_turn_keep_their_values(gpu_device, D, R, pairs, dt):
+    """Infinities and NaN behind the rotated dims stay in their elements, forward and (without a norm) backward; inside
+    them they reach their own pair and no other."""
+    from memory_amd import ops
+    g = gen(60)
+    x, dy = (torch.randn(2, 5, 4, D, generator=g).to(dt) for _ in range(2))
+    for i, bad in enumerate((float("inf"), float("-inf"), float("nan"))):
+        x[:, i, :, R + i::5] = bad
+        dy[:, i, :, R + i + 1::5] = bad
+    x, dy = x.to(gpu_device).requires_grad_(True), dy.to(gpu_device)
+    kw = dict(norm=False, inv_freq=ops.rope_frequencies(R, 10000.0, gpu_device), interleaved=pairs)
+    y = ops.head_norm_rotate(x, **kw)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    for got, want in ((y.detach(), x.detach()), (dx, dy)):
+        # NaN compares as one value; the rest of the elements to the bit
+        assert torch.equal(got[..., R:].nan_to_num(7.0, 8.0, 9.0), want[..., R:].nan_to_num(7.0, 8.0, 9.0))
+        assert torch.isfinite(got[..., :R]).all()
+    x = torch.randn(1, 1, 1, D, generator=g).to(dt)
+    other = torch.ones(D, dtype=torch.bool)
+    for p in {0, R // 2 - 1}:
+        z = x.clone()
+        a, b = (2 * p, 2 * p + 1) if pairs else (p, R // 2 + p)
+        z[..., a] = float("nan")
+        keep = other.clone()
+        keep[[a, b]] = False
+        y = ops.head_norm_rotate(z.to(gpu_device), positions=torch.tensor([3], device=gpu_device), **kw).cpu()
+        assert torch.isnan(y[..., ~keep]).all() and torch.isfinite(y[..., keep]).all()
