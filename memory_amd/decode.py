@@ -530,13 +530,14 @@ class PagedKVCache:
                     page_size: int = 64, memory_positions: Optional[torch.Tensor] = None) -> "PagedKVCache":
         """The keys and values of MemoryCrossAttention over an encoder's states (B, N, d), projected once for a
         generation (``memory_decode_step``); pages lie in the order of the sequences.  ``memory_lengths`` (B,) as in its
-        forward; ``memory_positions`` as there."""
+        forward; ``memory_positions`` as there.  A float16 module's pages are float32, as its attention is."""
         if memory.dim() != 3 or memory.shape[0] * memory.shape[1] == 0:
             raise ValueError(f"memory must be (B, N, d) with states, got {tuple(memory.shape)}")
         B, N, _ = memory.shape
         k, v = memory_attn.project_memory(memory, memory_positions)
         per = (N + page_size - 1) // page_size
-        self = cls.allocate(B * per, page_size, k.shape[2], k.shape[3], B, per, dtype=k.dtype, device=k.device)
+        dtype = k.dtype if k.dtype in (torch.float32, torch.bfloat16) else torch.float32
+        self = cls.allocate(B * per, page_size, k.shape[2], k.shape[3], B, per, dtype=dtype, device=k.device)
         self.block_table.copy_(torch.arange(B * per, device=k.device, dtype=torch.int32).view(B, per))
         self.append(k, v)
         if memory_lengths is not None:

@@ -379,3 +379,34 @@ def test_append_past_the_table(gpu_device):
         see = min(64, 63 + l)
         ref, bound = ca.reference(q[:, l:l + 1], k[None, :see], v[None, :see])
         ca.close(o[:, l:l + 1], ref, bound, f"token {l}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(qk_norm=True, rotary_dim=32)])
+def test_float16_layer_served(gpu_device, kw):
+    """A float16 module, served from float32 pages, equals its forward: keys and queries are the same float16 values in
+    both; the attention, float32 within 1e-5 of the largest value as in test_layer_served, is rounded to float16 in
+    both, and a row of o_proj adds 256 such differences (2^-11 each, half a step on either side, against o_proj's own
+    weights) before it is rounded itself."""
+    from memory_amd.decode import PagedKVCache, memory_decode_step
+    m = ca._module(gpu_device, dt=torch.float16, **kw)
+    h = torch.randn(3, 4, 256, generator=gen(53)).half().to(gpu_device)
+    mem = torch.randn(3, 50, 96, generator=gen(54)).half().to(gpu_device)
+    lens = torch.tensor([50, 0, 17], device=gpu_device)
+    pos = torch.arange(4, device=gpu_device) + 9 if kw else None
+    with torch.no_grad():
+        ref, _ = m(h, mem, memory_lengths=lens, query_positions=pos)
+        cache = PagedKVCache.from_memory(m, mem, lens, page_size=16)
+        assert cache.dtype == F32
+        k, v = m.project_memory(mem)
+        assert torch.equal(cache.k_pages[cache.block_table[0, 3], :2], k[0, 48:].float())
+        assert torch.equal(cache.v_pages[cache.block_table[2, 1], :1], v[2, 16:17].float())
+        whole = memory_decode_step(m, h, cache, positions=pos)
+        assert whole.dtype == torch.float16 and (whole[1] == 0).all()
+        a = m.attention_preproj(h, mem, memory_lengths=lens, query_positions=pos).double()
+        slack = (2 * 2.0 ** -11 * a.abs() + 1e-5 * a.abs().max()) @ m.o_proj.weight.double().abs().t().contiguous()
+        bound = slack + 2 * 2.0 ** -11 * ref.double().abs() + 2.0 ** -24
+        assert ((whole.double() - ref.double()).abs() <= bound).all()
+        for t in range(4):
+            one = memory_decode_step(m, h[:, t:t + 1], cache, positions=None if pos is None else pos[t:t + 1])
+            assert ((one.double() - ref[:, t:t + 1].double()).abs() <= bound[:, t:t + 1]).all()
