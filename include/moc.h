@@ -859,7 +859,7 @@ typedef struct {
 int64_t moc_cross_rows(int64_t L, int H, int HK);
 size_t moc_cross_fwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtype);
 int moc_cross_fwd(const moc_cross_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream);
-/* Gradients of the forward whose out and lse these are: dq (or NULL), dk and dv (both or neither NULL). */
+/* Gradients of the forward whose out and lse these are: dq, or dk and dv, or all three (the others NULL). */
 size_t moc_cross_bwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtype);
 int moc_cross_bwd(const moc_cross_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream);
 /* Packed key mask: mask one byte per key (0: does not count), element (b, n) at b * mb + n * mn. */

@@ -77,6 +77,7 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
     lse[qb] = ok ? a.lse[at] : INFINITY;
     if (g == 0 && sp == 0) a.ndelta[at] = -dl[qb];
   }
+  if (!a.dq) return;     // (the queries are not trained: -delta is all that dk needs)
   f32x4 acc[2][DB];
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb)
@@ -512,7 +513,7 @@ static int bwd_launch(CaArgs& a, const BwdPlan& p, hipStream_t stream) {
   constexpr int KEYS = 64 * DkvShape<T, D>::KB;
   const bool few = ca_few(a);
   CaArgs q = a, kv = a;
-  q.nsplit = p.dq_splits;
+  q.nsplit = a.dq ? p.dq_splits : 1;
   kv.nsplit = p.dkv_splits;
   kv.part = a.part + p.dq_part;
   const int64_t tiles = (int64_t)a.B * a.HK * q.nsplit * (a.Lp / kCaRows);
@@ -560,7 +561,7 @@ int moc_cross_bwd(const moc_cross_args* args, void* workspace, size_t workspace_
   CaArgs a;
   int rc = ca_check(who, args, &a);
   if (rc != MOC_OK) return rc;
-  MOC_REQUIRE(a.q && a.k && a.v && a.out && a.dout && a.lse && a.dq, MOC_ERR_ARG, "%s: null tensor", who);
+  MOC_REQUIRE(a.q && a.k && a.v && a.out && a.dout && a.lse && (a.dq || a.dk), MOC_ERR_ARG, "%s: null tensor", who);
   MOC_REQUIRE(!a.dk == !a.dv, MOC_ERR_ARG, "%s: dk and dv together or neither", who);
   // the rows of a step of dk, dv are read through one bounded buffer with 32-bit offsets
   const int64_t es = dtype_size(args->dtype);

@@ -1947,17 +1947,17 @@ class _CrossAttention(torch.autograd.Function):
             return (*(torch.zeros(t.shape, device=dev, dtype=t.dtype) if n else None for t, n in zip((q, k, v), need)), None,
                     None, None)
         dout = _attn_rows(dout, False)
-        dq, dk, dv = _contiguous_like(q), None, None
+        dq, dk, dv = _contiguous_like(q) if need[0] else None, None, None
         if need[1] or need[2]:
             dk, dv = _contiguous_like(k), _contiguous_like(v)
         with L.on_device(dev):
             nbytes = _cross_bwd_workspace(B, Lq, N, H, HK, D, dt)
             ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
             call("moc_cross_bwd", _pack_cross(q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(),
-                                              ptr0(low), dq.data_ptr(), ptr0(dk), ptr0(dv), lse.data_ptr(), ptr0(lengths),
+                                              ptr0(low), ptr0(dq), ptr0(dk), ptr0(dv), lse.data_ptr(), ptr0(lengths),
                                               ptr0(words), *_strides3(q), *_strides3(k), *_strides3(v), *_strides3(dout), B,
                                               Lq, N, H, HK, D, dt, ctx.scale), ptr(ws), nbytes, stream_ptr(dev))
-        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None
+        return dq, dk if need[1] else None, dv if need[2] else None, None, None, None
 
 
 def _key_words(key_mask, lengths, B: int, N: int):

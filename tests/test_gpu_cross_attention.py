@@ -454,3 +454,35 @@ def test_module_float16(gpu_device):
     mem = torch.randn(2, 20, 96, generator=gen(19)).half().to(gpu_device)
     out, _ = m(h, mem, memory_lengths=torch.tensor([20, 4], device=gpu_device))
     assert out.dtype == torch.float16 and torch.isfinite(out).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("shape", [(1, 4, 4, 2, 2, 64), (2, 200, 333, 4, 2, 64), (1, 30, 3000, 8, 2, 128), (3, 150, 150, 2, 1, 128)])
+def test_backward_entry_without_some_gradients(gpu_device, shape, dt):
+    """moc_cross_bwd gives dq alone, or dk and dv alone, to the bit of all three; it writes nothing else."""
+    from memory_amd import _lib as L
+    from memory_amd import ops
+    B, Lq, N, H, HK, D = shape
+    q, k, v, do = inputs(*shape, dt, gpu_device, seed=20)
+    out, low, lse = ops._cross_forward(q, k, v, None, None, D ** -0.5, True)
+    code = L.dtype_code(dt)
+    nbytes = L.query("moc_cross_bwd_workspace", B, Lq, N, H, HK, D, code)
+
+    def grads(want_q, want_kv):
+        g = [torch.full_like(q, 7.0) if want_q else None, *(torch.full_like(k, 7.0) if want_kv else None for _ in range(2))]
+        ws = torch.full((nbytes,), 0xff, device=gpu_device, dtype=torch.uint8)
+        L.call("moc_cross_bwd", ops._pack_cross(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), do.data_ptr(), out.data_ptr(), ops.ptr0(low), *map(ops.ptr0, g), lse.data_ptr(),
+            0, 0, *ops._strides3(q), *ops._strides3(k), *ops._strides3(v), *ops._strides3(do), B, Lq, N, H, HK, D, code, D ** -0.5),
+            ws.data_ptr(), nbytes, L.stream_ptr(gpu_device))
+        return g
+
+    whole = grads(True, True)
+    ref, bound = reference(q, k, v, None, do)
+    for name, x, a, b in zip(("dq", "dk", "dv"), whole, ref[1:], bound[1:]):
+        close(x, a, b, name)
+    only_q, only_kv = grads(True, False), grads(False, True)
+    assert torch.equal(only_q[0], whole[0]) and torch.equal(only_kv[1], whole[1]) and torch.equal(only_kv[2], whole[2])
+    with pytest.raises(ValueError, match="null"):
+        grads(False, False)
