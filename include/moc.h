@@ -854,7 +854,7 @@ typedef struct {
   int64_t qb, ql, qh, kb, kn, kh, vb, vn, vh, db, dl, dh; /* d: of dout */
   int64_t B, L, N;
   int H, HK, D, dtype;
-  float scale; /* > 0 */
+  float scale; /* > 0, < 2^127 */
 } moc_cross_args;
 int64_t moc_cross_rows(int64_t L, int H, int HK);
 size_t moc_cross_fwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtype);

@@ -306,7 +306,8 @@ int ca_check(const char* who, const moc_cross_args* p, CaArgs* c) {
   const int64_t G = a.H / a.HK, es = dtype_size(a.dtype);
   MOC_REQUIRE(a.L * G < (int64_t)1 << 30 && a.N < (int64_t)1 << 30 && a.B < (int64_t)1 << 24, MOC_ERR_UNSUPPORTED,
               "%s: sizes B=%lld L=%lld N=%lld", who, (long long)a.B, (long long)a.L, (long long)a.N);
-  MOC_REQUIRE(a.scale > 0.f && a.scale <= 3.4028234e38f, MOC_ERR_ARG, "%s: scale must be positive and finite", who);
+  // (scale log2(e) is finite then: a logit of 0 stays 0)
+  MOC_REQUIRE(a.scale > 0.f && a.scale < 0x1p127f, MOC_ERR_ARG, "%s: scale must be positive and less than 2^127", who);
   const int64_t st[] = {a.qb, a.ql, a.qh, a.kb, a.kn, a.kh, a.vb, a.vn, a.vh, a.db, a.dl, a.dh};
   for (int64_t s : st)
     MOC_REQUIRE(s >= 0 && s * es % 16 == 0, MOC_ERR_ARG, "%s: strides must be multiples of 16 bytes", who);

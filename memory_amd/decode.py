@@ -634,8 +634,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, *, causal: bool = Fals
     if len(shape) not in (3, 4) or shape[0] != B or shape[-1] != D or shape[-2] == 0 or shape[-2] % HK:
         raise ValueError(f"queries of shape {tuple(q.shape)}: expected ({B}, [tokens,] heads, {D}) with heads a multiple of {HK}")
     scale = float(D) ** -0.5 if softmax_scale is None else float(softmax_scale)
-    if not 0.0 < scale < 3e38:
-        raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
+    if not 0.0 < scale < 2.0 ** 127:
+        raise ValueError(f"softmax_scale must be positive and less than 2^127, got {softmax_scale}")
     if not q.is_floating_point():
         raise ValueError(f"queries of {q.dtype}")
     L.require_same_gpu(cache.k_pages, q)

@@ -1977,7 +1977,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     values: keys where it is False do not.  Keys that do not count may hold anything (NaN too) and get gradient 0; a
     sequence none of whose keys counts has result 0 and gives no gradient.  D is 64 or 128, L and N any; float32 or
     bfloat16 of one type (float16 runs as float32), with any strides (rows that are not 16-byte pieces are copied).
-    ``softmax_scale`` > 0, default D^-0.5.  Logits, sums and the running maximum are float32; in bfloat16 the
+    ``softmax_scale`` > 0 (and < 2^127), default D^-0.5.  Logits, sums and the running maximum are float32; in bfloat16 the
     probabilities enter their products rounded to it.  Differentiable once in q, k and v."""
     if k.dim() == 3 and v.dim() == 3:
         k, v = k.expand(q.shape[0], *k.shape), v.expand(q.shape[0], *v.shape)
@@ -1993,8 +1993,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     if q.dtype != k.dtype or q.dtype != v.dtype or not q.is_floating_point():
         raise ValueError(f"q, k and v of one floating-point type, got {q.dtype}, {k.dtype}, {v.dtype}")
     scale = float(D) ** -0.5 if softmax_scale is None else float(softmax_scale)
-    if not 0.0 < scale < 3e38:
-        raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
+    if not 0.0 < scale < 2.0 ** 127:
+        raise ValueError(f"softmax_scale must be positive and less than 2^127, got {softmax_scale}")
     L.require_same_gpu(q, k, v, kv_lengths, key_mask)
     if H * D >= 1 << 20 or HK * D >= 1 << 20:
         raise ValueError(f"{H} heads of {D}: rows of a million elements or more are not taken")

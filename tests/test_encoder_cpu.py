@@ -219,3 +219,21 @@ def test_pages_without_a_table():
         with pytest.raises(ValueError, match="null"):
             heads(**kw)
     heads(B=0, table=0)     # (no sequences: nothing is launched)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 127, 2.5e38])
+def test_scales_that_overflow_in_base_two(scale):
+    """scale log2(e) past float32 would make NaN of logits of 0."""
+    from memory_amd import _lib as L
+    from memory_amd import ops
+    from memory_amd.decode import PagedKVCache, paged_attention
+    with pytest.raises(ValueError, match="softmax_scale"):
+        ops.cross_attention(rnd(2, 3, 4, 64), rnd(2, 5, 2, 64), rnd(2, 5, 2, 64), softmax_scale=scale)
+    cache = PagedKVCache.__new__(PagedKVCache)
+    cache._sizes = (4, 16, 2, 64, 2, 2)
+    with pytest.raises(ValueError, match="softmax_scale"):
+        paged_attention(rnd(2, 4, 64), cache, softmax_scale=scale)
+    args = ops._pack_cross(16, 16, 16, 16, 16, 0, 16, 16, 16, 16, 0, 0, 0, 256, 64, 0, 128, 64, 0, 128, 64, 0, 256, 64, 1, 3, 5, 4,
+                           2, 64, L.MOC_BF16, scale)
+    with pytest.raises(ValueError, match="scale"):
+        L.call("moc_cross_fwd", args, None, 0, None)

@@ -486,3 +486,16 @@ def test_backward_entry_without_some_gradients(gpu_device, shape, dt):
     assert torch.equal(only_q[0], whole[0]) and torch.equal(only_kv[1], whole[1]) and torch.equal(only_kv[2], whole[2])
     with pytest.raises(ValueError, match="null"):
         grads(False, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L", [1, 200])
+def test_largest_scale(gpu_device, L):
+    """Logits of 0 under the largest scale: the mean of the values."""
+    from memory_amd import ops
+    q, k, v, _ = inputs(1, L, 5, 2, 1, 64, F32, gpu_device, seed=21)
+    with torch.no_grad():
+        o = ops.cross_attention(q, k * 0, v, softmax_scale=1.7e38)
+    ref = v.double().mean(1, keepdim=True).expand_as(o)
+    # (five probabilities and their sum, each exact but for the division, and five products and additions)
+    assert ((o.double() - ref).abs() <= 16 * U * v.double().abs().mean(1, keepdim=True)).all()
