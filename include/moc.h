@@ -843,7 +843,8 @@ int moc_gated_norm_bwd(const moc_gated_norm* a, const moc_gated_norm_grads* g, v
  * out, dq [B][L][H][D] and dk, dv [B][N][HK][D] contiguous.  lengths i32 [B] or NULL: keys from lengths[b] on do not
  * count (values are clamped to 0 .. N).  words u64 [B][ceil(N / 64)] or NULL: bit j of word t says whether key 64 t + j
  * counts (moc_key_words, which takes lengths in).  Keys that do not count may hold anything; rows without keys are 0 and
- * give no gradient.  lse f32 [B][HK][moc_cross_rows]: log2-domain log-sum-exp for the backward (forward: may be NULL).
+ * give no gradient.  lse f32 [B][HK][moc_cross_rows]: what the backward needs of the rows' logits, as the forward wrote it
+ * (forward: may be NULL).  Scaled logits of bf16 calls of more than 128 rows and keys must stay below 2^30.
  * out_low (bf16, as out, or NULL): what out's rounding left over, rounded; the backward's row sums dO . out take it in. */
 typedef struct {
   const void *q, *k, *v, *dout;

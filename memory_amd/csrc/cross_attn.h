@@ -50,7 +50,8 @@ __device__ __forceinline__ f32x4 ca_mma(const f32x8& a, const f32x8& b, const f3
   return x;
 }
 
-// s c - off; EXACT rounds the product by itself, so that a row's largest logit has exactly 2^0
+// s c - off; EXACT rounds the product by itself, so that a row's largest logit has exactly 2^0.  Fused, half a step of the
+// logit is left in the exponent: the same of a key's in the forward and the backward, so it cancels against the row's sum
 template <bool EXACT>
 __device__ __forceinline__ float ca_logit(float s, float c, float off) {
   if constexpr (EXACT) {
@@ -152,11 +153,18 @@ struct CaKeys {
 // heads and 10,813 keys: forward 45 -> 37 us and backward 117 -> 91 in bf16, 152 -> 92 and 326 -> 252 in float32).
 constexpr int kCaFew = 128;
 
+// Of each row the backward takes the reference of its logits (log2 units: their maximum, or less by up to kCaSlack) and
+// one over the sum of 2^(logit - reference).  In one number, reference + log2(sum), the logarithm's lower bits are lost
+// under a large logit, and where one key takes a row so is what the fused product leaves of it: dv was off by 8e-5 at
+// logits of 4,096 (float32), by 0.005 at 2^18 and by 0.4 at 2^24.  Partial results keep the two apart as well.
+// stats: [B][HK][2][Lp], the references (+inf in rows without keys, and behind the last) and the factors (0 there).
+__device__ __forceinline__ size_t ca_stat(size_t bh, int Lp, int r) { return 2 * bh * Lp + r; }
+
 // What a launch works on (moc_cross_args with the derived sizes)
 struct CaArgs {
   const void *q, *k, *v, *dout;
   void *out, *out_low, *dq, *dk, *dv;
-  float *lse, *ndelta, *part, *part_lse;
+  float *stats, *ndelta, *part, *part_m, *part_l;
   const int32_t* lengths;
   const uint64_t* words;
   int64_t qb, ql, qh, kb, kn, kh, vb, vn, vh, db, dl, dh;   // element strides
@@ -207,7 +215,7 @@ __device__ __forceinline__ T ca_low(float x, T rounded) { return from_f<T>(x - t
 inline bool ca_few(const CaArgs& a) { return a.N <= kCaFew || a.rows <= kCaFew; }
 
 int ca_check(const char* who, const moc_cross_args* a, CaArgs* c);
-// out (and lse) of a.nsplit partial results a.part, a.part_lse over rows [B][HK][Lp]
+// out (and stats) of a.nsplit partial results over rows [B][HK][Lp]: sums a.part, references a.part_m, row sums a.part_l
 int ca_merge(int dtype, int D, const CaArgs& a, hipStream_t stream);
 
 }  // namespace moc

@@ -1,5 +1,5 @@
 // Attention over keys and values of another length, backward (notation of cross_attn.h).
-//   P_ij = 2^(scale log2(e) q_i . k_j - lse_i),  delta_i = dO_i . o_i,  dS_ij = P_ij (dO_i . v_j - delta_i)
+//   P_ij = 2^(scale log2(e) q_i . k_j - m_i) / l_i,  delta_i = dO_i . o_i,  dS_ij = P_ij (dO_i . v_j - delta_i)
 //   dq_i = scale sum_j dS_ij k_j,   dk_j = scale sum_i dS_ij q_i,   dv_j = sum_i P_ij dO_i
 // delta takes the result before its rounding (out + out_low): where few keys share a row's weight, dO . v_j and delta
 // nearly cancel, and out's 2^-9 alone made dq and dk twice as inexact as everything else.
@@ -7,9 +7,10 @@
 // -delta behind; dk and dv run over the rows of a block of keys, so nothing is summed by atomics and every result has
 // one order.  P and dS enter their products rounded to the operands' type; sums, P itself and delta are f32.
 //
-// Measured (dq; dk and dv): 69 and 90 us for 8 x 1,024 rows of 12 heads of 64 over 1,500 ragged keys (640, 655 TFLOP/s),
-// 588 and 864 us for 4 x 2,048 of 32 heads of 128 over 4,097 masked ones (1,000 and 905 of the live keys, of 1,247 in a
-// large product).
+// Measured (dq; dk and dv): 68 and 94 us for 8 x 1,024 rows of 12 heads of 64 over 1,500 ragged keys (650, 630 TFLOP/s),
+// 596 and 881 us for 4 x 2,048 of 32 heads of 128 over 4,097 masked ones (990 and 890 of the live keys, of 1,247 in a
+// large product).  One over l as a number of its own (see ca_stat) costs dk and dv a product per probability: 867 -> 881 us
+// and 88 -> 94; dq, whose rows take it at the end, 1 %.
 #include "cross_attn.h"
 
 namespace moc {
@@ -45,7 +46,7 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
   const int t_end = SPLIT ? (int)((int64_t)nt * (sp + 1) / nsp) : nt;
 
   F8 qf[2][KS], dof[2][KS];
-  float lse[2], dl[2];
+  float ref[2], dl[2];
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
     const int r = r0 + 32 * wave + 16 * qb + c16;
@@ -74,7 +75,7 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
     const float del = __shfl(mine, 16 * (c16 >> 2) + c16, 64);
     const size_t at = ((size_t)b * a.HK + hk) * a.Lp + r;
     dl[qb] = del;
-    lse[qb] = ok ? a.lse[at] : INFINITY;
+    ref[qb] = ok ? a.stats[ca_stat((size_t)b * a.HK + hk, a.Lp, r)] : INFINITY;
     if (g == 0 && sp == 0) a.ndelta[at] = -dl[qb];
   }
   if (!a.dq) return;     // (the queries are not trained: -delta is all that dk needs)
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float ds = ca_exp2(st[kb][qb][e] * c - lse[qb]) * (kSub ? dp[kb][qb][e] - dl[qb] : dp[kb][qb][e]);
+              const float ds = ca_exp2(ca_logit<kSub>(st[kb][qb][e], c, ref[qb])) * (kSub ? dp[kb][qb][e] - dl[qb] : dp[kb][qb][e]);
               dsf[qb][4 * kb + e] = from_f<T>(ds);
               if constexpr (TWO) dsl[qb][4 * kb + e] = ca_low<T>(ds, dsf[qb][4 * kb + e]);
             }
@@ -178,14 +179,15 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int r = r0 + 32 * wave + 16 * qb + 4 * g + e;
+      const float inv = a.stats[ca_stat((size_t)b * a.HK + hk, a.Lp, r) + a.Lp];    // (of one over l, for the whole row)
       if constexpr (SPLIT) {
         float* dst = a.part + ((((size_t)sp * a.B + b) * a.HK + hk) * a.Lp + r) * D;
 #pragma unroll
-        for (int db = 0; db < DB; ++db) dst[16 * db + c16] = acc[qb][db][e];
+        for (int db = 0; db < DB; ++db) dst[16 * db + c16] = inv * acc[qb][db][e];
       } else if (r < a.rows) {
         T* dst = (T*)a.dq + (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D;
 #pragma unroll
-        for (int db = 0; db < DB; ++db) dst[16 * db + c16] = from_f<T>(a.scale * acc[qb][db][e]);
+        for (int db = 0; db < DB; ++db) dst[16 * db + c16] = from_f<T>(a.scale * inv * acc[qb][db][e]);
       }
     }
 }
@@ -213,7 +215,7 @@ __device__ __forceinline__ void dq_sum(const CaArgs& a, int64_t i) {
 // cycles of products and 480 of vector instructions on each SIMD; at 64 dims by the latter two.  A wave's 32 keys set
 // what is read (with 16, 1,196 us; with 64 the sums alone fill the registers).  VL: V stays in LDS, each wave reading
 // its own rows, where with it the registers of two waves per SIMD do not hold (one wave per SIMD: 1,280 us; spilled:
-// 1,330; now 864).
+// 1,330; now 881).
 template <typename T, int D> struct DkvShape;
 template <> struct DkvShape<bf16, 64> { static constexpr int KB = 2, QS = 128, VL = 0, WAVES = 2; };
 template <> struct DkvShape<bf16, 128> { static constexpr int KB = 2, QS = 32, VL = 1, WAVES = 2; };
@@ -232,7 +234,7 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
   using StageV = CaStage<T, D, KEYS, 4>;
   constexpr int VB = kVL ? KEYS * D * (int)sizeof(T) : 16;
   __shared__ __attribute__((aligned(16))) char sQ[2][TB], sD[2][TB], sV[VB];
-  __shared__ __attribute__((aligned(16))) float sL[2][QS], sDl[2][QS];
+  __shared__ __attribute__((aligned(16))) float sM[2][QS], sI[2][QS], sDl[2][QS];
   // what a lane's DMAs of a step need: offsets of its rows in Q and dO, and the rows' heads (out of registers meanwhile)
   __shared__ uint32_t sAt[3 * Stage::IPW][kCaThreads];
   const int nkb = (a.N + KEYS - 1) / KEYS;
@@ -297,7 +299,7 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
   const int nstep = (a.rows + QS - 1) / QS;
   const int s_begin = SPLIT ? (int)((int64_t)nstep * sp / nsp) : 0;
   const int s_end = any == 0 ? s_begin : SPLIT ? (int)((int64_t)nstep * (sp + 1) / nsp) : nstep;
-  const float* lse = a.lse + bh * a.Lp;
+  const float* stats = a.stats + ca_stat(bh, a.Lp, 0);
   const float* ndelta = a.ndelta + bh * a.Lp;
   // Rows of step s: row QS s + r is query l0 + (q0 + r) / G, head (q0 + r) % G of the group, with r = lr G + hr a
   // constant of the lane; so its offset from query l0 is that of (lr, hr), q0 heads on, and a query on where q0 + hr
@@ -335,13 +337,14 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
       q0 -= a.G;
       ++l0;
     }
-    // lse and -delta of the rows, padded to Lp, a multiple of QS, with +inf and 0
+    // reference, factor and -delta of the rows, padded to Lp, a multiple of QS, with +inf, 0 and 0
     if (64 * wave < QS) {
       const bool in = 64 * wave + lane < QS;
       const uint32_t o = in ? 4u * (64 * wave + lane) : kCaOut;
-      const Buf lb = ca_buf(lse + r0, 4 * QS), eb = ca_buf(ndelta + r0, 4 * QS);
+      const Buf mb = ca_buf(stats + r0, 4 * QS), ib = ca_buf(stats + a.Lp + r0, 4 * QS), eb = ca_buf(ndelta + r0, 4 * QS);
       if (in) {
-        ca_dma4(lb.r, o, &sL[buf][64 * wave]);
+        ca_dma4(mb.r, o, &sM[buf][64 * wave]);
+        ca_dma4(ib.r, o, &sI[buf][64 * wave]);
         ca_dma4(eb.r, o, &sDl[buf][64 * wave]);
       }
     }
@@ -369,7 +372,7 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
         F8 pa[KB], sa[KB], pb[KB], sb[KB];
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
-          const f32x4 ls = *reinterpret_cast<const f32x4*>(&sL[buf][r0 + 16 * qb + 4 * g]);
+          const f32x4 ms = *reinterpret_cast<const f32x4*>(&sM[buf][r0 + 16 * qb + 4 * g]);
           const f32x4 nd = *reinterpret_cast<const f32x4*>(&sDl[buf][r0 + 16 * qb + 4 * g]);
           f32x4 st[KB], dp[KB];
 #pragma unroll
@@ -385,11 +388,15 @@ __global__ __launch_bounds__(kCaThreads, (DkvShape<T, D>::WAVES)) void cross_dkv
                 dp[kb] = ca_mma(da, vf[kb][ks], d0);
             }
           }
+          // (read this late the factors take no registers from the products, which FEW does not have to spare: 49 spilled
+          // at 128 dims; the others have, and wait less if the compiler reads them early: 881 us, late 985)
+          if constexpr (FEW) asm volatile("" ::: "memory");
+          const f32x4 is = *reinterpret_cast<const f32x4*>(&sI[buf][r0 + 16 * qb + 4 * g]);
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float pt = ca_exp2(st[kb][e] * c - ls[e]);
+              const float pt = ca_exp2(ca_logit<kSub>(st[kb][e], c, ms[e])) * is[e];
               const float ds = pt * (kSub ? dp[kb][e] + nd[e] : dp[kb][e]);
               pa[kb][4 * qb + e] = from_f<T>(pt);
               sa[kb][4 * qb + e] = from_f<T>(ds);
@@ -561,7 +568,7 @@ int moc_cross_bwd(const moc_cross_args* args, void* workspace, size_t workspace_
   CaArgs a;
   int rc = ca_check(who, args, &a);
   if (rc != MOC_OK) return rc;
-  MOC_REQUIRE(a.q && a.k && a.v && a.out && a.dout && a.lse && (a.dq || a.dk), MOC_ERR_ARG, "%s: null tensor", who);
+  MOC_REQUIRE(a.q && a.k && a.v && a.out && a.dout && a.stats && (a.dq || a.dk), MOC_ERR_ARG, "%s: null tensor", who);
   MOC_REQUIRE(!a.dk == !a.dv, MOC_ERR_ARG, "%s: dk and dv together or neither", who);
   // the rows of a step of dk, dv are read through one bounded buffer with 32-bit offsets
   const int64_t es = dtype_size(args->dtype);

@@ -195,8 +195,8 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
     if (t < t_end) step(std::integral_constant<int, 1>());
   }
 
-  // rows without live keys: 0, and +inf as the backward's log-sum-exp (its probabilities are 0 then), as in the
-  // padding rows up to Lp
+  // rows without live keys: 0, and +inf as the backward's reference (its probabilities are 0 then), as in the padding
+  // rows up to Lp
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
     const float l = lsum[qb];
@@ -206,8 +206,11 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
       const size_t row = (((size_t)sp * a.B + b) * a.HK + hk) * a.Lp + r;
       float* pp = a.part + row * D + 4 * g;
 #pragma unroll
-      for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(pp + 16 * db) = o[db][qb] * inv;
-      if (g == 0) a.part_lse[row] = l == 0.f ? -INFINITY : m[qb] + log2f(l);
+      for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(pp + 16 * db) = o[db][qb];
+      if (g == 0) {
+        a.part_m[row] = m[qb];
+        a.part_l[row] = l;
+      }
     } else {
       if (r < a.rows) {
         const size_t at = (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + 4 * g;
@@ -216,13 +219,17 @@ __global__ __launch_bounds__(kCaThreads) void cross_fwd_kernel(CaArgs a) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) ca_store4<T>(op + 16 * db, lp ? lp + 16 * db : nullptr, o[db][qb] * inv);
       }
-      if (a.lse && g == 0)
-        a.lse[((size_t)b * a.HK + hk) * a.Lp + r] = r >= a.rows || l == 0.f ? INFINITY : m[qb] + log2f(l);
+      if (a.stats && g == 0) {
+        const bool none = r >= a.rows || l == 0.f;
+        float* st = a.stats + ca_stat((size_t)b * a.HK + hk, a.Lp, r);
+        st[0] = none ? INFINITY : m[qb];
+        st[a.Lp] = none ? 0.f : inv;
+      }
     }
   }
 }
 
-// out = sum_i 2^(lse_i - M) o_i / sum_i 2^(lse_i - M) over the splits of a row, and its log-sum-exp: D / 4 lanes of four
+// out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the splits of a row, and its stats: D / 4 lanes of four
 // dims in each of 1024 / D groups.  With few rows all groups of a workgroup share one, each taking every so many
 // splits, joined in LDS: a chain of two loads whatever the number of splits (32 of them one after the other took 7 us,
 // this 3).  With many rows (ALONE) each group has its own, which keeps more loads in flight.
@@ -236,23 +243,28 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(CaArgs a, int64_t nrow
   if (row >= nrow) return;
   const int r = (int)((uint32_t)row % (uint32_t)a.Lp);
   const uint32_t bh = (uint32_t)row / (uint32_t)a.Lp, b = bh / (uint32_t)a.HK, hk = bh - b * a.HK;
+  float* st = a.stats && ch == 0 ? a.stats + ca_stat(bh, a.Lp, r) : nullptr;
   if (r >= a.rows) {
-    if (a.lse && ch == 0) a.lse[row] = INFINITY;
+    if (st && (ALONE || gr == 0)) {
+      st[0] = INFINITY;
+      st[a.Lp] = 0.f;
+    }
     return;
   }
   float M = -INFINITY, den = 0.f;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
   auto take = [&](float d, const f32x4& o, float s) {
-    // (no weight for a split without live keys; a NaN goes through)
+    // (a split without live keys has sums of 0, one of NaN logits alone NaN: both go through with the weight 1)
     const float m = fmax_fast(M, d);
-    const float w = d == -INFINITY ? 0.f : ca_exp2(d - m), f = M == -INFINITY ? 0.f : ca_exp2(M - m);
+    const float w = d == -INFINITY ? 1.f : ca_exp2(d - m), f = M == -INFINITY ? 1.f : ca_exp2(M - m);
     acc = acc * f + o * w;
     den = den * f + s * w;
     M = m;
   };
 #pragma unroll 4
   for (int s = ALONE ? 0 : gr; s < a.nsplit; s += ALONE ? 1 : GR)
-    take(a.part_lse[s * nrow + row], *reinterpret_cast<const f32x4*>(a.part + (s * nrow + row) * D + 4 * ch), 1.f);
+    take(a.part_m[s * nrow + row], *reinterpret_cast<const f32x4*>(a.part + (s * nrow + row) * D + 4 * ch),
+         a.part_l[s * nrow + row]);
   if constexpr (!ALONE) {
     if (ch == 0) {
       sM[gr] = M;
@@ -267,7 +279,10 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(CaArgs a, int64_t nrow
   const float inv = den == 0.f ? 0.f : 1.f / den;
   const size_t at = (((size_t)b * a.L + r / a.G) * a.H + hk * a.G + r % a.G) * D + 4 * ch;
   ca_store4<T>((T*)a.out + at, a.out_low ? (T*)a.out_low + at : nullptr, acc * inv);
-  if (a.lse && ch == 0) a.lse[row] = den == 0.f ? INFINITY : M + log2f(den);
+  if (st) {
+    st[0] = den == 0.f ? INFINITY : M;
+    st[a.Lp] = inv;
+  }
 }
 
 // words[b][t]: the live keys of tile t, from one byte per key and the sequence's length; a wave per word
@@ -321,7 +336,7 @@ int ca_check(const char* who, const moc_cross_args* p, CaArgs* c) {
   CaArgs& o = *c;
   o = CaArgs{};
   o.q = a.q; o.k = a.k; o.v = a.v; o.out = a.out; o.out_low = a.dtype == MOC_BF16 ? a.out_low : nullptr; o.dout = a.dout;
-  o.dq = a.dq; o.dk = a.dk; o.dv = a.dv; o.lse = a.lse; o.lengths = a.lengths; o.words = a.words;
+  o.dq = a.dq; o.dk = a.dk; o.dv = a.dv; o.stats = a.lse; o.lengths = a.lengths; o.words = a.words;
   o.qb = a.qb; o.ql = a.ql; o.qh = a.qh; o.kb = a.kb; o.kn = a.kn; o.kh = a.kh; o.vb = a.vb; o.vn = a.vn; o.vh = a.vh;
   o.db = a.db; o.dl = a.dl; o.dh = a.dh;
   o.B = (int)a.B; o.L = (int)a.L; o.N = (int)a.N; o.H = a.H; o.HK = a.HK; o.G = (int)G;
@@ -378,13 +393,13 @@ extern "C" {
 
 int64_t moc_cross_rows(int64_t L, int H, int HK) {
   if (HK <= 0 || L <= 0) return 0;
-  return (L * (H / HK) + kCaRows - 1) / kCaRows * kCaRows;
+  return 2 * ((L * (H / HK) + kCaRows - 1) / kCaRows * kCaRows);
 }
 
 size_t moc_cross_fwd_workspace(int64_t B, int64_t L, int64_t N, int H, int HK, int D, int dtype) {
-  const int64_t Lp = moc_cross_rows(L, H, HK);
+  const int64_t Lp = moc_cross_rows(L, H, HK) / 2;
   const int s = ca_fwd_splits(B * HK * (Lp / kCaRows), (N + kCaKeys - 1) / kCaKeys, dtype);
-  return s == 1 ? 0 : (size_t)s * B * HK * Lp * (D + 1) * 4;
+  return s == 1 ? 0 : (size_t)s * B * HK * Lp * (D + 2) * 4;
 }
 
 int moc_cross_fwd(const moc_cross_args* args, void* workspace, size_t workspace_bytes, hipStream_t stream) {
@@ -398,7 +413,8 @@ int moc_cross_fwd(const moc_cross_args* args, void* workspace, size_t workspace_
   MOC_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), MOC_ERR_ARG, "moc_cross_fwd: workspace of %zu bytes, needs %zu",
               workspace_bytes, need);
   a.part = (float*)workspace;
-  a.part_lse = a.part + (size_t)a.nsplit * bhl * args->D;
+  a.part_m = a.part + (size_t)a.nsplit * bhl * args->D;
+  a.part_l = a.part_m + (size_t)a.nsplit * bhl;
   if (args->dtype == MOC_BF16) return args->D == 64 ? fwd_launch<bf16, 64>(a, stream) : fwd_launch<bf16, 128>(a, stream);
   return args->D == 64 ? fwd_launch<float, 64>(a, stream) : fwd_launch<float, 128>(a, stream);
 }

@@ -236,8 +236,11 @@ __global__ __launch_bounds__(64 * kKdWaves) void kv_decode_kernel(KdArgs p) {
       if (rr >= a.rows) continue;
       if constexpr (SPLIT) {
         const size_t at = (((size_t)sp * a.B + b) * a.HK + hk) * a.Lp + rr;
-        *reinterpret_cast<f32x4*>(a.part + at * D + d0) = acc * inv;
-        if (d0 == 0) a.part_lse[at] = den == 0.f ? -INFINITY : Mr + log2f(den);
+        *reinterpret_cast<f32x4*>(a.part + at * D + d0) = acc;
+        if (d0 == 0) {
+          a.part_m[at] = Mr;
+          a.part_l[at] = den;
+        }
       } else {
         T* op = (T*)a.out + (((size_t)b * a.L + rr / a.G) * a.H + hk * a.G + rr % a.G) * D + d0;
         ca_store4<T>(op, nullptr, acc * inv);
@@ -296,7 +299,7 @@ size_t moc_kv_decode_workspace(int64_t B, int64_t L, int64_t n_max, int H, int H
   if (HK <= 0) return 0;
   const int64_t rows = L * (H / HK), per = 16 * kd_row_blocks(rows, D, dtype), nrb = (rows + per - 1) / per;
   const int s = kd_splits(B * HK * nrb, n_max, D * dtype_size(dtype));
-  return s == 1 ? 0 : (size_t)s * B * HK * rows * (D + 1) * 4;
+  return s == 1 ? 0 : (size_t)s * B * HK * rows * (D + 2) * 4;
 }
 
 int moc_kv_decode(const moc_kv_decode_args* d, void* workspace, size_t workspace_bytes, hipStream_t stream) {
@@ -326,13 +329,14 @@ int moc_kv_decode(const moc_kv_decode_args* d, void* workspace, size_t workspace
   const int rb = kd_row_blocks(p.c.rows, x.D, x.dtype);
   p.nrb = (p.c.rows + 16 * rb - 1) / (16 * rb);
   p.c.Lp = p.c.rows;     // (of the partial results)
-  p.c.lse = nullptr;
+  p.c.stats = nullptr;
   p.c.nsplit = kd_splits((int64_t)p.c.B * p.c.HK * p.nrb, p.c.N, x.D * dtype_size(x.dtype));
   const size_t need = moc_kv_decode_workspace(x.B, x.L, x.N, x.H, x.HK, x.D, x.dtype);
   MOC_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), MOC_ERR_ARG, "%s: workspace of %zu bytes, needs %zu", who,
               workspace_bytes, need);
   p.c.part = (float*)workspace;
-  p.c.part_lse = p.c.part + (size_t)p.c.nsplit * p.c.B * p.c.HK * p.c.Lp * x.D;
+  p.c.part_m = p.c.part + (size_t)p.c.nsplit * p.c.B * p.c.HK * p.c.Lp * x.D;
+  p.c.part_l = p.c.part_m + (size_t)p.c.nsplit * p.c.B * p.c.HK * p.c.Lp;
   if (x.dtype == MOC_BF16)
     return x.D == 64 ? kd_launch<bf16, 64>(p, paged, rb, stream) : kd_launch<bf16, 128>(p, paged, rb, stream);
   return x.D == 64 ? kd_launch<float, 64>(p, paged, rb, stream) : kd_launch<float, 128>(p, paged, rb, stream);

@@ -1885,7 +1885,7 @@ def _strides3(t: torch.Tensor):
 
 @functools.lru_cache(maxsize=1024)
 def _cross_sizes(B: int, Lq: int, N: int, H: int, HK: int, D: int, dt: int):
-    """(bytes of the forward's workspace, rows of its log-sum-exp)"""
+    """(bytes of the forward's workspace, numbers that it keeps for the backward per sequence and kv head)"""
     return L.query("moc_cross_fwd_workspace", B, Lq, N, H, HK, D, dt), L.query("moc_cross_rows", Lq, H, HK)
 
 
@@ -1978,7 +1978,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     sequence none of whose keys counts has result 0 and gives no gradient.  D is 64 or 128, L and N any; float32 or
     bfloat16 of one type (float16 runs as float32), with any strides (rows that are not 16-byte pieces are copied).
     ``softmax_scale`` > 0 (and < 2^127), default D^-0.5.  Logits, sums and the running maximum are float32; in bfloat16 the
-    probabilities enter their products rounded to it.  Differentiable once in q, k and v."""
+    probabilities and their gradients enter their products rounded to it, in calls of at most 128 keys or rows of a kv head
+    (L x H / HK) in two pieces, 16 bits.  (Scaled logits of larger bfloat16 calls must stay below 2^30.)  Differentiable
+    once in q, k and v."""
     if k.dim() == 3 and v.dim() == 3:
         k, v = k.expand(q.shape[0], *k.shape), v.expand(q.shape[0], *v.shape)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:

@@ -499,3 +499,55 @@ def test_largest_scale(gpu_device, L):
     ref = v.double().mean(1, keepdim=True).expand_as(o)
     # (five probabilities and their sum, each exact but for the division, and five products and additions)
     assert ((o.double() - ref).abs() <= 16 * U * v.double().abs().mean(1, keepdim=True)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("power", [6, 12, 18, 24])
+@pytest.mark.parametrize("B,L,N,copies,apart", [(1, 40, 60, 1, 1), (2, 300, 400, 1, 1), (1, 300, 400, 4, 1), (1, 7, 5000, 1, 1),
+                                                (1, 1, 200, 2, 1), (1, 300, 400, 3, 130), (1, 7, 5000, 5, 999), (1, 1, 5000, 3, 7),
+                                                (1, 130, 5000, 3, 1200)])
+def test_one_key_takes_a_row(gpu_device, B, L, N, copies, apart, power, dt):
+    """Logits of up to 2^power with one key, or equal copies of it ``apart`` keys from each other, far above the others (by
+    more than 2^7, at 2^6 x 4): the weights are 1 / copies and 0, whatever the logits' own rounding.
+      out  the copies' mean value (copies roundings of float32, then the result's), dv sum_i dO_i / copies (L + 64 of
+           float32, then the weights' 2^-8 in bfloat16 calls of many rows and keys, and the result's),
+      dq, dk of one copy: 0 up to what dP - delta, both sums of D terms, leaves of them: 2 (D + 8 + copies) u
+           sum_d |dO_d v_d| (and 2^-16 of it in bfloat16: out's low piece) times scale |k|, |q|."""
+    from memory_amd import ops
+    D = 64
+    g = gen(22)
+    at = apart * torch.arange(copies)
+    u = torch.sign(torch.randn(D, generator=g))
+    q = (u * 2.0 ** ((power - 3) // 2)).expand(B, L, 1, D).contiguous()
+    k = torch.randn(B, N, 1, 1, generator=g).clamp(-1, 1) * u * 2.0 ** ((power - 3) // 2) / 64
+    k[:, at] = u * 2.0 ** (power - 3 - (power - 3) // 2) * (1 if power > 6 else 4)
+    v, do = torch.randn(B, N, 1, D, generator=g), torch.randn(B, L, 1, D, generator=g)
+    q, k, v, do = (x.to(dt).to(gpu_device) for x in (q, k, v, do))
+    s = (q[0, :1, 0].double() @ k[0, :, 0].double().t().contiguous())[0] / 8
+    rest = torch.ones(N, dtype=torch.bool)
+    rest[at] = False
+    assert (s[at] == s.max()).all() and s.max() - s[rest].max() > 128
+    q, k, v = (x.requires_grad_(True) for x in (q, k, v))
+    o = ops.cross_attention(q, k, v)
+    with torch.no_grad():
+        served = ops.cross_attention(q, k, v)
+    dq, dk, dv = torch.autograd.grad(o, [q, k, v], do)
+    t = 2.0 ** -24 if dt == F32 else 2.0 ** -8
+    r = 2.0 ** -8 if dt == BF and min(N, L) > 128 else 0.0 if dt == F32 else 2.0 ** -16
+    vd, dod = v.detach().double(), do.double()
+    mean, mag = vd[:, at].mean(1, keepdim=True), vd[:, at].abs().mean(1, keepdim=True)
+    for name, x in (("out", o.detach()), ("served", served)):
+        close(x, mean.expand_as(o), (t * mean.abs() + (2 * copies + 64) * U * mag).expand_as(o), name)
+    want, bound = torch.zeros_like(vd), torch.zeros_like(vd)
+    want[:, at] = dod.sum(1, keepdim=True) / copies
+    bound[:, at] = (t * dod.sum(1, keepdim=True).abs() + (r + (L + 64) * U) * dod.abs().sum(1, keepdim=True)) / copies
+    close(dv, want, bound, "dv")
+    if copies == 1:
+        noise = (2 * (D + 8 + copies) * U + (2.0 ** -16 if dt == BF else 0.0))
+        left = noise * (dod.abs() * vd[:, :1].abs()).sum(-1, keepdim=True)          # (B, L, 1, 1)
+        close(dq, torch.zeros_like(dod), left / 8 * k.detach().double()[:, :1].abs(), "dq")
+        close(dk[:, :1], torch.zeros_like(vd[:, :1]), (left / 8 * q.detach().double().abs()).sum(1, keepdim=True), "dk")
+        assert (dk[:, 1:] == 0).all()
+        if dt == F32 or min(N, L) <= 128:
+            assert (dq == 0).all() and (dk == 0).all()
