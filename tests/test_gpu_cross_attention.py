@@ -551,3 +551,16 @@ def test_one_key_takes_a_row(gpu_device, B, L, N, copies, apart, power, dt):
         assert (dk[:, 1:] == 0).all()
         if dt == F32 or min(N, L) <= 128:
             assert (dq == 0).all() and (dk == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("shape", [(2, 7, 1, 8, 2, 64), (1, 300, 1, 4, 1, 128), (3, 150, 1, 2, 2, 64), (1, 1, 1, 1, 1, 128)])
+def test_single_key(gpu_device, shape, dt):
+    """Over one key the result is its value to the bit, and dq and dk are exactly 0 (dP and delta are one sum, formed
+    alike), not its rounding."""
+    q, k, v, do = inputs(*shape, dt, gpu_device, seed=23, train=True)
+    o, dq, dk, dv = check(q, k, v, do)
+    G = shape[3] // shape[4]
+    assert torch.equal(o, v.detach().repeat_interleave(G, 2).expand_as(o))
+    assert (dq == 0).all() and (dk == 0).all()
