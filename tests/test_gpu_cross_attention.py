@@ -564,3 +564,22 @@ def test_single_key(gpu_device, shape, dt):
     G = shape[3] // shape[4]
     assert torch.equal(o, v.detach().repeat_interleave(G, 2).expand_as(o))
     assert (dq == 0).all() and (dk == 0).all()
+
+
+@pytest.mark.gpu
+def test_sublayer_attention_alone(gpu_device):
+    """What MemorySublayer adds to the residual, against the attention's own largest value: four chained products of at
+    most 256 terms and the attention, (512 + 8) u each at worst (1.2e-4), and the rounding of the sum."""
+    from memory_amd.memory_block import MemorySublayer
+    torch.manual_seed(4)
+    s = MemorySublayer(256, 4, 2, memory_dim=96, wo_init_zero=False, qk_norm=True, rotary_dim=64).to(gpu_device)
+    h = torch.randn(2, 11, 256, generator=gen(24)).to(gpu_device)
+    mem = torch.randn(2, 37, 96, generator=gen(25)).to(gpu_device)
+    lens = torch.tensor([37, 5], device=gpu_device)
+    with torch.no_grad():
+        out = s(h, mem, memory_lengths=lens).double()
+    hd = h.double()
+    normed = hd * (hd.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    live = torch.arange(37, device=gpu_device)[None] < lens[:, None]
+    ref = _module_reference(s.memory_attn, normed, mem, live)
+    assert ((out - hd - ref).abs() <= 1.2e-4 * ref.abs().max() + U * out.abs()).all()
