@@ -15,9 +15,9 @@
 
 namespace moc {
 
-// dq (bound as the forward is): one workgroup = 128 rows of one (sequence, kv head) as in the forward, K and V tiles double-buffered; K^T for
-// dS K is read from the K tile with the transposing LDS read.  A tile's 64 keys go in two halves, which halves the
-// score registers.  With SPLIT each of nsplit workgroups takes a share of the keys and writes f32 rows.
+// dq (bound as the forward is): one workgroup = 128 rows of one (sequence, kv head) as in the forward, K and V tiles
+// double-buffered; K^T for dS K is read from the K tile with the transposing LDS read.  A tile's 64 keys go in two halves,
+// which halves the score registers.  With SPLIT each of nsplit workgroups takes a share of the keys and writes f32 rows.
 template <typename T, int D, bool SPLIT, bool FEW>
 __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
   typedef typename Frag<T>::type F8;
@@ -55,8 +55,9 @@ __global__ __launch_bounds__(kCaThreads) void cross_dq_kernel(CaArgs a) {
     const T* qp = (const T*)a.q + b * a.qb + l * a.ql + h * a.qh;
     const T* dp = (const T*)a.dout + b * a.db + l * a.dl + h * a.dh;
     const size_t oat = (((size_t)b * a.L + l) * a.H + h) * D;
-    // delta is formed as dP is, by the matrix cores and in their order: the diagonal of dO o^T.  A row that one key
-    // takes whole (o = v) then has dP = delta to the bit, and no gradient.
+    // delta is formed as dP is, by the matrix cores and in their order: the diagonal of dO o^T.  With kSub a row that one
+    // key takes whole (o = v) then has dP = delta to the bit, and no gradient; where dP's sum starts from -delta it is left
+    // with that sum's roundings, some 2^-24 |dO| |v|.
     f32x4 dd = f32x4{0.f, 0.f, 0.f, 0.f}, dlow = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {

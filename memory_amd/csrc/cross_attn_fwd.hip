@@ -7,13 +7,15 @@
 // the rounded P.  Keys that do not count are fetched as zeros (whatever their memory holds) and their logits
 // start from -inf; tiles without live keys are passed over.  Few workgroups split the keys between them.
 //
-// Bound by products and vector instructions, which take turns on a SIMD: of 2 x 64 keys x 32 rows of 128 dims a
-// wave issues 68 products (1,088 cycles), 32 exponentials (512) and some 330 cycles of other vector
-// instructions; LDS is busy for 1,024 cycles per workgroup beside that.  Measured: 57 us for 8 x 1,024 rows of 12
-// heads of 64 over 1,500 ragged keys (520 TFLOP/s; its workgroups are one round of the card, as long as the longest
-// sequence), 458 us for 4 x 2,048 of 32 heads of 128 over 4,097 masked ones (850 TFLOP/s of the live keys, of 1,247 in
-// a large product), 85 + 7 us for one prompt of 509 rows, 16 heads on 4, over 16,001 keys (780).  Not kept: the next
-// tile's scores formed beside this one's exponentials (507 us, with the two interleaved by hand 486: 32 registers
+// Bound by products and vector instructions: of 2 x 64 keys x 32 rows of 128 dims a wave issues 68 products (1,088
+// cycles), 32 exponentials (512) and some 330 cycles of other vector instructions, one after the other; LDS is busy for
+// 1,024 cycles per workgroup beside that.  A SIMD has two waves, of two workgroups (three at 64 dims), which fill each
+// other's gaps only in part: counted over 4 x 2,048 rows of 32 heads of 128 over 4,097 masked keys, the matrix cores are
+// busy for 43 % of all cycles and vector instructions other than products issue in 31 % (dq: 49 and 24 %, dk and dv: 41 and
+// 19 %).  Measured: 56 us for 8 x 1,024 rows of 12 heads of 64 over 1,500 ragged keys (530 TFLOP/s; its workgroups are one
+// round of the card, as long as the longest sequence), 458 us for those of 128 dims above (850 TFLOP/s of the live keys, of
+// 1,247 in a large product), 84 + 7 us for one prompt of 509 rows, 16 heads on 4, over 16,001 keys (790).  Not kept: the
+// next tile's scores formed beside this one's exponentials (507 us, with the two interleaved by hand 486: 32 registers
 // more), waves without rows skipping the work (703: the loop no longer runs on scalars).
 #include "cross_attn.h"
 

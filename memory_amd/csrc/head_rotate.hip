@@ -5,8 +5,8 @@
 // A lane owns eight pairs of a head: with halves rotated elements p .. p + 7 and R / 2 + p .. + 7, with interleaved
 // pairs (and behind the rotated part) sixteen in a row, so a pair never leaves its lane and the norm's sums are over
 // the few neighbouring lanes of the head.  The angles are a token's, not a head's: a workgroup works each one out
-// once (f64 product and reduction: positions of any size keep f32 accuracy; then sin and cos in f32) and its rows
-// read them from LDS.
+// once (f64 product and reduction, whose error of 2^-53 times the position in turns stays below f32's for positions up
+// to 2^28; then sin and cos in f32) and its rows read them from LDS.
 //
 // Measured (forward; backward with the weights' sums): 16 us (62 MB, 3.9 TB/s; a copy of much more runs at 5.2) and 28 + 4
 // for 8,192 + 12,000 rows of 12 heads of 64; 33 us (167 MB, 5.0 TB/s) and 63 + 6 (250 MB, 3.9) for 8,156 rows of 32 and 8

@@ -626,9 +626,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, *, causal: bool = Fals
     """Attention of new tokens over their sequences' pages: q (B, H, D) or several tokens (B, L, H, D) -> the same shape
     in the cache's type.  Each sees the ``cache.lengths`` first keys of its sequence; with ``causal`` token l of L the
     first lengths - L + l + 1 (the tokens are the last ones appended; the values of the newer ones, which it gives no
-    weight, must be finite all the same).  Of those, keys
-    past the table's end or in no page do not exist (appended, they were dropped), and what lies there or behind a sequence's
-    length may be anything.  A token that sees no key gets 0."""
+    weight, must be finite all the same).  Of those, keys past the table's end or in no page do not exist (appended, they
+    were dropped), and what lies there or behind a sequence's length may be anything.  A token that sees no key gets 0."""
     P, page, HK, D, B, most = cache._sizes
     shape = q.shape
     if len(shape) not in (3, 4) or shape[0] != B or shape[-1] != D or shape[-2] == 0 or shape[-2] % HK:

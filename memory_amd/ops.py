@@ -1813,7 +1813,8 @@ def head_norm_rotate(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, 
     ``weight``: (head dim,), or one per head (heads, head dim).  ``inv_freq``: radians per position of the rotated pairs
     (``rope_frequencies``; without it nothing turns), at most head dim / 2, as float64 (other types are converted).  Of
     n frequencies pair p is elements (p, n + p), with ``interleaved`` (2 p, 2 p + 1); elements from 2 n on stay.
-    ``positions``: int32 or int64, (rows,) or (batch, rows); default 0, 1, ...  Angles are formed and reduced in float64.
+    ``positions``: int32 or int64, (rows,) or (batch, rows); default 0, 1, ...  Angles are formed and reduced in float64
+    (positions up to 2^28 keep float32 accuracy).
     x is float32 or bfloat16 (float16 runs as float32), with any strides; everything in between is float32, the result is
     rounded once.  Differentiable once in x and weight."""
     return _heads(x, None, weight, None, eps, norm, positions, None, inv_freq, interleaved)[0]
