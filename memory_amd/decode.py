@@ -533,6 +533,8 @@ class PagedKVCache:
         forward; ``memory_positions`` as there.  A float16 module's pages are float32, as its attention is."""
         if memory.dim() != 3 or memory.shape[0] * memory.shape[1] == 0:
             raise ValueError(f"memory must be (B, N, d) with states, got {tuple(memory.shape)}")
+        if page_size <= 0 or page_size % 16:
+            raise ValueError(f"pages of {page_size} tokens: expected a multiple of 16")
         B, N, _ = memory.shape
         k, v = memory_attn.project_memory(memory, memory_positions)
         per = (N + page_size - 1) // page_size

@@ -237,3 +237,11 @@ def test_scales_that_overflow_in_base_two(scale):
                            2, 64, L.MOC_BF16, scale)
     with pytest.raises(ValueError, match="scale"):
         L.call("moc_cross_fwd", args, None, 0, None)
+
+
+@pytest.mark.parametrize("page_size", [0, -16, 24])
+def test_from_memory_page_size(page_size):
+    from memory_amd.decode import PagedKVCache
+    from memory_amd.memory_attention import MemoryCrossAttention
+    with pytest.raises(ValueError, match="multiple of 16"):
+        PagedKVCache.from_memory(MemoryCrossAttention(256, 4, 2), rnd(1, 3, 256), page_size=page_size)
