@@ -583,3 +583,33 @@ def test_sublayer_attention_alone(gpu_device):
     live = torch.arange(37, device=gpu_device)[None] < lens[:, None]
     ref = _module_reference(s.memory_attn, normed, mem, live)
     assert ((out - hd - ref).abs() <= 1.2e-4 * ref.abs().max() + U * out.abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("L,N", [(1, 40), (1, 5000), (40, 60), (7, 5000), (300, 400), (200, 5000)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_that_are_not_finite_go_through(gpu_device, L, N, bad, dt):
+    """NaN or infinity in a key that counts, alone in its split too, makes NaN of every row of its kv head and of no
+    other; one in a query, of its row; a NaN in a value, of its column."""
+    from memory_amd import ops
+    q, k, v, do = inputs(2, L, N, 4, 2, 64, dt, gpu_device, seed=26)
+    q = q.abs()
+    k[0, N - 1, 0] = bad          # (every term of its logits is NaN or +inf)
+    q[1, L // 2, 3, 5] = float("nan")
+    v[1, N // 2, 0, 9] = float("nan")
+    q, k, v = (x.requires_grad_(True) for x in (q, k, v))
+    with torch.no_grad():
+        served = ops.cross_attention(q, k, v)
+    trained = ops.cross_attention(q, k, v)
+    want = torch.zeros(2, L, 4, 64, dtype=torch.bool, device=gpu_device)
+    want[0, :, :2] = True
+    want[1, L // 2, 3] = True
+    want[1, :, :2, 9] = True
+    for name, o in (("served", served), ("trained", trained.detach())):
+        assert torch.equal(torch.isnan(o), want), name
+    dq, dk, dv = torch.autograd.grad(trained, [q, k, v], do)
+    assert torch.isnan(dq[0, :, :2]).all() and torch.isfinite(dq[0, :, 2:]).all()
+    assert torch.isnan(dq[1, L // 2, 3]).all() and torch.isfinite(dq[1, :, 2]).all()
+    assert torch.isfinite(dk[0, :, 1]).all() and torch.isfinite(dv[0, :, 1]).all()
+    assert torch.isnan(dv[0, :, 0]).all() and torch.isnan(dv[1, :, 1]).all()
